@@ -30,39 +30,39 @@ LR, BETAS, EPS, DECAY = 2e-4, (0.9, 0.999), 1e-8, 0.01
 def listed():
     return [
         # One token through a small model's block: launches and host work.
-        {"name": "gated forward 1 row, 1.1B", "kind": "gated", "way": "forward", "rows": 1, "hidden": 2048,
+        {"name": "gated fwd 1 row (1.1B)", "kind": "gated", "way": "forward", "rows": 1, "hidden": 2048,
          "inter": 5632, "dtype": "bf16"},
         # An odd batch of sequences decoding through an 8B block: the packed weight is the traffic.
-        {"name": "gated forward 13 rows, 8B", "kind": "gated", "way": "forward", "rows": 13, "hidden": 4096,
+        {"name": "gated fwd 13 rows (8B)", "kind": "gated", "way": "forward", "rows": 13, "hidden": 4096,
          "inter": 14336, "dtype": "fp16"},
         # A short ragged prompt.
-        {"name": "gated forward 333 rows, 8B", "kind": "gated", "way": "forward", "rows": 333, "hidden": 4096,
+        {"name": "gated fwd 333 rows (8B)", "kind": "gated", "way": "forward", "rows": 333, "hidden": 4096,
          "inter": 14336, "dtype": "bf16"},
         # A training batch, forward only (the pass that a recomputing pipeline runs first).
-        {"name": "gated forward 8192 rows, 8B", "kind": "gated", "way": "forward", "rows": 8192, "hidden": 4096,
+        {"name": "gated fwd 8192 rows (8B)", "kind": "gated", "way": "forward", "rows": 8192, "hidden": 4096,
          "inter": 14336, "dtype": "bf16"},
         # A short fine-tuning sample on a small model: forward and the input's gradient.
-        {"name": "gated step 509 rows, 1.1B", "kind": "gated", "way": "step", "rows": 509, "hidden": 2048,
+        {"name": "gated step 509 rows (1.1B)", "kind": "gated", "way": "step", "rows": 509, "hidden": 2048,
          "inter": 5632, "dtype": "fp16"},
         # A training batch through an 8B block.
-        {"name": "gated step 4096 rows, 8B", "kind": "gated", "way": "step", "rows": 4096, "hidden": 4096,
+        {"name": "gated step 4096 rows (8B)", "kind": "gated", "way": "step", "rows": 4096, "hidden": 4096,
          "inter": 14336, "dtype": "bf16"},
         # Rank-16 adapters of one layer: the smallest set that is trained, launches and host work.
-        {"name": "adamw 32-bit, a 1.1B layer's adapters", "kind": "adamw", "bits": 32, "tensors": "adapters",
+        {"name": "adamw32 1.1B layer adapters", "kind": "adamw", "bits": 32, "tensors": "adapters",
          "hidden": 2048, "inter": 5632, "kv": 256, "layers": 1, "rank": 16, "param": "bf16", "master": False},
         # Rank-16 adapters on every projection of an 8B model, with 32-bit masters of the 16-bit parameters.
-        {"name": "adamw 32-bit, 8B adapters, masters", "kind": "adamw", "bits": 32, "tensors": "adapters",
+        {"name": "adamw32 8B adapters masters", "kind": "adamw", "bits": 32, "tensors": "adapters",
          "hidden": 4096, "inter": 14336, "kv": 1024, "layers": 32, "rank": 16, "param": "bf16", "master": True},
         # The same adapters in 32 bits, with 8-bit states.
-        {"name": "adamw 8-bit, 8B adapters", "kind": "adamw", "bits": 8, "tensors": "adapters", "hidden": 4096,
+        {"name": "adamw8 8B adapters", "kind": "adamw", "bits": 8, "tensors": "adapters", "hidden": 4096,
          "inter": 14336, "kv": 1024, "layers": 32, "rank": 16, "param": "fp32", "master": False},
         # Every projection of four small layers trained in full, with 8-bit states.
-        {"name": "adamw 8-bit, four 1.1B layers", "kind": "adamw", "bits": 8, "tensors": "dense", "hidden": 2048,
+        {"name": "adamw8 four 1.1B layers", "kind": "adamw", "bits": 8, "tensors": "dense", "hidden": 2048,
          "inter": 5632, "kv": 256, "layers": 4, "rank": 0, "param": "bf16", "master": False},
         # The norm over one layer's adapter gradients, and over those of a whole 8B model.
-        {"name": "norm, a 1.1B layer's adapters", "kind": "norm", "tensors": "adapters", "hidden": 2048,
+        {"name": "norm 1.1B layer adapters", "kind": "norm", "tensors": "adapters", "hidden": 2048,
          "inter": 5632, "kv": 256, "layers": 1, "rank": 16, "grad": "bf16"},
-        {"name": "norm, 8B adapters", "kind": "norm", "tensors": "adapters", "hidden": 4096, "inter": 14336,
+        {"name": "norm 8B adapters", "kind": "norm", "tensors": "adapters", "hidden": 4096, "inter": 14336,
          "kv": 1024, "layers": 32, "rank": 32, "grad": "bf16"},
     ]
 
