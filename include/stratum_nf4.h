@@ -316,6 +316,56 @@ int stm_nf4_dequantize_aug(const uint8_t* packed, const float* absmax, const voi
                            int64_t N, int64_t K, int blocksize, int dtype, void* stream);
 
 /*
+ * The end of a training step, over many tensors at once. No counterpart in the
+ * reference's NF4 path (its optimizer runs torch's AdamW per tensor on the host,
+ * stratum/optim.py:72); written for the adapters that the frozen base is trained with.
+ *
+ * stm_grad_norm: out[0] = |g| / loss_scale over all elements of all tensors, out[1] =
+ *   min(1, max_norm / (out[0] + 1e-6)) / loss_scale, the factor that clips and
+ *   unscales the gradients; NaN where the norm is not finite. out: two floats on the
+ *   device. max_norm >= 0 (INFINITY: no clipping). Sums in fp64 in a fixed order.
+ *   Workspace: stm_grad_norm_workspace_bytes(count, n) bytes, 8-byte aligned.
+ *   count, grads, n: host arrays of device pointers and element counts; one dtype.
+ *
+ * stm_adamw_step: step t = `step` (from 1) of AdamW on every tensor,
+ *     g' = scale g;  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ *   in fp32, rounded once to the parameter's type. scale = *grad_scale, a float on
+ *   the device (NULL: 1); where it is not finite, nothing is written. `master`, where
+ *   given, holds p in fp32 and `param` receives it rounded. state_bits 32: exp_avg and
+ *   exp_avg_sq are floats, the scales unused. state_bits 8: one code per element and
+ *   one float per 256 elements (ceil(n / 256)), see stm_state8_codes.
+ *   Any element-aligned pointers; 16-byte aligned ones (8 for 8-bit codes) are faster.
+ *   `tensors` is a host array, read before the call returns.
+ *
+ * stm_state8_codes / stm_state8_values: fp32 values to codes and scales, and back.
+ *   A block of 256 elements has its largest magnitude as scale. A code is a sign bit
+ *   (is_signed only: 7 bits of magnitude below it, K = 6; otherwise 8 bits, K = 7) and
+ *   a magnitude q: 0 is zero, else with k = floor(log2 q) the value is
+ *   (7 q + 7 - 6 * 2^k) * 2^(2 k - 3 - 3 K) times the scale, the nearest one; without
+ *   a sign a positive value never becomes zero.
+ */
+typedef struct {
+    void* param;
+    const void* grad;
+    float* master; /* or NULL */
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;    /* 8-bit states */
+    float* exp_avg_sq_scale; /* 8-bit states */
+    int64_t n;
+} stm_adamw_tensor;
+
+int64_t stm_grad_norm_workspace_bytes(int count, const int64_t* n);
+int stm_grad_norm(int count, const void* const* grads, const int64_t* n, int dtype, double max_norm,
+                  double loss_scale, float* out, void* workspace, int64_t workspace_bytes, void* stream);
+int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype, int state_bits,
+                   double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                   const float* grad_scale, void* stream);
+int stm_state8_codes(const float* x, int64_t n, int is_signed, uint8_t* codes, float* scales, void* stream);
+int stm_state8_values(const uint8_t* codes, const float* scales, int64_t n, int is_signed, float* out, void* stream);
+
+/*
  * Host-only introspection used by the CPU test suite (no GPU work):
  * the 15 fp32 decision boundaries of a rounding rule (code > i iff s >= b[i]),
  * and the 65-cell table the quantize kernel indexes with

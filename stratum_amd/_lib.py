@@ -32,6 +32,7 @@ ABI_VERSION = 5
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+_D = ctypes.c_double
 SIGNATURES = {
     "stm_nf4_abi_version": ([], _I),
     "stm_last_error": ([], ctypes.c_char_p),
@@ -58,6 +59,11 @@ SIGNATURES = {
     "stm_nf4_dequantize_aug": ([_P, _P, _P, _I, _P, _I64, _I64, _I, _I, _P], _I),
     "stm_lora_up": ([_P, _P, _P, _P, _I64, _I64, _I, _I, _I, _P], _I),
     "stm_lora_da": ([_P, _P, _P, _I64, _I64, _I, _I, _P, _I64, _P], _I),
+    "stm_grad_norm_workspace_bytes": ([_I, _P], _I64),
+    "stm_grad_norm": ([_I, _P, _P, _I, _D, _D, _P, _P, _I64, _P], _I),
+    "stm_adamw_step": ([_I, _P, _I, _I, _I, _D, _D, _D, _D, _D, _I64, _P, _P], _I),
+    "stm_state8_codes": ([_P, _I64, _I, _P, _P, _P], _I),
+    "stm_state8_values": ([_P, _P, _I64, _I, _P, _P], _I),
     "stm_nf4_decision_boundaries": ([_I, _P], _I),
     "stm_nf4_cell_table": ([_I, _P, _P], _I),
 }

@@ -1,0 +1,323 @@
+"""The end of a training step on the GPU: the norm of all gradients and AdamW over
+many tensors, each in a few launches of hand-written kernels.
+
+The reference steps its LoRA parameters with torch's AdamW, one tensor after another on
+the host (``stratum/optim.py:72``), and unscales and clips their gradients there
+(``stratum/grad_scaler.py``). Here nothing leaves the GPU: :func:`grad_norm` leaves the
+norm and the factor that clips (and unscales) the gradients in device memory, the step
+reads the factor there, and a step whose gradients are not finite changes nothing.
+
+* :class:`AdamW` is a ``torch.optim.Optimizer`` with states in 32 bits or in 8, and
+  optional fp32 masters of 16-bit parameters;
+* :class:`AdamWTensors` is the step over lists of tensors that the caller holds;
+* :func:`state_codes` and :func:`state_values` convert fp32 values to 8-bit states and back.
+
+An 8-bit state holds one code per element and one fp32 scale per 256 elements (the largest
+magnitude among them); the levels are dense near the scale and reach down to 8^-6 (first
+moment, which has a sign) or 8^-7 (second moment) of it. A step reads and writes 4 bytes
+of states per element instead of 16.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Iterable, Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import _lib
+
+__all__ = ["AdamW", "AdamWTensors", "STATE_BLOCK", "grad_norm", "state_codes", "state_values"]
+
+STATE_BLOCK = 256  # elements per scale of an 8-bit state
+
+# columns of a row of the tensor table (stm_adamw_tensor)
+_PARAM, _GRAD, _MASTER, _M, _V, _M_SCALE, _V_SCALE, _N = range(8)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // STATE_BLOCK)
+
+
+def _gpu(t: torch.Tensor, what: str) -> torch.device:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} runs on the GPU kernels; got a tensor on {t.device}")
+    return t.device
+
+
+def _held(name: str, t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype, numel: int) -> None:
+    """*t* can stand beside the parameter *like* in the tensor table."""
+    if t.dtype != dtype or t.numel() != numel or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {numel} elements on {like.device}, got "
+                         f"{t.dtype}, {t.numel()} elements on {t.device}, "
+                         f"{'' if t.is_contiguous() else 'not '}contiguous")
+
+
+class AdamWTensors:
+    """One AdamW step over lists of tensors: ``params`` of one dtype (fp32, bf16 or fp16),
+    their moments, and optionally fp32 ``masters`` of which the parameters are rounded
+    copies. ``scales`` = (first moments' scales, second moments' scales) makes the moments
+    8-bit codes (uint8, with ``ceil(numel / 256)`` fp32 scales each); without it they are
+    fp32. All contiguous, on one GPU. The tensors are checked once, here, and written in
+    place by :meth:`step`.
+    """
+
+    def __init__(self, params: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+                 exp_avg_sqs: Sequence[torch.Tensor], *, masters: Optional[Sequence[torch.Tensor]] = None,
+                 scales: Optional[tuple] = None):
+        params, exp_avgs, exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)
+        if not params:
+            raise ValueError("AdamWTensors needs at least one tensor")
+        first = params[0]
+        self.device, self.dtype = _gpu(first, "AdamW"), first.dtype
+        self.param_tag = _lib.dtype_tag(first.dtype)
+        self.state_bits = 8 if scales is not None else 32
+        state_dtype = torch.uint8 if scales is not None else torch.float32
+        columns = {"exp_avg": exp_avgs, "exp_avg_sq": exp_avg_sqs}
+        if masters is not None:
+            columns["master"] = masters = list(masters)
+        if scales is not None:
+            columns["exp_avg scale"], columns["exp_avg_sq scale"] = (list(s) for s in scales)
+        for name, column in columns.items():
+            if len(column) != len(params):
+                raise ValueError(f"{len(params)} parameters, but {len(column)} of {name}")
+        for i, p in enumerate(params):
+            n = p.numel()
+            _held(f"parameter {i}", p, first, first.dtype, n)
+            for name, column in columns.items():
+                dtype = state_dtype if name in ("exp_avg", "exp_avg_sq") else torch.float32
+                _held(f"{name} {i}", column[i], first, dtype, _blocks(n) if name.endswith("scale") else n)
+        self._sizes = [p.numel() for p in params]
+        table = np.zeros((len(params), 8), dtype=np.int64)
+        for at, column in ((_PARAM, params), (_M, exp_avgs), (_V, exp_avg_sqs), (_MASTER, columns.get("master")),
+                           (_M_SCALE, columns.get("exp_avg scale")), (_V_SCALE, columns.get("exp_avg_sq scale"))):
+            if column is not None:
+                table[:, at] = [t.data_ptr() for t in column]
+        table[:, _N] = self._sizes
+        self._table = table
+        # everything a step writes: held here (the table has bare addresses), and its versions counted up
+        self._written = [t for column in (params, *columns.values()) for t in column]
+
+    def at(self) -> list:
+        """The parameters' addresses."""
+        return self._table[:, _PARAM].tolist()
+
+    def step(self, grads: Sequence[Optional[torch.Tensor]], *, step: int, lr: float, betas: tuple = (0.9, 0.999),
+             eps: float = 1e-8, weight_decay: float = 0.01, grad_scale: Optional[torch.Tensor] = None) -> None:
+        """Step number ``step`` (from 1) with one gradient per parameter, of one dtype; a
+        tensor whose gradient is None stays as it is. ``grad_scale``, an fp32 scalar on the GPU, multiplies the
+        gradients first (``grad_norm(...)[1]``); where it is not finite the step writes nothing.
+        Runs on the current stream, without synchronising."""
+        if len(grads) != len(self._sizes):
+            raise ValueError(f"{len(self._sizes)} parameters, but {len(grads)} gradients")
+        if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
+                                       or grad_scale.device != self.device):
+            raise ValueError(f"grad_scale must be one fp32 value on {self.device}")
+        table, written, dtype, index = self._table, self._written, None, self.device.index
+        addresses, kept = [], None
+        for i, (g, n) in enumerate(zip(grads, self._sizes)):
+            if g is None:
+                addresses.append(0)
+                continue
+            if dtype is None:
+                dtype = g.dtype
+                tag = _lib.dtype_tag(dtype)
+            if g.dtype != dtype or g.numel() != n or g.get_device() != index:
+                raise ValueError(f"gradient {i} must hold {n} {dtype} elements on {self.device}, got {g.numel()} "
+                                 f"{g.dtype} on {g.device}")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                kept = (kept or []) + [g]  # until the launch, whose stream it was made on
+            addresses.append(g.data_ptr())
+        if dtype is None:
+            return
+        table[:, _GRAD] = addresses
+        if 0 in addresses:
+            some = [i for i, g in enumerate(grads) if g is not None]
+            per = len(self._sizes)
+            table = np.ascontiguousarray(table[some])
+            written = [written[c * per + i] for c in range(len(written) // per) for i in some]
+        with _lib.device_guard(self.device):
+            rc = _lib.lib().stm_adamw_step(
+                len(table), table.ctypes.data, self.param_tag, tag, self.state_bits, lr, betas[0], betas[1], eps,
+                weight_decay, step, grad_scale.data_ptr() if grad_scale is not None else None,
+                _lib.stream_handle(self.device))
+        _lib.check(rc, "stm_adamw_step")
+        torch.autograd.graph.increment_version(written)
+
+
+def grad_norm(grads: Iterable[Optional[torch.Tensor]], max_norm: float = math.inf, *,
+              loss_scale: float = 1.0) -> torch.Tensor:
+    """``[norm, factor]`` (fp32, on the GPU) over all elements of all gradients: the 2-norm
+    divided by ``loss_scale``, and ``min(1, max_norm / (norm + 1e-6)) / loss_scale``, the
+    factor to multiply the gradients with; NaN where the norm is not finite, which makes
+    the step that reads it change nothing. fp64 sums in a fixed order; no synchronisation."""
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        raise ValueError("grad_norm needs at least one gradient")
+    dev, dtype = _gpu(grads[0], "grad_norm"), grads[0].dtype
+    tag = _lib.dtype_tag(dtype)
+    for i, g in enumerate(grads):
+        if g.dtype != dtype or g.get_device() != dev.index:
+            raise ValueError(f"gradient {i} must be {dtype} on {dev}, got {g.dtype} on {g.device}")
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    sizes = np.array([g.numel() for g in grads], dtype=np.int64)
+    addresses = np.array([g.data_ptr() for g in grads], dtype=np.int64)
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    lib = _lib.lib()
+    nbytes = lib.stm_grad_norm_workspace_bytes(len(grads), sizes.ctypes.data)
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev)
+    with _lib.device_guard(dev):
+        rc = lib.stm_grad_norm(len(grads), addresses.ctypes.data, sizes.ctypes.data, tag, max_norm, loss_scale,
+                               out.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_handle(dev))
+    _lib.check(rc, "stm_grad_norm")
+    return out
+
+
+def state_codes(values: torch.Tensor, *, signed: bool) -> tuple:
+    """(codes uint8 like ``values``, scales fp32 [ceil(numel / 256)]) of an 8-bit state."""
+    dev = _gpu(values, "state_codes")
+    x = values.detach().to(torch.float32).contiguous()
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=dev)
+    scales = torch.empty(_blocks(x.numel()), dtype=torch.float32, device=dev)
+    with _lib.device_guard(dev):
+        rc = _lib.lib().stm_state8_codes(x.data_ptr(), x.numel(), int(signed), codes.data_ptr(), scales.data_ptr(),
+                                         _lib.stream_handle(dev))
+    _lib.check(rc, "stm_state8_codes")
+    return codes, scales
+
+
+def state_values(codes: torch.Tensor, scales: torch.Tensor, *, signed: bool) -> torch.Tensor:
+    """The fp32 values that an 8-bit state stands for, in the shape of ``codes``."""
+    dev = _gpu(codes, "state_values")
+    n = codes.numel()
+    if codes.dtype != torch.uint8:
+        raise ValueError(f"codes must be uint8, got {codes.dtype}")
+    if scales.dtype != torch.float32 or scales.numel() != _blocks(n) or scales.device != dev:
+        raise ValueError(f"scales must hold {_blocks(n)} fp32 values on {dev}")
+    c, s = codes.contiguous(), scales.contiguous()
+    out = torch.empty(codes.shape, dtype=torch.float32, device=dev)
+    with _lib.device_guard(dev):
+        rc = _lib.lib().stm_state8_values(c.data_ptr(), s.data_ptr(), n, int(signed), out.data_ptr(),
+                                          _lib.stream_handle(dev))
+    _lib.check(rc, "stm_state8_values")
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over parameters on one or several GPUs, a few launches per step.
+
+    ``state_bits`` = 32 or 8; ``master_weights`` keeps an fp32 master of every 16-bit
+    parameter, which takes the updates that bf16 or fp16 would round away (a parameter that
+    something else writes in place between two steps is taken over into its master).
+    ``max_grad_norm`` clips by the norm over all parameters (of one GPU each); ``grad_norm``
+    then holds the last norms, one tensor per GPU and gradient dtype, still on the device. A gradient that
+    is not finite makes the step change nothing (it still counts as a step)."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: tuple = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False,
+                 max_grad_norm: Optional[float] = None):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
+            raise ValueError("lr, eps and weight_decay must not be negative")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must lie in [0, 1), got {betas}")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"max_grad_norm must not be negative, got {max_grad_norm}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.master_weights, self.max_grad_norm = state_bits, master_weights, max_grad_norm
+        self.grad_norm: list = []
+        self._plans: dict = {}
+        self._versions: dict = {}  # of the parameters, as the last step left them
+
+    def _state(self, p: torch.Tensor) -> dict:
+        state = self.state[p]
+        if "step" not in state:
+            state["step"] = 0
+            dtype = torch.uint8 if self.state_bits == 8 else torch.float32
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.zeros(p.shape, dtype=dtype, device=p.device)
+                if self.state_bits == 8:
+                    state[name + "_scale"] = torch.zeros(_blocks(p.numel()), dtype=torch.float32, device=p.device)
+            if self.master_weights and p.dtype != torch.float32:
+                state["master"] = p.detach().to(torch.float32).contiguous()
+        elif "master" in state and self._versions.get(p, p._version) != p._version:
+            state["master"].copy_(p)
+        self._versions[p] = p._version
+        return state
+
+    def _plan(self, key: tuple, params: list) -> AdamWTensors:
+        """The checked tensor table of a group's parameters of one kind; made again when
+        one of them is no longer the same tensor or has moved."""
+        states = [self._state(p) for p in params]
+        held = [id(t) for s in states for name, t in s.items() if name != "step"]
+        plan = self._plans.get(key)
+        if plan is None or plan[0] != held or plan[1].at() != [p.data_ptr() for p in params]:
+            eight = self.state_bits == 8
+            tensors = AdamWTensors(
+                [p.detach() for p in params], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                masters=[s["master"] for s in states] if "master" in states[0] else None,
+                scales=([s["exp_avg_scale"] for s in states], [s["exp_avg_sq_scale"] for s in states]) if eight else None)
+            plan = self._plans[key] = (held, tensors)  # which keeps the tensors, so their ids stay theirs
+        return plan[1]
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale: Optional[torch.Tensor] = None):
+        """One step. ``grad_scale`` (an fp32 scalar on the GPU, as :func:`grad_norm` leaves
+        it) multiplies the gradients, in place of ``max_grad_norm``."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        # the tensors of one launch: one group, device, types and step number
+        sets: dict = {}
+        for gi, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError("AdamW does not take sparse gradients")
+                key = (gi, p.device, p.dtype, p.grad.dtype, self._state(p)["step"])
+                sets.setdefault(key, []).append(p)
+        factors: dict = {}
+        if grad_scale is None and self.max_grad_norm is not None:
+            factors = self._clip(sets)
+        for (gi, device, dtype, grad_dtype, count), params in sets.items():
+            group = self.param_groups[gi]
+            self._plan((gi, device, dtype, grad_dtype), params).step(
+                [p.grad for p in params], step=count + 1, lr=float(group["lr"]), betas=group["betas"],
+                eps=group["eps"], weight_decay=group["weight_decay"],
+                grad_scale=grad_scale if grad_scale is not None else factors.get(device))
+            for p in params:
+                self.state[p]["step"] = count + 1
+                self._versions[p] = p._version
+        return loss
+
+    def _clip(self, sets: dict) -> dict:
+        """The clip factor of each GPU, from the norm over all its gradients."""
+        grads: dict = {}
+        for (_, device, _, grad_dtype, _), params in sets.items():
+            grads.setdefault(device, {}).setdefault(grad_dtype, []).extend(p.grad for p in params)
+        self.grad_norm, factors = [], {}
+        for device, by_dtype in grads.items():
+            norms = [grad_norm(gs, self.max_grad_norm) for gs in by_dtype.values()]
+            if len(norms) == 1:
+                norm = norms[0]
+            else:  # several gradient types: the norm of their norms
+                norm = grad_norm([torch.stack([n[0] for n in norms])], self.max_grad_norm)
+            self.grad_norm.append(norm[0])
+            factors[device] = norm[1]
+        return factors
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """As torch's, but states keep their own types (torch casts them to the parameter's)."""
+        super().load_state_dict(state_dict)
+        self._plans, self._versions = {}, {}
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(saved, params):
+            if i in state_dict["state"]:
+                self.state[p] = {name: v.detach().clone().to(p.device) if isinstance(v, torch.Tensor) else v
+                                 for name, v in state_dict["state"][i].items()}
