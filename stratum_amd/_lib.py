@@ -52,6 +52,9 @@ SIGNATURES = {
     "stm_nf4_grouped_gemm_bwd_dx": ([_P, _P, _P, _P, _P, _I, _I64, _P, _I64, _I64, _I, _I, _P], _I),
     "stm_swiglu_fwd": ([_P, _P, _I64, _I64, _I, _P], _I),
     "stm_swiglu_bwd": ([_P, _P, _P, _I64, _I64, _I, _P], _I),
+    "stm_nf4_gated_workspace_bytes": ([_I64, _I64, _I64], _I64),
+    "stm_nf4_gated_fwd": ([_P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
+    "stm_nf4_gated_bwd": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
     "stm_lora_workspace_bytes": ([_I64, _I64, _I, _I], _I64),
     "stm_lora_down": ([_P, _P, _P, _I64, _I64, _I, ctypes.c_float, _I, _P, _I64, _P], _I),
     "stm_lora_dy": ([_P, _P, _P, _P, _P, _I64, _I64, _I, ctypes.c_float, _I, _P, _I64, _P], _I),

@@ -406,6 +406,50 @@ int stm_nf4_gemm_bwd_dx(const void* dY, const uint8_t* packed, const float* absm
     return launch_gemm_bwd(g, dtype, (hipStream_t)stream);
 }
 
+int64_t stm_nf4_gated_workspace_bytes(int64_t M, int64_t I, int64_t K) {
+    g_err[0] = 0;
+    if (M < 0 || I < 0 || K < 0) return set_error(STM_ERR_INVALID, "gated_workspace_bytes: negative size");
+    return gated_workspace_bytes(M, I, K);
+}
+
+// Both directions of the gated block; dH only for the backward.
+static int gated(const char* who, const void* dH, const void* X, const uint8_t* packed, const float* absmax, void* out,
+                 int64_t M, int64_t I, int64_t K, int blocksize, int dtype, bool backward, void* workspace,
+                 int64_t workspace_bytes, void* stream) {
+    g_err[0] = 0;
+    int rc = check_gemm_common(who, X, packed, absmax, out, M, I, K, blocksize, dtype);
+    if (rc <= 0) return rc;
+    if (I % 8 != 0) return set_error(STM_ERR_UNSUPPORTED, "%s: I = %lld must be a multiple of 8", who, (long long)I);
+    if (K == 0) return set_error(STM_ERR_UNSUPPORTED, "%s: K = 0", who);
+    // 32-bit offsets into the weight, and at least one 256-row tile of activations and outputs
+    if (I * K >= (int64_t)1 << 32 || K > (int64_t)1 << 22 || I > (int64_t)1 << 21)
+        return set_error(STM_ERR_UNSUPPORTED, "%s: a weight of [2 x %lld, %lld] is too large", who, (long long)I,
+                         (long long)K);
+    if (backward && (!dH || !aligned(dH, 16)))
+        return set_error(STM_ERR_INVALID, "%s: the gradient must be 16-byte aligned and not NULL", who);
+    const int64_t need = gated_workspace_bytes(M, I, K);
+    if (need > 0 && !workspace) return set_error(STM_ERR_INVALID, "%s: a workspace of %lld bytes is needed", who, (long long)need);
+    if ((rc = check_workspace(who, workspace, workspace_bytes, need)) != STM_OK) return rc;
+    GemmArgs g{};
+    g.a = X; g.packed = packed; g.absmax = absmax; g.out = out; g.M = M; g.N = 2 * I; g.K = K;
+    g.blocksize = blocksize; g.num_groups = 1; g.dh = dH;
+    g.partial = need ? (float*)workspace : nullptr;
+    return launch_gated(g, backward ? 2 : 1, dtype, (hipStream_t)stream);
+}
+
+int stm_nf4_gated_fwd(const void* X, const uint8_t* packed, const float* absmax, void* H, int64_t M, int64_t I,
+                      int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    return gated("gated_fwd", nullptr, X, packed, absmax, H, M, I, K, blocksize, dtype, false, workspace,
+                 workspace_bytes, stream);
+}
+
+int stm_nf4_gated_bwd(const void* dH, const void* X, const uint8_t* packed, const float* absmax, void* dGU, int64_t M,
+                      int64_t I, int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes,
+                      void* stream) {
+    return gated("gated_bwd", dH, X, packed, absmax, dGU, M, I, K, blocksize, dtype, true, workspace, workspace_bytes,
+                 stream);
+}
+
 // Host copy of a grouped call's expert offsets: offsets[0] = 0, non-decreasing,
 // and (max_rows >= 0) no expert above max_rows rows. Read entirely on the host,
 // before any launch.

@@ -1038,6 +1038,101 @@ __device__ __forceinline__ void store_tile_f32_rw(const f32x16_t (&acc)[FA][FB],
     }
 }
 
+// ------------------------------------------------------------ gated forward
+// h = silu(x Wg^T) * (x Wu^T) for the stacked weight W = [Wg; Wu] of N = 2 I rows, and its
+// backward dgu = [dh u silu'(g) | dh silu(g)] with g and u computed again: the
+// kernels of the plain forward over W's rows in another order, in which a gate row and
+// the up row of the same output column reach the same lane, and an epilogue on the fp32
+// sums (one rounding where the product and the SwiGLU pass as two kernels make two, and
+// no [M, 2 I] tensor written and read between them).
+
+// Physical row of output column c of part 0 (gate) or 1 (up); columns past I only feed
+// outputs that are never stored.
+__device__ __forceinline__ int64_t gated_row(int64_t c, int part, int64_t I) {
+    return part * I + (c < I ? c : I - 1);
+}
+
+__device__ __forceinline__ float gate_sigmoid(float g) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+}
+__device__ __forceinline__ float gate_fwd(float g, float u) { return g * gate_sigmoid(g) * u; }
+__device__ __forceinline__ void gate_bwd(float g, float u, float dh, float& dg, float& du) {
+    const float s = gate_sigmoid(g), gs = g * s;
+    du = dh * gs;
+    dg = dh * u * (s + gs * (1.0f - s));
+}
+
+// Epilogue of a wave that holds gate columns [c0, c0 + 32) in acc[0] and up columns in
+// acc[1] over 32 FB rows: MODE 1 stores h [rows, I], MODE 2 reads dh [rows, I] and
+// stores dgu [rows, 2 I]. Through LDS as store_tile_lds (rows of four 16-byte chunks
+// per output, chunk slot c ^ (row % 4)), FB / 2 fragments at a time. I % 8 == 0.
+template <typename Tr, int FB, int MODE>
+__device__ __forceinline__ void store_gated(const f32x16_t (&acc)[2][FB], const GemmArgs& g, int c0, int orow_base,
+                                            int orows, int lane, uint4* stage) {
+    constexpr int NP = 2, FP = FB / NP, RP = 32 * FP;
+    static_assert(FB % NP == 0, "two passes");
+    const int I = (int)(g.N / 2), ld = MODE * I, hi = lane >> 5;
+    uint8_t* st = reinterpret_cast<uint8_t*>(stage);
+    uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        if (orow_base + p * RP >= orows) break;  // no valid row left (uniform)
+#pragma unroll
+        for (int jj = 0; jj < FP; ++jj) {
+            const int rr = 32 * jj + (lane & 31);
+            uint2 dh[4];
+            if constexpr (MODE == 2) {
+                const int row = orow_base + p * RP + rr;
+                const uint16_t* src = reinterpret_cast<const uint16_t*>(g.dh) + (int64_t)(row < orows ? row : orows - 1) * I;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int col = c0 + 8 * q + 4 * hi;
+                    dh[q] = *reinterpret_cast<const uint2*>(src + (col < I ? col : 0));
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                // four columns at a time out of the accumulators
+                f32x4_t a, b;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = acc[0][p * FP + jj][4 * q + e], b[e] = acc[1][p * FP + jj][4 * q + e];
+                __asm__ volatile("" : "+v"(a), "+v"(b));
+                float v[4], w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (MODE == 1) {
+                        v[e] = gate_fwd(a[e], b[e]);
+                    } else {
+                        const uint32_t d = e < 2 ? dh[q].x : dh[q].y;
+                        gate_bwd(a[e], b[e], Tr::to_f32((uint16_t)(e & 1 ? d >> 16 : d & 0xFFFFu)), v[e], w[e]);
+                    }
+                }
+                const int slot = q ^ (rr & 3);
+                uint2 pk;
+                pk.x = Tr::pack2(v[0], v[1]);
+                pk.y = Tr::pack2(v[2], v[3]);
+                *reinterpret_cast<uint2*>(st + rr * 64 + slot * 16 + 8 * hi) = pk;
+                if constexpr (MODE == 2) {
+                    pk.x = Tr::pack2(w[0], w[1]);
+                    pk.y = Tr::pack2(w[2], w[3]);
+                    *reinterpret_cast<uint2*>(st + RP * 64 + rr * 64 + slot * 16 + 8 * hi) = pk;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int part = 0; part < MODE; ++part)
+#pragma unroll
+            for (int it = 0; it < RP / 16; ++it) {
+                const int rr = 16 * it + lane / 4, c = lane % 4;
+                const uint4 v = stage[part * RP * 4 + rr * 4 + (c ^ (rr & 3))];
+                const int orow = orow_base + p * RP + rr, col = c0 + 8 * c;
+                if (orow < orows && col < I)
+                    *reinterpret_cast<uint4*>(out + ((int64_t)orow * ld + part * I + col)) = v;
+            }
+    }
+}
+
 // Instruction order of one sub-step of the register-weight kernels: SLOTS
 // slots of 1 MFMA, 2 VALU (dequantization) and 1 LDS read (activation
 // fragment or level table), an order the compiler's scheduler must follow.
@@ -1059,8 +1154,9 @@ __device__ __forceinline__ void rw_slot_pattern() {
 #define STM_SHORT_ITEMS 1
 #endif
 
-template <typename Tr, int BM, int WM>
+template <typename Tr, int BM, int WM, int GATED = 0>
 __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
+    static_assert(!GATED || WM == 1, "a wave's gated columns are its own");
     constexpr int BN = 256, NT = 256 * WM, FB = BM / WM / 32;
     const int tid = threadIdx.x, lane0 = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave & 3, xrow0 = (wave >> 2) * (BM / WM);
@@ -1119,6 +1215,7 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
     for (int i = 0; i < 2; ++i) {
         int64_t n = col_base + i * 32 + (lane & 31);
         n = n < N ? n : N - 1;
+        if constexpr (GATED) n = gated_row(col_base / 2 + (lane & 31), i, N / 2);
         ws.woff[i] = (uint32_t)(n * (K / 2) + kbase / 2 + 16 * (lane >> 5));
         ws.aoff[i] = (uint32_t)(n * (K >> ws.bshift));
     }
@@ -1216,7 +1313,7 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
     // the item's valid rows decide (uniform over the work-group, so every wave
     // takes the same branch and meets the same barriers)
     const int64_t valid = grp.rows - m0;
-    if constexpr (STM_SHORT_ITEMS && FB == 8 && WM == 1) {
+    if constexpr (STM_SHORT_ITEMS && FB == 8 && WM == 1 && !GATED) {
         if (valid <= 64)
             main_loop(std::integral_constant<int, 2>{});
         else if (valid <= 128)
@@ -1228,6 +1325,19 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
     }
 
     const int lane_e = opaque_lane(lane);
+    if constexpr (GATED) {
+        constexpr int RPW = 16 * FB * 8, PER_BUF = BM * 8 / RPW;
+        uint4* stage = (wave < PER_BUF ? sA0 + wave * RPW : sA1 + (wave - PER_BUF) * RPW);
+        __syncthreads();  // every wave is done reading the activation buffers
+        // Without a matrix instruction behind the main loop the compiler would move the sums
+        // to vector registers at its end and spill; and so it does if the loop has the
+        // short items' other forms.
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int f = 0; f < FB; ++f) __asm__ volatile("" : "+a"(acc[i][f]));
+        store_gated<Tr, FB, GATED>(acc, g, (int)(col_base / 2), (int)m0, (int)grp.rows, lane_e, stage);
+    } else {
     if (g.lora_rank > 0 && z == 0)
         lora_term<Tr, 2, FB>(acc, reinterpret_cast<const uint16_t*>(g.lora_w), col_base, N,
                              reinterpret_cast<const uint16_t*>(g.lora_x) + grp.row0 * g.lora_rank, m0 + xrow0, grp.rows,
@@ -1248,6 +1358,7 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
         store_tile_rw<Tr, 2, FB>(acc, reinterpret_cast<uint16_t*>(g.out) + grp.row0 * N, (int)N, (int)col_base,
                                  (int)N, (int)(m0 + xrow0), (int)grp.rows, reinterpret_cast<const uint16_t*>(g.bias),
                                  lane_e);
+    }
     }
     __syncthreads();
     }
@@ -1903,7 +2014,8 @@ struct GvCfg {
 };
 constexpr int GV_GK = 256;  // group depth of k_gemv_ks
 
-template <typename Tr, int MB, int GK, bool GROUPED = false>
+// PARTIAL: the sums are left in fp32 even where one range holds the whole reduction.
+template <typename Tr, int MB, int GK, bool GROUPED = false, bool PARTIAL = false>
 __global__ __launch_bounds__((64 * GvCfg<MB, GK>::WAVES)) void k_gemv_fwd(GemmArgs g, int groups_per_split) {
     using C = GvCfg<MB, GK>;
     constexpr int R = C::R, WAVES = C::WAVES;
@@ -2087,7 +2199,7 @@ __global__ __launch_bounds__((64 * GvCfg<MB, GK>::WAVES)) void k_gemv_fwd(GemmAr
                 const int64_t m = 16 * mb + r;
                 const int64_t nc = n0 + 16 * t + 4 * h;
                 if (m >= rows || nc >= N) continue;  // N % 8 == 0: all four columns valid
-                if (!GROUPED && g.splits > 1) {
+                if (PARTIAL || (!GROUPED && g.splits > 1)) {
                     *reinterpret_cast<float4*>(g.partial + (int64_t)z * rows * N + m * N + nc) =
                         make_float4(v4[t][mb][0], v4[t][mb][1], v4[t][mb][2], v4[t][mb][3]);
                 } else {
@@ -2186,7 +2298,9 @@ struct GkCfg {
     static_assert(8 * TW * 64 * 16 <= kW, "the slice sums fit the weight buffer");
 };
 
-template <typename Tr, int T, int TW, int XR, bool GROUPED = false>
+// GATED: a 16-row tile holds 8 output columns, column 2 h + i with gate row 4 h + i and up
+// row 4 h + 2 + i (h = 0..3, i = 0, 1), so that a lane's four sums are two columns.
+template <typename Tr, int T, int TW, int XR, bool GROUPED = false, int GATED = 0>
 __global__ __launch_bounds__(512) void k_gemv_ks(GemmArgs g) {
     using C = GkCfg<T, TW, XR>;
     constexpr int S = C::S, ROWS = C::ROWS, P = C::P;
@@ -2213,6 +2327,9 @@ __global__ __launch_bounds__(512) void k_gemv_ks(GemmArgs g) {
     uint16_t* yo = reinterpret_cast<uint16_t*>(g.out);
     auto body = [&]() {
     auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane(v); };
+    [[maybe_unused]] auto tile_row = [&](int row) {  // GATED: physical weight row
+        return gated_row(n0 / 2 + 8 * (row >> 4) + 2 * ((row >> 2) & 3) + (row & 1), (row >> 1) & 1, N / 2);
+    };
 
     // copy sources, per thread. Packed weight: row-slice q = 16 TW wave + 8 i +
     // lane / 8 of the step's RS, 16-byte piece (lane % 8) ^ key(row).
@@ -2223,7 +2340,7 @@ __global__ __launch_bounds__(512) void k_gemv_ks(GemmArgs g) {
         const int q = 16 * TW * wave + 8 * i + (lane >> 3), row = q % ROWS;
         wsl[i] = q / ROWS;
         wpiece[i] = (lane & 7) ^ ((row >> 1) & 7);
-        const int64_t n = n0 + row < N ? n0 + row : N - 1;
+        const int64_t n = GATED ? tile_row(row) : n0 + row < N ? n0 + row : N - 1;
         wsrc[i] = wpk + n * (K / 2) + 16 * wpiece[i];
     }
     // absmax: thread tid copies entries e = tid + 512 i = (row-slice q) nfl + j
@@ -2236,7 +2353,7 @@ __global__ __launch_bounds__(512) void k_gemv_ks(GemmArgs g) {
         const int e = tid + 512 * i, q = (e < acount ? e : 0) / nfl;
         asl[i] = q / ROWS;
         aj[i] = e % nfl;
-        const int64_t n = n0 + q % ROWS < N ? n0 + q % ROWS : N - 1;
+        const int64_t n = GATED ? tile_row(q % ROWS) : n0 + q % ROWS < N ? n0 + q % ROWS : N - 1;
         asrc[i] = wab + n * kblocks;
     }
     // activations: piece p = tid + 512 i of S x XR x 32 (row xr of slice xs)
@@ -2385,6 +2502,21 @@ __global__ __launch_bounds__(512) void k_gemv_ks(GemmArgs g) {
             v[1] += o.y;
             v[2] += o.z;
             v[3] += o.w;
+        }
+        if constexpr (GATED) {
+            const int64_t I = N / 2, c = n0 / 2 + 8 * (t0 + u) + 2 * h;
+            if (r >= M || c >= I) continue;  // I % 8 == 0: both columns valid
+            if constexpr (GATED == 1) {
+                *reinterpret_cast<uint32_t*>(yo + r * I + c) = Tr::pack2(gate_fwd(v[0], v[2]), gate_fwd(v[1], v[3]));
+            } else {
+                const uint32_t d = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(g.dh) + r * I + c);
+                float dg[2], du[2];
+                gate_bwd(v[0], v[2], Tr::to_f32((uint16_t)(d & 0xFFFFu)), dg[0], du[0]);
+                gate_bwd(v[1], v[3], Tr::to_f32((uint16_t)(d >> 16)), dg[1], du[1]);
+                *reinterpret_cast<uint32_t*>(yo + r * N + c) = Tr::pack2(dg[0], dg[1]);
+                *reinterpret_cast<uint32_t*>(yo + r * N + I + c) = Tr::pack2(du[0], du[1]);
+            }
+            continue;
         }
         // C[4 h + i][r] of tile t0 + u: weight row n0 + 16 (t0 + u) + 4 h + i, activation row r
         const int64_t m = r, nc = n0 + 16 * (t0 + u) + 4 * h;
@@ -2761,6 +2893,64 @@ __global__ __launch_bounds__(256) void k_split_reduce(const float* __restrict__ 
     }
 }
 
+// The gated forward's reduce: g and u are columns c and I + c of the partials [split][m][2 I].
+template <typename Tr, int MODE>
+__global__ __launch_bounds__(256) void k_gated_reduce(const float* __restrict__ partial, int splits, int64_t rows,
+                                                      int64_t I, const uint16_t* __restrict__ dh,
+                                                      uint16_t* __restrict__ out) {
+    const int64_t total = rows * (I / 4), plane = rows * 2 * I;
+    for (int64_t v = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; v < total; v += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t row = v / (I / 4), c = (v - row * (I / 4)) * 4;
+        const float* src = partial + row * 2 * I + c;
+        float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + I);
+        for (int z = 1; z < splits; ++z) {
+            const float4 p = *reinterpret_cast<const float4*>(src + z * plane);
+            const float4 q = *reinterpret_cast<const float4*>(src + z * plane + I);
+            a.x += p.x, a.y += p.y, a.z += p.z, a.w += p.w;
+            b.x += q.x, b.y += q.y, b.z += q.z, b.w += q.w;
+        }
+        const float ga[4] = {a.x, a.y, a.z, a.w}, up[4] = {b.x, b.y, b.z, b.w};
+        float x[4], y[4];
+        if constexpr (MODE == 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = gate_fwd(ga[e], up[e]);
+        } else {
+            const uint2 d2 = *reinterpret_cast<const uint2*>(dh + row * I + c);
+            const uint32_t d[2] = {d2.x, d2.y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                gate_bwd(ga[e], up[e], Tr::to_f32((uint16_t)(e & 1 ? d[e / 2] >> 16 : d[e / 2] & 0xFFFFu)), x[e], y[e]);
+        }
+        uint2 pk;
+        pk.x = Tr::pack2(x[0], x[1]);
+        pk.y = Tr::pack2(x[2], x[3]);
+        *reinterpret_cast<uint2*>(out + row * MODE * I + c) = pk;
+        if constexpr (MODE == 2) {
+            pk.x = Tr::pack2(y[0], y[1]);
+            pk.y = Tr::pack2(y[2], y[3]);
+            *reinterpret_cast<uint2*>(out + row * 2 * I + I + c) = pk;
+        }
+    }
+}
+
+int launch_gated_reduce(const GemmArgs& g, int mode, int dtype, hipStream_t stream) {
+    const int64_t I = g.N / 2, blocks = (g.M * (I / 4) + 255) / 256;
+    const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384)), block(256);
+#define STM_GR_LAUNCH(TR, MODE)                                                                                  \
+    hipLaunchKernelGGL((k_gated_reduce<TR, MODE>), grid, block, 0, stream, g.partial, g.splits, g.M, I,          \
+                       (const uint16_t*)g.dh, (uint16_t*)g.out)
+    if (dtype == STM_BF16 && mode == 1)
+        STM_GR_LAUNCH(BF16, 1);
+    else if (dtype == STM_BF16)
+        STM_GR_LAUNCH(BF16, 2);
+    else if (mode == 1)
+        STM_GR_LAUNCH(F16, 1);
+    else
+        STM_GR_LAUNCH(F16, 2);
+#undef STM_GR_LAUNCH
+    return check_launch("gated reduce");
+}
+
 // lora: add the rank-R term here (the small-M forward leaves it to the reduce)
 int launch_split_reduce(const GemmArgs& g, int64_t cols, const void* bias, int dtype, hipStream_t stream,
                         bool lora = false) {
@@ -2842,7 +3032,8 @@ GemvPlan gemv_plan(int64_t M, int64_t N, int64_t K) {
 
 bool use_gemv(int64_t M, int num_groups) { return num_groups == 1 && M > 0 && M <= STM_GEMV_MAX_M; }
 
-int launch_gemv_fwd(GemmArgs g, const GemvPlan& p, int dtype, hipStream_t stream) {
+// gated: 0, or the mode of the gated reduce that takes the partials
+int launch_gemv_fwd(GemmArgs g, const GemvPlan& p, int dtype, hipStream_t stream, int gated = 0) {
     const int ngroups = (int)((g.K + p.gk - 1) / p.gk);
     const int gps = (ngroups + p.splits - 1) / p.splits;
     const int splits = gps ? (ngroups + gps - 1) / gps : 1;  // every range non-empty (K = 0: one empty range)
@@ -2853,7 +3044,11 @@ int launch_gemv_fwd(GemmArgs g, const GemvPlan& p, int dtype, hipStream_t stream
         static_assert(GvCfg<MB, GK>::ROWS > 0, "config");                                        \
         if (p.rows != GvCfg<MB, GK>::ROWS) return set_error(STM_ERR_INVALID, "gemv plan rows"); \
         dim3 block(64 * GvCfg<MB, GK>::WAVES);                                                   \
-        if (dtype == STM_BF16)                                                                   \
+        if (gated && dtype == STM_BF16)                                                          \
+            hipLaunchKernelGGL((k_gemv_fwd<BF16, MB, GK, false, true>), grid, block, 0, stream, g, gps); \
+        else if (gated)                                                                          \
+            hipLaunchKernelGGL((k_gemv_fwd<F16, MB, GK, false, true>), grid, block, 0, stream, g, gps);  \
+        else if (dtype == STM_BF16)                                                              \
             hipLaunchKernelGGL((k_gemv_fwd<BF16, MB, GK>), grid, block, 0, stream, g, gps);      \
         else                                                                                     \
             hipLaunchKernelGGL((k_gemv_fwd<F16, MB, GK>), grid, block, 0, stream, g, gps);       \
@@ -2873,6 +3068,7 @@ int launch_gemv_fwd(GemmArgs g, const GemvPlan& p, int dtype, hipStream_t stream
                          (long long)g.M);
 #undef STM_GV_LAUNCH
     int rc = check_launch("gemm_fwd (small M)");
+    if (rc == STM_OK && gated) return launch_gated_reduce(g, gated, dtype, stream);
     if (rc != STM_OK || g.splits == 1) return rc;
     return launch_split_reduce(g, g.N, g.bias, dtype, stream, true);
 }
@@ -3449,6 +3645,106 @@ int launch_gemm_fwd(const GemmArgs& g0, int dtype, hipStream_t stream) {
         rc = launch_fwd_cfg<128, 128, 2, 2>(g, dtype, stream);
     if (rc != STM_OK || g.splits == 1) return rc;
     return launch_split_reduce(g, g.N, g.bias, dtype, stream);
+}
+
+namespace {
+
+// How a gated forward of M rows over the stacked weight [2 I, K] runs.
+struct GatedPlan {
+    enum Kind { kKs, kGemv, kSplit, kTile } kind;
+    int cfg;       // kKs: its configuration; kTile: the tile's rows (128, 192 or 256)
+    GemvPlan gv;   // kGemv
+    int tile, splits;  // kSplit: tile kind and reduction ranges
+    int64_t partial;   // fp32 values of workspace
+};
+
+GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
+    GatedPlan p{};
+    if (M <= STM_GEMV_MAX_M && tile_override() < 0) {
+        p.cfg = gemv_ks_config(M, N, K);
+        if (p.cfg) {
+            p.kind = GatedPlan::kKs;
+            return p;
+        }
+        p.kind = GatedPlan::kGemv;
+        p.gv = gemv_plan(M, N, K);
+        p.partial = (int64_t)p.gv.splits * M * N;
+        return p;
+    }
+    const Plan t = plan(M, N, K, false, 1);
+    if (t.splits > 1) {
+        p.kind = GatedPlan::kSplit;
+        p.tile = t.kind;
+        p.splits = t.splits;
+        p.partial = (int64_t)t.splits * M * N;
+        return p;
+    }
+    p.kind = GatedPlan::kTile;
+    p.cfg = t.kind == kBig || t.kind == kBig8 ? 256 : 128;
+    return p;
+}
+
+template <typename Tr, int GATED>
+int launch_gated_mode(GemmArgs g, const GatedPlan& p, hipStream_t stream) {
+    if (p.kind == GatedPlan::kKs) {
+        const dim3 grid((unsigned)((g.N + 16 * (p.cfg & 15) - 1) / (16 * (p.cfg & 15)))), block(512);
+        switch (p.cfg) {
+            case 1 | 1 << 4 | 4 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 1, 1, 4, false, GATED>), grid, block, 0, stream, g); break;
+            case 2 | 1 << 4 | 8 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 2, 1, 8, false, GATED>), grid, block, 0, stream, g); break;
+            case 4 | 1 << 4 | 16 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 4, 1, 16, false, GATED>), grid, block, 0, stream, g); break;
+            case 8 | 1 << 4 | 16 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 8, 1, 16, false, GATED>), grid, block, 0, stream, g); break;
+            case 4 | 2 << 4 | 4 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 4, 2, 4, false, GATED>), grid, block, 0, stream, g); break;
+            default: return set_error(STM_ERR_INVALID, "gated: small-M configuration %d", p.cfg);
+        }
+        return check_launch("gated (small M)");
+    }
+    const int64_t tiles = (g.M + p.cfg - 1) / p.cfg * ((g.N + 255) / 256);
+    if (tiles > 0x7FFFFFFFLL) return set_error(STM_ERR_UNSUPPORTED, "gated: grid too large");
+    if (p.cfg == 256)
+        hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 256, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);
+    else
+        hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 128, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);
+    return check_launch("gated");
+}
+
+}  // namespace
+
+// Rows whose activations and outputs the tile kernels reach with their 32-bit offsets.
+static int64_t gated_max_rows(int64_t N, int64_t K) {
+    const int64_t by_x = ((int64_t)1 << 31) / K - 1, by_out = ((int64_t)1 << 31) / N - 1;
+    return (by_x < by_out ? by_x : by_out) / 256 * 256;
+}
+
+int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K) {
+    return M > 0 && I > 0 && K > 0 ? gated_plan(M, 2 * I, K).partial * (int64_t)sizeof(float) : 0;
+}
+
+int launch_gated(const GemmArgs& g0, int mode, int dtype, hipStream_t stream) {
+    GemmArgs g = g0;
+    g.splits = 1;
+    const GatedPlan p = gated_plan(g.M, g.N, g.K);
+    if (p.kind == GatedPlan::kTile && g.M > gated_max_rows(g.N, g.K)) {  // 32-bit offsets: in runs of rows
+        for (int64_t m = 0; m < g0.M; m += g.M) {
+            g = g0;
+            g.M = g0.M - m < gated_max_rows(g.N, g.K) ? g0.M - m : gated_max_rows(g.N, g.K);
+            g.a = (const uint16_t*)g0.a + m * g.K;
+            g.dh = mode == 2 ? (const uint16_t*)g0.dh + m * (g.N / 2) : nullptr;
+            g.out = (uint16_t*)g0.out + m * (mode == 2 ? g.N : g.N / 2);
+            const int rc = launch_gated(g, mode, dtype, stream);
+            if (rc != STM_OK) return rc;
+        }
+        return STM_OK;
+    }
+    if (p.kind == GatedPlan::kGemv) return launch_gemv_fwd(g, p.gv, dtype, stream, mode);
+    if (p.kind == GatedPlan::kSplit) {
+        g.splits = p.splits;
+        const int rc = p.tile == kSmall ? launch_fwd_cfg<128, 128, 2, 2>(g, dtype, stream)
+                                        : launch_fwd_cfg<STM_FWD_BM, STM_FWD_BN, STM_FWD_WM, STM_FWD_WN>(g, dtype, stream);
+        return rc != STM_OK ? rc : launch_gated_reduce(g, mode, dtype, stream);
+    }
+    if (dtype == STM_BF16)
+        return mode == 1 ? launch_gated_mode<BF16, 1>(g, p, stream) : launch_gated_mode<BF16, 2>(g, p, stream);
+    return mode == 1 ? launch_gated_mode<F16, 1>(g, p, stream) : launch_gated_mode<F16, 2>(g, p, stream);
 }
 
 int launch_gemv_bwd(GemmArgs g, int dtype, hipStream_t stream) {

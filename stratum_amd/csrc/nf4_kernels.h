@@ -41,6 +41,8 @@ struct GemmArgs {
     // they compete with that kernel's reads (the LoRA step's backward reads dY
     // right after the forward wrote a 235 MB output: 1.2 % per step).
     int stream_out;
+    // Gated backward: the gradient of h, [M, N / 2].
+    const void* dh;
 };
 
 constexpr int64_t kStreamOutBytes = 64ll << 20;
@@ -79,5 +81,9 @@ int launch_dequantize_host(int count, const uint8_t* const* packed, const float*
                            int bs, void* const* out, int out_dtype, hipStream_t stream);
 int launch_gemm_fwd(const GemmArgs& g, int dtype, hipStream_t stream);
 int launch_gemm_bwd(const GemmArgs& g, int dtype, hipStream_t stream);
+// Gated block over W [2 I, K]: mode 1 = forward (out [M, I]), 2 = backward from dh (out
+// [M, 2 I]); partial holds gated_workspace_bytes(M, I, K).
+int launch_gated(const GemmArgs& g, int mode, int dtype, hipStream_t stream);
+int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K);
 
 }  // namespace stm

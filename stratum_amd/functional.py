@@ -521,6 +521,81 @@ def nf4_gemm_bwd_dx(dy: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor
     return dx if len(lead) == 1 else dx.reshape(*lead, K)
 
 
+def gated_supported(inter: int, K: int, blocksize: int, backward: bool = False) -> bool:
+    """Widths that :func:`nf4_gated_fwd` takes (``backward``: also the input gradient behind it)."""
+    return K > 0 and not (K % 64 or K % blocksize or inter % (32 if backward else 8))
+
+
+def _gated_operands(x, packed, absmax, weight_shape, blocksize):
+    """(x as aligned rows, M, I, K, dtype tag, device) of a gated call, checked."""
+    N, K = int(weight_shape[0]), int(weight_shape[1])
+    if N % 2:
+        raise ValueError(f"weight_shape {tuple(weight_shape)}: the gate and up projections are stacked, so an even "
+                         "number of rows")
+    if x.shape[-1] != K:
+        raise ValueError(f"x has {x.shape[-1]} features, weight expects {K}")
+    tag = _gemm_dtype(x)
+    if not x.is_cuda:
+        raise RuntimeError("the gated block runs on the GPU kernels; x, packed and absmax must be on the GPU")
+    if not gated_supported(N // 2, K, blocksize):
+        raise ValueError(f"the gated block takes K a positive multiple of 64 and of the blocksize and I a multiple "
+                         f"of 8, got I = {N // 2}, K = {K}, blocksize {blocksize}")
+    x2 = _aligned(_rows(x, K))
+    _check_weight(packed, absmax, N, K, blocksize, x2.device)
+    return x2, x2.shape[0], N // 2, K, tag, x2.device
+
+
+def _gated_workspace(M: int, inter: int, K: int, device) -> Optional[torch.Tensor]:
+    nbytes = int(_lib.lib().stm_nf4_gated_workspace_bytes(M, inter, K))
+    if nbytes < 0:
+        _lib.check(nbytes, "stm_nf4_gated_workspace_bytes")
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+
+
+@_no_grad
+def nf4_gated_fwd(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, weight_shape: Sequence[int],
+                  blocksize: int = 64, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``silu(x @ Wg.T) * (x @ Wu.T)`` as [..., I] in x's dtype, for the stacked NF4 weight
+    [Wg; Wu] of shape ``weight_shape`` = (2 I, K): both projections and the gating in one
+    kernel, fp32 throughout, one rounding. (``swiglu_fwd(nf4_gemm_fwd(...))`` rounds the
+    projections first and writes and reads them.) ``out`` as for :func:`nf4_gemm_fwd`."""
+    x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
+    h = _out_buffer(out, (M, inter), x.dtype, dev)
+    with _lib.device_guard(dev):
+        ws = _gated_workspace(M, inter, K, dev)
+        rc = _lib.lib().stm_nf4_gated_fwd(
+            x2.data_ptr(), _aligned(packed).data_ptr(), _aligned(absmax, 4).data_ptr(), h.data_ptr(), M, inter, K,
+            blocksize, tag, ws.data_ptr() if ws is not None else None, 4 * ws.numel() if ws is not None else 0,
+            _lib.stream_handle(dev))
+    _lib.check(rc, "stm_nf4_gated_fwd")
+    return h if x.dim() == 2 else h.reshape(*x.shape[:-1], inter)
+
+
+@_no_grad
+def nf4_gated_bwd(grad_out: torch.Tensor, x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor,
+                  weight_shape: Sequence[int], blocksize: int = 64,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of :func:`nf4_gated_fwd` with respect to the two projections' outputs:
+    [..., 2 I] = [d gate | d up] in x's dtype, both projections computed again in the same
+    kernel. The input's gradient is ``nf4_gemm_bwd_dx`` of it with the same weight."""
+    x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
+    if grad_out.shape[-1] != inter or grad_out.dtype != x.dtype:
+        raise ValueError(f"grad_out must be [..., {inter}] {x.dtype}, got {tuple(grad_out.shape)} {grad_out.dtype}")
+    d2 = _aligned(_rows(grad_out, inter))
+    if d2.shape[0] != M:
+        raise ValueError(f"grad_out has {d2.shape[0]} rows, x has {M}")
+    _on_device(dev, grad_out=d2)
+    dgu = _out_buffer(out, (M, 2 * inter), x.dtype, dev)
+    with _lib.device_guard(dev):
+        ws = _gated_workspace(M, inter, K, dev)
+        rc = _lib.lib().stm_nf4_gated_bwd(
+            d2.data_ptr(), x2.data_ptr(), _aligned(packed).data_ptr(), _aligned(absmax, 4).data_ptr(), dgu.data_ptr(), M,
+            inter, K, blocksize, tag, ws.data_ptr() if ws is not None else None,
+            4 * ws.numel() if ws is not None else 0, _lib.stream_handle(dev))
+    _lib.check(rc, "stm_nf4_gated_bwd")
+    return dgu if x.dim() == 2 else dgu.reshape(*x.shape[:-1], 2 * inter)
+
+
 _OFFSETS_CACHE: "OrderedDict[tuple, tuple]" = OrderedDict()
 _OFFSETS_CACHE_SIZE = 8
 
