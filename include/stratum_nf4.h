@@ -382,6 +382,19 @@ int stm_grad_norm(int count, const void* const* grads, const int64_t* n, int dty
 int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype, int state_bits,
                    double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
                    const float* grad_scale, void* stream);
+/*
+ * stm_adamw_step with the list in device memory, one launch for any number of tensors
+ * (stm_adamw_step makes one per 56): stm_adamw_fill_table checks a list and writes
+ * stm_adamw_table_bytes(count) bytes of table to host memory (8-byte aligned) and returns
+ * the launch's work-groups (or a negative status); the caller copies them to the device
+ * on `stream` and passes them with the same count, types and state_bits.
+ */
+int64_t stm_adamw_table_bytes(int count);
+int stm_adamw_fill_table(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype, int state_bits,
+                         void* table);
+int stm_adamw_step_table(int count, const void* table, int groups, int param_dtype, int grad_dtype, int state_bits,
+                         double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                         const float* grad_scale, void* stream);
 int stm_state8_codes(const float* x, int64_t n, int is_signed, uint8_t* codes, float* scales, void* stream);
 int stm_state8_values(const uint8_t* codes, const float* scales, int64_t n, int is_signed, float* out, void* stream);
 

@@ -10,7 +10,12 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libstratum_nf4.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ["nf4_abi.hip", "nf4_quant.hip", "nf4_gemm.hip", "swiglu.hip", "lora.hip", "optim.hip"]
+SOURCES = ["nf4_abi.hip", "nf4_quant.hip", "nf4_gemm.hip", "swiglu.hip", "lora.hip", "gated_dense.hip",
+           "optim.hip"]
+
+# The host code of launch-bound calls, a CPython module against torch's headers.
+FAST_SOURCE = "fast_path.cpp"
+FAST_PATH = os.path.join(PKG_DIR, "_fast.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -58,6 +63,19 @@ def _finish(proc: subprocess.Popen, what: str, verbose: bool) -> None:
         print("\n".join(msgs), flush=True)
 
 
+def _start_fast(out: str, verbose: bool) -> subprocess.Popen:
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include = [sysconfig.get_paths()["include"], os.path.join(root, "include"),
+               os.path.join(root, "include", "torch", "csrc", "api", "include")]
+    return _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                 *(f"-I{d}" for d in include), os.path.join(CSRC, FAST_SOURCE), "-o", out,
+                 "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"], verbose)
+
+
 def build(verbose: bool = False) -> str:
     """Compile every source to an object (in parallel), then link the library.
     Objects go to a private temporary directory; nothing but the library is
@@ -66,6 +84,7 @@ def build(verbose: bool = False) -> str:
     compile_flags = [f for f in FLAGS if f != "-shared"]
     with tempfile.TemporaryDirectory(prefix="stm_build_") as tmpdir:
         objs, procs = [], []
+        fast = _start_fast(FAST_PATH + ".tmp", verbose)
         for src in SOURCES:
             obj = os.path.join(tmpdir, os.path.splitext(src)[0] + ".o")
             objs.append(obj)
@@ -74,9 +93,11 @@ def build(verbose: bool = False) -> str:
                           src))
         for proc, src in procs:
             _finish(proc, src, verbose)
+        _finish(fast, FAST_SOURCE, verbose)
         tmp = LIB_PATH + ".tmp"
         _finish(_run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs], verbose), LIB_NAME,
                 verbose)
+    os.replace(FAST_PATH + ".tmp", FAST_PATH)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 
@@ -65,6 +66,9 @@ SIGNATURES = {
     "stm_grad_norm_workspace_bytes": ([_I, _P], _I64),
     "stm_grad_norm": ([_I, _P, _P, _I, _D, _D, _P, _P, _I64, _P], _I),
     "stm_adamw_step": ([_I, _P, _I, _I, _I, _D, _D, _D, _D, _D, _I64, _P, _P], _I),
+    "stm_adamw_table_bytes": ([_I], _I64),
+    "stm_adamw_fill_table": ([_I, _P, _I, _I, _I, _P], _I),
+    "stm_adamw_step_table": ([_I, _P, _I, _I, _I, _I, _D, _D, _D, _D, _D, _I64, _P, _P], _I),
     "stm_state8_codes": ([_P, _I64, _I, _P, _P, _P], _I),
     "stm_state8_values": ([_P, _P, _I64, _I, _P, _P], _I),
     "stm_nf4_decision_boundaries": ([_I, _P], _I),
@@ -111,6 +115,28 @@ def lib():
                 raise NF4LibraryError(f"ABI version {L.stm_nf4_abi_version()} != {ABI_VERSION}")
             _lib = L
     return _lib
+
+
+_fast = None
+
+
+def fast():
+    """The native host code of launch-bound calls (csrc/fast_path.cpp)."""
+    global _fast
+    if _fast is None:
+        try:
+            from . import _fast as module
+        except ImportError as exc:
+            raise NF4LibraryError(f"{PKG_DIR}/_fast.so is not built or does not load ({exc}); build it with "
+                                  "`python -m stratum_amd._build` (or __graft_entry__.build())") from exc
+        _fast = module
+    return _fast
+
+
+@functools.lru_cache(maxsize=None)
+def address(name: str) -> int:
+    """Address of an entry point, for native callers."""
+    return ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
 
 
 def check(rc: int, what: str) -> None:

@@ -84,6 +84,11 @@ int launch_gemm_bwd(const GemmArgs& g, int dtype, hipStream_t stream);
 // Gated block over W [2 I, K]: mode 1 = forward (out [M, I]), 2 = backward from dh (out
 // [M, 2 I]); partial holds gated_workspace_bytes(M, I, K).
 int launch_gated(const GemmArgs& g, int mode, int dtype, hipStream_t stream);
+// The same from the weight's tiles at w (launch_dequantize_tiles: ceil(I / 128) * 256 * K values), `grid`
+// work-groups over the tiles.
+int launch_gated_dense(const GemmArgs& g, const void* w, int mode, int dtype, unsigned grid, hipStream_t stream);
+int launch_dequantize_tiles(const uint8_t* packed, const float* absmax, int64_t inter, int64_t K, int bs, void* out,
+                            int dtype, hipStream_t stream);
 int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K);
 
 }  // namespace stm

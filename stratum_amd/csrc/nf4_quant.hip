@@ -625,6 +625,73 @@ __global__ __launch_bounds__(256) void k_dequantize_aug(const uint32_t* __restri
     }
 }
 
+// Stacked [gate; up] weight [2 I, K] as the tiles of k_gated_dense: tile t holds the output
+// columns [128 t, + 128), its row r (of 256) the gate (fragment r / 32 even) or up row of
+// column 128 t + 32 (r / 64) + r % 32, and 32-deep step h of it is 16 KB in one piece,
+// [256 rows][4 chunks of 8 values], chunk c of row r in slot c ^ (r / 4) % 4. The product
+// then copies whole KBs in order; from rows of K values (stride 2 K bytes) the same copies
+// made it 4 % slower (8192 rows, W [2 x 14336, 4096], us: 1474 -> 1420). Columns past I
+// repeat the last one and are never stored.
+//
+// Bound by HBM. A work-group takes 64 rows of a tile over 16 steps: it reads 256
+// consecutive bytes of every row into LDS, then every wave takes 16 rows, four lanes a
+// row, so that its stores are 1 KB in one piece. (Words read straight into those lanes, 16
+// bytes of a row at a time: 94 us for W [2 x 14336, 4096].)
+template <int DT>
+__global__ __launch_bounds__(256) void k_dequantize_tiles(const uint4* __restrict__ q, const float* __restrict__ absmax,
+                                                          void* __restrict__ out, uint32_t inter, uint32_t steps,
+                                                          int gshift) {
+    constexpr uint32_t HS = 16, RS = HS + 1;  // steps of a work-group; 16-byte words of a staged row (padded)
+    __shared__ float2 lut[256];
+    __shared__ uint4 stage[64 * RS];
+    const uint32_t tile = blockIdx.x >> 2, wn = blockIdx.x & 3, h0 = blockIdx.y * HS;
+    auto weight_row = [&](uint32_t r) {  // of row r (of 64): gate rows, then up rows, of 32 columns
+        uint32_t col = tile * 128 + wn * 32 + (r & 31);
+        col = col < inter ? col : inter - 1;
+        return (r >> 5) * inter + col;
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t r = i * 16 + (threadIdx.x >> 4), h = threadIdx.x & 15;
+        stage[r * RS + h] = q[weight_row(r) * steps + (h0 + h < steps ? h0 + h : steps - 1)];
+    }
+    fill_byte_lut(lut);  // ends with a barrier
+    const uint32_t r = threadIdx.x >> 2, c = threadIdx.x & 3, rt = wn * 64 + r;
+    const uint32_t word0 = (weight_row(r) * steps + h0) * 4, slot = rt * 4 + (c ^ ((rt >> 2) & 3));
+    const uint32_t count = steps - h0 < HS ? steps - h0 : HS;  // even
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(stage) + r * (RS * 4) + c;
+    float a[HS / 2];  // a 64-deep block at least has one scale
+#pragma unroll
+    for (uint32_t j = 0; j < HS / 2; ++j) a[j] = absmax[(word0 + (2 * j < count ? 8 * j : 0)) >> gshift];
+#pragma unroll
+    for (uint32_t j = 0; j < HS; ++j) {
+        if (j >= count) break;
+        const uint32_t w = words[j * 4];
+        float v[8];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float2 l = lut[(w >> (8 * b)) & 0xFFu];
+            v[2 * b] = opaque(l.x * a[j / 2]);
+            v[2 * b + 1] = opaque(l.y * a[j / 2]);
+        }
+        store8<DT>(out, (int64_t)(tile * steps + h0 + j) * 1024 + slot, v);
+    }
+}
+
+int launch_dequantize_tiles(const uint8_t* packed, const float* absmax, int64_t inter, int64_t K, int bs, void* out,
+                            int dtype, hipStream_t stream) {
+    const dim3 grid((unsigned)((inter + 127) / 128 * 4), (unsigned)((K / 32 + 15) / 16)), block(256);
+    const int gshift = ilog2(bs) - 3;
+    const uint4* q = (const uint4*)packed;
+    if (dtype == STM_BF16)
+        hipLaunchKernelGGL(k_dequantize_tiles<STM_BF16>, grid, block, 0, stream, q, absmax, out, (uint32_t)inter,
+                           (uint32_t)(K / 32), gshift);
+    else
+        hipLaunchKernelGGL(k_dequantize_tiles<STM_F16>, grid, block, 0, stream, q, absmax, out, (uint32_t)inter,
+                           (uint32_t)(K / 32), gshift);
+    return check_launch("dequantize (tiles)");
+}
+
 int launch_dequantize_aug(const uint8_t* packed, const float* absmax, const void* L, int64_t rows, int64_t cols, int R,
                           int bs, void* out, int dtype, hipStream_t stream) {
     const int64_t total = rows * (cols / 8 + 8);

@@ -12,8 +12,8 @@
 // each (no contraction), so that a plain evaluation gives the same states bit for bit.
 //
 // Tensors travel as kernel arguments (pointers and sizes, one launch for up to
-// kAdamTensors / kNormTensors of them); a work-group finds its tensor by a ballot over
-// the prefix sums of work-groups.
+// kAdamTensors / kNormTensors of them), those of a long AdamW list in a table in device
+// memory; a work-group finds its tensor by a search in the prefix sums of work-groups.
 //
 // States in 8 bits. Blocks of 256 elements of a tensor share an fp32 scale, their
 // largest magnitude. A code holds a magnitude q of K + 1 bits (K = 6 below a sign bit
@@ -27,6 +27,8 @@
 // not zero never becomes zero (it takes the lowest level): with a first moment left,
 // a zero would divide by eps alone in a later step. Levels are dyadic, so the code is
 // arithmetic both ways: no table, no LDS.
+#include <type_traits>
+
 #include "nf4_common.h"
 
 namespace stm {
@@ -35,18 +37,36 @@ namespace {
 constexpr int kBlock8 = 256;      // elements per scale of an 8-bit state
 constexpr int kAdamTensors = 56;  // tensors per launch (below 4 KB of kernel arguments)
 constexpr int kNormTensors = 160;
-constexpr int kTile = 2048;       // elements per work-group: 256 threads of 8
+// Rows of 256 elements per wave: with one, a 32-bit step of 42 M elements takes 219 us, with two
+// 227, with four 240 (four accesses of a lane stand between a row's loads and its stores); an
+// 8-bit step of 176 M 477, 419 and 500 (two rows share a division).
+constexpr int rows_of(int bits) { return bits == 8 ? 2 : 1; }
+constexpr int tile_of(int bits) { return 4 * rows_of(bits) * kBlock8; }  // elements per work-group
+constexpr int kRows = rows_of(8), kTile = tile_of(8);                    // of the conversions
 constexpr int kNormTile = 16384;  // elements per work-group of the norm
 
-struct AdamArgs {
-    stm_adamw_tensor t[kAdamTensors];
-    int first[kAdamTensors];  // first work-group of tensor i
-    int count;
+struct AdamNumbers {
     float beta1, beta2, rest1, rest2;  // rest = 1 - beta
     float decay, step_size, inv_root2, eps;
     const float* scale;
 };
+
+// Up to kAdamTensors tensors in the kernel's arguments,
+struct AdamArgs {
+    stm_adamw_tensor t[kAdamTensors];
+    int first[kAdamTensors];  // first work-group of tensor i
+    int count;
+    AdamNumbers h;
+};
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
+
+// or any number in a table in device memory: `count` tensors, then their first work-groups.
+struct AdamTable {
+    const stm_adamw_tensor* t;
+    const int* first;
+    int count;
+    AdamNumbers h;
+};
 
 struct NormArgs {
     const void* g[kNormTensors];
@@ -56,17 +76,18 @@ struct NormArgs {
 };
 static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
 
-// The tensor that work-group b belongs to: the last one whose first work-group is at
-// or before b. Every lane of the wave takes part.
-template <int CAP>
-__device__ __forceinline__ int tensor_of(const int* first, int count, int b, int lane) {
-    int below = 0;
-#pragma unroll
-    for (int i0 = 0; i0 < CAP; i0 += 64) {
-        const int i = i0 + lane;
-        below += __popcll(__ballot(i < count && first[i < count ? i : 0] <= b));
+// The tensor that work-group b belongs to: the last one whose first work-group is at or
+// before b. Every read is uniform (scalar loads of the kernel arguments).
+__device__ __forceinline__ int tensor_of(const int* first, int count, int b) {
+    int lo = 0, hi = count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (first[mid] <= b)
+            lo = mid;
+        else
+            hi = mid;
     }
-    return __builtin_amdgcn_readfirstlane(below - 1);
+    return lo;
 }
 
 // ------------------------------------------------------------ element access
@@ -74,102 +95,92 @@ struct F32 {
     static constexpr int tag = STM_F32;
 };
 
+// Four elements at i of a tensor of n; `vec`: the base is aligned for one access.
 template <typename T>
-__device__ __forceinline__ void load8(const void* base, int64_t i, int64_t n, bool vec, float (&f)[8]) {
+__device__ __forceinline__ void load4(const void* base, int64_t i, int64_t n, bool vec, float (&f)[4]) {
     if constexpr (T::tag == STM_F32) {
         const float* p = reinterpret_cast<const float*>(base) + i;
-        if (vec && i + 8 <= n) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+        if (vec && i + 4 <= n) {
+            const float4 a = *reinterpret_cast<const float4*>(p);
+            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = i + e < n ? p[e] : 0.0f;
+            for (int e = 0; e < 4; ++e) f[e] = i + e < n ? p[e] : 0.0f;
         }
     } else {
         const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + i;
-        if (vec && i + 8 <= n) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f[2 * e] = T::to_f32((uint16_t)(w[e] & 0xFFFFu));
-                f[2 * e + 1] = T::to_f32((uint16_t)(w[e] >> 16));
-            }
+        if (vec && i + 4 <= n) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            f[0] = T::to_f32((uint16_t)(v.x & 0xFFFFu)), f[1] = T::to_f32((uint16_t)(v.x >> 16));
+            f[2] = T::to_f32((uint16_t)(v.y & 0xFFFFu)), f[3] = T::to_f32((uint16_t)(v.y >> 16));
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = i + e < n ? T::to_f32(p[e]) : 0.0f;
+            for (int e = 0; e < 4; ++e) f[e] = i + e < n ? T::to_f32(p[e]) : 0.0f;
         }
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(void* base, int64_t i, int64_t n, bool vec, const float (&f)[8]) {
+__device__ __forceinline__ void store4(void* base, int64_t i, int64_t n, bool vec, const float (&f)[4]) {
     if constexpr (T::tag == STM_F32) {
         float* p = reinterpret_cast<float*>(base) + i;
-        if (vec && i + 8 <= n) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        if (vec && i + 4 <= n) {
+            *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 4; ++e)
                 if (i + e < n) p[e] = f[e];
         }
     } else {
         uint16_t* p = reinterpret_cast<uint16_t*>(base) + i;
-        if (vec && i + 8 <= n) {
-            *reinterpret_cast<uint4*>(p) = make_uint4(T::pack2(f[0], f[1]), T::pack2(f[2], f[3]), T::pack2(f[4], f[5]),
-                                                      T::pack2(f[6], f[7]));
+        if (vec && i + 4 <= n) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(T::pack2(f[0], f[1]), T::pack2(f[2], f[3]));
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 4; ++e)
                 if (i + e < n) p[e] = T::from_f32(f[e]);
         }
     }
 }
 
-__device__ __forceinline__ void load_codes(const uint8_t* base, int64_t i, int64_t n, bool vec, uint32_t (&c)[8]) {
+// Four codes in a word, element 0 in the low byte.
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* base, int64_t i, int64_t n, bool vec) {
     const uint8_t* p = base + i;
-    if (vec && i + 8 <= n) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
+    if (vec && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(p);
+    uint32_t c = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = (v.x >> (8 * e)) & 255u, c[4 + e] = (v.y >> (8 * e)) & 255u;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = i + e < n ? p[e] : 0u;
-    }
+    for (int e = 0; e < 4; ++e) c |= i + e < n ? (uint32_t)p[e] << (8 * e) : 0u;
+    return c;
 }
 
-__device__ __forceinline__ void store_codes(uint8_t* base, int64_t i, int64_t n, bool vec, const uint32_t (&c)[8]) {
+__device__ __forceinline__ void store_codes(uint8_t* base, int64_t i, int64_t n, bool vec, uint32_t c) {
     uint8_t* p = base + i;
-    if (vec && i + 8 <= n) {
-        uint2 v;
-        v.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-        v.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-        *reinterpret_cast<uint2*>(p) = v;
+    if (vec && i + 4 <= n) {
+        *reinterpret_cast<uint32_t*>(p) = c;
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (i + e < n) p[e] = (uint8_t)c[e];
+        for (int e = 0; e < 4; ++e)
+            if (i + e < n) p[e] = (uint8_t)(c >> (8 * e));
     }
 }
 
 // ------------------------------------------------------------ the 8-bit code
-// level(q) for q in 0..2^(K+1) - 1
+// Value of magnitude q, given as a float: exact up to the product with the scale.
 template <int K>
-__device__ __forceinline__ float level8(uint32_t q) {
-    const int k = 31 - __builtin_clz(q | 1u);
-    const float a = (float)(int)(7u * q + 7u - (6u << k));
-    const float l = a * __uint_as_float((uint32_t)(127 + 2 * k - 3 - 3 * K) << 23);
-    return q ? l : 0.0f;
+__device__ __forceinline__ float level8(float q) {
+    const float top = __uint_as_float(__float_as_uint(q) & 0xFF800000u);  // 2^k, 0 for q = 0
+    const float a = fmaf(top, -6.0f, fmaf(q, 7.0f, 7.0f));
+    return a * top * (top * __uint_as_float((uint32_t)(127 - 3 - 3 * K) << 23));
 }
 
+// Values of the four codes of a word.
 template <bool SIGNED>
-__device__ __forceinline__ float decode8(uint32_t code, float scale) {
-    if constexpr (SIGNED) {
-        const float v = level8<6>(code & 127u);
-        return (code & 128u ? -v : v) * scale;
-    } else {
-        return level8<7>(code) * scale;
+__device__ __forceinline__ void decode4(uint32_t c, float scale, float (&f)[4]) {
+    const uint32_t q = SIGNED ? c & 0x7F7F7F7Fu : c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float v = level8<SIGNED ? 6 : 7>((float)((q >> (8 * e)) & 255u)) * scale;
+        f[e] = SIGNED ? __uint_as_float(__float_as_uint(v) ^ ((c << (24 - 8 * e)) & 0x80000000u)) : v;
     }
 }
 
@@ -177,115 +188,167 @@ __device__ __forceinline__ float decode8(uint32_t code, float scale) {
 // (zero, subnormal, infinite, NaN): its codes are zero (v: the lowest level).
 __device__ __forceinline__ float inverse_scale(float top) { return top >= 0x1p-126f ? 1.0f / top : 0.0f; }
 
+// Code of x in a block with that inverse scale. With s = |x| inv in segment z (8^-(z+1) <= s <
+// 8^-z; z = K: everything below), n = 2^(K-z) and c = 8/7 n, the step above the segment's
+// lower end is j = rint((8^z s - 1/8) c). The difference is exact in fp32, so one fma of s with
+// 8^z c and -c/8 gives the product rounded once, as the formula does; the rounding to a
+// whole number is that of adding 1.5 * 2^23. In the last segment j = rint(8^K s).
 template <bool SIGNED>
 __device__ __forceinline__ uint32_t encode8(float x, float inv) {
     constexpr int K = SIGNED ? 6 : 7;
+    constexpr uint32_t kC = 0x3F924925u, kMagic = 0x4B400000u;  // 8/7; 1.5 * 2^23
     const float s = fminf(fabsf(x) * inv, 1.0f);  // 1 also for an infinite x (inv is 0)
-    // segment z: 8^-(z+1) <= s < 8^-z (z = K: everything below), from the exponent
-    const int e = 126 - (int)(__float_as_uint(s) >> 23);
-    int z = e <= 0 ? 0 : (e * 43) >> 7;  // e / 3 for e <= 127
-    z = z < K ? z : K;
-    const float y = s * __uint_as_float((uint32_t)(127 + 3 * z) << 23);
-    // steps from the segment's lower end, 2^(K - z) of them between 1/8 and 1
-    const float per = __uint_as_float(__float_as_uint(8.0f / 7.0f) + ((uint32_t)(K - z) << 23));
-    const float j = z == K ? y : (y - 0.125f) * per;
-    const int q = (1 << (K - z)) - 1 + (int)rintf(j);
-    if constexpr (SIGNED) return (uint32_t)q | (x < 0.0f ? 128u : 0u);
-    return (uint32_t)(q == 0 && x > 0.0f ? 1 : q);
+    // z from the biased exponent E: floor((126 - E) / 3), in [0, K]
+    const int E = (int)(__float_as_uint(s) >> 23);
+    int z = (126 * 43 - 43 * E) >> 7;  // exact for 0 <= 126 - E <= 126
+    z = z < 0 ? 0 : z;
+    const bool last = z >= K;
+    z = last ? K : z;
+    const float mul = __uint_as_float(last ? (uint32_t)(127 + 3 * K) << 23 : kC + ((uint32_t)(2 * z + K) << 23));
+    const float sub = last ? 0.0f : __uint_as_float(kC + ((uint32_t)(K - 3 - z) << 23));
+    const uint32_t j = __float_as_uint(fmaf(s, mul, -sub) + 12582912.0f);
+    const uint32_t q = j + (((1u << K) >> z) - 1u - kMagic);
+    if constexpr (SIGNED) return q | ((__float_as_uint(x) >> 24) & 128u);
+    const uint32_t some = __float_as_uint(x) < 1u ? 0u : 1u;
+    return q > some ? q : some;
 }
 
-// The largest magnitude of the 32 lanes that share a block (8 elements each). Compared
-// as integers: the order of non-negative floats, with NaN above everything.
-__device__ __forceinline__ float block_top(const float (&f)[8]) {
+// The largest magnitude of a wave's 256 elements, the same in every lane. Compared as
+// integers: the order of non-negative floats, with NaN above everything.
+__device__ __forceinline__ float block_top(const float (&f)[4]) {
     uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4; ++e) {
         const uint32_t b = __float_as_uint(f[e]) & 0x7FFFFFFFu;
         top = top > b ? top : b;
     }
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)top, d);
+    auto step = [&](auto ctrl) {  // the maximum with another lane's, zero where there is none
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xF, 0xF, false);
         top = top > o ? top : o;
-    }
-    return __uint_as_float(top);
+    };
+    step(std::integral_constant<int, 0x111>());  // row_shr 1, 2, 4, 8: lane 15 of every row of 16 has its row's
+    step(std::integral_constant<int, 0x112>());
+    step(std::integral_constant<int, 0x114>());
+    step(std::integral_constant<int, 0x118>());
+    step(std::integral_constant<int, 0x142>());  // row_bcast 15, 31: lane 63 has the wave's
+    step(std::integral_constant<int, 0x143>());
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)top, 63));
+}
+
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t encode4(const float (&f)[4], float inv) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c |= encode8<SIGNED>(f[e], inv) << (8 * e);
+    return c;
 }
 
 // ------------------------------------------------------------ AdamW
-template <typename P, typename G, int BITS>
-__global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
+// A work-group takes kTile consecutive elements of one tensor: wave w, kRows rows of 256
+// elements, four a lane, so that every access of a wave is one contiguous piece and a row is a
+// block of an 8-bit state. All loads are issued before the first result is needed.
+template <typename P, typename G, int BITS, typename Args>
+__global__ __launch_bounds__(256) void k_adamw(Args args) {
+    const AdamNumbers& a = args.h;
     float scale = 1.0f;
     if (a.scale) {
         scale = *a.scale;
         if (!(fabsf(scale) < INFINITY)) return;  // the whole launch alike
     }
+    constexpr int kRows = rows_of(BITS);
     const int lane = threadIdx.x & 63;
-    const int ti = tensor_of<kAdamTensors>(a.first, a.count, (int)blockIdx.x, lane);
-    const stm_adamw_tensor t = a.t[ti];
-    const int64_t n = t.n, i = ((int64_t)blockIdx.x - a.first[ti]) * kTile + threadIdx.x * 8;
+    const int ti = tensor_of(args.first, args.count, (int)blockIdx.x);
+    const stm_adamw_tensor t = args.t[ti];
+    const int64_t n = t.n;
+    const int64_t base = ((int64_t)blockIdx.x - args.first[ti]) * tile_of(BITS) + (threadIdx.x >> 6) * (kRows * kBlock8) + lane * 4;
     auto al = [](const void* p, uintptr_t b) { return ((uintptr_t)p & (b - 1)) == 0; };
-    const bool vp = al(t.param, 16), vg = al(t.grad, 16);
-    const bool vs = al(t.exp_avg, BITS == 8 ? 8 : 16) && al(t.exp_avg_sq, BITS == 8 ? 8 : 16);
+    const bool vp = al(t.param, P::tag == STM_F32 ? 16 : 8), vg = al(t.grad, G::tag == STM_F32 ? 16 : 8);
+    const bool vs = al(t.exp_avg, BITS == 8 ? 4 : 16) && al(t.exp_avg_sq, BITS == 8 ? 4 : 16), vm = al(t.master, 16);
 
-    float p[8], g[8], m[8], v[8];
-    load8<G>(t.grad, i, n, vg, g);
-    if (t.master)
-        load8<F32>(t.master, i, n, al(t.master, 16), p);
-    else
-        load8<P>(t.param, i, n, vp, p);
-    if constexpr (BITS == 32) {
-        load8<F32>(t.exp_avg, i, n, vs, m);
-        load8<F32>(t.exp_avg_sq, i, n, vs, v);
-    } else {
-        uint32_t cm[8], cv[8];
-        load_codes((const uint8_t*)t.exp_avg, i, n, vs, cm);
-        load_codes((const uint8_t*)t.exp_avg_sq, i, n, vs, cv);
-        const int64_t b = i / kBlock8;
-        const float sm = i < n ? t.exp_avg_scale[b] : 0.0f, sv = i < n ? t.exp_avg_sq_scale[b] : 0.0f;
+    float p[kRows][4], g[kRows][4], m[kRows][4], v[kRows][4];
+    [[maybe_unused]] uint32_t cm[kRows], cv[kRows];
+    [[maybe_unused]] float sm[kRows], sv[kRows], tops[2 * kRows];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m[e] = decode8<true>(cm[e], sm), v[e] = decode8<false>(cv[e], sv);
+    for (int r = 0; r < kRows; ++r) {
+        const int64_t i = base + r * kBlock8;
+        load4<G>(t.grad, i, n, vg, g[r]);
+        if (t.master)
+            load4<F32>(t.master, i, n, vm, p[r]);
+        else
+            load4<P>(t.param, i, n, vp, p[r]);
+        if constexpr (BITS == 32) {
+            load4<F32>(t.exp_avg, i, n, vs, m[r]);
+            load4<F32>(t.exp_avg_sq, i, n, vs, v[r]);
+        } else {
+            cm[r] = load_codes((const uint8_t*)t.exp_avg, i, n, vs);
+            cv[r] = load_codes((const uint8_t*)t.exp_avg_sq, i, n, vs);
+            sm[r] = i < n ? t.exp_avg_scale[i / kBlock8] : 0.0f;
+            sv[r] = i < n ? t.exp_avg_sq_scale[i / kBlock8] : 0.0f;
+        }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float ge = g[e] * scale;
-        m[e] = m[e] * a.beta1 + ge * a.rest1;
-        v[e] = v[e] * a.beta2 + ge * a.rest2 * ge;
-        const float d = sqrtf(v[e]) * a.inv_root2 + a.eps;
-        p[e] = p[e] * a.decay - a.step_size * m[e] / d;
+    for (int r = 0; r < kRows; ++r) {
+        const int64_t i = base + r * kBlock8;
+        if constexpr (BITS == 8) {
+            decode4<true>(cm[r], sm[r], m[r]);
+            decode4<false>(cv[r], sv[r], v[r]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float ge = g[r][e] * scale;
+            m[r][e] = m[r][e] * a.beta1 + ge * a.rest1;
+            v[r][e] = v[r][e] * a.beta2 + ge * a.rest2 * ge;
+            // the update's root and reciprocal are the instructions' (one ulp each): it is added to p,
+            // where its last bits do not count, and neither state depends on it
+            const float d = __builtin_amdgcn_sqrtf(v[r][e]) * a.inv_root2 + a.eps;
+            p[r][e] = p[r][e] * a.decay - a.step_size * m[r][e] * __builtin_amdgcn_rcpf(d);
+        }
+        if (t.master) store4<F32>(t.master, i, n, vm, p[r]);
+        store4<P>(t.param, i, n, vp, p[r]);
+        if constexpr (BITS == 32) {
+            store4<F32>(t.exp_avg, i, n, vs, m[r]);
+            store4<F32>(t.exp_avg_sq, i, n, vs, v[r]);
+        } else {
+            if (i + 4 > n) {  // past the tensor: no part in the block's scale
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e >= n) m[r][e] = v[r][e] = 0.0f;
+            }
+            tops[2 * r] = block_top(m[r]);
+            tops[2 * r + 1] = block_top(v[r]);
+        }
     }
-    if (t.master) store8<F32>(t.master, i, n, al(t.master, 16), p);
-    store8<P>(t.param, i, n, vp, p);
-    if constexpr (BITS == 32) {
-        store8<F32>(t.exp_avg, i, n, vs, m);
-        store8<F32>(t.exp_avg_sq, i, n, vs, v);
-    } else {
+    if constexpr (BITS == 8) {
+        // one division for the wave's scales: lane i inverts number i
+        float mine = tops[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (i + e >= n) m[e] = v[e] = 0.0f;  // past the tensor: no part in the block's scale
-        const float tm = block_top(m), tv = block_top(v);
-        const float im = inverse_scale(tm), iv = inverse_scale(tv);
-        uint32_t cm[8], cv[8];
+        for (int k = 1; k < 2 * kRows; ++k) mine = lane == k ? tops[k] : mine;
+        const int inverse = (int)__float_as_uint(inverse_scale(mine));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) cm[e] = encode8<true>(m[e], im), cv[e] = encode8<false>(v[e], iv);
-        store_codes((uint8_t*)t.exp_avg, i, n, vs, cm);
-        store_codes((uint8_t*)t.exp_avg_sq, i, n, vs, cv);
-        if ((lane & 31) == 0 && i < n) {
-            t.exp_avg_scale[i / kBlock8] = tm;
-            t.exp_avg_sq_scale[i / kBlock8] = tv;
+        for (int r = 0; r < kRows; ++r) {
+            const int64_t i = base + r * kBlock8;
+            const float im = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(inverse, 2 * r));
+            const float iv = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(inverse, 2 * r + 1));
+            store_codes((uint8_t*)t.exp_avg, i, n, vs, encode4<true>(m[r], im));
+            store_codes((uint8_t*)t.exp_avg_sq, i, n, vs, encode4<false>(v[r], iv));
+            if (lane == 0 && i < n) {
+                t.exp_avg_scale[i / kBlock8] = tops[2 * r];
+                t.exp_avg_sq_scale[i / kBlock8] = tops[2 * r + 1];
+            }
         }
     }
 }
 
-template <typename P, typename G>
-void launch_adamw(const AdamArgs& a, int bits, unsigned grid, hipStream_t st) {
+template <typename P, typename G, typename Args>
+void launch_adamw(const Args& a, int bits, unsigned grid, hipStream_t st) {
     if (bits == 8)
-        hipLaunchKernelGGL((k_adamw<P, G, 8>), dim3(grid), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_adamw<P, G, 8, Args>), dim3(grid), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((k_adamw<P, G, 32>), dim3(grid), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_adamw<P, G, 32, Args>), dim3(grid), dim3(256), 0, st, a);
 }
 
-template <typename P>
-void launch_adamw(const AdamArgs& a, int grad_dtype, int bits, unsigned grid, hipStream_t st) {
+template <typename P, typename Args>
+void launch_adamw(const Args& a, int grad_dtype, int bits, unsigned grid, hipStream_t st) {
     if (grad_dtype == STM_F32)
         launch_adamw<P, F32>(a, bits, grid, st);
     else if (grad_dtype == STM_BF16)
@@ -294,19 +357,37 @@ void launch_adamw(const AdamArgs& a, int grad_dtype, int bits, unsigned grid, hi
         launch_adamw<P, F16>(a, bits, grid, st);
 }
 
+template <typename Args>
+int launch_adamw(const Args& a, int param_dtype, int grad_dtype, int bits, int64_t grid, hipStream_t st) {
+    if (param_dtype == STM_F32)
+        launch_adamw<F32>(a, grad_dtype, bits, (unsigned)grid, st);
+    else if (param_dtype == STM_BF16)
+        launch_adamw<BF16>(a, grad_dtype, bits, (unsigned)grid, st);
+    else
+        launch_adamw<F16>(a, grad_dtype, bits, (unsigned)grid, st);
+    return check_launch("adamw_step");
+}
+
 // ------------------------------------------------------------ 8-bit states as values
 template <bool SIGNED>
 __global__ __launch_bounds__(256) void k_state_values(const uint8_t* __restrict__ codes,
                                                       const float* __restrict__ scales, int64_t n,
                                                       float* __restrict__ out, int vec) {
-    for (int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * kTile) {
-        uint32_t c[8];
-        float f[8];
-        load_codes(codes, i, n, vec, c);
-        const float s = scales[i / kBlock8];
+    const int lane = threadIdx.x & 63;
+    const int64_t base = (int64_t)blockIdx.x * kTile + (threadIdx.x >> 6) * (kRows * kBlock8) + lane * 4;
+    uint32_t c[kRows];
+    float s[kRows];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = decode8<SIGNED>(c[e], s);
-        store8<F32>(out, i, n, vec, f);
+    for (int r = 0; r < kRows; ++r) {
+        const int64_t i = base + r * kBlock8;
+        c[r] = load_codes(codes, i, n, vec);
+        s[r] = i < n ? scales[i / kBlock8] : 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        float f[4];
+        decode4<SIGNED>(c[r], s[r], f);
+        store4<F32>(out, base + r * kBlock8, n, vec, f);
     }
 }
 
@@ -314,17 +395,16 @@ template <bool SIGNED>
 __global__ __launch_bounds__(256) void k_state_codes(const float* __restrict__ x, int64_t n,
                                                      uint8_t* __restrict__ codes, float* __restrict__ scales,
                                                      int vec) {
-    // whole waves stay in the loop together: a block's 32 lanes meet in the reduction
-    for (int64_t base = blockIdx.x * (int64_t)kTile; base < n; base += (int64_t)gridDim.x * kTile) {
-        const int64_t i = base + threadIdx.x * 8;
-        float f[8];
-        load8<F32>(x, i, n, vec, f);
-        const float top = block_top(f), inv = inverse_scale(top);
-        uint32_t c[8];
+    const int lane = threadIdx.x & 63;
+    const int64_t base = (int64_t)blockIdx.x * kTile + (threadIdx.x >> 6) * (kRows * kBlock8) + lane * 4;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = encode8<SIGNED>(f[e], inv);
-        store_codes(codes, i, n, vec, c);
-        if ((threadIdx.x & 31) == 0 && i < n) scales[i / kBlock8] = top;
+    for (int r = 0; r < kRows; ++r) {
+        const int64_t i = base + r * kBlock8;
+        float f[4];
+        load4<F32>(x, i, n, vec, f);
+        const float top = block_top(f);
+        store_codes(codes, i, n, vec, encode4<SIGNED>(f, inverse_scale(top)));
+        if (lane == 0 && i < n) scales[i / kBlock8] = top;
     }
 }
 
@@ -343,17 +423,20 @@ __device__ __forceinline__ double group_sum(double v, double* lds) {
 template <typename G>
 __global__ __launch_bounds__(256) void k_norm_partial(NormArgs a, double* __restrict__ partial) {
     __shared__ double lds[4];
-    const int ti = tensor_of<kNormTensors>(a.first, a.count, (int)blockIdx.x, threadIdx.x & 63);
+    const int ti = tensor_of(a.first, a.count, (int)blockIdx.x);
     const void* g = a.g[ti];
     const int64_t n = a.n[ti], base = ((int64_t)blockIdx.x - a.first[ti]) * kNormTile;
-    const bool vec = ((uintptr_t)g & 15) == 0;
+    const bool vec = ((uintptr_t)g & (G::tag == STM_F32 ? 15 : 7)) == 0;
     double sum = 0.0;
-#pragma unroll 4
-    for (int k = 0; k < kNormTile / kTile; ++k) {
-        float f[8];
-        load8<G>(g, base + k * kTile + threadIdx.x * 8, n, vec, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fma((double)f[e], (double)f[e], sum);
+    for (int k = 0; k < kNormTile / 1024; k += 8) {  // eight loads in flight
+        float f[8][4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) load4<G>(g, base + (k + j) * 1024 + threadIdx.x * 4, n, vec, f[j]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum = fma((double)f[j][e], (double)f[j][e], sum);
     }
     sum = group_sum(sum, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -382,17 +465,20 @@ bool valid_dtype(int dt) { return dt == STM_F16 || dt == STM_BF16 || dt == STM_F
 
 using namespace stm;
 
-extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype,
-                              int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay,
-                              int64_t step, const float* grad_scale, void* stream) {
-    if (count < 0 || (count && !tensors)) return set_error(STM_ERR_INVALID, "adamw_step: bad tensor list");
+constexpr int64_t kMostGroups = 0x3FFFFFFF;  // work-groups of a launch
+
+static int check_adamw_types(int param_dtype, int grad_dtype, int state_bits) {
     if (!valid_dtype(param_dtype) || !valid_dtype(grad_dtype))
         return set_error(STM_ERR_INVALID, "adamw_step: unknown dtype");
     if (state_bits != 8 && state_bits != 32)
         return set_error(STM_ERR_INVALID, "adamw_step: states have 8 or 32 bits, got %d", state_bits);
-    if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
-        return set_error(STM_ERR_INVALID, "adamw_step: betas must lie in [0, 1)");
-    if (step < 1) return set_error(STM_ERR_INVALID, "adamw_step: the first step is step 1");
+    return STM_OK;
+}
+
+static int check_adamw_tensors(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype,
+                               int state_bits) {
+    if (count < 0 || (count && !tensors)) return set_error(STM_ERR_INVALID, "adamw_step: bad tensor list");
+    const int64_t tile = tile_of(state_bits);
     for (int i = 0; i < count; ++i) {
         const stm_adamw_tensor& t = tensors[i];
         if (t.n < 0) return set_error(STM_ERR_INVALID, "adamw_step: tensor %d has a negative size", i);
@@ -405,25 +491,44 @@ extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int pa
         if (!aligned(t.param, pa) || !aligned(t.grad, ga) || !aligned(t.master, 4) || !aligned(t.exp_avg, sa) ||
             !aligned(t.exp_avg_sq, sa) || !aligned(t.exp_avg_scale, 4) || !aligned(t.exp_avg_sq_scale, 4))
             return set_error(STM_ERR_INVALID, "adamw_step: tensor %d is not aligned to its elements", i);
-        if ((t.n + kTile - 1) / kTile > 0x3FFFFFFF)
+        if ((t.n + tile - 1) / tile > kMostGroups)
             return set_error(STM_ERR_UNSUPPORTED, "adamw_step: tensor %d is too large", i);
     }
+    return STM_OK;
+}
+
+static int adamw_numbers(double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                         const float* grad_scale, AdamNumbers& h) {
+    if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
+        return set_error(STM_ERR_INVALID, "adamw_step: betas must lie in [0, 1)");
+    if (step < 1) return set_error(STM_ERR_INVALID, "adamw_step: the first step is step 1");
+    h.beta1 = (float)beta1;
+    h.beta2 = (float)beta2;
+    h.rest1 = (float)(1.0 - beta1);
+    h.rest2 = (float)(1.0 - beta2);
+    h.decay = (float)(1.0 - lr * weight_decay);
+    h.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+    h.inv_root2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+    h.eps = (float)eps;
+    h.scale = grad_scale;
+    return STM_OK;
+}
+
+extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype,
+                              int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay,
+                              int64_t step, const float* grad_scale, void* stream) {
     AdamArgs a;
-    a.beta1 = (float)beta1;
-    a.beta2 = (float)beta2;
-    a.rest1 = (float)(1.0 - beta1);
-    a.rest2 = (float)(1.0 - beta2);
-    a.decay = (float)(1.0 - lr * weight_decay);
-    a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
-    a.inv_root2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
-    a.eps = (float)eps;
-    a.scale = grad_scale;
+    int rc = check_adamw_types(param_dtype, grad_dtype, state_bits);
+    if (rc == STM_OK) rc = adamw_numbers(lr, beta1, beta2, eps, weight_decay, step, grad_scale, a.h);
+    if (rc == STM_OK) rc = check_adamw_tensors(count, tensors, param_dtype, grad_dtype, state_bits);
+    if (rc != STM_OK) return rc;
+    const int64_t tile = tile_of(state_bits);
     for (int i = 0; i < count;) {
         a.count = 0;
         int64_t groups = 0;
         while (i < count && a.count < kAdamTensors) {
-            const int64_t g = (tensors[i].n + kTile - 1) / kTile;
-            if (groups + g > 0x3FFFFFFF) break;
+            const int64_t g = (tensors[i].n + tile - 1) / tile;
+            if (groups + g > kMostGroups) break;
             if (g) {
                 a.t[a.count] = tensors[i];
                 a.first[a.count++] = (int)groups;
@@ -432,16 +537,50 @@ extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int pa
             ++i;
         }
         if (!groups) continue;
-        if (param_dtype == STM_F32)
-            launch_adamw<F32>(a, grad_dtype, state_bits, (unsigned)groups, (hipStream_t)stream);
-        else if (param_dtype == STM_BF16)
-            launch_adamw<BF16>(a, grad_dtype, state_bits, (unsigned)groups, (hipStream_t)stream);
-        else
-            launch_adamw<F16>(a, grad_dtype, state_bits, (unsigned)groups, (hipStream_t)stream);
-        const int rc = check_launch("adamw_step");
-        if (rc) return rc;
+        rc = launch_adamw(a, param_dtype, grad_dtype, state_bits, groups, (hipStream_t)stream);
+        if (rc != STM_OK) return rc;
     }
     return STM_OK;
+}
+
+extern "C" int64_t stm_adamw_table_bytes(int count) {
+    if (count < 0) return set_error(STM_ERR_INVALID, "adamw_table: bad tensor list");
+    return (int64_t)count * (int64_t)(sizeof(stm_adamw_tensor) + sizeof(int));
+}
+
+extern "C" int stm_adamw_fill_table(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype,
+                                    int state_bits, void* table) {
+    int rc = check_adamw_types(param_dtype, grad_dtype, state_bits);
+    if (rc == STM_OK) rc = check_adamw_tensors(count, tensors, param_dtype, grad_dtype, state_bits);
+    if (rc != STM_OK) return rc;
+    if (count && (!table || !aligned(table, 8))) return set_error(STM_ERR_INVALID, "adamw_table: bad table");
+    auto* t = static_cast<stm_adamw_tensor*>(table);
+    auto* first = reinterpret_cast<int*>(t + count);
+    const int64_t tile = tile_of(state_bits);
+    int64_t groups = 0;
+    for (int i = 0; i < count; ++i) {
+        t[i] = tensors[i];
+        first[i] = (int)groups;
+        groups += (tensors[i].n + tile - 1) / tile;
+        if (groups > kMostGroups) return set_error(STM_ERR_UNSUPPORTED, "adamw_table: too many elements");
+    }
+    return (int)groups;
+}
+
+extern "C" int stm_adamw_step_table(int count, const void* table, int groups, int param_dtype, int grad_dtype,
+                                    int state_bits, double lr, double beta1, double beta2, double eps,
+                                    double weight_decay, int64_t step, const float* grad_scale, void* stream) {
+    AdamTable a;
+    int rc = check_adamw_types(param_dtype, grad_dtype, state_bits);
+    if (rc == STM_OK) rc = adamw_numbers(lr, beta1, beta2, eps, weight_decay, step, grad_scale, a.h);
+    if (rc != STM_OK) return rc;
+    if (count < 0 || groups < 0 || groups > kMostGroups || (groups && (!count || !table || !aligned(table, 8))))
+        return set_error(STM_ERR_INVALID, "adamw_step_table: bad table");
+    if (!groups) return STM_OK;
+    a.t = static_cast<const stm_adamw_tensor*>(table);
+    a.first = reinterpret_cast<const int*>(a.t + count);
+    a.count = count;
+    return launch_adamw(a, param_dtype, grad_dtype, state_bits, groups, (hipStream_t)stream);
 }
 
 extern "C" int stm_state8_values(const uint8_t* codes, const float* scales, int64_t n, int is_signed, float* out,
@@ -450,9 +589,10 @@ extern "C" int stm_state8_values(const uint8_t* codes, const float* scales, int6
     if (n == 0) return STM_OK;
     if (!codes || !scales || !out) return set_error(STM_ERR_INVALID, "state8_values: null pointer");
     if (!aligned(scales, 4) || !aligned(out, 4)) return set_error(STM_ERR_INVALID, "state8_values: unaligned fp32");
-    const int vec = aligned(codes, 8) && aligned(out, 16);
+    const int vec = aligned(codes, 4) && aligned(out, 16);
     const int64_t tiles = (n + kTile - 1) / kTile;
-    const dim3 grid((unsigned)(tiles < 65536 ? tiles : 65536));
+    if (tiles > 0x3FFFFFFF) return set_error(STM_ERR_UNSUPPORTED, "state8: %lld elements", (long long)n);
+    const dim3 grid((unsigned)tiles);
     if (is_signed)
         hipLaunchKernelGGL(k_state_values<true>, grid, dim3(256), 0, (hipStream_t)stream, codes, scales, n, out, vec);
     else
@@ -466,9 +606,10 @@ extern "C" int stm_state8_codes(const float* x, int64_t n, int is_signed, uint8_
     if (n == 0) return STM_OK;
     if (!codes || !scales || !x) return set_error(STM_ERR_INVALID, "state8_codes: null pointer");
     if (!aligned(scales, 4) || !aligned(x, 4)) return set_error(STM_ERR_INVALID, "state8_codes: unaligned fp32");
-    const int vec = aligned(codes, 8) && aligned(x, 16);
+    const int vec = aligned(codes, 4) && aligned(x, 16);
     const int64_t tiles = (n + kTile - 1) / kTile;
-    const dim3 grid((unsigned)(tiles < 65536 ? tiles : 65536));
+    if (tiles > 0x3FFFFFFF) return set_error(STM_ERR_UNSUPPORTED, "state8: %lld elements", (long long)n);
+    const dim3 grid((unsigned)tiles);
     if (is_signed)
         hipLaunchKernelGGL(k_state_codes<true>, grid, dim3(256), 0, (hipStream_t)stream, x, n, codes, scales, vec);
     else

@@ -545,6 +545,18 @@ def _gated_operands(x, packed, absmax, weight_shape, blocksize):
     return x2, x2.shape[0], N // 2, K, tag, x2.device
 
 
+def _gated_plain(entry: str, x, packed, absmax, weight_shape, blocksize, grad):
+    """The call made by the native host code, or None where an operand has to be copied or refused."""
+    if not x.is_cuda:
+        return None
+    y = _lib.fast().gated(_lib.address(entry), _lib.address("stm_nf4_gated_workspace_bytes"), x, packed, absmax,
+                          int(weight_shape[0]), int(weight_shape[1]), blocksize, grad,
+                          torch._C._cuda_getCurrentRawStream(x.get_device()))
+    if type(y) is int:
+        _lib.check(y, entry)
+    return y
+
+
 def _gated_workspace(M: int, inter: int, K: int, device) -> Optional[torch.Tensor]:
     nbytes = int(_lib.lib().stm_nf4_gated_workspace_bytes(M, inter, K))
     if nbytes < 0:
@@ -559,6 +571,10 @@ def nf4_gated_fwd(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, w
     [Wg; Wu] of shape ``weight_shape`` = (2 I, K): both projections and the gating in one
     kernel, fp32 throughout, one rounding. (``swiglu_fwd(nf4_gemm_fwd(...))`` rounds the
     projections first and writes and reads them.) ``out`` as for :func:`nf4_gemm_fwd`."""
+    if out is None:
+        h = _gated_plain("stm_nf4_gated_fwd", x, packed, absmax, weight_shape, blocksize, None)
+        if h is not None:
+            return h
     x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
     h = _out_buffer(out, (M, inter), x.dtype, dev)
     with _lib.device_guard(dev):
@@ -578,6 +594,10 @@ def nf4_gated_bwd(grad_out: torch.Tensor, x: torch.Tensor, packed: torch.Tensor,
     """Gradient of :func:`nf4_gated_fwd` with respect to the two projections' outputs:
     [..., 2 I] = [d gate | d up] in x's dtype, both projections computed again in the same
     kernel. The input's gradient is ``nf4_gemm_bwd_dx`` of it with the same weight."""
+    if out is None:
+        dgu = _gated_plain("stm_nf4_gated_bwd", x, packed, absmax, weight_shape, blocksize, grad_out)
+        if dgu is not None:
+            return dgu
     x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
     if grad_out.shape[-1] != inter or grad_out.dtype != x.dtype:
         raise ValueError(f"grad_out must be [..., {inter}] {x.dtype}, got {tuple(grad_out.shape)} {grad_out.dtype}")

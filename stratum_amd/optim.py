@@ -32,6 +32,11 @@ __all__ = ["AdamW", "AdamWTensors", "STATE_BLOCK", "grad_norm", "state_codes", "
 
 STATE_BLOCK = 256  # elements per scale of an 8-bit state
 
+# Lists up to this length go as kernel arguments (one launch); longer ones as a table that is copied to
+# the GPU, which costs 10 us and saves the drain between launches of 56 tensors (448 adapters of an
+# 8B model: 257 us in 8 launches, where one launch over as many elements takes 219).
+_ARGUMENT_TENSORS = 56
+
 # columns of a row of the tensor table (stm_adamw_tensor)
 _PARAM, _GRAD, _MASTER, _M, _V, _M_SCALE, _V_SCALE, _N = range(8)
 
@@ -52,6 +57,12 @@ def _held(name: str, t: torch.Tensor, like: torch.Tensor, dtype: torch.dtype, nu
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {numel} elements on {like.device}, got "
                          f"{t.dtype}, {t.numel()} elements on {t.device}, "
                          f"{'' if t.is_contiguous() else 'not '}contiguous")
+
+
+def _laid_out(i: int, g: torch.Tensor, first: torch.Tensor) -> torch.Tensor:
+    if g.is_contiguous():
+        raise ValueError(f"gradient {i} is on {g.device}, the first one on {first.device}")
+    return g.contiguous()
 
 
 class AdamWTensors:
@@ -82,19 +93,23 @@ class AdamWTensors:
         for name, column in columns.items():
             if len(column) != len(params):
                 raise ValueError(f"{len(params)} parameters, but {len(column)} of {name}")
-        for i, p in enumerate(params):
-            n = p.numel()
-            _held(f"parameter {i}", p, first, first.dtype, n)
-            for name, column in columns.items():
-                dtype = state_dtype if name in ("exp_avg", "exp_avg_sq") else torch.float32
-                _held(f"{name} {i}", column[i], first, dtype, _blocks(n) if name.endswith("scale") else n)
-        self._sizes = [p.numel() for p in params]
+        sizes = np.array([p.numel() for p in params], dtype=np.int64)
+        blocks = -(-sizes // STATE_BLOCK)
         table = np.zeros((len(params), 8), dtype=np.int64)
-        for at, column in ((_PARAM, params), (_M, exp_avgs), (_V, exp_avg_sqs), (_MASTER, columns.get("master")),
-                           (_M_SCALE, columns.get("exp_avg scale")), (_V_SCALE, columns.get("exp_avg_sq scale"))):
-            if column is not None:
-                table[:, at] = [t.data_ptr() for t in column]
-        table[:, _N] = self._sizes
+        for name, at, column, dtype in (("parameter", _PARAM, params, first.dtype),
+                                        ("exp_avg", _M, exp_avgs, state_dtype),
+                                        ("exp_avg_sq", _V, exp_avg_sqs, state_dtype),
+                                        ("master", _MASTER, columns.get("master"), torch.float32),
+                                        ("exp_avg scale", _M_SCALE, columns.get("exp_avg scale"), torch.float32),
+                                        ("exp_avg_sq scale", _V_SCALE, columns.get("exp_avg_sq scale"), torch.float32)):
+            if column is None:
+                continue
+            want = blocks if name.endswith("scale") else sizes
+            _, index, _, bad = _lib.fast().collect(column, table.ctypes.data + 8 * at, 8, want.ctypes.data, 0)
+            if bad >= 0 or index != self.device.index or column[0].dtype != dtype:
+                for i, t in enumerate(column):
+                    _held(f"{name} {i}", t, first, dtype, int(want[i]))
+        table[:, _N] = self._sizes = sizes
         self._table = table
         # everything a step writes: held here (the table has bare addresses), and its versions counted up
         self._written = [t for column in (params, *columns.values()) for t in column]
@@ -102,6 +117,18 @@ class AdamWTensors:
     def at(self) -> list:
         """The parameters' addresses."""
         return self._table[:, _PARAM].tolist()
+
+    def _plain(self, i: int, grads: list) -> torch.Tensor:
+        """Gradient *i* in the parameter's order of elements; raises if that is not what is wrong with it."""
+        g, n = grads[i], int(self._sizes[i])
+        first = next(x for x in grads if x is not None)
+        if not isinstance(g, torch.Tensor) or g.layout != torch.strided:
+            raise ValueError(f"gradient {i} must be a dense tensor")
+        _lib.dtype_tag(first.dtype)
+        if g.dtype != first.dtype or g.numel() != n or g.device != self.device:
+            raise ValueError(f"gradient {i} must hold {n} {first.dtype} elements on {self.device}, got {g.numel()} "
+                             f"{g.dtype} on {g.device}")
+        return _laid_out(i, g, first)  # held by the list until the launch, on the stream it was made on
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], *, step: int, lr: float, betas: tuple = (0.9, 0.999),
              eps: float = 1e-8, weight_decay: float = 0.01, grad_scale: Optional[torch.Tensor] = None) -> None:
@@ -114,37 +141,52 @@ class AdamWTensors:
         if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
                                        or grad_scale.device != self.device):
             raise ValueError(f"grad_scale must be one fp32 value on {self.device}")
-        table, written, dtype, index = self._table, self._written, None, self.device.index
-        addresses, kept = [], None
-        for i, (g, n) in enumerate(zip(grads, self._sizes)):
-            if g is None:
-                addresses.append(0)
-                continue
-            if dtype is None:
-                dtype = g.dtype
-                tag = _lib.dtype_tag(dtype)
-            if g.dtype != dtype or g.numel() != n or g.get_device() != index:
-                raise ValueError(f"gradient {i} must hold {n} {dtype} elements on {self.device}, got {g.numel()} "
-                                 f"{g.dtype} on {g.device}")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                kept = (kept or []) + [g]  # until the launch, whose stream it was made on
-            addresses.append(g.data_ptr())
-        if dtype is None:
+        grads, table, written = list(grads), self._table, self._written
+        sizes = self._sizes.ctypes.data
+        while True:
+            tag, index, count, bad = _lib.fast().collect(grads, table.ctypes.data + 8 * _GRAD, 8, sizes, 0)
+            if bad < 0:
+                break
+            grads[bad] = self._plain(bad, grads)
+        if count == 0:
             return
-        table[:, _GRAD] = addresses
-        if 0 in addresses:
+        if tag < 0:
+            raise ValueError("gradients must be float16, bfloat16 or float32")
+        if index != self.device.index:
+            raise ValueError(f"the gradients are on GPU {index}, the parameters on {self.device}")
+        if count < len(grads):
             some = [i for i, g in enumerate(grads) if g is not None]
-            per = len(self._sizes)
+            per = len(grads)
             table = np.ascontiguousarray(table[some])
             written = [written[c * per + i] for c in range(len(written) // per) for i in some]
+        numbers = (lr, betas[0], betas[1], eps, weight_decay, step,
+                   grad_scale.data_ptr() if grad_scale is not None else None)
+        types = (self.param_tag, tag, self.state_bits)
+        lib, n = _lib.lib(), len(table)
         with _lib.device_guard(self.device):
-            rc = _lib.lib().stm_adamw_step(
-                len(table), table.ctypes.data, self.param_tag, tag, self.state_bits, lr, betas[0], betas[1], eps,
-                weight_decay, step, grad_scale.data_ptr() if grad_scale is not None else None,
-                _lib.stream_handle(self.device))
+            stream = _lib.stream_handle(self.device)
+            if n <= _ARGUMENT_TENSORS or torch.cuda.is_current_stream_capturing():
+                rc = lib.stm_adamw_step(n, table.ctypes.data, *types, *numbers, stream)
+            else:
+                host = torch.empty(lib.stm_adamw_table_bytes(n), dtype=torch.uint8, pin_memory=True)
+                rc = lib.stm_adamw_fill_table(n, table.ctypes.data, *types, host.data_ptr())
+                if rc >= 0:  # the caching host allocator keeps the pinned block until the copy has run
+                    held = host.to(self.device, non_blocking=True)
+                    rc = lib.stm_adamw_step_table(n, held.data_ptr(), rc, *types, *numbers, stream)
         _lib.check(rc, "stm_adamw_step")
-        torch.autograd.graph.increment_version(written)
+        _lib.fast().bump(written)
+
+
+def _plain_gradient(i: int, grads: list) -> torch.Tensor:
+    """Gradient *i* as a contiguous tensor; raises if that is not what is wrong with it."""
+    g, first = grads[i], next(x for x in grads if x is not None)
+    if not isinstance(g, torch.Tensor) or g.layout != torch.strided:
+        raise ValueError(f"gradient {i} must be a dense tensor")
+    _gpu(first, "grad_norm")
+    _lib.dtype_tag(first.dtype)
+    if g.dtype != first.dtype or g.device != first.device:
+        raise ValueError(f"gradient {i} must be {first.dtype} on {first.device}, got {g.dtype} on {g.device}")
+    return _laid_out(i, g, first)
 
 
 def grad_norm(grads: Iterable[Optional[torch.Tensor]], max_norm: float = math.inf, *,
@@ -153,17 +195,19 @@ def grad_norm(grads: Iterable[Optional[torch.Tensor]], max_norm: float = math.in
     divided by ``loss_scale``, and ``min(1, max_norm / (norm + 1e-6)) / loss_scale``, the
     factor to multiply the gradients with; NaN where the norm is not finite, which makes
     the step that reads it change nothing. fp64 sums in a fixed order; no synchronisation."""
-    grads = [g for g in grads if g is not None]
-    if not grads:
+    grads = list(grads)
+    table = np.empty((2, len(grads)), dtype=np.int64)
+    addresses, sizes = table[0], table[1]
+    while True:
+        tag, index, count, bad = _lib.fast().collect(grads, addresses.ctypes.data, 1, 0, sizes.ctypes.data)
+        if bad < 0:
+            break
+        grads[bad] = _plain_gradient(bad, grads)
+    if count == 0:
         raise ValueError("grad_norm needs at least one gradient")
-    dev, dtype = _gpu(grads[0], "grad_norm"), grads[0].dtype
-    tag = _lib.dtype_tag(dtype)
-    for i, g in enumerate(grads):
-        if g.dtype != dtype or g.get_device() != dev.index:
-            raise ValueError(f"gradient {i} must be {dtype} on {dev}, got {g.dtype} on {g.device}")
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    sizes = np.array([g.numel() for g in grads], dtype=np.int64)
-    addresses = np.array([g.data_ptr() for g in grads], dtype=np.int64)
+    if tag < 0:
+        raise ValueError("gradients must be float16, bfloat16 or float32")
+    dev = torch.device("cuda", index)
     out = torch.empty(2, dtype=torch.float32, device=dev)
     lib = _lib.lib()
     nbytes = lib.stm_grad_norm_workspace_bytes(len(grads), sizes.ctypes.data)
