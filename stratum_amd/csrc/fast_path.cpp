@@ -13,8 +13,10 @@
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <climits>
 #include <cstdint>
 #include <exception>
+#include <vector>
 
 #include "../../include/stratum_nf4.h"
 
@@ -30,52 +32,95 @@ bool aligned16(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data
 // Writes the address of tensors[i] (None: 0) to ((int64 *)addresses)[i * stride], and, where sizes_out is
 // not 0, its size there. bad: the first tensor that is not contiguous, on the first one's GPU, of its
 // type (of 16 or 32 bits, or uint8: tag -1) and, where sizes_in is not 0, of that size; -1: none.
-PyObject* collect(PyObject*, PyObject* args) {
+struct Collected {
+    long long tag = -1, device = -1, count = 0, bad = -1;
+};
+
+Collected collect(PyObject* list, int64_t* out, int64_t stride, const int64_t* want, int64_t* sizes) {
+    Collected c;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    at::ScalarType type = at::kByte;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        PyObject* item = PyList_GET_ITEM(list, i);
+        if (item == Py_None) {
+            out[i * stride] = 0;
+            if (sizes) sizes[i] = 0;
+            continue;
+        }
+        c.bad = i;
+        if (!THPVariable_Check(item)) return c;
+        const at::Tensor& t = THPVariable_Unpack(item);
+        if (t.layout() != at::kStrided || !t.is_cuda()) return c;
+        if (c.count == 0) {
+            type = t.scalar_type();
+            c.tag = dtype_tag(type);
+            c.device = t.get_device();
+        }
+        if ((c.tag < 0 && type != at::kByte) || t.scalar_type() != type || t.get_device() != c.device ||
+            !t.is_contiguous() || (want && t.numel() != want[i]))
+            return c;
+        out[i * stride] = reinterpret_cast<int64_t>(t.data_ptr());
+        if (sizes) sizes[i] = t.numel();
+        ++c.count;
+        c.bad = -1;
+    }
+    return c;
+}
+
+PyObject* py_collect(PyObject*, PyObject* args) {
     PyObject* list;
     long long addresses, stride, sizes_in, sizes_out;
     if (!PyArg_ParseTuple(args, "O!LLLL", &PyList_Type, &list, &addresses, &stride, &sizes_in, &sizes_out)) return nullptr;
-    auto* out = reinterpret_cast<int64_t*>(addresses);
-    const auto* want = reinterpret_cast<const int64_t*>(sizes_in);
-    auto* sizes = reinterpret_cast<int64_t*>(sizes_out);
-    long long tag = -1, device = -1, count = 0, bad = -1;
-    const Py_ssize_t n = PyList_GET_SIZE(list);
-    at::ScalarType type = at::kByte;
     try {
-        for (Py_ssize_t i = 0; i < n; ++i) {
-            PyObject* item = PyList_GET_ITEM(list, i);
-            if (item == Py_None) {
-                out[i * stride] = 0;
-                if (sizes) sizes[i] = 0;
-                continue;
-            }
-            if (!THPVariable_Check(item)) {
-                bad = i;
-                break;
-            }
-            const at::Tensor& t = THPVariable_Unpack(item);
-            if (t.layout() != at::kStrided || !t.is_cuda()) {
-                bad = i;
-                break;
-            }
-            if (count == 0) {
-                type = t.scalar_type();
-                tag = dtype_tag(type);
-                device = t.get_device();
-            }
-            if ((tag < 0 && type != at::kByte) || t.scalar_type() != type || t.get_device() != device || !t.is_contiguous() ||
-                (want && t.numel() != want[i])) {
-                bad = i;
-                break;
-            }
-            out[i * stride] = reinterpret_cast<int64_t>(t.data_ptr());
-            if (sizes) sizes[i] = t.numel();
-            ++count;
-        }
+        const Collected c = collect(list, reinterpret_cast<int64_t*>(addresses), stride,
+                                    reinterpret_cast<const int64_t*>(sizes_in), reinterpret_cast<int64_t*>(sizes_out));
+        return Py_BuildValue("LLLL", c.tag, c.device, c.count, c.bad);
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
         return nullptr;
     }
-    return Py_BuildValue("LLLL", tag, device, count, bad);
+}
+
+// Whether `device` is the current GPU.
+bool is_current(const c10::Device& device) {
+    return c10::impl::getDeviceGuardImpl(device.type())->getDevice() == device;
+}
+
+typedef int64_t (*NormBytes)(int, const int64_t*);
+typedef int (*Norm)(int, const void* const*, const int64_t*, int, double, double, float*, void*, int64_t, void*);
+
+// grad_norm(function, workspace function, gradients, max_norm, loss_scale, raw stream of a GPU)
+//   -> the two values; None where a gradient has to be copied or refused, or the list is empty.
+PyObject* grad_norm(PyObject*, PyObject* args) {
+    long long fn, ws_fn;
+    PyObject *list, *stream_of;
+    double max_norm, loss_scale;
+    if (!PyArg_ParseTuple(args, "LLO!ddO", &fn, &ws_fn, &PyList_Type, &list, &max_norm, &loss_scale, &stream_of))
+        return nullptr;
+    try {
+        const Py_ssize_t n = PyList_GET_SIZE(list);
+        std::vector<int64_t> addresses(n), sizes(n);
+        const Collected c = collect(list, addresses.data(), 1, nullptr, sizes.data());
+        if (c.bad >= 0 || c.count == 0 || c.tag < 0 || n > INT_MAX) Py_RETURN_NONE;
+        const c10::Device device(c10::DeviceType::CUDA, (c10::DeviceIndex)c.device);
+        if (!is_current(device)) Py_RETURN_NONE;
+        PyObject* raw = PyObject_CallFunction(stream_of, "L", c.device);
+        if (!raw) return nullptr;
+        void* stream = PyLong_AsVoidPtr(raw);
+        Py_DECREF(raw);
+        const int64_t bytes = reinterpret_cast<NormBytes>(ws_fn)((int)n, sizes.data());
+        if (bytes < 0) return PyLong_FromLongLong(bytes);
+        const auto options = at::TensorOptions().device(device);
+        at::Tensor out = at::empty({2}, options.dtype(at::kFloat)), ws = at::empty({bytes / 8}, options.dtype(at::kDouble));
+        const int rc = reinterpret_cast<Norm>(fn)((int)n, reinterpret_cast<const void* const*>(addresses.data()),
+                                                  sizes.data(), (int)c.tag, max_norm, loss_scale, out.data_ptr<float>(),
+                                                  ws.data_ptr(), bytes, stream);
+        if (rc != STM_OK) return PyLong_FromLong(rc);
+        return THPVariable_Wrap(out);
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
 }
 
 // bump(tensors): count their versions up, as an in-place operation of torch does.
@@ -129,7 +174,7 @@ PyObject* gated(PyObject*, PyObject* args) {
             !q.is_contiguous() || !a.is_contiguous() || !aligned16(x) || !aligned16(q) ||
             q.numel() < inter * K || a.numel() * bs < N * K)
             Py_RETURN_NONE;
-        if (c10::impl::getDeviceGuardImpl(device.type())->getDevice() != device) Py_RETURN_NONE;
+        if (!is_current(device)) Py_RETURN_NONE;
         const int64_t M = x.numel() / K;
         const void* grad = nullptr;
         if (pg != Py_None) {
@@ -162,8 +207,9 @@ PyObject* gated(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {
-    {"collect", collect, METH_VARARGS, "addresses, sizes, type and device of a list of tensors"},
+    {"collect", py_collect, METH_VARARGS, "addresses, sizes, type and device of a list of tensors"},
     {"bump", bump, METH_O, "count the versions of a list of tensors up"},
+    {"grad_norm", grad_norm, METH_VARARGS, "the gradient norm of a list of tensors in its plain form"},
     {"gated", gated, METH_VARARGS, "a gated block's call in its plain form"},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -196,6 +196,12 @@ def grad_norm(grads: Iterable[Optional[torch.Tensor]], max_norm: float = math.in
     factor to multiply the gradients with; NaN where the norm is not finite, which makes
     the step that reads it change nothing. fp64 sums in a fixed order; no synchronisation."""
     grads = list(grads)
+    out = _lib.fast().grad_norm(_lib.address("stm_grad_norm"), _lib.address("stm_grad_norm_workspace_bytes"), grads,
+                                max_norm, loss_scale, torch._C._cuda_getCurrentRawStream)
+    if isinstance(out, torch.Tensor):
+        return out
+    if out is not None:
+        _lib.check(out, "stm_grad_norm")
     table = np.empty((2, len(grads)), dtype=np.int64)
     addresses, sizes = table[0], table[1]
     while True:
