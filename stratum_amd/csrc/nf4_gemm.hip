@@ -3423,13 +3423,27 @@ struct GatedPlan {
     int64_t partial;   // fp32 values of workspace: the partials, or (kDense) the 16-bit weight
 };
 
-#ifndef STM_GATED_DENSE_M
-#define STM_GATED_DENSE_M 768
-#endif
+// Time of `tiles` work items of one reduction depth, one work-group per CU, in us: every round of
+// 256 takes steps x (c0 + c1 x the share of the CUs it fills) + 8.
+double gated_rounds(int64_t tiles, int64_t steps, double c0, double c1) {
+    const double full = (double)(tiles / kCUs), last = (double)(tiles % kCUs) / kCUs;
+    return full * ((double)steps * (c0 + c1) + 8.0) + (last > 0.0 ? (double)steps * (c0 + c1 * last) + 8.0 : 0.0);
+}
 
+// The least estimated time, in us. Up to 64 rows the weight-streaming kernels run. Above that:
+//  * tiles of 128, 192 or 256 rows that dequantize their own weight (k_gemm_fwd_rw);
+//  * the LDS-weight tiles of 128 x 128 or 256 x 256 over 2-8 ranges of the reduction, whose
+//    fp32 partials k_gated_reduce sums and gates: few rows on a narrow weight;
+//  * the weight dequantized once and k_gated_dense over it: many rows.
+// The constants are fitted to 7 weights (K 640-5120, I 512-14336) x 13-15 row counts from 65 to
+// 8192, all ways timed on each: the pick is 0.3 % above the fastest on average and 5 % at
+// worst. E.g. us, [2 x 14336, 4096]: 100 rows 65 (128-row tiles; dense 129, split 66), 333 rows 85
+// (192; 256-row tiles 102), 1024 rows 207 (256; 192: 250), 8192 rows dense 1510 (256: 1600);
+// [2 x 512, 4096]: 509 rows 21 (eight ranges of 128 x 128; unsplit 50).
 GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
     GatedPlan p{};
-    if (M <= STM_GEMV_MAX_M && tile_override() < 0) {
+    const int only = tile_override();
+    if (M <= STM_GEMV_MAX_M && only < 0) {
         p.cfg = gemv_ks_config(M, N, K);
         if (p.cfg) {
             p.kind = GatedPlan::kKs;
@@ -3440,21 +3454,30 @@ GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
         p.partial = (int64_t)p.gv.splits * M * N;
         return p;
     }
-    if (M >= STM_GATED_DENSE_M && N * K < (int64_t)1 << 31 && tile_override() < 0) {
-        p.kind = GatedPlan::kDense;
-        p.partial = (N / 2 + 127) / 128 * 128 * K;  // 256 x K values of 2 bytes a tile
-        return p;
+    const int64_t steps = K / BK;
+    auto tiles = [&](int64_t bm, int64_t bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
+    double best = 1e30;
+    auto offer = [&](double t, GatedPlan::Kind kind, int cfg, int splits, int64_t partial) {
+        if (t >= best) return;
+        best = t;
+        p.kind = kind, p.cfg = cfg, p.tile = cfg, p.splits = splits, p.partial = partial;
+    };
+    if (only < 0 || only == kMid || only == kSmall)
+        offer(gated_rounds(tiles(128, 256), steps, 0.66, 0.34), GatedPlan::kTile, 128, 1, 0);
+    if (only < 0 || only == kBig8) offer(gated_rounds(tiles(192, 256), steps, 0.89, 0.36), GatedPlan::kTile, 192, 1, 0);
+    if (only < 0 || only == kBig) offer(gated_rounds(tiles(256, 256), steps, 1.12, 0.40), GatedPlan::kTile, 256, 1, 0);
+    for (int sp = 2; sp <= 8 && sp * 8 <= steps; ++sp) {
+        const int64_t partial = sp * M * N, per = (steps + sp - 1) / sp;
+        const double reduce = 3.5 + (double)partial * 8.0 / 4.0e6;
+        auto rounds = [&](int64_t items) { return (double)((items + kCUs - 1) / kCUs); };
+        if (only < 0 || only == kSmall)
+            offer(rounds(tiles(128, 128) * sp) * (0.62 * (double)per + 7.0) + reduce, GatedPlan::kSplit, kSmall, sp, partial);
+        if (only < 0 || only == kBig)
+            offer(rounds(tiles(256, 256) * sp) * (1.62 * (double)per + 5.0) + reduce, GatedPlan::kSplit, kBig, sp, partial);
     }
-    const Plan t = plan(M, N, K, false, 1);
-    if (t.splits > 1) {
-        p.kind = GatedPlan::kSplit;
-        p.tile = t.kind;
-        p.splits = t.splits;
-        p.partial = (int64_t)t.splits * M * N;
-        return p;
-    }
-    p.kind = GatedPlan::kTile;
-    p.cfg = t.kind == kBig || t.kind == kBig8 ? 256 : 128;
+    if (only < 0 && N * K < (int64_t)1 << 31)
+        offer(gated_rounds(tiles(256, 256), steps, 1.0, 0.36) + (double)(N * K) * 2.5625 / 3.9e6 + 2.0, GatedPlan::kDense, 0, 1,
+              (N / 2 + 127) / 128 * 128 * K);  // 256 x K values of 2 bytes a tile
     return p;
 }
 
@@ -3476,6 +3499,8 @@ int launch_gated_mode(GemmArgs g, const GatedPlan& p, hipStream_t stream) {
     if (tiles > 0x7FFFFFFFLL) return set_error(STM_ERR_UNSUPPORTED, "gated: grid too large");
     if (p.cfg == 256)
         hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 256, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);
+    else if (p.cfg == 192)
+        hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 192, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);
     else
         hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 128, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);
     return check_launch("gated");

@@ -90,7 +90,13 @@ def test_a_large_weight(cuda, M):
     check(M, 14336, 4096, torch.bfloat16 if M % 2 else torch.float16)
 
 
-@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("M,inter,K", [(6200, 5640, 2112), (8150, 3080, 1600), (8200, 2824, 2112)])
+def test_many_rows_ragged(cuda, M, inter, K):
+    """Rows, columns and reductions that fill no tile of the many-rows kernel."""
+    check(M, inter, K, torch.float16)
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2, 3])
 @pytest.mark.parametrize("M", [5, 100, 257, 520])
 def test_every_tile_kind(cuda, kind, M):
     from stratum_amd import _lib
