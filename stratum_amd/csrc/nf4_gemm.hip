@@ -3423,6 +3423,24 @@ struct GatedPlan {
     int64_t partial;   // fp32 values of workspace: the partials, or (kDense) the 16-bit weight
 };
 
+// Configuration of the split-free small-M kernel for a gated call, by its time in us: every round of
+// work-groups (one per CU) 1.45 and 1.0 a step (1.85 with two tiles a wave), the launch 1.5. Fitted to
+// 7 weights x 5 row counts, every configuration that takes the rows timed on each: the pick is
+// within 2 % of the fastest on all. E.g. one row, us: [2 x 5632, 2048] 6.7 (T = 4, TW = 2; T = 1 8.7),
+// [2 x 512, 4096] 4.9 (T = 1; T = 4 10.5), [2 x 14336, 4096] 19.1 (T = 8; T = 1 28.0).
+int gated_ks_config(int64_t M, int64_t N, int64_t K, double* time) {
+    int best = 0;
+    const int64_t groups = (K + GV_GK - 1) / GV_GK, cus = device_cus();
+    for (const auto& c : kKsConfigs) {
+        const int T = c[0], TW = c[1], S = 8 * TW / T;
+        if (M > c[2]) continue;
+        const int64_t rounds = ((N + 16 * T - 1) / (16 * T) + cus - 1) / cus;
+        const double t = 1.5 + (double)rounds * (1.45 + (double)((groups + S - 1) / S) * (TW == 1 ? 1.0 : 1.85));
+        if (!best || t < *time) *time = t, best = c[0] | c[1] << 4 | c[2] << 8;
+    }
+    return best;
+}
+
 // Time of `tiles` work items of one reduction depth, one work-group per CU, in us: every round of
 // 256 takes steps x (c0 + c1 x the share of the CUs it fills) + 8.
 double gated_rounds(int64_t tiles, int64_t steps, double c0, double c1) {
@@ -3444,13 +3462,14 @@ GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
     GatedPlan p{};
     const int only = tile_override();
     if (M <= STM_GEMV_MAX_M && only < 0) {
-        p.cfg = gemv_ks_config(M, N, K);
-        if (p.cfg) {
+        p.gv = gemv_plan(M, N, K);
+        double t = 0.0;
+        p.cfg = gated_ks_config(M, N, K, &t);
+        if (p.cfg && t < p.gv.est) {
             p.kind = GatedPlan::kKs;
             return p;
         }
         p.kind = GatedPlan::kGemv;
-        p.gv = gemv_plan(M, N, K);
         p.partial = (int64_t)p.gv.splits * M * N;
         return p;
     }

@@ -655,14 +655,14 @@ __global__ __launch_bounds__(256) void k_dequantize_tiles(const uint4* __restric
         const uint32_t r = i * 16 + (threadIdx.x >> 4), h = threadIdx.x & 15;
         stage[r * RS + h] = q[weight_row(r) * steps + (h0 + h < steps ? h0 + h : steps - 1)];
     }
-    fill_byte_lut(lut);  // ends with a barrier
     const uint32_t r = threadIdx.x >> 2, c = threadIdx.x & 3, rt = wn * 64 + r;
     const uint32_t word0 = (weight_row(r) * steps + h0) * 4, slot = rt * 4 + (c ^ ((rt >> 2) & 3));
     const uint32_t count = steps - h0 < HS ? steps - h0 : HS;  // even
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(stage) + r * (RS * 4) + c;
     float a[HS / 2];  // a 64-deep block at least has one scale
 #pragma unroll
     for (uint32_t j = 0; j < HS / 2; ++j) a[j] = absmax[(word0 + (2 * j < count ? 8 * j : 0)) >> gshift];
+    fill_byte_lut(lut);  // ends with a barrier
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(stage) + r * (RS * 4) + c;
 #pragma unroll
     for (uint32_t j = 0; j < HS; ++j) {
         if (j >= count) break;

@@ -545,15 +545,22 @@ def _gated_operands(x, packed, absmax, weight_shape, blocksize):
     return x2, x2.shape[0], N // 2, K, tag, x2.device
 
 
-def _gated_plain(entry: str, x, packed, absmax, weight_shape, blocksize, grad):
+@functools.lru_cache(maxsize=None)
+def _gated_native() -> tuple:
+    """(native caller, and the addresses of the forward, the backward and their workspace size)."""
+    return (_lib.fast().gated, _lib.address("stm_nf4_gated_fwd"), _lib.address("stm_nf4_gated_bwd"),
+            _lib.address("stm_nf4_gated_workspace_bytes"))
+
+
+def _gated_plain(x, packed, absmax, weight_shape, blocksize, grad):
     """The call made by the native host code, or None where an operand has to be copied or refused."""
     if not x.is_cuda:
         return None
-    y = _lib.fast().gated(_lib.address(entry), _lib.address("stm_nf4_gated_workspace_bytes"), x, packed, absmax,
-                          int(weight_shape[0]), int(weight_shape[1]), blocksize, grad,
-                          torch._C._cuda_getCurrentRawStream(x.get_device()))
+    native, fwd, bwd, ws = _gated_native()
+    y = native(fwd if grad is None else bwd, ws, x, packed, absmax, int(weight_shape[0]), int(weight_shape[1]),
+               blocksize, grad, torch._C._cuda_getCurrentRawStream(x.get_device()))
     if type(y) is int:
-        _lib.check(y, entry)
+        _lib.check(y, "stm_nf4_gated_fwd" if grad is None else "stm_nf4_gated_bwd")
     return y
 
 
@@ -572,7 +579,7 @@ def nf4_gated_fwd(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, w
     kernel, fp32 throughout, one rounding. (``swiglu_fwd(nf4_gemm_fwd(...))`` rounds the
     projections first and writes and reads them.) ``out`` as for :func:`nf4_gemm_fwd`."""
     if out is None:
-        h = _gated_plain("stm_nf4_gated_fwd", x, packed, absmax, weight_shape, blocksize, None)
+        h = _gated_plain(x, packed, absmax, weight_shape, blocksize, None)
         if h is not None:
             return h
     x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
@@ -595,7 +602,7 @@ def nf4_gated_bwd(grad_out: torch.Tensor, x: torch.Tensor, packed: torch.Tensor,
     [..., 2 I] = [d gate | d up] in x's dtype, both projections computed again in the same
     kernel. The input's gradient is ``nf4_gemm_bwd_dx`` of it with the same weight."""
     if out is None:
-        dgu = _gated_plain("stm_nf4_gated_bwd", x, packed, absmax, weight_shape, blocksize, grad_out)
+        dgu = _gated_plain(x, packed, absmax, weight_shape, blocksize, grad_out)
         if dgu is not None:
             return dgu
     x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
