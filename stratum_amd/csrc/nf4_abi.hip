@@ -422,7 +422,7 @@ static int gated(const char* who, const void* dH, const void* X, const uint8_t* 
     if (I % 8 != 0) return set_error(STM_ERR_UNSUPPORTED, "%s: I = %lld must be a multiple of 8", who, (long long)I);
     if (K == 0) return set_error(STM_ERR_UNSUPPORTED, "%s: K = 0", who);
     // 32-bit offsets into the weight, and at least one 256-row tile of activations and outputs
-    if (I * K >= (int64_t)1 << 32 || K > (int64_t)1 << 22 || I > (int64_t)1 << 21)
+    if (K > (int64_t)1 << 22 || I > (int64_t)1 << 21 || I * K >= (int64_t)1 << 32)
         return set_error(STM_ERR_UNSUPPORTED, "%s: a weight of [2 x %lld, %lld] is too large", who, (long long)I,
                          (long long)K);
     if (backward && (!dH || !aligned(dH, 16)))

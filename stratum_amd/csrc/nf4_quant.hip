@@ -665,7 +665,6 @@ __global__ __launch_bounds__(256) void k_dequantize_tiles(const uint4* __restric
     const uint32_t* words = reinterpret_cast<const uint32_t*>(stage) + r * (RS * 4) + c;
 #pragma unroll
     for (uint32_t j = 0; j < HS; ++j) {
-        if (j >= count) break;
         const uint32_t w = words[j * 4];
         float v[8];
 #pragma unroll
@@ -674,7 +673,7 @@ __global__ __launch_bounds__(256) void k_dequantize_tiles(const uint4* __restric
             v[2 * b] = opaque(l.x * a[j / 2]);
             v[2 * b + 1] = opaque(l.y * a[j / 2]);
         }
-        store8<DT>(out, (int64_t)(tile * steps + h0 + j) * 1024 + slot, v);
+        if (j < count) store8<DT>(out, (int64_t)(tile * steps + h0 + j) * 1024 + slot, v);
     }
 }
 

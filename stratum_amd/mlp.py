@@ -25,6 +25,10 @@ work:
   projection's output);
 * ``_ModuleRows`` otherwise: the module's own projections, with the input
   gradient of a chunk taken by a backward pass over that chunk's recompute.
+
+``NF4GatedMLP`` is the MLP for a whole batch at once: gate, up and the gating in one
+kernel (``nf4_gated``), then the module's own down projection, which may train a LoRA
+adapter.
 """
 
 from __future__ import annotations
@@ -36,13 +40,14 @@ from typing import Any, NamedTuple, Optional
 import torch
 import torch.nn as nn
 
-from .functional import (QuantState, dequantize_4bit, fused_supported, nf4_gemm_bwd_dx, nf4_gemm_fwd, quantize_4bit,
-                         swiglu_bwd, swiglu_fwd)
-from .nf4_linear import NF4Linear, fused_max_rows
+from .functional import (QuantState, dequantize_4bit, fused_supported, gated_supported, nf4_gemm_bwd_dx, nf4_gemm_fwd,
+                         quantize_4bit, swiglu_bwd, swiglu_fwd)
+from .nf4_linear import NF4Linear, fused_max_rows, nf4_gated
 
 __all__ = [
     "MemoryFlatFrozenMLP",
     "MemoryFlatFrozenMLPFunction",
+    "NF4GatedMLP",
     "NF4StackedMLP",
     "quantize_mlp_",
 ]
@@ -327,6 +332,43 @@ class MemoryFlatFrozenMLP(nn.Module):
 
     def named_buffers(self, prefix: str = "", recurse: bool = True, remove_duplicate: bool = True):
         yield from self.module.named_buffers(prefix=prefix, recurse=recurse, remove_duplicate=remove_duplicate)
+
+
+class NF4GatedMLP(nn.Module):
+    """``down(silu(gate(x)) * up(x))`` with the two frozen NF4 projections and the gating as
+    one kernel: neither [tokens, 2 I] nor its gradient outlives the call that needs it, and
+    the backward keeps only x (and what the down projection keeps of h).
+
+    ``module`` is an MLP whose gate and up projections are plain ``NF4Linear`` (``quantize_mlp_``
+    makes them, stacked in one payload) with a SiLU ``act_fn``; its down projection is called as
+    it is and may be an ``NF4LoRALinear``."""
+
+    def __init__(self, module: nn.Module):
+        super().__init__()
+        names = _mlp_projection_names(module)
+        gate, up, down = (getattr(module, n) for n in names)
+        for name, proj in zip(names, (gate, up)):
+            if type(proj) is not NF4Linear or proj.bias is not None:
+                raise TypeError(f"NF4GatedMLP needs a bias-free NF4Linear as {name}, got {type(proj)!r}")
+        if not _is_silu(module.act_fn):
+            raise TypeError("NF4GatedMLP computes SiLU; act_fn is another activation")
+        gs, us = gate.quant_state, up.quant_state
+        if tuple(gs.shape) != tuple(us.shape) or gs.blocksize != us.blocksize:
+            raise ValueError("gate and up must share one shape and one blocksize")
+        inter, hidden = (int(d) for d in gs.shape)
+        if not gated_supported(inter, hidden, gs.blocksize, backward=True):
+            raise ValueError(f"gate/up [{inter}, {hidden}], blocksize {gs.blocksize}: unsupported widths")
+        self.shape, self.blocksize = (2 * inter, hidden), gs.blocksize
+        payloads = gate.quantized.reshape(-1), up.quantized.reshape(-1)
+        scales = gs.absmax.reshape(-1).float(), us.absmax.reshape(-1).float()
+        # plain attributes, as NF4Linear's: .to(dtype) and .half() leave the fp32 scales alone
+        self.gate_up_packed, self.gate_up_absmax = (v if (v := _adjacent_view(*p)) is not None else torch.cat(p)
+                                                    for p in (payloads, scales))
+        self.down = down
+
+    def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
+        return self.down(nf4_gated(hidden_states, self.gate_up_packed, self.gate_up_absmax, self.shape,
+                                   self.blocksize))
 
 
 @torch.no_grad()
