@@ -36,14 +36,16 @@ namespace {
 
 constexpr int kBlock8 = 256;      // elements per scale of an 8-bit state
 constexpr int kAdamTensors = 56;  // tensors per launch (below 4 KB of kernel arguments)
-constexpr int kNormTensors = 160;
+constexpr int kNormTensors = 254;
 // Rows of 256 elements per wave: with one, a 32-bit step of 42 M elements takes 219 us, with two
 // 227, with four 240 (four accesses of a lane stand between a row's loads and its stores); an
 // 8-bit step of 176 M 477, 419 and 500 (two rows share a division).
 constexpr int rows_of(int bits) { return bits == 8 ? 2 : 1; }
 constexpr int tile_of(int bits) { return 4 * rows_of(bits) * kBlock8; }  // elements per work-group
 constexpr int kRows = rows_of(8), kTile = tile_of(8);                    // of the conversions
-constexpr int kNormTile = 16384;  // elements per work-group of the norm
+// Elements per work-group of the norm, all in flight at once: 84 M elements in 16 bits 42.5 us, 16384
+// 43.3, 32768 60; 21 M in 32 bits 36.5, 42, 56.
+constexpr int kNormTile = 8192;
 
 struct AdamNumbers {
     float beta1, beta2, rest1, rest2;  // rest = 1 - beta
@@ -70,8 +72,8 @@ struct AdamTable {
 
 struct NormArgs {
     const void* g[kNormTensors];
-    int64_t n[kNormTensors];
-    int first[kNormTensors];
+    int first[kNormTensors + 1];  // first work-group of tensor i; of `count`: all of them
+    int last[kNormTensors];       // elements of tensor i's last work-group
     int count;
 };
 static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
@@ -409,13 +411,17 @@ __global__ __launch_bounds__(256) void k_state_codes(const float* __restrict__ x
 }
 
 // ------------------------------------------------------------ gradient norm
-// Sum of v over the work-group's 256 threads, in a fixed order; valid in thread 0.
-__device__ __forceinline__ double group_sum(double v, double* lds) {
+// Sum of v over the work-group's threads, in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ double group_sum(double v, double (&lds)[THREADS / 64]) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+    v = lds[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; ++i) v += lds[i];
+    return v;
 }
 
 // Squares are summed in fp64: exact products of the 16-bit types, no overflow for any
@@ -425,29 +431,37 @@ __global__ __launch_bounds__(256) void k_norm_partial(NormArgs a, double* __rest
     __shared__ double lds[4];
     const int ti = tensor_of(a.first, a.count, (int)blockIdx.x);
     const void* g = a.g[ti];
-    const int64_t n = a.n[ti], base = ((int64_t)blockIdx.x - a.first[ti]) * kNormTile;
+    const int64_t base = ((int64_t)blockIdx.x - a.first[ti]) * kNormTile;
+    const int64_t n = (int64_t)(a.first[ti + 1] - a.first[ti] - 1) * kNormTile + a.last[ti];
     const bool vec = ((uintptr_t)g & (G::tag == STM_F32 ? 15 : 7)) == 0;
     double sum = 0.0;
+    constexpr int kLoads = kNormTile / 1024;
+    float f[kLoads][4];
 #pragma unroll
-    for (int k = 0; k < kNormTile / 1024; k += 8) {  // eight loads in flight
-        float f[8][4];
+    for (int j = 0; j < kLoads; ++j) load4<G>(g, base + j * 1024 + threadIdx.x * 4, n, vec, f[j]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) load4<G>(g, base + (k + j) * 1024 + threadIdx.x * 4, n, vec, f[j]);
+    for (int j = 0; j < kLoads; ++j)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum = fma((double)f[j][e], (double)f[j][e], sum);
-    }
-    sum = group_sum(sum, lds);
+        for (int e = 0; e < 4; ++e) sum = fma((double)f[j][e], (double)f[j][e], sum);
+    sum = group_sum<256>(sum, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-__global__ __launch_bounds__(256) void k_norm_final(const double* __restrict__ partial, int64_t count, double max_norm,
-                                                    double loss_scale, float* __restrict__ out) {
-    __shared__ double lds[4];
+// One work-group with eight loads a thread in flight: the 10 240 partial sums of 84 M elements.
+constexpr int kFinalThreads = 1024;
+__global__ __launch_bounds__(kFinalThreads) void k_norm_final(const double* __restrict__ partial, int64_t count,
+                                                              double max_norm, double loss_scale,
+                                                              float* __restrict__ out) {
+    __shared__ double lds[kFinalThreads / 64];
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < count; i += 256) sum += partial[i];
-    sum = group_sum(sum, lds);
+    for (int64_t i = threadIdx.x; i < count; i += 8 * kFinalThreads) {  // eight loads in flight
+        double v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = i + j * kFinalThreads < count ? partial[i + j * kFinalThreads] : 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += v[j];
+    }
+    sum = group_sum<kFinalThreads>(sum, lds);
     if (threadIdx.x == 0) {
         const double norm = sqrt(sum) / loss_scale;
         const double factor = max_norm / (norm + 1e-6);
@@ -654,13 +668,14 @@ extern "C" int stm_grad_norm(int count, const void* const* grads, const int64_t*
             if (groups + g > 0x3FFFFFFF) break;
             if (g) {
                 a.g[a.count] = grads[i];
-                a.n[a.count] = n[i];
+                a.last[a.count] = (int)(n[i] - (g - 1) * kNormTile);
                 a.first[a.count++] = (int)groups;
                 groups += g;
             }
             ++i;
         }
         if (!groups) continue;
+        a.first[a.count] = (int)groups;
         const dim3 grid((unsigned)groups), block(256);
         if (dtype == STM_F32)
             hipLaunchKernelGGL(k_norm_partial<F32>, grid, block, 0, (hipStream_t)stream, a, partial);
@@ -672,7 +687,7 @@ extern "C" int stm_grad_norm(int count, const void* const* grads, const int64_t*
         if (rc) return rc;
         partial += groups;
     }
-    hipLaunchKernelGGL(k_norm_final, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)workspace, need / 8,
+    hipLaunchKernelGGL(k_norm_final, dim3(1), dim3(kFinalThreads), 0, (hipStream_t)stream, (const double*)workspace, need / 8,
                        max_norm, loss_scale, out);
     return check_launch("grad_norm");
 }
