@@ -268,12 +268,16 @@ int stm_swiglu_bwd(const void* grad_out, const void* gate_up, void* grad_gate_up
  * first, the payload of stack_nf4 or quantize_mlp_), in one pass:
  *   stm_nf4_gated_fwd: H[M, I]      = silu(X Wg^T) * (X Wu^T)
  *   stm_nf4_gated_bwd: dGU[M, 2 I]  = [dH u silu'(g) | dH silu(g)], g = X Wg^T, u = X Wu^T computed again
+ *   stm_nf4_gated_fwd_keep: the forward, which also stores the fp32 sums [M, 2 I] = [g | u]
+ *   stm_gated_bwd_kept: dGU from those sums, without the product
  * Replaces act_fn(gate_proj(x)) * up_proj(x) and its recompute in the backward
  * (stratum/model/mlp_opt.py:178-180, :203-212); the input gradient is then
  * stm_nf4_gemm_bwd_dx of dGU against the same weight. W is dequantized as by
  * stm_nf4_dequantize; fp32 sums and gating, one rounding of each output.
  *   X [M, K], H / dH [M, I], dGU [M, 2 I]: row-major, dtype STM_BF16 or STM_F16
  *   workspace   : stm_nf4_gated_workspace_bytes(M, I, K) bytes, 16-byte aligned (NULL where that is 0)
+ *   sums        : stm_nf4_gated_sums_bytes(M, I, K) bytes, 16-byte aligned; where that is 0 (few rows: reading
+ *                 the weight again costs as little), fwd_keep is refused
  *   constraints : K % 64 == 0, K % blocksize == 0, K > 0, I % 8 == 0, pointers 16-byte aligned
  */
 int64_t stm_nf4_gated_workspace_bytes(int64_t M, int64_t I, int64_t K);
@@ -282,6 +286,11 @@ int stm_nf4_gated_fwd(const void* X, const uint8_t* packed, const float* absmax,
 int stm_nf4_gated_bwd(const void* dH, const void* X, const uint8_t* packed, const float* absmax, void* dGU, int64_t M,
                       int64_t I, int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes,
                       void* stream);
+int64_t stm_nf4_gated_sums_bytes(int64_t M, int64_t I, int64_t K);
+int stm_nf4_gated_fwd_keep(const void* X, const uint8_t* packed, const float* absmax, void* H, float* sums, int64_t M,
+                           int64_t I, int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+int stm_gated_bwd_kept(const void* dH, const float* sums, void* dGU, int64_t M, int64_t I, int dtype, void* stream);
 
 /*
  * Rank-R side products of a LoRA adapter on the frozen NF4 base. They replace the

@@ -56,6 +56,9 @@ SIGNATURES = {
     "stm_nf4_gated_workspace_bytes": ([_I64, _I64, _I64], _I64),
     "stm_nf4_gated_fwd": ([_P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
     "stm_nf4_gated_bwd": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
+    "stm_nf4_gated_sums_bytes": ([_I64, _I64, _I64], _I64),
+    "stm_nf4_gated_fwd_keep": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
+    "stm_gated_bwd_kept": ([_P, _P, _P, _I64, _I64, _I, _P], _I),
     "stm_lora_workspace_bytes": ([_I64, _I64, _I, _I], _I64),
     "stm_lora_down": ([_P, _P, _P, _I64, _I64, _I, ctypes.c_float, _I, _P, _I64, _P], _I),
     "stm_lora_dy": ([_P, _P, _P, _P, _P, _I64, _I64, _I, ctypes.c_float, _I, _P, _I64, _P], _I),

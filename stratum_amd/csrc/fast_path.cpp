@@ -1,7 +1,8 @@
 // Host code of the calls whose time is the host's (CPython module stratum_amd._fast): reading
-// a list of tensors into an address table, and the gated block's call in its plain form.
+// a list of tensors into an address table, and the gated block's calls in their plain form.
 // 448 tensors, us: dtype, device, size, layout and address of each read from Python
-// 110, here 6; a call of the gated block on one row 10.4, here 6.
+// 110, here 6; a forward of the gated block on one row 10.4, here 6.5; its forward and backward
+// through autograd 118, here 42.
 //
 // Nothing is decided here that the Python layer does not decide as well: what is not the
 // plain form is handed back (None, or the index of the tensor), and Python converts it or
@@ -149,57 +150,139 @@ PyObject* bump(PyObject*, PyObject* list) {
 typedef int64_t (*GatedBytes)(int64_t, int64_t, int64_t);
 typedef int (*GatedFwd)(const void*, const uint8_t*, const float*, void*, int64_t, int64_t, int64_t, int, int, void*,
                         int64_t, void*);
+typedef int (*GatedKeep)(const void*, const uint8_t*, const float*, void*, float*, int64_t, int64_t, int64_t, int, int,
+                         void*, int64_t, void*);
 typedef int (*GatedBwd)(const void*, const void*, const uint8_t*, const float*, void*, int64_t, int64_t, int64_t, int,
                         int, void*, int64_t, void*);
+typedef int (*GatedKept)(const void*, const float*, void*, int64_t, int64_t, int, void*);
+typedef int64_t (*GemmBytes)(int64_t, int64_t, int64_t, int);
+typedef int (*GemmDx)(const void*, const uint8_t*, const float*, const void*, const void*, int, void*, int64_t, int64_t,
+                      int64_t, int, int, void*, int64_t, void*);
 
-// gated(function, workspace function, x, packed, absmax, N, K, blocksize, gradient or None, stream)
-//   -> the output; None where the operands are not in the plain form (contiguous, aligned, on the
-//   current GPU, sizes that fit: the Python layer copies or refuses them); a status if the call failed.
-PyObject* gated(PyObject*, PyObject* args) {
-    long long fn, ws_fn, N, K, bs, stream;
-    PyObject *px, *pq, *pa, *pg;
-    if (!PyArg_ParseTuple(args, "LLOOOLLLOL", &fn, &ws_fn, &px, &pq, &pa, &N, &K, &bs, &pg, &stream)) return nullptr;
-    if (!THPVariable_Check(px) || !THPVariable_Check(pq) || !THPVariable_Check(pa)) Py_RETURN_NONE;
-    if (pg != Py_None && !THPVariable_Check(pg)) Py_RETURN_NONE;
+// Contiguous aligned rows of `width` on `device`.
+bool rows_of(const at::Tensor& t, c10::Device device, int64_t width) {
+    return t.device() == device && t.is_contiguous() && aligned16(t) && t.dim() >= 1 && t.size(-1) == width;
+}
+
+// A stacked NF4 weight [N, K] in the plain form, its payload on the current GPU.
+struct Weight {
+    const uint8_t* packed = nullptr;
+    const float* absmax = nullptr;
+    int64_t N, K;
+    int bs;
+
+    bool read(PyObject* pq, PyObject* pa, int64_t n, int64_t k, int64_t blocksize, c10::Device* device) {
+        if (!THPVariable_Check(pq) || !THPVariable_Check(pa)) return false;
+        const at::Tensor &q = THPVariable_Unpack(pq), &a = THPVariable_Unpack(pa);
+        if (!q.is_cuda() || q.device() != a.device() || n <= 0 || n % 16 || k <= 0 || k % 64 || blocksize < 64 ||
+            blocksize > 4096 || (blocksize & (blocksize - 1)) || k % blocksize || q.scalar_type() != at::kByte ||
+            a.scalar_type() != at::kFloat || !q.is_contiguous() || !a.is_contiguous() || !aligned16(q) ||
+            q.numel() < n / 2 * k || a.numel() * blocksize < n * k || !is_current(q.device()))
+            return false;
+        packed = static_cast<const uint8_t*>(q.data_ptr()), absmax = static_cast<const float*>(a.data_ptr());
+        N = n, K = k, bs = (int)blocksize, *device = q.device();
+        return true;
+    }
+};
+
+at::Tensor bytes_on(int64_t bytes, const at::Tensor& like) {
+    return at::empty({bytes}, like.options().dtype(at::kByte).requires_grad(false));
+}
+
+// Tensor of x's leading sizes and `width` columns.
+at::Tensor shaped(const at::Tensor& x, int64_t width) {
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = width;
+    return at::empty(shape, x.options().requires_grad(false));
+}
+
+// gated_fwd(function, workspace function, keeping function, sums function, x, packed, absmax, N, K, blocksize, stream)
+//   -> h, or with a sums function (not 0) (h, the kept sums or None); None where the operands are not in the
+//   plain form (the Python layer copies or refuses them); a status if the call failed.
+PyObject* gated_fwd(PyObject*, PyObject* args) {
+    long long fn, ws_fn, keep_fn, sums_fn, N, K, bs, stream;
+    PyObject *px, *pq, *pa;
+    if (!PyArg_ParseTuple(args, "LLLLOOOLLLL", &fn, &ws_fn, &keep_fn, &sums_fn, &px, &pq, &pa, &N, &K, &bs, &stream))
+        return nullptr;
     try {
-        const at::Tensor &x = THPVariable_Unpack(px), &q = THPVariable_Unpack(pq), &a = THPVariable_Unpack(pa);
-        const int64_t inter = N / 2;
-        if (!x.is_cuda() || !q.is_cuda() || !a.is_cuda() || x.dim() < 1 || N <= 0 || N % 16 || K <= 0 || K % 64 ||
-            bs < 64 || bs > 4096 || (bs & (bs - 1)) || K % bs)
-            Py_RETURN_NONE;
+        Weight w;
+        c10::Device device(c10::DeviceType::CPU);
+        if (!THPVariable_Check(px) || !w.read(pq, pa, N, K, bs, &device)) Py_RETURN_NONE;
+        const at::Tensor& x = THPVariable_Unpack(px);
         const int tag = dtype_tag(x.scalar_type());
-        const auto device = x.device();
-        if ((tag != STM_BF16 && tag != STM_F16) || x.size(-1) != K || q.scalar_type() != at::kByte ||
-            a.scalar_type() != at::kFloat || q.device() != device || a.device() != device || !x.is_contiguous() ||
-            !q.is_contiguous() || !a.is_contiguous() || !aligned16(x) || !aligned16(q) ||
-            q.numel() < inter * K || a.numel() * bs < N * K)
-            Py_RETURN_NONE;
-        if (!is_current(device)) Py_RETURN_NONE;
-        const int64_t M = x.numel() / K;
-        const void* grad = nullptr;
-        if (pg != Py_None) {
-            const at::Tensor& g = THPVariable_Unpack(pg);
-            if (g.device() != device || g.scalar_type() != x.scalar_type() || !g.is_contiguous() || g.dim() < 1 ||
-                g.size(-1) != inter || g.numel() != M * inter || !aligned16(g))
-                Py_RETURN_NONE;
-            grad = g.data_ptr();
-        }
-        at::DimVector shape(x.sizes().begin(), x.sizes().end());
-        shape.back() = grad || pg != Py_None ? N : inter;
-        at::Tensor out = at::empty(shape, x.options().requires_grad(false));
+        if ((tag != STM_BF16 && tag != STM_F16) || !rows_of(x, device, K)) Py_RETURN_NONE;
+        const int64_t M = x.numel() / K, inter = N / 2;
         const int64_t bytes = reinterpret_cast<GatedBytes>(ws_fn)(M, inter, K);
-        if (bytes < 0) return PyLong_FromLongLong(bytes);
-        at::Tensor ws;
-        if (bytes) ws = at::empty({bytes}, a.options().dtype(at::kByte).requires_grad(false));
+        const int64_t kept = sums_fn ? reinterpret_cast<GatedBytes>(sums_fn)(M, inter, K) : 0;
+        if (bytes < 0 || kept < 0) return PyLong_FromLongLong(bytes < 0 ? bytes : kept);
+        at::Tensor h = shaped(x, inter), ws, sums;
+        if (bytes) ws = bytes_on(bytes, x);
         void* wp = bytes ? ws.data_ptr() : nullptr;
-        const auto* qp = static_cast<const uint8_t*>(q.data_ptr());
-        const auto* ap = static_cast<const float*>(a.data_ptr());
         void* st = reinterpret_cast<void*>(stream);
-        const int rc = pg == Py_None
-                           ? reinterpret_cast<GatedFwd>(fn)(x.data_ptr(), qp, ap, out.data_ptr(), M, inter, K, (int)bs, tag, wp, bytes, st)
-                           : reinterpret_cast<GatedBwd>(fn)(grad, x.data_ptr(), qp, ap, out.data_ptr(), M, inter, K, (int)bs, tag, wp, bytes, st);
+        int rc;
+        if (kept) {
+            sums = at::empty({M, N}, x.options().dtype(at::kFloat).requires_grad(false));
+            rc = reinterpret_cast<GatedKeep>(keep_fn)(x.data_ptr(), w.packed, w.absmax, h.data_ptr(),
+                                                      sums.data_ptr<float>(), M, inter, K, w.bs, tag, wp, bytes, st);
+        } else {
+            rc = reinterpret_cast<GatedFwd>(fn)(x.data_ptr(), w.packed, w.absmax, h.data_ptr(), M, inter, K, w.bs, tag,
+                                                wp, bytes, st);
+        }
         if (rc != STM_OK) return PyLong_FromLong(rc);
-        return THPVariable_Wrap(out);
+        if (!sums_fn) return THPVariable_Wrap(h);
+        if (!kept) return Py_BuildValue("NO", THPVariable_Wrap(h), Py_None);
+        return Py_BuildValue("NN", THPVariable_Wrap(h), THPVariable_Wrap(sums));
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// gated_bwd(function, workspace function, function on kept sums, gradient, x or the kept sums, packed, absmax,
+//           N, K, blocksize, input gradient's function and workspace function or 0, stream)
+//   -> the gradient of the projections' outputs, or of x with an input gradient's function; otherwise as gated_fwd.
+PyObject* gated_bwd(PyObject*, PyObject* args) {
+    long long fn, ws_fn, kept_fn, N, K, bs, dx_fn, dx_ws_fn, stream;
+    PyObject *pg, *px, *pq, *pa;
+    if (!PyArg_ParseTuple(args, "LLLOOOOLLLLLL", &fn, &ws_fn, &kept_fn, &pg, &px, &pq, &pa, &N, &K, &bs, &dx_fn,
+                          &dx_ws_fn, &stream))
+        return nullptr;
+    try {
+        Weight w;
+        c10::Device device(c10::DeviceType::CPU);
+        if (!THPVariable_Check(px) || !THPVariable_Check(pg) || !w.read(pq, pa, N, K, bs, &device)) Py_RETURN_NONE;
+        const at::Tensor &x = THPVariable_Unpack(px), &g = THPVariable_Unpack(pg);
+        const int64_t inter = N / 2;
+        const bool kept = x.scalar_type() == at::kFloat;
+        const int tag = dtype_tag(g.scalar_type());
+        if ((tag != STM_BF16 && tag != STM_F16) || !rows_of(g, device, inter) || !rows_of(x, device, kept ? N : K) ||
+            (!kept && x.scalar_type() != g.scalar_type()) || (dx_fn && N % 64))
+            Py_RETURN_NONE;
+        const int64_t M = g.numel() / inter;
+        if (x.numel() != M * (kept ? N : K)) Py_RETURN_NONE;
+        void* st = reinterpret_cast<void*>(stream);
+        at::Tensor dgu = shaped(g, N);
+        int rc;
+        if (kept) {
+            rc = reinterpret_cast<GatedKept>(kept_fn)(g.data_ptr(), x.data_ptr<float>(), dgu.data_ptr(), M, inter, tag, st);
+        } else {
+            const int64_t bytes = reinterpret_cast<GatedBytes>(ws_fn)(M, inter, K);
+            if (bytes < 0) return PyLong_FromLongLong(bytes);
+            at::Tensor ws;
+            if (bytes) ws = bytes_on(bytes, g);
+            rc = reinterpret_cast<GatedBwd>(fn)(g.data_ptr(), x.data_ptr(), w.packed, w.absmax, dgu.data_ptr(), M, inter,
+                                                K, w.bs, tag, bytes ? ws.data_ptr() : nullptr, bytes, st);
+        }
+        if (rc != STM_OK) return PyLong_FromLong(rc);
+        if (!dx_fn) return THPVariable_Wrap(dgu);
+        const int64_t bytes = reinterpret_cast<GemmBytes>(dx_ws_fn)(M, N, K, 1);
+        if (bytes < 0) return PyLong_FromLongLong(bytes);
+        at::Tensor dx = shaped(g, K), ws;
+        if (bytes) ws = bytes_on(bytes, g);
+        rc = reinterpret_cast<GemmDx>(dx_fn)(dgu.data_ptr(), w.packed, w.absmax, nullptr, nullptr, 0, dx.data_ptr(), M, N,
+                                             K, w.bs, tag, bytes ? ws.data_ptr() : nullptr, bytes, st);
+        if (rc != STM_OK) return PyLong_FromLong(rc);
+        return THPVariable_Wrap(dx);
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
         return nullptr;
@@ -210,7 +293,8 @@ PyMethodDef methods[] = {
     {"collect", py_collect, METH_VARARGS, "addresses, sizes, type and device of a list of tensors"},
     {"bump", bump, METH_O, "count the versions of a list of tensors up"},
     {"grad_norm", grad_norm, METH_VARARGS, "the gradient norm of a list of tensors in its plain form"},
-    {"gated", gated, METH_VARARGS, "a gated block's call in its plain form"},
+    {"gated_fwd", gated_fwd, METH_VARARGS, "a gated block's forward in its plain form"},
+    {"gated_bwd", gated_bwd, METH_VARARGS, "a gated block's backward in its plain form"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", "Host code of launch-bound calls.", -1, methods,

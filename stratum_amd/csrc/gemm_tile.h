@@ -175,14 +175,15 @@ __device__ __forceinline__ void gate_bwd(float g, float u, float dh, float& dg, 
 
 // Epilogue of a wave that holds gate columns [c0, c0 + 32) in acc[0] and up columns in
 // acc[1] over 32 FB rows: MODE 1 stores h [rows, I], MODE 2 reads dh [rows, I] and
-// stores dgu [rows, 2 I]. Through LDS as store_tile_lds (rows of four 16-byte chunks
+// stores dgu [rows, 2 I], MODE 3 stores h and the sums (g.sums [rows, 2 I], fp32). Through LDS as store_tile_lds (rows of four 16-byte chunks
 // per output, chunk slot c ^ (row % 4)), FB / 2 fragments at a time. I % 8 == 0.
 template <typename Tr, int FB, int MODE>
 __device__ __forceinline__ void store_gated(const f32x16_t (&acc)[2][FB], const GemmArgs& g, int c0, int orow_base,
                                             int orows, int lane, uint4* stage) {
     constexpr int NP = 2, FP = FB / NP, RP = 32 * FP;
     static_assert(FB % NP == 0, "two passes");
-    const int I = (int)(g.N / 2), ld = MODE * I, hi = lane >> 5;
+    constexpr int PARTS = MODE == 2 ? 2 : 1;
+    const int I = (int)(g.N / 2), ld = PARTS * I, hi = lane >> 5;
     uint8_t* st = reinterpret_cast<uint8_t*>(stage);
     uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
 #pragma unroll
@@ -211,12 +212,17 @@ __device__ __forceinline__ void store_gated(const f32x16_t (&acc)[2][FB], const 
                 float v[4], w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if constexpr (MODE == 1) {
+                    if constexpr (MODE != 2) {
                         v[e] = gate_fwd(a[e], b[e]);
                     } else {
                         const uint32_t d = e < 2 ? dh[q].x : dh[q].y;
                         gate_bwd(a[e], b[e], Tr::to_f32((uint16_t)(e & 1 ? d >> 16 : d & 0xFFFFu)), v[e], w[e]);
                     }
+                }
+                if constexpr (MODE == 3) {
+                    const int row = orow_base + p * RP + rr, col = c0 + 8 * q + 4 * hi;
+                    float* dst = g.sums + ((int64_t)row * 2 * I + col);
+                    if (row < orows && col < I) *reinterpret_cast<f32x4_t*>(dst) = a, *reinterpret_cast<f32x4_t*>(dst + I) = b;
                 }
                 const int slot = q ^ (rr & 3);
                 uint2 pk;
@@ -232,7 +238,7 @@ __device__ __forceinline__ void store_gated(const f32x16_t (&acc)[2][FB], const 
             }
         }
 #pragma unroll
-        for (int part = 0; part < MODE; ++part)
+        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
             for (int it = 0; it < RP / 16; ++it) {
                 const int rr = 16 * it + lane / 4, c = lane % 4;

@@ -412,9 +412,9 @@ int64_t stm_nf4_gated_workspace_bytes(int64_t M, int64_t I, int64_t K) {
     return gated_workspace_bytes(M, I, K);
 }
 
-// Both directions of the gated block; dH only for the backward.
+// Every direction of the gated block: dH for the backward, sums for the forward that keeps them.
 static int gated(const char* who, const void* dH, const void* X, const uint8_t* packed, const float* absmax, void* out,
-                 int64_t M, int64_t I, int64_t K, int blocksize, int dtype, bool backward, void* workspace,
+                 float* sums, int64_t M, int64_t I, int64_t K, int blocksize, int dtype, int mode, void* workspace,
                  int64_t workspace_bytes, void* stream) {
     g_err[0] = 0;
     int rc = check_gemm_common(who, X, packed, absmax, out, M, I, K, blocksize, dtype);
@@ -425,29 +425,59 @@ static int gated(const char* who, const void* dH, const void* X, const uint8_t* 
     if (K > (int64_t)1 << 22 || I > (int64_t)1 << 21 || I * K >= (int64_t)1 << 32)
         return set_error(STM_ERR_UNSUPPORTED, "%s: a weight of [2 x %lld, %lld] is too large", who, (long long)I,
                          (long long)K);
-    if (backward && (!dH || !aligned(dH, 16)))
+    if (mode == 2 && (!dH || !aligned(dH, 16)))
         return set_error(STM_ERR_INVALID, "%s: the gradient must be 16-byte aligned and not NULL", who);
+    if (mode == 3 && (!sums || !aligned(sums, 16)))
+        return set_error(STM_ERR_INVALID, "%s: the sums must be 16-byte aligned and not NULL", who);
+    if (mode == 3 && M <= kGatedKeepRows)
+        return set_error(STM_ERR_UNSUPPORTED, "%s: takes more than %d rows", who, kGatedKeepRows);
     const int64_t need = gated_workspace_bytes(M, I, K);
     if (need > 0 && !workspace) return set_error(STM_ERR_INVALID, "%s: a workspace of %lld bytes is needed", who, (long long)need);
     if ((rc = check_workspace(who, workspace, workspace_bytes, need)) != STM_OK) return rc;
     GemmArgs g{};
     g.a = X; g.packed = packed; g.absmax = absmax; g.out = out; g.M = M; g.N = 2 * I; g.K = K;
-    g.blocksize = blocksize; g.num_groups = 1; g.dh = dH;
+    g.blocksize = blocksize; g.num_groups = 1; g.dh = dH; g.sums = sums;
     g.partial = need ? (float*)workspace : nullptr;
-    return launch_gated(g, backward ? 2 : 1, dtype, (hipStream_t)stream);
+    return launch_gated(g, mode, dtype, (hipStream_t)stream);
 }
 
 int stm_nf4_gated_fwd(const void* X, const uint8_t* packed, const float* absmax, void* H, int64_t M, int64_t I,
                       int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-    return gated("gated_fwd", nullptr, X, packed, absmax, H, M, I, K, blocksize, dtype, false, workspace,
+    return gated("gated_fwd", nullptr, X, packed, absmax, H, nullptr, M, I, K, blocksize, dtype, 1, workspace,
                  workspace_bytes, stream);
+}
+
+int64_t stm_nf4_gated_sums_bytes(int64_t M, int64_t I, int64_t K) {
+    g_err[0] = 0;
+    if (M < 0 || I < 0 || K < 0) return set_error(STM_ERR_INVALID, "gated_sums_bytes: negative size");
+    return gated_sums_bytes(M, I, K);
+}
+
+int stm_nf4_gated_fwd_keep(const void* X, const uint8_t* packed, const float* absmax, void* H, float* sums, int64_t M,
+                           int64_t I, int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
+    return gated("gated_fwd_keep", nullptr, X, packed, absmax, H, sums, M, I, K, blocksize, dtype, 3, workspace,
+                 workspace_bytes, stream);
+}
+
+int stm_gated_bwd_kept(const void* dH, const float* sums, void* dGU, int64_t M, int64_t I, int dtype, void* stream) {
+    g_err[0] = 0;
+    if (!is_16bit(dtype)) return set_error(STM_ERR_INVALID, "gated_bwd_kept: dtype %d is not bf16/fp16", dtype);
+    if (M < 0 || I < 0) return set_error(STM_ERR_INVALID, "gated_bwd_kept: negative size");
+    if (M == 0 || I == 0) return STM_OK;
+    if (I % 8 != 0) return set_error(STM_ERR_UNSUPPORTED, "gated_bwd_kept: I = %lld must be a multiple of 8", (long long)I);
+    if (!dH || !sums || !dGU || !aligned(dH, 16) || !aligned(sums, 16) || !aligned(dGU, 16))
+        return set_error(STM_ERR_INVALID, "gated_bwd_kept: operands must be 16-byte aligned and not NULL");
+    GemmArgs g{};
+    g.M = M; g.N = 2 * I; g.dh = dH; g.out = dGU; g.partial = const_cast<float*>(sums);
+    return launch_gated_kept(g, dtype, (hipStream_t)stream);
 }
 
 int stm_nf4_gated_bwd(const void* dH, const void* X, const uint8_t* packed, const float* absmax, void* dGU, int64_t M,
                       int64_t I, int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes,
                       void* stream) {
-    return gated("gated_bwd", dH, X, packed, absmax, dGU, M, I, K, blocksize, dtype, true, workspace, workspace_bytes,
-                 stream);
+    return gated("gated_bwd", dH, X, packed, absmax, dGU, nullptr, M, I, K, blocksize, dtype, 2, workspace,
+                 workspace_bytes, stream);
 }
 
 // Host copy of a grouped call's expert offsets: offsets[0] = 0, non-decreasing,

@@ -2658,11 +2658,12 @@ __global__ __launch_bounds__(256) void k_split_reduce(const float* __restrict__ 
     }
 }
 
-// The gated forward's reduce: g and u are columns c and I + c of the partials [split][m][2 I].
+// The gated block from partials [split][m][2 I], g and u in columns c and I + c: the forward (MODE 1), the
+// forward that also keeps the sums (3), and the backward (2), also from kept sums (one split).
 template <typename Tr, int MODE>
 __global__ __launch_bounds__(256) void k_gated_reduce(const float* __restrict__ partial, int splits, int64_t rows,
                                                       int64_t I, const uint16_t* __restrict__ dh,
-                                                      uint16_t* __restrict__ out) {
+                                                      uint16_t* __restrict__ out, float* __restrict__ sums) {
     const int64_t total = rows * (I / 4), plane = rows * 2 * I;
     for (int64_t v = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; v < total; v += (int64_t)gridDim.x * blockDim.x) {
         const int64_t row = v / (I / 4), c = (v - row * (I / 4)) * 4;
@@ -2676,7 +2677,11 @@ __global__ __launch_bounds__(256) void k_gated_reduce(const float* __restrict__ 
         }
         const float ga[4] = {a.x, a.y, a.z, a.w}, up[4] = {b.x, b.y, b.z, b.w};
         float x[4], y[4];
-        if constexpr (MODE == 1) {
+        if constexpr (MODE == 3) {
+            *reinterpret_cast<float4*>(sums + row * 2 * I + c) = a;
+            *reinterpret_cast<float4*>(sums + row * 2 * I + I + c) = b;
+        }
+        if constexpr (MODE != 2) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = gate_fwd(ga[e], up[e]);
         } else {
@@ -2689,7 +2694,7 @@ __global__ __launch_bounds__(256) void k_gated_reduce(const float* __restrict__ 
         uint2 pk;
         pk.x = Tr::pack2(x[0], x[1]);
         pk.y = Tr::pack2(x[2], x[3]);
-        *reinterpret_cast<uint2*>(out + row * MODE * I + c) = pk;
+        *reinterpret_cast<uint2*>(out + row * (MODE == 2 ? 2 : 1) * I + c) = pk;
         if constexpr (MODE == 2) {
             pk.x = Tr::pack2(y[0], y[1]);
             pk.y = Tr::pack2(y[2], y[3]);
@@ -2703,15 +2708,19 @@ int launch_gated_reduce(const GemmArgs& g, int mode, int dtype, hipStream_t stre
     const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384)), block(256);
 #define STM_GR_LAUNCH(TR, MODE)                                                                                  \
     hipLaunchKernelGGL((k_gated_reduce<TR, MODE>), grid, block, 0, stream, g.partial, g.splits, g.M, I,          \
-                       (const uint16_t*)g.dh, (uint16_t*)g.out)
-    if (dtype == STM_BF16 && mode == 1)
-        STM_GR_LAUNCH(BF16, 1);
-    else if (dtype == STM_BF16)
-        STM_GR_LAUNCH(BF16, 2);
-    else if (mode == 1)
-        STM_GR_LAUNCH(F16, 1);
+                       (const uint16_t*)g.dh, (uint16_t*)g.out, g.sums)
+    if (dtype == STM_BF16)
+        switch (mode) {
+            case 1: STM_GR_LAUNCH(BF16, 1); break;
+            case 2: STM_GR_LAUNCH(BF16, 2); break;
+            default: STM_GR_LAUNCH(BF16, 3);
+        }
     else
-        STM_GR_LAUNCH(F16, 2);
+        switch (mode) {
+            case 1: STM_GR_LAUNCH(F16, 1); break;
+            case 2: STM_GR_LAUNCH(F16, 2); break;
+            default: STM_GR_LAUNCH(F16, 3);
+        }
 #undef STM_GR_LAUNCH
     return check_launch("gated reduce");
 }
@@ -3501,19 +3510,21 @@ GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
 }
 
 template <typename Tr, int GATED>
-int launch_gated_mode(GemmArgs g, const GatedPlan& p, hipStream_t stream) {
-    if (p.kind == GatedPlan::kKs) {
-        const dim3 grid((unsigned)((g.N + 16 * (p.cfg & 15) - 1) / (16 * (p.cfg & 15)))), block(512);
-        switch (p.cfg) {
-            case 1 | 1 << 4 | 4 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 1, 1, 4, false, GATED>), grid, block, 0, stream, g); break;
-            case 2 | 1 << 4 | 8 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 2, 1, 8, false, GATED>), grid, block, 0, stream, g); break;
-            case 4 | 1 << 4 | 16 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 4, 1, 16, false, GATED>), grid, block, 0, stream, g); break;
-            case 8 | 1 << 4 | 16 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 8, 1, 16, false, GATED>), grid, block, 0, stream, g); break;
-            case 4 | 2 << 4 | 4 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 4, 2, 4, false, GATED>), grid, block, 0, stream, g); break;
-            default: return set_error(STM_ERR_INVALID, "gated: small-M configuration %d", p.cfg);
-        }
-        return check_launch("gated (small M)");
+int launch_gated_ks(const GemmArgs& g, const GatedPlan& p, hipStream_t stream) {
+    const dim3 grid((unsigned)((g.N + 16 * (p.cfg & 15) - 1) / (16 * (p.cfg & 15)))), block(512);
+    switch (p.cfg) {
+        case 1 | 1 << 4 | 4 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 1, 1, 4, false, GATED>), grid, block, 0, stream, g); break;
+        case 2 | 1 << 4 | 8 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 2, 1, 8, false, GATED>), grid, block, 0, stream, g); break;
+        case 4 | 1 << 4 | 16 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 4, 1, 16, false, GATED>), grid, block, 0, stream, g); break;
+        case 8 | 1 << 4 | 16 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 8, 1, 16, false, GATED>), grid, block, 0, stream, g); break;
+        case 4 | 2 << 4 | 4 << 8: hipLaunchKernelGGL((k_gemv_ks<Tr, 4, 2, 4, false, GATED>), grid, block, 0, stream, g); break;
+        default: return set_error(STM_ERR_INVALID, "gated: small-M configuration %d", p.cfg);
     }
+    return check_launch("gated (small M)");
+}
+
+template <typename Tr, int GATED>
+int launch_gated_tiles(const GemmArgs& g, const GatedPlan& p, hipStream_t stream) {
     const int64_t tiles = (g.M + p.cfg - 1) / p.cfg * ((g.N + 255) / 256);
     if (tiles > 0x7FFFFFFFLL) return set_error(STM_ERR_UNSUPPORTED, "gated: grid too large");
     if (p.cfg == 256)
@@ -3523,6 +3534,12 @@ int launch_gated_mode(GemmArgs g, const GatedPlan& p, hipStream_t stream) {
     else
         hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 128, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);
     return check_launch("gated");
+}
+
+template <typename Tr>
+int launch_gated_tiles(const GemmArgs& g, const GatedPlan& p, int mode, hipStream_t stream) {
+    return mode == 1 ? launch_gated_tiles<Tr, 1>(g, p, stream)
+                     : mode == 2 ? launch_gated_tiles<Tr, 2>(g, p, stream) : launch_gated_tiles<Tr, 3>(g, p, stream);
 }
 
 }  // namespace
@@ -3535,6 +3552,17 @@ static int64_t gated_max_rows(int64_t N, int64_t K) {
 
 int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K) {
     return M > 0 && I > 0 && K > 0 ? gated_plan(M, 2 * I, K).partial * (int64_t)sizeof(float) : 0;
+}
+
+// A training step's two directions, us, the backward computing the sums again -> from kept ones.
+// Keeping costs 22 bytes an element at the rate of the copies, computing again 4 K operations:
+// [2 x 5632, 2048] 70 rows 46 -> 35, 509 rows 77 -> 52, 8192 rows 678 -> 528; [2 x 14336, 4096] 4096 rows
+// 1601 -> 994. Short reductions lose once the sums leave the 256 MB cache: [2 x 5632, 512] 4096 rows
+// (185 MB) 141 -> 138, 8192 rows (369 MB) 267 -> 326; [2 x 12000, 640] 4096 rows (393 MB) 338 -> 345, 8192
+// rows 603 -> 773. Up to kGatedKeepRows both directions are a pass over the weight.
+int64_t gated_sums_bytes(int64_t M, int64_t I, int64_t K) {
+    const int64_t bytes = M * 2 * I * (int64_t)sizeof(float);
+    return M > kGatedKeepRows && (K >= 1280 || bytes <= (int64_t)192 << 20) ? bytes : 0;
 }
 
 int launch_gated(const GemmArgs& g0, int mode, int dtype, hipStream_t stream) {
@@ -3554,13 +3582,12 @@ int launch_gated(const GemmArgs& g0, int mode, int dtype, hipStream_t stream) {
             g.a = (const uint16_t*)g0.a + m * g.K;
             g.dh = mode == 2 ? (const uint16_t*)g0.dh + m * (g.N / 2) : nullptr;
             g.out = (uint16_t*)g0.out + m * (mode == 2 ? g.N : g.N / 2);
+            g.sums = mode == 3 ? g0.sums + m * g.N : nullptr;
             const int64_t tiles = (g.M + 255) / 256 * ((g.N + 255) / 256);
             const int rc = p.kind == GatedPlan::kDense
                                ? launch_gated_dense(g, g.partial, mode, dtype, work_grid(tiles).x, stream)
-                           : dtype == STM_BF16 ? (mode == 1 ? launch_gated_mode<BF16, 1>(g, p, stream)
-                                                            : launch_gated_mode<BF16, 2>(g, p, stream))
-                                               : (mode == 1 ? launch_gated_mode<F16, 1>(g, p, stream)
-                                                            : launch_gated_mode<F16, 2>(g, p, stream));
+                           : dtype == STM_BF16 ? launch_gated_tiles<BF16>(g, p, mode, stream)
+                                               : launch_gated_tiles<F16>(g, p, mode, stream);
             if (rc != STM_OK) return rc;
         }
         return STM_OK;
@@ -3573,8 +3600,14 @@ int launch_gated(const GemmArgs& g0, int mode, int dtype, hipStream_t stream) {
         return rc != STM_OK ? rc : launch_gated_reduce(g, mode, dtype, stream);
     }
     if (dtype == STM_BF16)
-        return mode == 1 ? launch_gated_mode<BF16, 1>(g, p, stream) : launch_gated_mode<BF16, 2>(g, p, stream);
-    return mode == 1 ? launch_gated_mode<F16, 1>(g, p, stream) : launch_gated_mode<F16, 2>(g, p, stream);
+        return mode == 1 ? launch_gated_ks<BF16, 1>(g, p, stream) : launch_gated_ks<BF16, 2>(g, p, stream);
+    return mode == 1 ? launch_gated_ks<F16, 1>(g, p, stream) : launch_gated_ks<F16, 2>(g, p, stream);
+}
+
+int launch_gated_kept(const GemmArgs& g0, int dtype, hipStream_t stream) {
+    GemmArgs g = g0;
+    g.splits = 1;
+    return launch_gated_reduce(g, 2, dtype, stream);
 }
 
 int launch_gemv_bwd(GemmArgs g, int dtype, hipStream_t stream) {

@@ -43,6 +43,8 @@ struct GemmArgs {
     int stream_out;
     // Gated backward: the gradient of h, [M, N / 2].
     const void* dh;
+    // Gated forward: where to keep both projections' sums, [M, N].
+    float* sums;
 };
 
 constexpr int64_t kStreamOutBytes = 64ll << 20;
@@ -82,13 +84,18 @@ int launch_dequantize_host(int count, const uint8_t* const* packed, const float*
 int launch_gemm_fwd(const GemmArgs& g, int dtype, hipStream_t stream);
 int launch_gemm_bwd(const GemmArgs& g, int dtype, hipStream_t stream);
 // Gated block over W [2 I, K]: mode 1 = forward (out [M, I]), 2 = backward from dh (out
-// [M, 2 I]); partial holds gated_workspace_bytes(M, I, K).
+// [M, 2 I]), 3 = forward that also keeps the sums (M > kGatedKeepRows); partial holds
+// gated_workspace_bytes(M, I, K).
+constexpr int kGatedKeepRows = 64;
 int launch_gated(const GemmArgs& g, int mode, int dtype, hipStream_t stream);
-// The same from the weight's tiles at w (launch_dequantize_tiles: ceil(I / 128) * 256 * K values), `grid`
+// Mode 2 from the kept sums, which g.partial holds.
+int launch_gated_kept(const GemmArgs& g, int dtype, hipStream_t stream);
+// Every mode from the weight's tiles at w (launch_dequantize_tiles: ceil(I / 128) * 256 * K values), `grid`
 // work-groups over the tiles.
 int launch_gated_dense(const GemmArgs& g, const void* w, int mode, int dtype, unsigned grid, hipStream_t stream);
 int launch_dequantize_tiles(const uint8_t* packed, const float* absmax, int64_t inter, int64_t K, int bs, void* out,
                             int dtype, hipStream_t stream);
 int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K);
+int64_t gated_sums_bytes(int64_t M, int64_t I, int64_t K);  // worth keeping; 0: not
 
 }  // namespace stm

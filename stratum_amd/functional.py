@@ -547,20 +547,35 @@ def _gated_operands(x, packed, absmax, weight_shape, blocksize):
 
 @functools.lru_cache(maxsize=None)
 def _gated_native() -> tuple:
-    """(native caller, and the addresses of the forward, the backward and their workspace size)."""
-    return (_lib.fast().gated, _lib.address("stm_nf4_gated_fwd"), _lib.address("stm_nf4_gated_bwd"),
-            _lib.address("stm_nf4_gated_workspace_bytes"))
+    """The native callers of the forward and the backward, and the addresses that they take."""
+    f, at = _lib.fast(), _lib.address
+    return (f.gated_fwd, (at("stm_nf4_gated_fwd"), at("stm_nf4_gated_workspace_bytes"), at("stm_nf4_gated_fwd_keep")),
+            at("stm_nf4_gated_sums_bytes"),
+            f.gated_bwd, (at("stm_nf4_gated_bwd"), at("stm_nf4_gated_workspace_bytes"), at("stm_gated_bwd_kept")),
+            (at("stm_nf4_gemm_bwd_dx"), at("stm_nf4_gemm_workspace_bytes")))
 
 
-def _gated_plain(x, packed, absmax, weight_shape, blocksize, grad):
-    """The call made by the native host code, or None where an operand has to be copied or refused."""
+def _gated_plain(x, packed, absmax, weight_shape, blocksize, keep=False):
+    """The forward made by the native host code, or None where an operand has to be copied or refused."""
     if not x.is_cuda:
         return None
-    native, fwd, bwd, ws = _gated_native()
-    y = native(fwd if grad is None else bwd, ws, x, packed, absmax, int(weight_shape[0]), int(weight_shape[1]),
-               blocksize, grad, torch._C._cuda_getCurrentRawStream(x.get_device()))
+    native, entries, sums = _gated_native()[:3]
+    y = native(*entries, sums if keep else 0, x, packed, absmax, int(weight_shape[0]), int(weight_shape[1]), blocksize,
+               torch._C._cuda_getCurrentRawStream(x.get_device()))
     if type(y) is int:
-        _lib.check(y, "stm_nf4_gated_fwd" if grad is None else "stm_nf4_gated_bwd")
+        _lib.check(y, "stm_nf4_gated_fwd")
+    return y
+
+
+def _gated_plain_bwd(grad, saved, packed, absmax, weight_shape, blocksize, dx=False):
+    """The backward from x or the kept sums (``dx``: and the input gradient behind it), as :func:`_gated_plain`."""
+    if not grad.is_cuda:
+        return None
+    native, entries, products = _gated_native()[3:]
+    y = native(*entries, grad, saved, packed, absmax, int(weight_shape[0]), int(weight_shape[1]), blocksize,
+               *(products if dx else (0, 0)), torch._C._cuda_getCurrentRawStream(grad.get_device()))
+    if type(y) is int:
+        _lib.check(y, "stm_nf4_gated_bwd")
     return y
 
 
@@ -579,7 +594,7 @@ def nf4_gated_fwd(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, w
     kernel, fp32 throughout, one rounding. (``swiglu_fwd(nf4_gemm_fwd(...))`` rounds the
     projections first and writes and reads them.) ``out`` as for :func:`nf4_gemm_fwd`."""
     if out is None:
-        h = _gated_plain(x, packed, absmax, weight_shape, blocksize, None)
+        h = _gated_plain(x, packed, absmax, weight_shape, blocksize)
         if h is not None:
             return h
     x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
@@ -595,6 +610,65 @@ def nf4_gated_fwd(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, w
 
 
 @_no_grad
+def nf4_gated_fwd_keep(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, weight_shape: Sequence[int],
+                       blocksize: int = 64) -> tuple:
+    """:func:`nf4_gated_fwd` that also keeps the projections' fp32 sums for :func:`nf4_gated_bwd`:
+    (h, sums [rows, 2 I]); sums is None where the backward computes them again as cheaply."""
+    kept = _gated_plain(x, packed, absmax, weight_shape, blocksize, keep=True)
+    if kept is not None:
+        return kept
+    x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)
+    if not _lib.lib().stm_nf4_gated_sums_bytes(M, inter, K):
+        return nf4_gated_fwd(x, packed, absmax, weight_shape, blocksize), None
+    h = torch.empty(*x.shape[:-1], inter, dtype=x.dtype, device=dev)
+    sums = torch.empty(M, 2 * inter, dtype=torch.float32, device=dev)
+    with _lib.device_guard(dev):
+        ws = _gated_workspace(M, inter, K, dev)
+        rc = _lib.lib().stm_nf4_gated_fwd_keep(
+            x2.data_ptr(), _aligned(packed).data_ptr(), _aligned(absmax, 4).data_ptr(), h.data_ptr(), sums.data_ptr(), M,
+            inter, K, blocksize, tag, ws.data_ptr() if ws is not None else None, 4 * ws.numel() if ws is not None else 0,
+            _lib.stream_handle(dev))
+    _lib.check(rc, "stm_nf4_gated_fwd_keep")
+    return h, sums
+
+
+@_no_grad
+def nf4_gated_bwd_dx(grad_out: torch.Tensor, saved: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor,
+                     weight_shape: Sequence[int], blocksize: int = 64) -> torch.Tensor:
+    """Gradient of the gated block's input from that of its output and what the forward kept (its
+    sums, or x): :func:`nf4_gated_bwd_kept` or :func:`nf4_gated_bwd`, then :func:`nf4_gemm_bwd_dx`."""
+    dx = _gated_plain_bwd(grad_out, saved, packed, absmax, weight_shape, blocksize, dx=True)
+    if dx is not None:
+        return dx
+    if saved.dtype == torch.float32:
+        dgu = nf4_gated_bwd_kept(grad_out, saved)
+    else:
+        dgu = nf4_gated_bwd(grad_out, saved, packed, absmax, weight_shape, blocksize)
+    return nf4_gemm_bwd_dx(dgu, packed, absmax, weight_shape, blocksize)
+
+
+@_no_grad
+def nf4_gated_bwd_kept(grad_out: torch.Tensor, sums: torch.Tensor) -> torch.Tensor:
+    """:func:`nf4_gated_bwd` from the sums of :func:`nf4_gated_fwd_keep`."""
+    inter = sums.shape[-1] // 2
+    if sums.dtype != torch.float32 or sums.dim() != 2 or sums.shape[1] % 16 or not sums.is_contiguous():
+        raise ValueError("sums must be contiguous fp32 [rows, 2 I], I a multiple of 8, as nf4_gated_fwd_keep gives them")
+    tag = _gemm_dtype(grad_out)
+    if not sums.is_cuda:
+        raise RuntimeError("the gated block runs on the GPU kernels; its operands must be on the GPU")
+    if grad_out.shape[-1] != inter or grad_out.numel() != sums.shape[0] * inter:
+        raise ValueError(f"grad_out must hold [{sums.shape[0]}, {inter}], got {tuple(grad_out.shape)}")
+    _on_device(sums.device, grad_out=grad_out)
+    d2 = _aligned(_rows(grad_out, inter))
+    dgu = torch.empty(*grad_out.shape[:-1], 2 * inter, dtype=grad_out.dtype, device=sums.device)
+    with _lib.device_guard(sums.device):
+        rc = _lib.lib().stm_gated_bwd_kept(d2.data_ptr(), _aligned(sums).data_ptr(), dgu.data_ptr(), sums.shape[0], inter,
+                                           tag, _lib.stream_handle(sums.device))
+    _lib.check(rc, "stm_gated_bwd_kept")
+    return dgu
+
+
+@_no_grad
 def nf4_gated_bwd(grad_out: torch.Tensor, x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor,
                   weight_shape: Sequence[int], blocksize: int = 64,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -602,7 +676,9 @@ def nf4_gated_bwd(grad_out: torch.Tensor, x: torch.Tensor, packed: torch.Tensor,
     [..., 2 I] = [d gate | d up] in x's dtype, both projections computed again in the same
     kernel. The input's gradient is ``nf4_gemm_bwd_dx`` of it with the same weight."""
     if out is None:
-        dgu = _gated_plain(x, packed, absmax, weight_shape, blocksize, grad_out)
+        dgu = None
+        if x.dtype == grad_out.dtype:
+            dgu = _gated_plain_bwd(grad_out, x, packed, absmax, weight_shape, blocksize)
         if dgu is not None:
             return dgu
     x2, M, inter, K, tag, dev = _gated_operands(x, packed, absmax, weight_shape, blocksize)

@@ -336,15 +336,16 @@ class MemoryFlatFrozenMLP(nn.Module):
 
 class NF4GatedMLP(nn.Module):
     """``down(silu(gate(x)) * up(x))`` with the two frozen NF4 projections and the gating as
-    one kernel: neither [tokens, 2 I] nor its gradient outlives the call that needs it, and
-    the backward keeps only x (and what the down projection keeps of h).
+    one kernel (``nf4_gated``). The backward keeps the projections' fp32 sums [tokens, 2 I], or
+    with ``recompute=True`` only x (and what the down projection keeps of h).
 
     ``module`` is an MLP whose gate and up projections are plain ``NF4Linear`` (``quantize_mlp_``
     makes them, stacked in one payload) with a SiLU ``act_fn``; its down projection is called as
     it is and may be an ``NF4LoRALinear``."""
 
-    def __init__(self, module: nn.Module):
+    def __init__(self, module: nn.Module, recompute: bool = False):
         super().__init__()
+        self.recompute = recompute
         names = _mlp_projection_names(module)
         gate, up, down = (getattr(module, n) for n in names)
         for name, proj in zip(names, (gate, up)):
@@ -368,7 +369,7 @@ class NF4GatedMLP(nn.Module):
 
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         return self.down(nf4_gated(hidden_states, self.gate_up_packed, self.gate_up_absmax, self.shape,
-                                   self.blocksize))
+                                   self.blocksize, recompute=self.recompute))
 
 
 @torch.no_grad()

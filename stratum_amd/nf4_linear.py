@@ -44,8 +44,8 @@ import torch.nn.functional as F
 import os
 
 from .functional import (QuantState, _rows, dequantize_4bit, dequantize_4bit_aug, fused_supported, lora_aug_supported,
-                         gated_supported, lora_da, lora_down, lora_down_aug, lora_dy, lora_supported, lora_up, nf4_gated_bwd,
-                         nf4_gated_fwd, nf4_gemm_bwd_dx, nf4_gemm_fwd)
+                         gated_supported, lora_da, lora_down, lora_down_aug, lora_dy, lora_supported, lora_up,
+                         nf4_gated_bwd_dx, nf4_gated_fwd, nf4_gated_fwd_keep, nf4_gemm_bwd_dx, nf4_gemm_fwd)
 
 _DEFAULT_FUSED_MAX_ROWS = 768
 # With a LoRA adapter the fused kernels fold the rank-R terms into their
@@ -216,34 +216,43 @@ def nf4_linear(x: torch.Tensor, quantized: torch.Tensor, quant_state: QuantState
 
 
 class _NF4GatedFn(torch.autograd.Function):
-    """h = silu(x . Wg^T) * (x . Wu^T) with [Wg; Wu] frozen in NF4. Only x is kept: the
-    backward computes both projections again inside the kernel that differentiates them."""
+    """h = silu(x . Wg^T) * (x . Wu^T) with [Wg; Wu] frozen in NF4. Kept for the backward: the
+    projections' fp32 sums, or (``recompute``, or few rows) x alone, from which the kernel
+    that differentiates them computes them again."""
 
     @staticmethod
-    def forward(ctx, x, packed, absmax, shape, blocksize):
+    def forward(ctx, x, packed, absmax, shape, blocksize, recompute):
         if ctx.needs_input_grad[0] and not gated_supported(shape[0] // 2, shape[1], blocksize, backward=True):
             raise ValueError(f"the gated block's gradient takes I a multiple of 32, got {shape[0] // 2}")
-        ctx.save_for_backward(x, packed, absmax)
-        ctx.shape, ctx.blocksize = shape, blocksize
-        return nf4_gated_fwd(x, packed, absmax, shape, blocksize)
+        ctx.shape, ctx.blocksize, sums = shape, blocksize, None
+        if recompute or not ctx.needs_input_grad[0]:
+            h = nf4_gated_fwd(x, packed, absmax, shape, blocksize)
+        else:
+            h, sums = nf4_gated_fwd_keep(x, packed, absmax, shape, blocksize)
+        ctx.save_for_backward(x if sums is None else sums, packed, absmax)
+        return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, packed, absmax = ctx.saved_tensors
-        dgu = nf4_gated_bwd(grad, x, packed, absmax, ctx.shape, ctx.blocksize)
-        return nf4_gemm_bwd_dx(dgu, packed, absmax, ctx.shape, ctx.blocksize), None, None, None, None
+        saved, packed, absmax = ctx.saved_tensors
+        dx = nf4_gated_bwd_dx(grad, saved, packed, absmax, ctx.shape, ctx.blocksize)
+        return dx, None, None, None, None, None
 
 
 def nf4_gated(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, weight_shape: Sequence[int],
-              blocksize: int = 64) -> torch.Tensor:
+              blocksize: int = 64, recompute: bool = False) -> torch.Tensor:
     """``silu(x @ Wg.T) * (x @ Wu.T)`` with the stacked NF4 weight [Wg; Wu] of shape
     ``weight_shape`` = (2 I, K) (``stack_nf4``, ``quantize_mlp_``), one kernel; differentiable in x. The
-    step ``act_fn(gate_proj(x)) * up_proj(x)`` of stratum/model/mlp_opt.py:178-180."""
+    step ``act_fn(gate_proj(x)) * up_proj(x)`` of stratum/model/mlp_opt.py:178-180.
+
+    For the backward the projections' fp32 sums are kept, 8 bytes per output column and row
+    (16 I bytes a row more than h), from the forward to the backward of this call;
+    ``recompute=True`` keeps x alone and computes them again."""
     shape = tuple(int(d) for d in weight_shape)
     if not (torch.is_grad_enabled() and x.requires_grad):
         return nf4_gated_fwd(x, packed, absmax, shape, blocksize)
-    return _NF4GatedFn.apply(x, packed, absmax, shape, blocksize)
+    return _NF4GatedFn.apply(x, packed, absmax, shape, blocksize, recompute)
 
 
 class NF4Linear(nn.Module):

@@ -118,3 +118,25 @@ def test_module_takes_adjacent_payloads_as_they_are_and_keeps_fp32_scales():
     assert mlp.gate_up_absmax.dtype == torch.float32 and torch.equal(mlp.gate_up_absmax, scales)
     apart = NF4GatedMLP(MLP(projection(64, 128), projection(64, 128), nn.Linear(64, 128, bias=False)))
     assert apart.gate_up_packed.numel() == 64 * 128 and apart.gate_up_absmax.numel() == 256
+
+
+def test_c_abi_of_the_kept_sums(L):
+    err = lambda: L.stm_last_error().decode()  # noqa: E731
+
+    def keep(sums=BASE, M=100, I=64, K=128):  # noqa: E741
+        return L.stm_nf4_gated_fwd_keep(BASE, BASE, BASE, BASE, sums, M, I, K, 64, 1, BASE, 1 << 30, None)
+
+    def kept(dh=BASE, sums=BASE, out=BASE, M=100, I=64, dtype=1):  # noqa: E741
+        return L.stm_gated_bwd_kept(dh, sums, out, M, I, dtype, None)
+    assert keep(sums=None) < 0 and "sums" in err()
+    assert keep(sums=BASE + 4) < 0 and "sums" in err()
+    assert keep(M=64) < 0 and "rows" in err()
+    assert keep(M=0) == 0
+    for bad in (dict(dh=None), dict(sums=None), dict(out=None), dict(dh=BASE + 2), dict(sums=BASE + 4),
+                dict(out=BASE + 8), dict(I=12), dict(M=-1), dict(I=-8), dict(dtype=2)):
+        assert kept(**bad) < 0 and err(), bad
+    assert kept(M=0, dh=None, sums=None, out=None) == 0 and kept(I=0, dh=None) == 0
+    assert L.stm_nf4_gated_sums_bytes(64, 64, 128) == 0 and L.stm_nf4_gated_sums_bytes(-1, 64, 128) < 0
+    assert L.stm_nf4_gated_sums_bytes(100, 64, 128) == 100 * 2 * 64 * 4
+    # a short reduction whose sums outgrow the cache is computed again
+    assert L.stm_nf4_gated_sums_bytes(8192, 5632, 512) == 0 and L.stm_nf4_gated_sums_bytes(8192, 5632, 2048) > 0
