@@ -43,9 +43,7 @@ constexpr int kNormTensors = 254;
 constexpr int rows_of(int bits) { return bits == 8 ? 2 : 1; }
 constexpr int tile_of(int bits) { return 4 * rows_of(bits) * kBlock8; }  // elements per work-group
 constexpr int kRows = rows_of(8), kTile = tile_of(8);                    // of the conversions
-// Elements per work-group of the norm, all in flight at once: 84 M elements in 16 bits 42.5 us, 16384
-// 43.3, 32768 60; 21 M in 32 bits 36.5, 42, 56.
-constexpr int kNormTile = 8192;
+constexpr int kNormThreads = 512, kNormTile = 16384;  // elements per work-group of the norm
 
 struct AdamNumbers {
     float beta1, beta2, rest1, rest2;  // rest = 1 - beta
@@ -69,6 +67,8 @@ struct AdamTable {
     int count;
     AdamNumbers h;
 };
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct NormArgs {
     const void* g[kNormTensors];
@@ -426,28 +426,52 @@ __device__ __forceinline__ double group_sum(double v, double (&lds)[THREADS / 64
 
 // Squares are summed in fp64: exact products of the 16-bit types, no overflow for any
 // fp32 gradient, and an order of its own would not show in the fp32 result.
+//
+// A whole tile of an aligned tensor is asked for at once, 16 bytes a lane and load; the last
+// tile of a tensor, and tensors that start between, four elements at a time with bounds.
+// 84 M elements in bf16 (168 MB, 448 tensors): 38.5 us where four elements a load took 52;
+// 168 M in fp32 118 us (5.7 TB/s), against 133. With 256 threads 38 and 121.
 template <typename G>
-__global__ __launch_bounds__(256) void k_norm_partial(NormArgs a, double* __restrict__ partial) {
-    __shared__ double lds[4];
+__global__ __launch_bounds__(kNormThreads) void k_norm_partial(NormArgs a, double* __restrict__ partial) {
+    __shared__ double lds[kNormThreads / 64];
     const int ti = tensor_of(a.first, a.count, (int)blockIdx.x);
     const void* g = a.g[ti];
     const int64_t base = ((int64_t)blockIdx.x - a.first[ti]) * kNormTile;
     const int64_t n = (int64_t)(a.first[ti + 1] - a.first[ti] - 1) * kNormTile + a.last[ti];
-    const bool vec = ((uintptr_t)g & (G::tag == STM_F32 ? 15 : 7)) == 0;
     double sum = 0.0;
-    constexpr int kLoads = kNormTile / 1024;
-    float f[kLoads][4];
+    auto add = [&](float f) { sum = fma((double)f, (double)f, sum); };
+    if (((uintptr_t)g & 15) == 0 && base + kNormTile <= n) {
+        constexpr int kBytes = G::tag == STM_F32 ? 4 : 2, kLoads = kNormTile * kBytes / (16 * kNormThreads);
+        const u32x4* src = reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(g) + base * kBytes);
+        u32x4 raw[kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) load4<G>(g, base + j * 1024 + threadIdx.x * 4, n, vec, f[j]);
+        for (int j = 0; j < kLoads; ++j) raw[j] = src[j * kNormThreads + threadIdx.x];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j)
+        for (int j = 0; j < kLoads; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum = fma((double)f[j][e], (double)f[j][e], sum);
-    sum = group_sum<256>(sum, lds);
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (G::tag == STM_F32) {
+                    add(__builtin_bit_cast(float, raw[j][e]));
+                } else {
+                    add(G::to_f32((uint16_t)(raw[j][e] & 0xFFFFu)));
+                    add(G::to_f32((uint16_t)(raw[j][e] >> 16)));
+                }
+            }
+    } else {
+        const bool vec = ((uintptr_t)g & (G::tag == STM_F32 ? 15 : 7)) == 0;
+#pragma unroll 4
+        for (int j = 0; j < kNormTile; j += 4 * kNormThreads) {
+            float f[4];
+            load4<G>(g, base + j + threadIdx.x * 4, n, vec, f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add(f[e]);
+        }
+    }
+    sum = group_sum<kNormThreads>(sum, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// One work-group with eight loads a thread in flight: the 10 240 partial sums of 84 M elements.
+// One work-group with eight loads a thread in flight: the 5 120 partial sums of 84 M elements.
 constexpr int kFinalThreads = 1024;
 __global__ __launch_bounds__(kFinalThreads) void k_norm_final(const double* __restrict__ partial, int64_t count,
                                                               double max_norm, double loss_scale,
@@ -676,7 +700,7 @@ extern "C" int stm_grad_norm(int count, const void* const* grads, const int64_t*
         }
         if (!groups) continue;
         a.first[a.count] = (int)groups;
-        const dim3 grid((unsigned)groups), block(256);
+        const dim3 grid((unsigned)groups), block(kNormThreads);
         if (dtype == STM_F32)
             hipLaunchKernelGGL(k_norm_partial<F32>, grid, block, 0, (hipStream_t)stream, a, partial);
         else if (dtype == STM_BF16)
