@@ -430,7 +430,7 @@ __device__ __forceinline__ double group_sum(double v, double (&lds)[THREADS / 64
 // A whole tile of an aligned tensor is asked for at once, 16 bytes a lane and load; the last
 // tile of a tensor, and tensors that start between, four elements at a time with bounds.
 // 84 M elements in bf16 (168 MB, 448 tensors): 38.5 us where four elements a load took 52;
-// 168 M in fp32 118 us (5.7 TB/s), against 133. With 256 threads 38 and 121.
+// 168 M in fp32 120 us (5.6 TB/s), against 133. (256 threads: the same.)
 template <typename G>
 __global__ __launch_bounds__(kNormThreads) void k_norm_partial(NormArgs a, double* __restrict__ partial) {
     __shared__ double lds[kNormThreads / 64];
@@ -450,11 +450,12 @@ __global__ __launch_bounds__(kNormThreads) void k_norm_partial(NormArgs a, doubl
         for (int j = 0; j < kLoads; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
+                const uint32_t word = raw[j][e];
                 if constexpr (G::tag == STM_F32) {
-                    add(__builtin_bit_cast(float, raw[j][e]));
+                    add(__uint_as_float(word));
                 } else {
-                    add(G::to_f32((uint16_t)(raw[j][e] & 0xFFFFu)));
-                    add(G::to_f32((uint16_t)(raw[j][e] >> 16)));
+                    add(G::to_f32((uint16_t)(word & 0xFFFFu)));
+                    add(G::to_f32((uint16_t)(word >> 16)));
                 }
             }
     } else {
