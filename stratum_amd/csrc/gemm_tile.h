@@ -176,12 +176,11 @@ __device__ __forceinline__ void gate_bwd(float g, float u, float dh, float& dg, 
 // Epilogue of a wave that holds gate columns [c0, c0 + 32) in acc[0] and up columns in
 // acc[1] over 32 FB rows: MODE 1 stores h [rows, I], MODE 2 reads dh [rows, I] and
 // stores dgu [rows, 2 I], MODE 3 stores h and the sums (g.sums [rows, 2 I], fp32). Through LDS as store_tile_lds (rows of four 16-byte chunks
-// per output, chunk slot c ^ (row % 4)), FB / 2 fragments at a time. I % 8 == 0.
+// per output, chunk slot c ^ (row % 4)), half of the fragments (an odd number: one) at a time. I % 8 == 0.
 template <typename Tr, int FB, int MODE>
 __device__ __forceinline__ void store_gated(const f32x16_t (&acc)[2][FB], const GemmArgs& g, int c0, int orow_base,
                                             int orows, int lane, uint4* stage) {
-    constexpr int NP = 2, FP = FB / NP, RP = 32 * FP;
-    static_assert(FB % NP == 0, "two passes");
+    constexpr int NP = FB % 2 ? FB : 2, FP = FB / NP, RP = 32 * FP;
     constexpr int PARTS = MODE == 2 ? 2 : 1;
     const int I = (int)(g.N / 2), ld = PARTS * I, hi = lane >> 5;
     uint8_t* st = reinterpret_cast<uint8_t*>(stage);

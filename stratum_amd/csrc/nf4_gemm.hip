@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "gemm_tile.h"
+#include <cstdlib>
 #include "nf4_kernels.h"
 
 // Tile shapes (measured best on MI355X at M = 8192, N = 14336, K = 4096):
@@ -919,15 +920,19 @@ __device__ __forceinline__ void rw_slot_pattern() {
 #define STM_SHORT_ITEMS 1
 #endif
 
-template <typename Tr, int BM, int WM, int GATED = 0>
+// KW = 2 (gated): the tile has 128 weight rows, and two pairs of waves take half of the reduction each, on
+// activation tiles of their own; at the end they exchange halves of the sums through LDS. Twice the tiles
+// of half the depth, for row counts whose tiles leave half of the CUs without one.
+template <typename Tr, int BM, int WM, int GATED = 0, int KW = 1>
 __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
     static_assert(!GATED || WM == 1, "a wave's gated columns are its own");
-    constexpr int BN = 256, NT = 256 * WM, FB = BM / WM / 32;
+    static_assert(KW == 1 || (KW == 2 && GATED), "split within the work-group: gated only");
+    constexpr int BN = 256 / KW, NT = 256 * WM, FB = BM / WM / 32, XT = BM * 8;  // XT: 16-byte words of an activation tile
     const int tid = threadIdx.x, lane0 = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wn = wave & 3, xrow0 = (wave >> 2) * (BM / WM);
+    const int wn = wave & (4 / KW - 1), xrow0 = (wave >> 2) * (BM / WM), kw = KW == 2 ? wave >> 1 : 0;
 
     __shared__ float2 lut_all[256 * RW_LUT_COPIES];
-    __shared__ uint4 sA0[BM * 8], sA1[BM * 8];
+    __shared__ uint4 sA0[KW * XT], sA1[KW * XT];
 
     fill_lut_rw<NT>(lut_all, tid);
 
@@ -936,7 +941,7 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
     int64_t work = tiles * g.num_groups * g.splits, main_work = 0;
     __shared__ GroupedPlan plan;
     bool use_plan = false;
-    if constexpr (NT == 256) {
+    if constexpr (NT == 256 && KW == 1) {
         use_plan = plan_usable(g);
         if (use_plan) {
             build_plan<BM>(g, plan, tid);
@@ -963,7 +968,10 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
     if (m0 >= grp.rows) continue;
 
     int s_begin, KT;
-    split_range((int)(K / BK), g.splits, z, s_begin, KT);
+    if constexpr (KW == 2)
+        KT = (int)(K / BK) / 2, s_begin = kw * KT;  // an even number of steps
+    else
+        split_range((int)(K / BK), g.splits, z, s_begin, KT);
     const int64_t kbase = (int64_t)s_begin * BK;
     const uint16_t* X = reinterpret_cast<const uint16_t*>(g.a) + grp.row0 * K + kbase;
     const int lane = opaque_lane(lane0);
@@ -984,8 +992,8 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
         ws.woff[i] = (uint32_t)(n * (K / 2) + kbase / 2 + 16 * (lane >> 5));
         ws.aoff[i] = (uint32_t)(n * (K >> ws.bshift));
     }
-    ActStageS<BM, 4 * WM> as;
-    as.init(X, K, m0, grp.rows, sA0, sA1, wave, lane);
+    ActStageS<BM, 4 * WM / KW> as;
+    as.init(X, K, m0, grp.rows, sA0 + kw * XT, sA1 + kw * XT, KW == 2 ? wn : wave, lane);
 
     f32x16_t acc[2][FB];
     zero_acc(acc);
@@ -1034,7 +1042,7 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
         }
         ws.issue(raw0, 3, pa);
         ws.load_words((KT > 2 ? 2 : KT - 1) * (int64_t)BK, raw0);
-        read_x<FB, FBA>(x, sA0, xrow0, lane, 0);
+        read_x<FB, FBA>(x, sA0 + kw * XT, xrow0, lane, 0);
         sched_fence();
 
         auto sub = [&](const uint4 (&w)[2], const uint4* sx, int jn, const typename RwWeights<Tr>::Raw& r_next,
@@ -1068,11 +1076,12 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
             sched_fence();
         };
         int s = 0;
+        const uint4 *x0 = sA0 + kw * XT, *x1 = sA1 + kw * XT;
         for (; s + 1 < KT; s += 2) {
-            step(s, sA0, sA1, 0, raw0, raw1);
-            step(s + 1, sA1, sA0, 1, raw1, raw0);
+            step(s, x0, x1, 0, raw0, raw1);
+            step(s + 1, x1, x0, 1, raw1, raw0);
         }
-        if (s < KT) step(s, sA0, sA1, 0, raw0, raw1);
+        if (s < KT) step(s, x0, x1, 0, raw0, raw1);
         wait_vmem();  // the loads past the last step (clamped to it) land before the epilogue reuses LDS
     };
     // the item's valid rows decide (uniform over the work-group, so every wave
@@ -1101,7 +1110,43 @@ __global__ __launch_bounds__(256 * WM) void k_gemm_fwd_rw(GemmArgs g) {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int f = 0; f < FB; ++f) __asm__ volatile("" : "+a"(acc[i][f]));
-        store_gated<Tr, FB, GATED>(acc, g, (int)(col_base / 2), (int)m0, (int)grp.rows, lane_e, stage);
+        if constexpr (KW == 2) {
+            // wave (kw, wn) hands the other half of its rows to wave (1 - kw, wn) and gates its own
+            constexpr int FH = FB / 2;
+            f32x4_t* send = reinterpret_cast<f32x4_t*>(kw ? sA1 : sA0) + wn * (FB * 256) + lane_e;
+            const f32x4_t* recv = reinterpret_cast<const f32x4_t*>(kw ? sA0 : sA1) + wn * (FB * 256) + lane_e;
+            f32x16_t half[2][FH];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int f = 0; f < FH; ++f) {
+                    const f32x16_t other = kw ? acc[i][f] : acc[i][FH + f];
+                    half[i][f] = kw ? acc[i][FH + f] : acc[i][f];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        f32x4_t v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = other[4 * q + e];
+                        send[((i * FH + f) * 4 + q) * 64] = v;
+                    }
+                }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int f = 0; f < FH; ++f)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x4_t v = recv[((i * FH + f) * 4 + q) * 64];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) half[i][f][4 * q + e] += v[e];
+                    }
+            __syncthreads();  // the halves are read: LDS stages the output
+            store_gated<Tr, FH, GATED>(half, g, (int)(col_base / 2), (int)(m0 + 32 * FH * kw), (int)grp.rows, lane_e,
+                                       stage);
+        } else {
+            store_gated<Tr, FB, GATED>(acc, g, (int)(col_base / 2), (int)m0, (int)grp.rows, lane_e, stage);
+        }
     } else {
     if (g.lora_rank > 0 && z == 0)
         lora_term<Tr, 2, FB>(acc, reinterpret_cast<const uint16_t*>(g.lora_w), col_base, N,
@@ -3426,7 +3471,7 @@ namespace {
 // How a gated forward of M rows over the stacked weight [2 I, K] runs.
 struct GatedPlan {
     enum Kind { kKs, kGemv, kSplit, kTile, kDense } kind;
-    int cfg;       // kKs: its configuration; kTile: the tile's rows (128, 192 or 256)
+    int cfg;       // kKs: its configuration; kTile: the tile's rows (128, 192 or 256), + 1 with KW = 2
     GemvPlan gv;   // kGemv
     int tile, splits;  // kSplit: tile kind and reduction ranges
     int64_t partial;   // fp32 values of workspace: the partials, or (kDense) the 16-bit weight
@@ -3451,20 +3496,23 @@ int gated_ks_config(int64_t M, int64_t N, int64_t K, double* time) {
 }
 
 // Time of `tiles` work items of one reduction depth, one work-group per CU, in us: every round of
-// 256 takes steps x (c0 + c1 x the share of the CUs it fills) + 8.
-double gated_rounds(int64_t tiles, int64_t steps, double c0, double c1) {
+// 256 takes steps x (c0 + c1 x the share of the CUs it fills) + `fixed`.
+double gated_rounds(int64_t tiles, int64_t steps, double c0, double c1, double fixed = 8.0) {
     const double full = (double)(tiles / kCUs), last = (double)(tiles % kCUs) / kCUs;
-    return full * ((double)steps * (c0 + c1) + 8.0) + (last > 0.0 ? (double)steps * (c0 + c1 * last) + 8.0 : 0.0);
+    return full * ((double)steps * (c0 + c1) + fixed) + (last > 0.0 ? (double)steps * (c0 + c1 * last) + fixed : 0.0);
 }
 
 // The least estimated time, in us. Up to 64 rows the weight-streaming kernels run. Above that:
-//  * tiles of 128, 192 or 256 rows that dequantize their own weight (k_gemm_fwd_rw);
+//  * tiles of 128, 192 or 256 rows that dequantize their own weight (k_gemm_fwd_rw), and of 128 or
+//    192 rows with half the weight rows and the reduction split between their waves (KW = 2; 256
+//    rows of two activation tiles do not fit LDS): fewer than 128 of the former;
 //  * the LDS-weight tiles of 128 x 128 or 256 x 256 over 2-8 ranges of the reduction, whose
 //    fp32 partials k_gated_reduce sums and gates: few rows on a narrow weight;
 //  * the weight dequantized once and k_gated_dense over it: many rows.
 // The constants are fitted to 7 weights (K 640-5120, I 512-14336) x 13-15 row counts from 65 to
 // 8192, all ways timed on each: the pick is 0.3 % above the fastest on average and 5 % at
-// worst. E.g. us, [2 x 14336, 4096]: 100 rows 65 (128-row tiles; dense 129, split 66), 333 rows 85
+// worst (those with KW = 2 to 9 weights x 12 row counts up to 768: 0.1 % and 4 %). E.g. us, [2 x 14336, 4096]:
+// 100 rows 46 (128 rows, KW = 2; KW = 1 65, dense 129, split 66), 180 rows 53 (192, KW = 2; 128, KW = 1 67), 333 rows 85
 // (192; 256-row tiles 102), 1024 rows 207 (256; 192: 250), 8192 rows dense 1510 (256: 1600);
 // [2 x 512, 4096]: 509 rows 21 (eight ranges of 128 x 128; unsplit 50).
 GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
@@ -3494,6 +3542,10 @@ GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
         offer(gated_rounds(tiles(128, 256), steps, 0.66, 0.34), GatedPlan::kTile, 128, 1, 0);
     if (only < 0 || only == kBig8) offer(gated_rounds(tiles(192, 256), steps, 0.89, 0.36), GatedPlan::kTile, 192, 1, 0);
     if (only < 0 || only == kBig) offer(gated_rounds(tiles(256, 256), steps, 1.12, 0.40), GatedPlan::kTile, 256, 1, 0);
+    if (only < 0 && steps % 2 == 0) {
+        offer(gated_rounds(tiles(128, 128), steps / 2, 0.94, 0.25, 5.7), GatedPlan::kTile, 128 + 1, 1, 0);
+        offer(gated_rounds(tiles(192, 128), steps / 2, 1.14, 0.23, 8.3), GatedPlan::kTile, 192 + 1, 1, 0);
+    }
     for (int sp = 2; sp <= 8 && sp * 8 <= steps; ++sp) {
         const int64_t partial = sp * M * N, per = (steps + sp - 1) / sp;
         const double reduce = 3.5 + (double)partial * 8.0 / 4.0e6;
@@ -3525,9 +3577,14 @@ int launch_gated_ks(const GemmArgs& g, const GatedPlan& p, hipStream_t stream) {
 
 template <typename Tr, int GATED>
 int launch_gated_tiles(const GemmArgs& g, const GatedPlan& p, hipStream_t stream) {
-    const int64_t tiles = (g.M + p.cfg - 1) / p.cfg * ((g.N + 255) / 256);
+    const int rows = p.cfg & ~1, cols = p.cfg & 1 ? 128 : 256;
+    const int64_t tiles = (g.M + rows - 1) / rows * ((g.N + cols - 1) / cols);
     if (tiles > 0x7FFFFFFFLL) return set_error(STM_ERR_UNSUPPORTED, "gated: grid too large");
-    if (p.cfg == 256)
+    if (p.cfg == 129)
+        hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 128, 1, GATED, 2>), work_grid(tiles), dim3(256), 0, stream, g);
+    else if (p.cfg == 193)
+        hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 192, 1, GATED, 2>), work_grid(tiles), dim3(256), 0, stream, g);
+    else if (p.cfg == 256)
         hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 256, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);
     else if (p.cfg == 192)
         hipLaunchKernelGGL((k_gemm_fwd_rw<Tr, 192, 1, GATED>), work_grid(tiles), dim3(256), 0, stream, g);

@@ -115,3 +115,14 @@ def test_replayed_graph(cuda):
         torch.cuda.synchronize()
         assert torch.equal(h, expected[0]) and torch.equal(dgu, expected[1])
         x.mul_(-0.9)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,inter,K", [(65, 8200, 128), (128, 8200, 256), (150, 8200, 256), (192, 8200, 384), (257, 1000, 1024),
+                                       (380, 4104, 2048)])
+def test_reductions_that_two_pairs_of_waves_share(cuda, M, inter, K, dtype):
+    from stratum_amd import nf4_gated_bwd
+    check(M, inter, K, dtype)
+    q, a, w = weight(inter, K, dtype)
+    x, dh = (seeded((M, n), M + n, 1.0, dtype).cuda() for n in (K, inter))
+    assert_within(nf4_gated_bwd(dh, x, q, a, (2 * inter, K)), *reference(x, w, dh), dtype)
