@@ -24,8 +24,9 @@
 // 1622; copies behind the operand reads 1474; weight in tiles 1452; steps of 32 in four
 // buffers 1420 (five: 1429). Without copies 1240, without the epilogue as well 1210: what
 // is left is the copies' share of LDS and L1, of which x, read in rows with a stride of
-// 2 K bytes, has 60 us (packed into tiles as the weight is: 1354, and 27 for the packing).
-// Copies issued between the matrix instructions: 1543-1576.
+// 2 K bytes, has 60 us (tiles as the weight's: 1354, but with the kernel that makes them the
+// call went from 1502 to 1485, and on [2 x 5632, 2048] from 313 to 317). Copies issued
+// between the matrix instructions: 1543-1576. The weight straight into registers: 1628.
 #include "gemm_tile.h"
 
 namespace stm {

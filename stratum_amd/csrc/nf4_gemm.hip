@@ -3509,9 +3509,9 @@ double gated_rounds(int64_t tiles, int64_t steps, double c0, double c1, double f
 //  * the LDS-weight tiles of 128 x 128 or 256 x 256 over 2-8 ranges of the reduction, whose
 //    fp32 partials k_gated_reduce sums and gates: few rows on a narrow weight;
 //  * the weight dequantized once and k_gated_dense over it: many rows.
-// The constants are fitted to 7 weights (K 640-5120, I 512-14336) x 13-15 row counts from 65 to
-// 8192, all ways timed on each: the pick is 0.3 % above the fastest on average and 5 % at
-// worst (those with KW = 2 to 9 weights x 12 row counts up to 768: 0.1 % and 4 %). E.g. us, [2 x 14336, 4096]:
+// The constants are fitted to 9 weights (K 640-5120, I 512-14336) x 20 row counts from 65 to
+// 8192, all ways timed on each: the pick is 0.2 % above the fastest on average and 4 % at
+// worst. E.g. us, [2 x 14336, 4096]:
 // 100 rows 46 (128 rows, KW = 2; KW = 1 65, dense 129, split 66), 180 rows 53 (192, KW = 2; 128, KW = 1 67), 333 rows 85
 // (192; 256-row tiles 102), 1024 rows 207 (256; 192: 250), 8192 rows dense 1510 (256: 1600);
 // [2 x 512, 4096]: 509 rows 21 (eight ranges of 128 x 128; unsplit 50).
@@ -3556,7 +3556,7 @@ GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
             offer(rounds(tiles(256, 256) * sp) * (1.62 * (double)per + 5.0) + reduce, GatedPlan::kSplit, kBig, sp, partial);
     }
     if (only < 0 && N * K < (int64_t)1 << 31)
-        offer(gated_rounds(tiles(256, 256), steps, 1.0, 0.36) + (double)(N * K) * 2.5625 / 3.9e6 + 2.0, GatedPlan::kDense, 0, 1,
+        offer(gated_rounds(tiles(256, 256), steps, 1.0, 0.34, 7.0) + (double)(N * K) * 2.5625 / 4.2e6 + 2.0, GatedPlan::kDense, 0, 1,
               (N / 2 + 127) / 128 * 128 * K);  // 256 x K values of 2 bytes a tile
     return p;
 }

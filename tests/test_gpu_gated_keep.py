@@ -126,3 +126,43 @@ def test_reductions_that_two_pairs_of_waves_share(cuda, M, inter, K, dtype):
     q, a, w = weight(inter, K, dtype)
     x, dh = (seeded((M, n), M + n, 1.0, dtype).cuda() for n in (K, inter))
     assert_within(nf4_gated_bwd(dh, x, q, a, (2 * inter, K)), *reference(x, w, dh), dtype)
+
+
+@pytest.mark.parametrize("recompute", [False, True])
+def test_gradients_of_other_layouts(cuda, recompute):
+    """An expanded, a transposed and a sliced gradient, and x with leading sizes, as their copies."""
+    from stratum_amd import nf4_gated
+    q, a, _ = weight(96, 128, torch.bfloat16)
+    x = seeded((5, 20, 128), 3, 1.0, torch.bfloat16).cuda()
+    wide = seeded((5, 20, 192), 4, 1.0, torch.bfloat16).cuda()
+    for grad in (torch.ones(1, 1, 1, dtype=x.dtype, device=cuda).expand(5, 20, 96), wide[..., 1:97],
+                 wide.permute(2, 0, 1)[:96].permute(1, 2, 0)):
+        got = []
+        for g in (grad, grad.clone(memory_format=torch.contiguous_format)):
+            t = x.clone().requires_grad_(True)
+            nf4_gated(t, q, a, (192, 128), recompute=recompute).backward(g)
+            got.append(t.grad)
+        assert got[0].shape == x.shape and torch.equal(got[0], got[1])
+
+
+def test_kept_sums_on_another_stream(cuda):
+    """Forward and backward on a side stream while the default stream is busy."""
+    from stratum_amd import nf4_gated
+    q, a, _ = weight(320, 512, torch.bfloat16)
+    x = seeded((300, 512), 5, 1.0, torch.bfloat16).cuda()
+    dh = seeded((300, 320), 6, 1.0, torch.bfloat16).cuda()
+
+    def step():
+        t = x.clone().requires_grad_(True)
+        nf4_gated(t, q, a, (640, 512)).backward(dh)
+        return t.grad
+    expected = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    busy = torch.randn(4096, 4096, device=cuda)
+    for _ in range(4):
+        busy = busy @ busy * 1e-4
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert torch.equal(got, expected)
