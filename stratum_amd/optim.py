@@ -111,6 +111,7 @@ class AdamWTensors:
                     _held(f"{name} {i}", t, first, dtype, int(want[i]))
         table[:, _N] = self._sizes = sizes
         self._table = table
+        self._addresses = table.ctypes.data, sizes.ctypes.data  # (a microsecond each to ask numpy for)
         # everything a step writes: held here (the table has bare addresses), and its versions counted up
         self._written = [t for column in (params, *columns.values()) for t in column]
 
@@ -141,10 +142,10 @@ class AdamWTensors:
         if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
                                        or grad_scale.device != self.device):
             raise ValueError(f"grad_scale must be one fp32 value on {self.device}")
-        grads, table, written = list(grads), self._table, self._written
-        sizes = self._sizes.ctypes.data
+        grads, written = list(grads), self._written
+        rows, sizes = self._addresses
         while True:
-            tag, index, count, bad = _lib.fast().collect(grads, table.ctypes.data + 8 * _GRAD, 8, sizes, 0)
+            tag, index, count, bad = _lib.fast().collect(grads, rows + 8 * _GRAD, 8, sizes, 0)
             if bad < 0:
                 break
             grads[bad] = self._plain(bad, grads)
@@ -157,19 +158,20 @@ class AdamWTensors:
         if count < len(grads):
             some = [i for i, g in enumerate(grads) if g is not None]
             per = len(grads)
-            table = np.ascontiguousarray(table[some])
+            table = np.ascontiguousarray(self._table[some])
+            rows = table.ctypes.data
             written = [written[c * per + i] for c in range(len(written) // per) for i in some]
         numbers = (lr, betas[0], betas[1], eps, weight_decay, step,
                    grad_scale.data_ptr() if grad_scale is not None else None)
         types = (self.param_tag, tag, self.state_bits)
-        lib, n = _lib.lib(), len(table)
+        lib, n = _lib.lib(), count
         with _lib.device_guard(self.device):
             stream = _lib.stream_handle(self.device)
             if n <= _ARGUMENT_TENSORS or torch.cuda.is_current_stream_capturing():
-                rc = lib.stm_adamw_step(n, table.ctypes.data, *types, *numbers, stream)
+                rc = lib.stm_adamw_step(n, rows, *types, *numbers, stream)
             else:
                 host = torch.empty(lib.stm_adamw_table_bytes(n), dtype=torch.uint8, pin_memory=True)
-                rc = lib.stm_adamw_fill_table(n, table.ctypes.data, *types, host.data_ptr())
+                rc = lib.stm_adamw_fill_table(n, rows, *types, host.data_ptr())
                 if rc >= 0:  # the caching host allocator keeps the pinned block until the copy has run
                     held = host.to(self.device, non_blocking=True)
                     rc = lib.stm_adamw_step_table(n, held.data_ptr(), rc, *types, *numbers, stream)
