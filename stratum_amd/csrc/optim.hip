@@ -8,7 +8,8 @@
 //             and nothing at all where scale is not finite
 //
 // Both are bound by HBM: the norm reads every gradient once; a step reads p, g, m
-// and v and writes p, m and v. All arithmetic is fp32 in the order above, one rounding
+// and v and writes p, m and v (with 8-bit states some 90 vector instructions an element are as
+// much: 176 M bf16 elements 377 us, their 1.77 GB 328). All arithmetic is fp32 in the order above, one rounding
 // each (no contraction), so that a plain evaluation gives the same states bit for bit.
 //
 // Tensors travel as kernel arguments (pointers and sizes, one launch for up to
@@ -39,7 +40,7 @@ constexpr int kAdamTensors = 56;  // tensors per launch (below 4 KB of kernel ar
 constexpr int kNormTensors = 254;
 // Rows of 256 elements per wave: with one, a 32-bit step of 42 M elements takes 219 us, with two
 // 227, with four 240 (four accesses of a lane stand between a row's loads and its stores); an
-// 8-bit step of 176 M 477, 419 and 500 (two rows share a division).
+// 8-bit step of 176 M 394, 377 and 388 (two rows share a division).
 constexpr int rows_of(int bits) { return bits == 8 ? 2 : 1; }
 constexpr int tile_of(int bits) { return 4 * rows_of(bits) * kBlock8; }  // elements per work-group
 constexpr int kRows = rows_of(8), kTile = tile_of(8);                    // of the conversions
@@ -249,24 +250,14 @@ __device__ __forceinline__ uint32_t encode4(const float (&f)[4], float inv) {
 // A work-group takes kTile consecutive elements of one tensor: wave w, kRows rows of 256
 // elements, four a lane, so that every access of a wave is one contiguous piece and a row is a
 // block of an 8-bit state. All loads are issued before the first result is needed.
-template <typename P, typename G, int BITS, typename Args>
-__global__ __launch_bounds__(256) void k_adamw(Args args) {
-    const AdamNumbers& a = args.h;
-    float scale = 1.0f;
-    if (a.scale) {
-        scale = *a.scale;
-        if (!(fabsf(scale) < INFINITY)) return;  // the whole launch alike
-    }
+//
+// FULL: the tile lies inside its tensor and every base is aligned for whole accesses; then no
+// access has a test of its own (8-bit states of 176 M elements: 400 -> 377 us).
+template <typename P, typename G, int BITS, bool FULL>
+__device__ __forceinline__ void adamw_tile(const AdamNumbers& a, const stm_adamw_tensor& t, int64_t base, int lane,
+                                           float scale, bool vp, bool vg, bool vs, bool vm) {
     constexpr int kRows = rows_of(BITS);
-    const int lane = threadIdx.x & 63;
-    const int ti = tensor_of(args.first, args.count, (int)blockIdx.x);
-    const stm_adamw_tensor t = args.t[ti];
-    const int64_t n = t.n;
-    const int64_t base = ((int64_t)blockIdx.x - args.first[ti]) * tile_of(BITS) + (threadIdx.x >> 6) * (kRows * kBlock8) + lane * 4;
-    auto al = [](const void* p, uintptr_t b) { return ((uintptr_t)p & (b - 1)) == 0; };
-    const bool vp = al(t.param, P::tag == STM_F32 ? 16 : 8), vg = al(t.grad, G::tag == STM_F32 ? 16 : 8);
-    const bool vs = al(t.exp_avg, BITS == 8 ? 4 : 16) && al(t.exp_avg_sq, BITS == 8 ? 4 : 16), vm = al(t.master, 16);
-
+    const int64_t n = FULL ? INT64_MAX : t.n;
     float p[kRows][4], g[kRows][4], m[kRows][4], v[kRows][4];
     [[maybe_unused]] uint32_t cm[kRows], cv[kRows];
     [[maybe_unused]] float sm[kRows], sv[kRows], tops[2 * kRows];
@@ -284,8 +275,8 @@ __global__ __launch_bounds__(256) void k_adamw(Args args) {
         } else {
             cm[r] = load_codes((const uint8_t*)t.exp_avg, i, n, vs);
             cv[r] = load_codes((const uint8_t*)t.exp_avg_sq, i, n, vs);
-            sm[r] = i < n ? t.exp_avg_scale[i / kBlock8] : 0.0f;
-            sv[r] = i < n ? t.exp_avg_sq_scale[i / kBlock8] : 0.0f;
+            sm[r] = FULL || i < n ? t.exp_avg_scale[i / kBlock8] : 0.0f;
+            sv[r] = FULL || i < n ? t.exp_avg_sq_scale[i / kBlock8] : 0.0f;
         }
     }
 #pragma unroll
@@ -311,7 +302,7 @@ __global__ __launch_bounds__(256) void k_adamw(Args args) {
             store4<F32>(t.exp_avg, i, n, vs, m[r]);
             store4<F32>(t.exp_avg_sq, i, n, vs, v[r]);
         } else {
-            if (i + 4 > n) {  // past the tensor: no part in the block's scale
+            if (!FULL && i + 4 > n) {  // past the tensor: no part in the block's scale
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (i + e >= n) m[r][e] = v[r][e] = 0.0f;
@@ -333,12 +324,34 @@ __global__ __launch_bounds__(256) void k_adamw(Args args) {
             const float iv = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(inverse, 2 * r + 1));
             store_codes((uint8_t*)t.exp_avg, i, n, vs, encode4<true>(m[r], im));
             store_codes((uint8_t*)t.exp_avg_sq, i, n, vs, encode4<false>(v[r], iv));
-            if (lane == 0 && i < n) {
+            if (lane == 0 && (FULL || i < n)) {
                 t.exp_avg_scale[i / kBlock8] = tops[2 * r];
                 t.exp_avg_sq_scale[i / kBlock8] = tops[2 * r + 1];
             }
         }
     }
+}
+
+template <typename P, typename G, int BITS, typename Args>
+__global__ __launch_bounds__(256) void k_adamw(Args args) {
+    const AdamNumbers& a = args.h;
+    float scale = 1.0f;
+    if (a.scale) {
+        scale = *a.scale;
+        if (!(fabsf(scale) < INFINITY)) return;  // the whole launch alike
+    }
+    const int lane = threadIdx.x & 63;
+    const int ti = tensor_of(args.first, args.count, (int)blockIdx.x);
+    const stm_adamw_tensor t = args.t[ti];
+    const int64_t tile = ((int64_t)blockIdx.x - args.first[ti]) * tile_of(BITS);
+    const int64_t base = tile + (threadIdx.x >> 6) * (rows_of(BITS) * kBlock8) + lane * 4;
+    auto al = [](const void* p, uintptr_t b) { return ((uintptr_t)p & (b - 1)) == 0; };
+    const bool vp = al(t.param, P::tag == STM_F32 ? 16 : 8), vg = al(t.grad, G::tag == STM_F32 ? 16 : 8);
+    const bool vs = al(t.exp_avg, BITS == 8 ? 4 : 16) && al(t.exp_avg_sq, BITS == 8 ? 4 : 16), vm = al(t.master, 16);
+    if (vp && vg && vs && vm && tile + tile_of(BITS) <= t.n)
+        adamw_tile<P, G, BITS, true>(a, t, base, lane, scale, true, true, true, true);
+    else
+        adamw_tile<P, G, BITS, false>(a, t, base, lane, scale, vp, vg, vs, vm);
 }
 
 template <typename P, typename G, typename Args>
