@@ -158,18 +158,14 @@ int launch_gated_dense(const GemmArgs& g, const void* w, int mode, int dtype, un
     d.g = g;
     d.w = (const uint16_t*)w;
 #define STM_GD_LAUNCH(TR, MODE) hipLaunchKernelGGL((k_gated_dense<TR, MODE>), dim3(grid), dim3(512), 0, stream, d)
-    if (dtype == STM_BF16)
-        switch (mode) {
-            case 1: STM_GD_LAUNCH(BF16, 1); break;
-            case 2: STM_GD_LAUNCH(BF16, 2); break;
-            default: STM_GD_LAUNCH(BF16, 3);
-        }
+    if (dtype == STM_BF16 && mode == 1)
+        STM_GD_LAUNCH(BF16, 1);
+    else if (dtype == STM_BF16)
+        STM_GD_LAUNCH(BF16, 2);
+    else if (mode == 1)
+        STM_GD_LAUNCH(F16, 1);
     else
-        switch (mode) {
-            case 1: STM_GD_LAUNCH(F16, 1); break;
-            case 2: STM_GD_LAUNCH(F16, 2); break;
-            default: STM_GD_LAUNCH(F16, 3);
-        }
+        STM_GD_LAUNCH(F16, 2);
 #undef STM_GD_LAUNCH
     return check_launch("gated (dense)");
 }

@@ -3515,7 +3515,10 @@ double gated_rounds(int64_t tiles, int64_t steps, double c0, double c1, double f
 // 100 rows 46 (128 rows, KW = 2; KW = 1 65, dense 129, split 66), 180 rows 53 (192, KW = 2; 128, KW = 1 67), 333 rows 85
 // (192; 256-row tiles 102), 1024 rows 207 (256; 192: 250), 8192 rows dense 1510 (256: 1600);
 // [2 x 512, 4096]: 509 rows 21 (eight ranges of 128 x 128; unsplit 50).
-GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
+// A forward that keeps its sums (mode 3) does not take the dense way, which loses more by the stores, us:
+// [2 x 14336, 4096] 4096 rows 884 against 841 (256-row tiles), 8192 rows 1724 against 1697, [2 x 8192, 4096]
+// 8192 rows 1029 against 958, [2 x 2816, 1024] 118 against 121.
+GatedPlan gated_plan(int64_t M, int64_t N, int64_t K, int mode) {
     GatedPlan p{};
     const int only = tile_override();
     if (M <= STM_GEMV_MAX_M && only < 0) {
@@ -3555,7 +3558,7 @@ GatedPlan gated_plan(int64_t M, int64_t N, int64_t K) {
         if (only < 0 || only == kBig)
             offer(rounds(tiles(256, 256) * sp) * (1.62 * (double)per + 5.0) + reduce, GatedPlan::kSplit, kBig, sp, partial);
     }
-    if (only < 0 && N * K < (int64_t)1 << 31)
+    if (only < 0 && mode != 3 && N * K < (int64_t)1 << 31)
         offer(gated_rounds(tiles(256, 256), steps, 1.0, 0.34, 7.0) + (double)(N * K) * 2.5625 / 4.2e6 + 2.0, GatedPlan::kDense, 0, 1,
               (N / 2 + 127) / 128 * 128 * K);  // 256 x K values of 2 bytes a tile
     return p;
@@ -3608,7 +3611,9 @@ static int64_t gated_max_rows(int64_t N, int64_t K) {
 }
 
 int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K) {
-    return M > 0 && I > 0 && K > 0 ? gated_plan(M, 2 * I, K).partial * (int64_t)sizeof(float) : 0;
+    if (M <= 0 || I <= 0 || K <= 0) return 0;
+    const int64_t a = gated_plan(M, 2 * I, K, 1).partial, b = gated_plan(M, 2 * I, K, 3).partial;
+    return (a > b ? a : b) * (int64_t)sizeof(float);
 }
 
 // A training step's two directions, us, the backward computing the sums again -> from kept ones.
@@ -3625,7 +3630,7 @@ int64_t gated_sums_bytes(int64_t M, int64_t I, int64_t K) {
 int launch_gated(const GemmArgs& g0, int mode, int dtype, hipStream_t stream) {
     GemmArgs g = g0;
     g.splits = 1;
-    const GatedPlan p = gated_plan(g.M, g.N, g.K);
+    const GatedPlan p = gated_plan(g.M, g.N, g.K, mode);
     if (p.kind == GatedPlan::kDense) {
         const int rc = launch_dequantize_tiles(g.packed, g.absmax, g.N / 2, g.K, g.blocksize, g.partial, dtype, stream);
         if (rc != STM_OK) return rc;

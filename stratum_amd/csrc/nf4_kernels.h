@@ -90,7 +90,7 @@ constexpr int kGatedKeepRows = 64;
 int launch_gated(const GemmArgs& g, int mode, int dtype, hipStream_t stream);
 // Mode 2 from the kept sums, which g.partial holds.
 int launch_gated_kept(const GemmArgs& g, int dtype, hipStream_t stream);
-// Every mode from the weight's tiles at w (launch_dequantize_tiles: ceil(I / 128) * 256 * K values), `grid`
+// Modes 1 and 2 from the weight's tiles at w (launch_dequantize_tiles: ceil(I / 128) * 256 * K values), `grid`
 // work-groups over the tiles.
 int launch_gated_dense(const GemmArgs& g, const void* w, int mode, int dtype, unsigned grid, hipStream_t stream);
 int launch_dequantize_tiles(const uint8_t* packed, const float* absmax, int64_t inter, int64_t K, int bs, void* out,
