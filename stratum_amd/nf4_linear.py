@@ -40,6 +40,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 import os
 
@@ -250,7 +251,8 @@ def nf4_gated(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, weigh
     (16 I bytes a row more than h), from the forward to the backward of this call;
     ``recompute=True`` keeps x alone and computes them again."""
     shape = tuple(int(d) for d in weight_shape)
-    if not (torch.is_grad_enabled() and x.requires_grad):
+    # the raw kernel knows no autograd: a forward-mode dual goes to the function, which refuses it
+    if not (torch.is_grad_enabled() and x.requires_grad) and forward_ad.unpack_dual(x).tangent is None:
         return nf4_gated_fwd(x, packed, absmax, shape, blocksize)
     return _NF4GatedFn.apply(x, packed, absmax, shape, blocksize, recompute)
 
