@@ -363,7 +363,9 @@ int stm_nf4_dequantize_aug(const uint8_t* packed, const float* absmax, const voi
  *   the device (NULL: 1); where it is not finite, nothing is written. `master`, where
  *   given, holds p in fp32 and `param` receives it rounded. state_bits 32: exp_avg and
  *   exp_avg_sq are floats, the scales unused. state_bits 8: one code per element and
- *   one float per 256 elements (ceil(n / 256)), see stm_state8_codes.
+ *   one float per 256 elements (ceil(n / 256)), see stm_state8_codes. With STM_ADAMW_FOLLOW or'ed to
+ *   state_bits, an element of `param` that is not its master rounded (something else has written
+ *   it) replaces the master before the step; without it `param` is not read where there is a master.
  *   Any element-aligned pointers; 16-byte aligned ones (8 for 8-bit codes) are faster.
  *   `tensors` is a host array, read before the call returns.
  *
@@ -384,6 +386,8 @@ typedef struct {
     float* exp_avg_sq_scale; /* 8-bit states */
     int64_t n;
 } stm_adamw_tensor;
+
+#define STM_ADAMW_FOLLOW 0x100 /* in state_bits: masters follow their parameters */
 
 int64_t stm_grad_norm_workspace_bytes(int count, const int64_t* n);
 int stm_grad_norm(int count, const void* const* grads, const int64_t* n, int dtype, double max_norm,

@@ -146,6 +146,15 @@ __device__ __forceinline__ void store4(void* base, int64_t i, int64_t n, bool ve
     }
 }
 
+// x as the type holds it.
+template <typename T>
+__device__ __forceinline__ float rounded(float x) {
+    if constexpr (T::tag == STM_F32)
+        return x;
+    else
+        return T::to_f32(T::from_f32(x));
+}
+
 // Four codes in a word, element 0 in the low byte.
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* base, int64_t i, int64_t n, bool vec) {
     const uint8_t* p = base + i;
@@ -253,12 +262,18 @@ __device__ __forceinline__ uint32_t encode4(const float (&f)[4], float inv) {
 //
 // FULL: the tile lies inside its tensor and every base is aligned for whole accesses; then no
 // access has a test of its own (8-bit states of 176 M elements: 400 -> 377 us).
-template <typename P, typename G, int BITS, bool FULL>
+//
+// FOLLOW: an element of the parameter that is not its master rounded was written by something
+// else since the last step, and replaces the master. No other trace of such a write is certain (a
+// tensor's version counts no write through .data), so the parameter is read as well: 42 M bf16 elements
+// with masters 240 -> 255 us, with 8-bit states 145 -> 162.
+template <typename P, typename G, int BITS, bool FOLLOW, bool FULL>
 __device__ __forceinline__ void adamw_tile(const AdamNumbers& a, const stm_adamw_tensor& t, int64_t base, int lane,
                                            float scale, bool vp, bool vg, bool vs, bool vm) {
     constexpr int kRows = rows_of(BITS);
     const int64_t n = FULL ? INT64_MAX : t.n;
     float p[kRows][4], g[kRows][4], m[kRows][4], v[kRows][4];
+    [[maybe_unused]] float held[kRows][4];  // FOLLOW: the parameter beside its master
     [[maybe_unused]] uint32_t cm[kRows], cv[kRows];
     [[maybe_unused]] float sm[kRows], sv[kRows], tops[2 * kRows];
 #pragma unroll
@@ -269,6 +284,7 @@ __device__ __forceinline__ void adamw_tile(const AdamNumbers& a, const stm_adamw
             load4<F32>(t.master, i, n, vm, p[r]);
         else
             load4<P>(t.param, i, n, vp, p[r]);
+        if constexpr (FOLLOW) load4<P>(t.param, i, n, vp, held[r]);
         if constexpr (BITS == 32) {
             load4<F32>(t.exp_avg, i, n, vs, m[r]);
             load4<F32>(t.exp_avg_sq, i, n, vs, v[r]);
@@ -285,6 +301,10 @@ __device__ __forceinline__ void adamw_tile(const AdamNumbers& a, const stm_adamw
         if constexpr (BITS == 8) {
             decode4<true>(cm[r], sm[r], m[r]);
             decode4<false>(cv[r], sv[r], v[r]);
+        }
+        if constexpr (FOLLOW) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[r][e] = rounded<P>(p[r][e]) == held[r][e] ? p[r][e] : held[r][e];
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -332,7 +352,7 @@ __device__ __forceinline__ void adamw_tile(const AdamNumbers& a, const stm_adamw
     }
 }
 
-template <typename P, typename G, int BITS, typename Args>
+template <typename P, typename G, int BITS, bool FOLLOW, typename Args>
 __global__ __launch_bounds__(256) void k_adamw(Args args) {
     const AdamNumbers& a = args.h;
     float scale = 1.0f;
@@ -349,37 +369,48 @@ __global__ __launch_bounds__(256) void k_adamw(Args args) {
     const bool vp = al(t.param, P::tag == STM_F32 ? 16 : 8), vg = al(t.grad, G::tag == STM_F32 ? 16 : 8);
     const bool vs = al(t.exp_avg, BITS == 8 ? 4 : 16) && al(t.exp_avg_sq, BITS == 8 ? 4 : 16), vm = al(t.master, 16);
     if (vp && vg && vs && vm && tile + tile_of(BITS) <= t.n)
-        adamw_tile<P, G, BITS, true>(a, t, base, lane, scale, true, true, true, true);
+        adamw_tile<P, G, BITS, FOLLOW, true>(a, t, base, lane, scale, true, true, true, true);
     else
-        adamw_tile<P, G, BITS, false>(a, t, base, lane, scale, vp, vg, vs, vm);
+        adamw_tile<P, G, BITS, FOLLOW, false>(a, t, base, lane, scale, vp, vg, vs, vm);
 }
 
+// How a step is asked for: its types, the bits of a state, and whether masters follow their parameters.
+struct AdamKind {
+    int param_dtype, grad_dtype, bits;
+    bool follow;
+};
+
 template <typename P, typename G, typename Args>
-void launch_adamw(const Args& a, int bits, unsigned grid, hipStream_t st) {
-    if (bits == 8)
-        hipLaunchKernelGGL((k_adamw<P, G, 8, Args>), dim3(grid), dim3(256), 0, st, a);
+void launch_adamw(const Args& a, const AdamKind& k, unsigned grid, hipStream_t st) {
+    const dim3 block(256);
+    if (k.bits == 8 && k.follow)
+        hipLaunchKernelGGL((k_adamw<P, G, 8, true, Args>), dim3(grid), block, 0, st, a);
+    else if (k.bits == 8)
+        hipLaunchKernelGGL((k_adamw<P, G, 8, false, Args>), dim3(grid), block, 0, st, a);
+    else if (k.follow)
+        hipLaunchKernelGGL((k_adamw<P, G, 32, true, Args>), dim3(grid), block, 0, st, a);
     else
-        hipLaunchKernelGGL((k_adamw<P, G, 32, Args>), dim3(grid), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_adamw<P, G, 32, false, Args>), dim3(grid), block, 0, st, a);
 }
 
 template <typename P, typename Args>
-void launch_adamw(const Args& a, int grad_dtype, int bits, unsigned grid, hipStream_t st) {
-    if (grad_dtype == STM_F32)
-        launch_adamw<P, F32>(a, bits, grid, st);
-    else if (grad_dtype == STM_BF16)
-        launch_adamw<P, BF16>(a, bits, grid, st);
+void launch_adamw(const Args& a, const AdamKind& k, unsigned grid, hipStream_t st) {
+    if (k.grad_dtype == STM_F32)
+        launch_adamw<P, F32>(a, k, grid, st);
+    else if (k.grad_dtype == STM_BF16)
+        launch_adamw<P, BF16>(a, k, grid, st);
     else
-        launch_adamw<P, F16>(a, bits, grid, st);
+        launch_adamw<P, F16>(a, k, grid, st);
 }
 
 template <typename Args>
-int launch_adamw(const Args& a, int param_dtype, int grad_dtype, int bits, int64_t grid, hipStream_t st) {
-    if (param_dtype == STM_F32)
-        launch_adamw<F32>(a, grad_dtype, bits, (unsigned)grid, st);
-    else if (param_dtype == STM_BF16)
-        launch_adamw<BF16>(a, grad_dtype, bits, (unsigned)grid, st);
+int launch_adamw(const Args& a, const AdamKind& k, int64_t grid, hipStream_t st) {
+    if (k.param_dtype == STM_F32)
+        launch_adamw<F32>(a, k, (unsigned)grid, st);
+    else if (k.param_dtype == STM_BF16)
+        launch_adamw<BF16>(a, k, (unsigned)grid, st);
     else
-        launch_adamw<F16>(a, grad_dtype, bits, (unsigned)grid, st);
+        launch_adamw<F16>(a, k, (unsigned)grid, st);
     return check_launch("adamw_step");
 }
 
@@ -519,27 +550,27 @@ using namespace stm;
 
 constexpr int64_t kMostGroups = 0x3FFFFFFF;  // work-groups of a launch
 
-static int check_adamw_types(int param_dtype, int grad_dtype, int state_bits) {
+static int adamw_kind(int param_dtype, int grad_dtype, int state_bits, AdamKind& k) {
     if (!valid_dtype(param_dtype) || !valid_dtype(grad_dtype))
         return set_error(STM_ERR_INVALID, "adamw_step: unknown dtype");
-    if (state_bits != 8 && state_bits != 32)
-        return set_error(STM_ERR_INVALID, "adamw_step: states have 8 or 32 bits, got %d", state_bits);
+    k = {param_dtype, grad_dtype, state_bits & ~STM_ADAMW_FOLLOW, (state_bits & STM_ADAMW_FOLLOW) != 0};
+    if (k.bits != 8 && k.bits != 32)
+        return set_error(STM_ERR_INVALID, "adamw_step: states have 8 or 32 bits, got %d", k.bits);
     return STM_OK;
 }
 
-static int check_adamw_tensors(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype,
-                               int state_bits) {
+static int check_adamw_tensors(int count, const stm_adamw_tensor* tensors, const AdamKind& k) {
     if (count < 0 || (count && !tensors)) return set_error(STM_ERR_INVALID, "adamw_step: bad tensor list");
-    const int64_t tile = tile_of(state_bits);
+    const int64_t tile = tile_of(k.bits);
     for (int i = 0; i < count; ++i) {
         const stm_adamw_tensor& t = tensors[i];
         if (t.n < 0) return set_error(STM_ERR_INVALID, "adamw_step: tensor %d has a negative size", i);
         if (t.n == 0) continue;
         if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq ||
-            (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))
+            (k.bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))
             return set_error(STM_ERR_INVALID, "adamw_step: tensor %d has a null pointer", i);
-        const uintptr_t pa = param_dtype == STM_F32 ? 4 : 2, ga = grad_dtype == STM_F32 ? 4 : 2;
-        const uintptr_t sa = state_bits == 32 ? 4 : 1;
+        const uintptr_t pa = k.param_dtype == STM_F32 ? 4 : 2, ga = k.grad_dtype == STM_F32 ? 4 : 2;
+        const uintptr_t sa = k.bits == 32 ? 4 : 1;
         if (!aligned(t.param, pa) || !aligned(t.grad, ga) || !aligned(t.master, 4) || !aligned(t.exp_avg, sa) ||
             !aligned(t.exp_avg_sq, sa) || !aligned(t.exp_avg_scale, 4) || !aligned(t.exp_avg_sq_scale, 4))
             return set_error(STM_ERR_INVALID, "adamw_step: tensor %d is not aligned to its elements", i);
@@ -570,11 +601,12 @@ extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int pa
                               int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay,
                               int64_t step, const float* grad_scale, void* stream) {
     AdamArgs a;
-    int rc = check_adamw_types(param_dtype, grad_dtype, state_bits);
+    AdamKind k;
+    int rc = adamw_kind(param_dtype, grad_dtype, state_bits, k);
     if (rc == STM_OK) rc = adamw_numbers(lr, beta1, beta2, eps, weight_decay, step, grad_scale, a.h);
-    if (rc == STM_OK) rc = check_adamw_tensors(count, tensors, param_dtype, grad_dtype, state_bits);
+    if (rc == STM_OK) rc = check_adamw_tensors(count, tensors, k);
     if (rc != STM_OK) return rc;
-    const int64_t tile = tile_of(state_bits);
+    const int64_t tile = tile_of(k.bits);
     for (int i = 0; i < count;) {
         a.count = 0;
         int64_t groups = 0;
@@ -589,7 +621,7 @@ extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int pa
             ++i;
         }
         if (!groups) continue;
-        rc = launch_adamw(a, param_dtype, grad_dtype, state_bits, groups, (hipStream_t)stream);
+        rc = launch_adamw(a, k, groups, (hipStream_t)stream);
         if (rc != STM_OK) return rc;
     }
     return STM_OK;
@@ -602,13 +634,14 @@ extern "C" int64_t stm_adamw_table_bytes(int count) {
 
 extern "C" int stm_adamw_fill_table(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype,
                                     int state_bits, void* table) {
-    int rc = check_adamw_types(param_dtype, grad_dtype, state_bits);
-    if (rc == STM_OK) rc = check_adamw_tensors(count, tensors, param_dtype, grad_dtype, state_bits);
+    AdamKind k;
+    int rc = adamw_kind(param_dtype, grad_dtype, state_bits, k);
+    if (rc == STM_OK) rc = check_adamw_tensors(count, tensors, k);
     if (rc != STM_OK) return rc;
     if (count && (!table || !aligned(table, 8))) return set_error(STM_ERR_INVALID, "adamw_table: bad table");
     auto* t = static_cast<stm_adamw_tensor*>(table);
     auto* first = reinterpret_cast<int*>(t + count);
-    const int64_t tile = tile_of(state_bits);
+    const int64_t tile = tile_of(k.bits);
     int64_t groups = 0;
     for (int i = 0; i < count; ++i) {
         t[i] = tensors[i];
@@ -623,7 +656,8 @@ extern "C" int stm_adamw_step_table(int count, const void* table, int groups, in
                                     int state_bits, double lr, double beta1, double beta2, double eps,
                                     double weight_decay, int64_t step, const float* grad_scale, void* stream) {
     AdamTable a;
-    int rc = check_adamw_types(param_dtype, grad_dtype, state_bits);
+    AdamKind k;
+    int rc = adamw_kind(param_dtype, grad_dtype, state_bits, k);
     if (rc == STM_OK) rc = adamw_numbers(lr, beta1, beta2, eps, weight_decay, step, grad_scale, a.h);
     if (rc != STM_OK) return rc;
     if (count < 0 || groups < 0 || groups > kMostGroups || (groups && (!count || !table || !aligned(table, 8))))
@@ -632,7 +666,7 @@ extern "C" int stm_adamw_step_table(int count, const void* table, int groups, in
     a.t = static_cast<const stm_adamw_tensor*>(table);
     a.first = reinterpret_cast<const int*>(a.t + count);
     a.count = count;
-    return launch_adamw(a, param_dtype, grad_dtype, state_bits, groups, (hipStream_t)stream);
+    return launch_adamw(a, k, groups, (hipStream_t)stream);
 }
 
 extern "C" int stm_state8_values(const uint8_t* codes, const float* scales, int64_t n, int is_signed, float* out,

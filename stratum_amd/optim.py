@@ -37,6 +37,8 @@ STATE_BLOCK = 256  # elements per scale of an 8-bit state
 # 8B model: 257 us in 8 launches, where one launch over as many elements takes 219).
 _ARGUMENT_TENSORS = 56
 
+_FOLLOW = 0x100  # STM_ADAMW_FOLLOW
+
 # columns of a row of the tensor table (stm_adamw_tensor)
 _PARAM, _GRAD, _MASTER, _M, _V, _M_SCALE, _V_SCALE, _N = range(8)
 
@@ -71,12 +73,14 @@ class AdamWTensors:
     copies. ``scales`` = (first moments' scales, second moments' scales) makes the moments
     8-bit codes (uint8, with ``ceil(numel / 256)`` fp32 scales each); without it they are
     fp32. All contiguous, on one GPU. The tensors are checked once, here, and written in
-    place by :meth:`step`.
+    place by :meth:`step`. A step takes the masters as they are and does not read the
+    parameters beside them; with ``follow`` it does, and an element of a parameter that is not its
+    master rounded (something else has written it) replaces the master first.
     """
 
     def __init__(self, params: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
                  exp_avg_sqs: Sequence[torch.Tensor], *, masters: Optional[Sequence[torch.Tensor]] = None,
-                 scales: Optional[tuple] = None):
+                 scales: Optional[tuple] = None, follow: bool = False):
         params, exp_avgs, exp_avg_sqs = list(params), list(exp_avgs), list(exp_avg_sqs)
         if not params:
             raise ValueError("AdamWTensors needs at least one tensor")
@@ -84,6 +88,7 @@ class AdamWTensors:
         self.device, self.dtype = _gpu(first, "AdamW"), first.dtype
         self.param_tag = _lib.dtype_tag(first.dtype)
         self.state_bits = 8 if scales is not None else 32
+        self.follow = bool(follow) and masters is not None
         state_dtype = torch.uint8 if scales is not None else torch.float32
         columns = {"exp_avg": exp_avgs, "exp_avg_sq": exp_avg_sqs}
         if masters is not None:
@@ -163,7 +168,7 @@ class AdamWTensors:
             written = [written[c * per + i] for c in range(len(written) // per) for i in some]
         numbers = (lr, betas[0], betas[1], eps, weight_decay, step,
                    grad_scale.data_ptr() if grad_scale is not None else None)
-        types = (self.param_tag, tag, self.state_bits)
+        types = (self.param_tag, tag, self.state_bits | (_FOLLOW if self.follow else 0))
         lib, n = _lib.lib(), count
         with _lib.device_guard(self.device):
             stream = _lib.stream_handle(self.device)
@@ -261,8 +266,9 @@ class AdamW(torch.optim.Optimizer):
     """AdamW over parameters on one or several GPUs, a few launches per step.
 
     ``state_bits`` = 32 or 8; ``master_weights`` keeps an fp32 master of every 16-bit
-    parameter, which takes the updates that bf16 or fp16 would round away (a parameter that
-    something else writes in place between two steps is taken over into its master).
+    parameter, which takes the updates that bf16 or fp16 would round away; an element of a
+    parameter that something else wrote between two steps, in place, through ``.data`` or by loading,
+    is taken over into its master (the step sees that it is not the master rounded).
     ``max_grad_norm`` clips by the norm over all parameters (of one GPU each); ``grad_norm``
     then holds the last norms, one tensor per GPU and gradient dtype, still on the device. A gradient that
     is not finite makes the step change nothing (it still counts as a step)."""
@@ -282,7 +288,6 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.max_grad_norm = state_bits, master_weights, max_grad_norm
         self.grad_norm: list = []
         self._plans: dict = {}
-        self._versions: dict = {}  # of the parameters, as the last step left them
 
     def _state(self, p: torch.Tensor) -> dict:
         state = self.state[p]
@@ -295,9 +300,6 @@ class AdamW(torch.optim.Optimizer):
                     state[name + "_scale"] = torch.zeros(_blocks(p.numel()), dtype=torch.float32, device=p.device)
             if self.master_weights and p.dtype != torch.float32:
                 state["master"] = p.detach().to(torch.float32).contiguous()
-        elif "master" in state and self._versions.get(p, p._version) != p._version:
-            state["master"].copy_(p)
-        self._versions[p] = p._version
         return state
 
     def _plan(self, key: tuple, params: list) -> AdamWTensors:
@@ -311,7 +313,8 @@ class AdamW(torch.optim.Optimizer):
             tensors = AdamWTensors(
                 [p.detach() for p in params], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                 masters=[s["master"] for s in states] if "master" in states[0] else None,
-                scales=([s["exp_avg_scale"] for s in states], [s["exp_avg_sq_scale"] for s in states]) if eight else None)
+                scales=([s["exp_avg_scale"] for s in states], [s["exp_avg_sq_scale"] for s in states]) if eight else None,
+                follow=True)
             plan = self._plans[key] = (held, tensors)  # which keeps the tensors, so their ids stay theirs
         return plan[1]
 
@@ -344,7 +347,6 @@ class AdamW(torch.optim.Optimizer):
                 grad_scale=grad_scale if grad_scale is not None else factors.get(device))
             for p in params:
                 self.state[p]["step"] = count + 1
-                self._versions[p] = p._version
         return loss
 
     def _clip(self, sets: dict) -> dict:
@@ -366,7 +368,7 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, but states keep their own types (torch casts them to the parameter's)."""
         super().load_state_dict(state_dict)
-        self._plans, self._versions = {}, {}
+        self._plans = {}
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
         for i, p in zip(saved, params):
