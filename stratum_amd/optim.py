@@ -269,9 +269,10 @@ class AdamW(torch.optim.Optimizer):
     parameter, which takes the updates that bf16 or fp16 would round away; an element of a
     parameter that something else wrote between two steps, in place, through ``.data`` or by loading,
     is taken over into its master (the step sees that it is not the master rounded).
-    ``max_grad_norm`` clips by the norm over all parameters (of one GPU each); ``grad_norm``
-    then holds the last norms, one tensor per GPU and gradient dtype, still on the device. A gradient that
-    is not finite makes the step change nothing (it still counts as a step)."""
+    ``max_grad_norm`` clips by the norm over all parameters (of one GPU each). ``grad_norm``
+    holds the last norms, one tensor per GPU, still on the device; they are taken without clipping
+    too, since a gradient that is not finite makes the step change nothing on its GPU (it still counts as
+    a step). With a ``grad_scale`` no norm is taken and that factor alone decides."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False,
@@ -321,7 +322,8 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: Optional[torch.Tensor] = None):
         """One step. ``grad_scale`` (an fp32 scalar on the GPU, as :func:`grad_norm` leaves
-        it) multiplies the gradients, in place of ``max_grad_norm``."""
+        it) multiplies the gradients, in place of ``max_grad_norm``; a step whose factor is
+        not finite changes nothing."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -337,7 +339,7 @@ class AdamW(torch.optim.Optimizer):
                 key = (gi, p.device, p.dtype, p.grad.dtype, self._state(p)["step"])
                 sets.setdefault(key, []).append(p)
         factors: dict = {}
-        if grad_scale is None and self.max_grad_norm is not None:
+        if grad_scale is None:
             factors = self._clip(sets)
         for (gi, device, dtype, grad_dtype, count), params in sets.items():
             group = self.param_groups[gi]
@@ -350,17 +352,19 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _clip(self, sets: dict) -> dict:
-        """The clip factor of each GPU, from the norm over all its gradients."""
+        """The clip factor of each GPU, from the norm over all its gradients; 1 without clipping, and
+        NaN where the norm is not finite."""
+        most = math.inf if self.max_grad_norm is None else self.max_grad_norm
         grads: dict = {}
         for (_, device, _, grad_dtype, _), params in sets.items():
             grads.setdefault(device, {}).setdefault(grad_dtype, []).extend(p.grad for p in params)
         self.grad_norm, factors = [], {}
         for device, by_dtype in grads.items():
-            norms = [grad_norm(gs, self.max_grad_norm) for gs in by_dtype.values()]
+            norms = [grad_norm(gs, most) for gs in by_dtype.values()]
             if len(norms) == 1:
                 norm = norms[0]
             else:  # several gradient types: the norm of their norms
-                norm = grad_norm([torch.stack([n[0] for n in norms])], self.max_grad_norm)
+                norm = grad_norm([torch.stack([n[0] for n in norms])], most)
             self.grad_norm.append(norm[0])
             factors[device] = norm[1]
         return factors
