@@ -290,6 +290,15 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: list = []
         self._plans: dict = {}
 
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "state_bits": self.state_bits, "master_weights": self.master_weights,
+                "max_grad_norm": self.max_grad_norm}
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        self._plans = {}
+        self.__dict__.setdefault("grad_norm", [])
+
     def _state(self, p: torch.Tensor) -> dict:
         state = self.state[p]
         if "step" not in state:
