@@ -308,9 +308,12 @@ class AdamW(torch.optim.Optimizer):
                 state[name] = torch.zeros(p.shape, dtype=dtype, device=p.device)
                 if self.state_bits == 8:
                     state[name + "_scale"] = torch.zeros(_blocks(p.numel()), dtype=torch.float32, device=p.device)
-            if self.master_weights and p.dtype != torch.float32:
+            if self._mastered(p):
                 state["master"] = p.detach().to(torch.float32).contiguous()
         return state
+
+    def _mastered(self, p: torch.Tensor) -> bool:
+        return self.master_weights and p.dtype != torch.float32
 
     def _plan(self, key: tuple, params: list) -> AdamWTensors:
         """The checked tensor table of a group's parameters of one kind; made again when
@@ -379,12 +382,38 @@ class AdamW(torch.optim.Optimizer):
         return factors
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As torch's, but states keep their own types (torch casts them to the parameter's)."""
+        """As torch's, but states keep fp32 or their codes (torch casts them to the parameter's type). A
+        checkpoint of other settings, torch's own AdamW among them, is made one of these: its moments
+        take ``state_bits``, and masters are made from the parameters, or dropped, as ``master_weights``
+        says."""
         super().load_state_dict(state_dict)
         self._plans = {}
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
         for i, p in zip(saved, params):
             if i in state_dict["state"]:
-                self.state[p] = {name: v.detach().clone().to(p.device) if isinstance(v, torch.Tensor) else v
-                                 for name, v in state_dict["state"][i].items()}
+                self.state[p] = self._taken(p, state_dict["state"][i])
+
+    def _taken(self, p: torch.Tensor, saved: dict) -> dict:
+        """The state of *p* from a saved one of any width, with or without a master."""
+        missing = [name for name in ("step", "exp_avg", "exp_avg_sq") if name not in saved]
+        if missing:
+            raise ValueError(f"not the state of an AdamW: {', '.join(missing)} missing")
+        state = {"step": int(saved["step"])}
+        for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+            value, scale = saved[name].detach(), saved.get(name + "_scale")
+            if value.numel() != p.numel():
+                raise ValueError(f"{name} has {value.numel()} elements, its parameter {p.numel()}")
+            if self.state_bits == 8 and scale is not None:
+                state[name] = value.to(p.device, copy=True).contiguous()
+                state[name + "_scale"] = scale.detach().to(p.device, copy=True).contiguous()
+            elif self.state_bits == 8:
+                state[name], state[name + "_scale"] = state_codes(value.to(p.device), signed=signed)
+            elif scale is not None:
+                state[name] = state_values(value.to(p.device), scale.detach().to(p.device), signed=signed)
+            else:
+                state[name] = value.to(p.device, torch.float32, copy=True).contiguous()
+        if self._mastered(p):
+            master = saved["master"].detach() if "master" in saved else p.detach()
+            state["master"] = master.to(p.device, torch.float32, copy=True).contiguous()
+        return state

@@ -41,3 +41,51 @@ def test_a_copied_optimizer_goes_on_with_the_same_bits(cuda, bits, way):
     run(other, qs, range(3, 6))
     assert all(p.data_ptr() != q.data_ptr() and torch.equal(p, q) for p, q in zip(ps, qs))
     assert all(torch.equal(opt.state[p]["master"], other.state[q]["master"]) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("masters", [(False, True), (True, False), (True, True)])
+@pytest.mark.parametrize("bits", [(32, 8), (8, 32)])
+def test_a_checkpoint_of_the_other_width(cuda, bits, masters):
+    """The moments become the nearest codes, or the values that the codes stand for, and training goes on."""
+    from stratum_amd.optim import AdamW, state_codes, state_values
+    ps, qs = params(1), params(1)
+    first = AdamW(ps, lr=1e-2, state_bits=bits[0], master_weights=masters[0])
+    second = AdamW(qs, lr=1e-2, state_bits=bits[1], master_weights=masters[1])
+    run(first, ps, range(3))
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+    second.load_state_dict(first.state_dict())
+    for p, q in zip(ps, qs):
+        a, b = first.state[p], second.state[q]
+        for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+            if bits[1] == 8:
+                codes, scales = state_codes(a[name], signed=signed)
+                assert torch.equal(b[name], codes) and torch.equal(b[name + "_scale"], scales)
+            else:
+                want = state_values(a[name], a[name + "_scale"], signed=signed)
+                assert torch.equal(b[name], want) and name + "_scale" not in b
+        assert ("master" in b) == masters[1]
+        if masters == (True, True):
+            assert torch.equal(a["master"], b["master"])
+    run(second, qs, range(3, 5))
+    assert all(second.state[q]["step"] == 5 and torch.isfinite(q).all() for q in qs)
+    assert all(not torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("masters", [True, False])
+def test_a_checkpoint_of_torchs_adamw_goes_on(cuda, masters):
+    """Three steps of torch's AdamW in fp32, then one here: within fp32 rounding of its fourth."""
+    from stratum_amd.optim import AdamW
+    ps, qs = params(2, torch.float32), params(2, torch.float32)
+    first, second = torch.optim.AdamW(ps, lr=1e-2), AdamW(qs, lr=0.5, master_weights=masters)
+    run(first, ps, range(3))
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+    second.load_state_dict(first.state_dict())
+    run(first, ps, [3])
+    run(second, qs, [3])
+    # an update of at most 3.2 lr with 20 roundings here and as many there, 3 of the parameter each
+    u = 2.0 ** -24
+    assert all(((p - q).abs() <= 40 * u * 3.2e-2 + 6 * u * p.abs()).all() for p, q in zip(ps, qs))

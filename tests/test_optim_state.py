@@ -60,3 +60,68 @@ def test_a_copied_optimizer_keeps_its_settings_and_steps(on_cpu, bits, masters, 
         assert (q == 1.0 - 0.25 * (steps + 1)).all() and (p == 1.0 - 0.25 * steps).all()
         assert other.state[q]["step"] == steps + 1 and set(other.state[q]) >= {"exp_avg", "exp_avg_sq"}
         assert ("master" in other.state[q]) == masters and ("exp_avg_scale" in other.state[q]) == (bits == 8)
+
+
+def test_a_checkpoint_without_masters_gets_them(on_cpu):
+    p, q = parameter(300, torch.bfloat16), parameter(300, torch.bfloat16)
+    opt, other = optim.AdamW([p], lr=0.25), optim.AdamW([q], lr=0.25, master_weights=True)
+    opt.step()
+    with torch.no_grad():
+        q.copy_(p)
+    other.load_state_dict(opt.state_dict())
+    master = other.state[q]["master"]
+    assert master.dtype == torch.float32 and torch.equal(master, p.detach().float())
+    master.zero_()
+    assert (q == 0.75).all()
+    # a parameter that joins later has one too, in the same set of tensors
+    late = parameter(5, torch.bfloat16)
+    other.add_param_group({"params": [late]})
+    other.step()
+    assert "master" in other.state[late]
+
+
+def test_a_checkpoint_with_masters_loses_them_where_none_are_kept(on_cpu):
+    p, q = parameter(300, torch.bfloat16), parameter(300, torch.bfloat16)
+    opt, other = optim.AdamW([p], master_weights=True), optim.AdamW([q])
+    opt.step()
+    other.load_state_dict(opt.state_dict())
+    assert "master" not in other.state[q]
+    other.step()
+
+
+def test_a_checkpoint_of_torchs_adamw(on_cpu):
+    p, q = parameter(300, torch.bfloat16), parameter(300, torch.bfloat16)
+    opt, other = torch.optim.AdamW([p], lr=0.125), optim.AdamW([q], master_weights=True)
+    for _ in range(3):
+        opt.step()
+    other.load_state_dict(opt.state_dict())
+    state = other.state[q]
+    assert state["step"] == 3 and type(state["step"]) is int
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert state[name].dtype == torch.float32 and torch.equal(state[name], opt.state[p][name].float())
+    assert other.param_groups[0]["lr"] == 0.125
+    other.step()
+    assert other.state[q]["step"] == 4
+
+
+def test_what_is_no_state_of_an_adamw_is_refused(on_cpu):
+    p, q = parameter(), parameter()
+    sgd = torch.optim.SGD([p], lr=0.1, momentum=0.9)
+    sgd.step()
+    with pytest.raises(ValueError, match="exp_avg"):
+        optim.AdamW([q]).load_state_dict(sgd.state_dict())
+    good = optim.AdamW([p])
+    good.step()
+    with pytest.raises(ValueError, match="elements"):
+        optim.AdamW([parameter(11)]).load_state_dict(good.state_dict())
+
+
+def test_loaded_states_are_copies(on_cpu):
+    p, q = parameter(300, torch.bfloat16), parameter(300, torch.bfloat16)
+    opt, other = (optim.AdamW([x], state_bits=8, master_weights=True) for x in (p, q))
+    opt.step()
+    other.load_state_dict(opt.state_dict())
+    for name, t in opt.state[p].items():
+        if name != "step":
+            assert t.data_ptr() != other.state[q][name].data_ptr() and torch.equal(t, other.state[q][name])
+            assert t.dtype == other.state[q][name].dtype
