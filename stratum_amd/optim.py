@@ -386,7 +386,13 @@ class AdamW(torch.optim.Optimizer):
         checkpoint of other settings, torch's own AdamW among them, is made one of these: its moments
         take ``state_bits``, and masters are made from the parameters, or dropped, as ``master_weights``
         says."""
-        super().load_state_dict(state_dict)
+        loaded: dict = {}  # what the hooks before loading leave of it
+        last = self.register_load_state_dict_pre_hook(lambda _, given: loaded.update(given))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
+        state_dict = loaded
         self._plans = {}
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]

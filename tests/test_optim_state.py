@@ -125,3 +125,17 @@ def test_loaded_states_are_copies(on_cpu):
         if name != "step":
             assert t.data_ptr() != other.state[q][name].data_ptr() and torch.equal(t, other.state[q][name])
             assert t.dtype == other.state[q][name].dtype
+
+
+def test_a_hook_before_loading_changes_what_is_loaded(on_cpu):
+    p, q = parameter(), parameter()
+    opt, other = optim.AdamW([p]), optim.AdamW([q])
+    opt.step()
+
+    def hook(_, given):
+        return {**given, "state": {i: {**s, "exp_avg": torch.full_like(s["exp_avg"], 7.0)} for i, s in given["state"].items()}}
+    other.register_load_state_dict_pre_hook(hook)
+    for _ in range(2):
+        other.load_state_dict(opt.state_dict())
+        assert (other.state[q]["exp_avg"] == 7.0).all()
+    assert len(other._optimizer_load_state_dict_pre_hooks) == 1
