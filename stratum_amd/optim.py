@@ -316,9 +316,9 @@ class AdamW(torch.optim.Optimizer):
         return self.master_weights and p.dtype != torch.float32
 
     def _plan(self, key: tuple, params: list) -> AdamWTensors:
-        """The checked tensor table of a group's parameters of one kind; made again when
+        """The checked tensor table of one set of a step's tensors; made again when
         one of them is no longer the same tensor or has moved."""
-        states = [self._state(p) for p in params]
+        states = [self.state[p] for p in params]
         held = [id(t) for s in states for name, t in s.items() if name != "step"]
         plan = self._plans.get(key)
         if plan is None or plan[0] != held or plan[1].at() != [p.data_ptr() for p in params]:
@@ -340,7 +340,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # the tensors of one launch: one group, device, types and step number
+        # the tensors of one launch: one group, device, types, with masters or without, and step number
         sets: dict = {}
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
@@ -348,14 +348,18 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if p.grad.is_sparse:
                     raise ValueError("AdamW does not take sparse gradients")
-                key = (gi, p.device, p.dtype, p.grad.dtype, self._state(p)["step"])
+                state = self._state(p)
+                key = (gi, p.device, p.dtype, p.grad.dtype, "master" in state, state["step"])
                 sets.setdefault(key, []).append(p)
         factors: dict = {}
         if grad_scale is None:
             factors = self._clip(sets)
-        for (gi, device, dtype, grad_dtype, count), params in sets.items():
-            group = self.param_groups[gi]
-            self._plan((gi, device, dtype, grad_dtype), params).step(
+        alike: dict = {}  # sets that differ in their step number alone, so far
+        for (*kind, count), params in sets.items():
+            gi, device, kind = kind[0], kind[1], tuple(kind)
+            group, place = self.param_groups[gi], alike.setdefault(kind, 0)
+            alike[kind] = place + 1
+            self._plan((kind, place), params).step(
                 [p.grad for p in params], step=count + 1, lr=float(group["lr"]), betas=group["betas"],
                 eps=group["eps"], weight_decay=group["weight_decay"],
                 grad_scale=grad_scale if grad_scale is not None else factors.get(device))
@@ -368,7 +372,7 @@ class AdamW(torch.optim.Optimizer):
         NaN where the norm is not finite."""
         most = math.inf if self.max_grad_norm is None else self.max_grad_norm
         grads: dict = {}
-        for (_, device, _, grad_dtype, _), params in sets.items():
+        for (_, device, _, grad_dtype, _, _), params in sets.items():
             grads.setdefault(device, {}).setdefault(grad_dtype, []).extend(p.grad for p in params)
         self.grad_norm, factors = [], {}
         for device, by_dtype in grads.items():

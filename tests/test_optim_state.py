@@ -13,10 +13,13 @@ optim = importlib.import_module("stratum_amd.optim")
 
 class Tensors:
     """Stands for AdamWTensors: counts what is built and stepped, and moves the parameters by lr."""
-    built = 0
+    built, newest = 0, []
 
     def __init__(self, params, exp_avgs, exp_avg_sqs, *, masters=None, scales=None, follow=False):
         type(self).built += 1
+        assert masters is None or len(masters) == len(params)
+        self.kept = None if masters is None else [m.data_ptr() for m in masters]
+        type(self).newest.append(self)
         self.params, self.masters, self.scales = params, masters, scales
 
     def at(self):
@@ -32,6 +35,7 @@ def on_cpu(monkeypatch):
     monkeypatch.setattr(optim, "AdamWTensors", Tensors)
     monkeypatch.setattr(optim, "grad_norm", lambda grads, most: torch.tensor([1.0, 1.0]))
     Tensors.built = 0
+    Tensors.newest.clear()
 
 
 def parameter(n=10, dtype=torch.float32):
@@ -139,3 +143,32 @@ def test_a_hook_before_loading_changes_what_is_loaded(on_cpu):
         other.load_state_dict(opt.state_dict())
         assert (other.state[q]["exp_avg"] == 7.0).all()
     assert len(other._optimizer_load_state_dict_pre_hooks) == 1
+
+
+def test_sets_that_differ_in_their_step_count_keep_their_plans(on_cpu):
+    early, late = parameter(), parameter()
+    opt = optim.AdamW([early, late], lr=0.25)
+    late.grad = None
+    opt.step()
+    late.grad = torch.ones_like(late)
+    opt.step()
+    before = Tensors.built
+    for _ in range(5):
+        opt.step()
+    assert Tensors.built == before
+    assert (opt.state[early]["step"], opt.state[late]["step"]) == (7, 6)
+    assert (early == 1 - 7 * 0.25).all() and (late == 1 - 6 * 0.25).all()
+
+
+def test_masters_switched_on_later_stand_apart_from_states_without(on_cpu):
+    p, q = (parameter(4, torch.bfloat16) for _ in range(2))
+    opt = optim.AdamW([p], lr=0.25)
+    opt.step()
+    opt.master_weights = True
+    opt.add_param_group({"params": [q]})
+    opt.param_groups[0]["params"].append(opt.param_groups.pop()["params"][0])
+    opt.state[p]["step"] = 0
+    opt.step()
+    assert "master" in opt.state[q] and "master" not in opt.state[p]
+    assert (p == 0.5).all() and (q == 0.75).all()
+    assert [opt.state[q]["master"].data_ptr()] in [t.kept for t in Tensors.newest]  # the step writes it
