@@ -367,7 +367,8 @@ int stm_nf4_dequantize_aug(const uint8_t* packed, const float* absmax, const voi
  *   state_bits, an element of `param` that is not its master rounded (something else has written
  *   it) replaces the master before the step; without it `param` is not read where there is a master.
  *   Any element-aligned pointers; 16-byte aligned ones (8 for 8-bit codes) are faster.
- *   `tensors` is a host array, read before the call returns.
+ *   `tensors` is a host array, read before the call returns. All numbers are arguments of the launch: a
+ *   captured step repeats its lr, step and bias corrections on every replay; *grad_scale is read anew.
  *
  * stm_state8_codes / stm_state8_values: fp32 values to codes and scales, and back.
  *   A block of 256 elements has its largest magnitude as scale. A code is a sign bit

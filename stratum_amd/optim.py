@@ -141,7 +141,9 @@ class AdamWTensors:
         """Step number ``step`` (from 1) with one gradient per parameter, of one dtype; a
         tensor whose gradient is None stays as it is. ``grad_scale``, an fp32 scalar on the GPU, multiplies the
         gradients first (``grad_norm(...)[1]``); where it is not finite the step writes nothing.
-        Runs on the current stream, without synchronising."""
+        Runs on the current stream, without synchronising. Captured into a graph, a replay repeats
+        these numbers: the rate, the step number and its bias corrections are part of the launch,
+        and only what lies on the GPU (gradients, ``grad_scale``) is read anew."""
         if len(grads) != len(self._sizes):
             raise ValueError(f"{len(self._sizes)} parameters, but {len(grads)} gradients")
         if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
@@ -335,7 +337,8 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None, *, grad_scale: Optional[torch.Tensor] = None):
         """One step. ``grad_scale`` (an fp32 scalar on the GPU, as :func:`grad_norm` leaves
         it) multiplies the gradients, in place of ``max_grad_norm``; a step whose factor is
-        not finite changes nothing."""
+        not finite changes nothing. A captured step repeats its own rate and step number on every
+        replay (:meth:`AdamWTensors.step`) and counts once."""
         loss = None
         if closure is not None:
             with torch.enable_grad():

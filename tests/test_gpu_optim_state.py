@@ -89,3 +89,27 @@ def test_a_checkpoint_of_torchs_adamw_goes_on(cuda, masters):
     # an update of at most 3.2 lr with 20 roundings here and as many there, 3 of the parameter each
     u = 2.0 ** -24
     assert all(((p - q).abs() <= 40 * u * 3.2e-2 + 6 * u * p.abs()).all() for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_repeats_its_numbers(cuda, bits):
+    """Replays of the optimizer's third step against eager steps of the number three; it counts once."""
+    from stratum_amd.optim import AdamW, AdamWTensors
+    ps = params(3, torch.float32)
+    opt = AdamW(ps, lr=1e-2, state_bits=bits)
+    run(opt, ps, range(2))
+    mine = [p.detach().clone() for p in ps]
+    names = ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if bits == 8 else ())
+    m, v, *scales = ([opt.state[p][name].clone() for p in ps] for name in names)
+    tensors = AdamWTensors(mine, m, v, scales=tuple(scales) or None)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        for p in ps:
+            p.grad.mul_(-0.7)
+        graph.replay()
+        tensors.step([p.grad for p in ps], step=3, lr=1e-2, grad_scale=torch.ones((), device=cuda))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, mine))
+    assert all(opt.state[p]["step"] == 3 for p in ps)
