@@ -397,8 +397,9 @@ int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int param_dtype, 
                    double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
                    const float* grad_scale, void* stream);
 /*
- * stm_adamw_step with the list in device memory, one launch for any number of tensors
- * (stm_adamw_step makes one per 56): stm_adamw_fill_table checks a list and writes
+ * stm_adamw_step with the list in device memory, one launch for any number of tensors (stm_adamw_step
+ * makes one per 56) of up to 2^24 - 1 work-groups of 1024 elements (8-bit states: 2048; above that
+ * fill_table returns STM_ERR_UNSUPPORTED, and stm_adamw_step makes several launches): stm_adamw_fill_table checks a list and writes
  * stm_adamw_table_bytes(count) bytes of table to host memory (8-byte aligned) and returns
  * the launch's work-groups (or a negative status); the caller copies them to the device
  * on `stream` and passes them with the same count, types and state_bits.

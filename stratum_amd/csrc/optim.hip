@@ -548,7 +548,10 @@ bool valid_dtype(int dt) { return dt == STM_F16 || dt == STM_BF16 || dt == STM_F
 
 using namespace stm;
 
-constexpr int64_t kMostGroups = 0x3FFFFFFF;  // work-groups of a launch
+// Work-groups of a launch: HIP takes fewer than 2^32 threads. What needs more goes in several launches.
+constexpr int64_t most_groups(int threads) { return ((int64_t)1 << 32) / threads - 1; }
+constexpr int64_t kMostGroups = most_groups(256);  // of a step and of the conversions
+constexpr int64_t kMostElements = (int64_t)1 << 48;
 
 static int adamw_kind(int param_dtype, int grad_dtype, int state_bits, AdamKind& k) {
     if (!valid_dtype(param_dtype) || !valid_dtype(grad_dtype))
@@ -561,7 +564,6 @@ static int adamw_kind(int param_dtype, int grad_dtype, int state_bits, AdamKind&
 
 static int check_adamw_tensors(int count, const stm_adamw_tensor* tensors, const AdamKind& k) {
     if (count < 0 || (count && !tensors)) return set_error(STM_ERR_INVALID, "adamw_step: bad tensor list");
-    const int64_t tile = tile_of(k.bits);
     for (int i = 0; i < count; ++i) {
         const stm_adamw_tensor& t = tensors[i];
         if (t.n < 0) return set_error(STM_ERR_INVALID, "adamw_step: tensor %d has a negative size", i);
@@ -574,7 +576,7 @@ static int check_adamw_tensors(int count, const stm_adamw_tensor* tensors, const
         if (!aligned(t.param, pa) || !aligned(t.grad, ga) || !aligned(t.master, 4) || !aligned(t.exp_avg, sa) ||
             !aligned(t.exp_avg_sq, sa) || !aligned(t.exp_avg_scale, 4) || !aligned(t.exp_avg_sq_scale, 4))
             return set_error(STM_ERR_INVALID, "adamw_step: tensor %d is not aligned to its elements", i);
-        if ((t.n + tile - 1) / tile > kMostGroups)
+        if (t.n > kMostElements)
             return set_error(STM_ERR_UNSUPPORTED, "adamw_step: tensor %d is too large", i);
     }
     return STM_OK;
@@ -597,6 +599,16 @@ static int adamw_numbers(double lr, double beta1, double beta2, double eps, doub
     return STM_OK;
 }
 
+// Elements [start, start + n) of a tensor, start a multiple of a tile's elements.
+static stm_adamw_tensor piece_of(const stm_adamw_tensor& t, int64_t start, int64_t n, const AdamKind& k) {
+    auto at = [&](const void* p, int bytes) { return (void*)((uintptr_t)p + (uintptr_t)(start * bytes)); };
+    auto floats = [&](float* p, int64_t i) { return p ? p + i : nullptr; };
+    const int state = k.bits == 32 ? 4 : 1;
+    return {at(t.param, k.param_dtype == STM_F32 ? 4 : 2), at(t.grad, k.grad_dtype == STM_F32 ? 4 : 2),
+            floats(t.master, start), at(t.exp_avg, state), at(t.exp_avg_sq, state),
+            floats(t.exp_avg_scale, start / kBlock8), floats(t.exp_avg_sq_scale, start / kBlock8), n};
+}
+
 extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int param_dtype, int grad_dtype,
                               int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay,
                               int64_t step, const float* grad_scale, void* stream) {
@@ -607,18 +619,21 @@ extern "C" int stm_adamw_step(int count, const stm_adamw_tensor* tensors, int pa
     if (rc == STM_OK) rc = check_adamw_tensors(count, tensors, k);
     if (rc != STM_OK) return rc;
     const int64_t tile = tile_of(k.bits);
+    int64_t done = 0;  // tiles of tensor i that earlier launches hold
     for (int i = 0; i < count;) {
         a.count = 0;
         int64_t groups = 0;
-        while (i < count && a.count < kAdamTensors) {
-            const int64_t g = (tensors[i].n + tile - 1) / tile;
-            if (groups + g > kMostGroups) break;
+        while (i < count && a.count < kAdamTensors && groups < kMostGroups) {
+            const int64_t all = (tensors[i].n + tile - 1) / tile, left = all - done;
+            const int64_t g = left < kMostGroups - groups ? left : kMostGroups - groups;
             if (g) {
-                a.t[a.count] = tensors[i];
+                const int64_t start = done * tile, rest = tensors[i].n - start;
+                a.t[a.count] = piece_of(tensors[i], start, rest < g * tile ? rest : g * tile, k);
                 a.first[a.count++] = (int)groups;
                 groups += g;
+                done += g;
             }
-            ++i;
+            if (done == all) ++i, done = 0;
         }
         if (!groups) continue;
         rc = launch_adamw(a, k, groups, (hipStream_t)stream);
@@ -676,14 +691,15 @@ extern "C" int stm_state8_values(const uint8_t* codes, const float* scales, int6
     if (!codes || !scales || !out) return set_error(STM_ERR_INVALID, "state8_values: null pointer");
     if (!aligned(scales, 4) || !aligned(out, 4)) return set_error(STM_ERR_INVALID, "state8_values: unaligned fp32");
     const int vec = aligned(codes, 4) && aligned(out, 16);
-    const int64_t tiles = (n + kTile - 1) / kTile;
-    if (tiles > 0x3FFFFFFF) return set_error(STM_ERR_UNSUPPORTED, "state8: %lld elements", (long long)n);
-    const dim3 grid((unsigned)tiles);
-    if (is_signed)
-        hipLaunchKernelGGL(k_state_values<true>, grid, dim3(256), 0, (hipStream_t)stream, codes, scales, n, out, vec);
-    else
-        hipLaunchKernelGGL(k_state_values<false>, grid, dim3(256), 0, (hipStream_t)stream, codes, scales, n, out, vec);
-    return check_launch("state8_values");
+    auto* kernel = is_signed ? k_state_values<true> : k_state_values<false>;
+    for (int64_t i = 0; i < n; i += kMostGroups * kTile) {
+        const int64_t m = n - i < kMostGroups * kTile ? n - i : kMostGroups * kTile;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((m + kTile - 1) / kTile)), dim3(256), 0, (hipStream_t)stream, codes + i,
+                           scales + i / kBlock8, m, out + i, vec);
+        const int rc = check_launch("state8_values");
+        if (rc != STM_OK) return rc;
+    }
+    return STM_OK;
 }
 
 extern "C" int stm_state8_codes(const float* x, int64_t n, int is_signed, uint8_t* codes, float* scales,
@@ -693,14 +709,15 @@ extern "C" int stm_state8_codes(const float* x, int64_t n, int is_signed, uint8_
     if (!codes || !scales || !x) return set_error(STM_ERR_INVALID, "state8_codes: null pointer");
     if (!aligned(scales, 4) || !aligned(x, 4)) return set_error(STM_ERR_INVALID, "state8_codes: unaligned fp32");
     const int vec = aligned(codes, 4) && aligned(x, 16);
-    const int64_t tiles = (n + kTile - 1) / kTile;
-    if (tiles > 0x3FFFFFFF) return set_error(STM_ERR_UNSUPPORTED, "state8: %lld elements", (long long)n);
-    const dim3 grid((unsigned)tiles);
-    if (is_signed)
-        hipLaunchKernelGGL(k_state_codes<true>, grid, dim3(256), 0, (hipStream_t)stream, x, n, codes, scales, vec);
-    else
-        hipLaunchKernelGGL(k_state_codes<false>, grid, dim3(256), 0, (hipStream_t)stream, x, n, codes, scales, vec);
-    return check_launch("state8_codes");
+    auto* kernel = is_signed ? k_state_codes<true> : k_state_codes<false>;
+    for (int64_t i = 0; i < n; i += kMostGroups * kTile) {
+        const int64_t m = n - i < kMostGroups * kTile ? n - i : kMostGroups * kTile;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((m + kTile - 1) / kTile)), dim3(256), 0, (hipStream_t)stream, x + i, m,
+                           codes + i, scales + i / kBlock8, vec);
+        const int rc = check_launch("state8_codes");
+        if (rc != STM_OK) return rc;
+    }
+    return STM_OK;
 }
 
 extern "C" int64_t stm_grad_norm_workspace_bytes(int count, const int64_t* n) {
@@ -728,7 +745,7 @@ extern "C" int stm_grad_norm(int count, const void* const* grads, const int64_t*
         if (n[i] == 0) continue;
         if (!grads[i] || !aligned(grads[i], dtype == STM_F32 ? 4 : 2))
             return set_error(STM_ERR_INVALID, "grad_norm: tensor %d is null or not aligned to its elements", i);
-        if (norm_groups(n[i]) > 0x3FFFFFFF) return set_error(STM_ERR_UNSUPPORTED, "grad_norm: tensor %d is too large", i);
+        if (norm_groups(n[i]) > most_groups(kNormThreads)) return set_error(STM_ERR_UNSUPPORTED, "grad_norm: tensor %d is too large", i);
     }
     double* partial = (double*)workspace;
     NormArgs a;
@@ -737,7 +754,7 @@ extern "C" int stm_grad_norm(int count, const void* const* grads, const int64_t*
         int64_t groups = 0;
         while (i < count && a.count < kNormTensors) {
             const int64_t g = norm_groups(n[i]);
-            if (groups + g > 0x3FFFFFFF) break;
+            if (groups + g > most_groups(kNormThreads)) break;
             if (g) {
                 a.g[a.count] = grads[i];
                 a.last[a.count] = (int)(n[i] - (g - 1) * kNormTile);

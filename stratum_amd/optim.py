@@ -179,7 +179,9 @@ class AdamWTensors:
             else:
                 host = torch.empty(lib.stm_adamw_table_bytes(n), dtype=torch.uint8, pin_memory=True)
                 rc = lib.stm_adamw_fill_table(n, rows, *types, host.data_ptr())
-                if rc >= 0:  # the caching host allocator keeps the pinned block until the copy has run
+                if rc == _lib.STM_ERR_UNSUPPORTED:  # more elements than one launch takes
+                    rc = lib.stm_adamw_step(n, rows, *types, *numbers, stream)
+                elif rc >= 0:  # the caching host allocator keeps the pinned block until the copy has run
                     held = host.to(self.device, non_blocking=True)
                     rc = lib.stm_adamw_step_table(n, held.data_ptr(), rc, *types, *numbers, stream)
         _lib.check(rc, "stm_adamw_step")

@@ -113,3 +113,25 @@ def test_a_captured_step_repeats_its_numbers(cuda, bits):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(ps, mine))
     assert all(opt.state[p]["step"] == 3 for p in ps)
+
+
+def test_a_tensor_of_more_threads_than_one_launch_takes(cuda):
+    """2^24 tiles of 1024 elements and some more: two launches. The elements around their seam."""
+    from stratum_amd.optim import AdamWTensors
+    seam, n = ((1 << 24) - 1) * 1024, (1 << 24) * 1024 + 5001
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 13 * n:  # 2 + 2 + 4 + 4 bytes an element
+        pytest.skip("takes 206 GB")
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    m, v = (torch.zeros(n, device=cuda) for _ in range(2))
+    spots = torch.tensor([0, 1 << 32, seam - 1, seam, seam + 1, seam + 1024, n - 1], device=cuda)
+    g[spots] = torch.tensor([1., -2., 3., -4., 5., -6., 7.], dtype=torch.bfloat16, device=cuda)
+    AdamWTensors([p], [m], [v]).step([g], step=1, lr=0.125, weight_decay=0.0)
+    want = torch.tensor([-0.125, 0.125] * 3 + [-0.125], dtype=torch.bfloat16, device=cuda)  # lr sign(g)
+    assert torch.equal(p[spots], want)
+    around = seam - (1 << 20)
+    assert int((p[:1 << 20] != 0).sum()) == 1
+    for t in (p, m, v):  # the five spots of the last stretch, and nothing else there
+        assert int((t[around:] != 0).sum()) == 5
+    del p, g, m, v, t
+    torch.cuda.empty_cache()

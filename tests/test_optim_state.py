@@ -2,11 +2,15 @@
 stand-in for the GPU's step where one is taken."""
 
 import copy
+import ctypes
 import importlib
 import pickle
 
+import numpy as np
 import pytest
 import torch
+
+from stratum_amd import _lib
 
 optim = importlib.import_module("stratum_amd.optim")
 
@@ -172,3 +176,38 @@ def test_masters_switched_on_later_stand_apart_from_states_without(on_cpu):
     assert "master" in opt.state[q] and "master" not in opt.state[p]
     assert (p == 0.5).all() and (q == 0.75).all()
     assert [opt.state[q]["master"].data_ptr()] in [t.kept for t in Tensors.newest]  # the step writes it
+
+
+# ------------------------------------------------------------------ launches of 2^32 threads and more
+
+def row(n, where):
+    return np.array([[where] * 2 + [0] + [where] * 4 + [n]], np.int64)
+
+
+@pytest.mark.parametrize("bits,tile", [(32, 1024), (8, 2048)])
+def test_a_table_holds_no_more_work_groups_than_a_launch_takes(bits, tile):
+    L = _lib.lib()
+    where = ctypes.addressof(ctypes.create_string_buffer(64)) // 16 * 16 + 16  # never read: the table is only filled
+    table = ctypes.create_string_buffer(2 * 128)
+    most = (1 << 24) - 1  # groups of 256 threads below 2^32 threads
+
+    def fill(*sizes):
+        rows = np.concatenate([row(n, where) for n in sizes])
+        return L.stm_adamw_fill_table(len(sizes), rows.ctypes.data, 1, 1, bits, ctypes.addressof(table) + 15 & ~15)
+    assert fill(most * tile) == most
+    assert fill(most * tile + 1) == _lib.STM_ERR_UNSUPPORTED
+    assert fill((most - 1) * tile, tile) == most
+    assert fill((most - 1) * tile, tile + 1) == _lib.STM_ERR_UNSUPPORTED
+
+    def step(groups):
+        return L.stm_adamw_step_table(1, where, groups, 1, 1, bits, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None, None)
+    assert step(most + 1) == _lib.STM_ERR_INVALID and step(0) == 0
+
+
+def test_a_norm_refuses_a_tensor_of_more_work_groups_than_a_launch_takes():
+    L = _lib.lib()
+    where = ctypes.addressof(ctypes.create_string_buffer(64)) // 16 * 16 + 16
+    most = (1 << 23) - 1  # groups of 512 threads
+    one, n = np.array([where], np.int64), np.array([most * 16384 + 1], np.int64)
+    assert L.stm_grad_norm(1, one.ctypes.data, n.ctypes.data, 1, 1.0, 1.0, where, where, 1 << 40,
+                           None) == _lib.STM_ERR_UNSUPPORTED
