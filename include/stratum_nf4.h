@@ -275,12 +275,15 @@ int stm_swiglu_bwd(const void* grad_out, const void* gate_up, void* grad_gate_up
  * stm_nf4_gemm_bwd_dx of dGU against the same weight. W is dequantized as by
  * stm_nf4_dequantize; fp32 sums and gating, one rounding of each output.
  *   X [M, K], H / dH [M, I], dGU [M, 2 I]: row-major, dtype STM_BF16 or STM_F16
- *   workspace   : stm_nf4_gated_workspace_bytes(M, I, K) bytes, 16-byte aligned (NULL where that is 0)
+ *   workspace   : stm_nf4_gated_workspace_bytes(M, I, K) bytes, 16-byte aligned (NULL where that is 0), enough for
+ *                 every direction; fwd_keep alone takes stm_nf4_gated_keep_workspace_bytes(M, I, K), which
+ *                 for many rows, where the others hold the dequantized weight, is less
  *   sums        : stm_nf4_gated_sums_bytes(M, I, K) bytes, 16-byte aligned; where that is 0 (few rows: reading
  *                 the weight again costs as little), fwd_keep is refused
  *   constraints : K % 64 == 0, K % blocksize == 0, K > 0, I % 8 == 0, pointers 16-byte aligned
  */
 int64_t stm_nf4_gated_workspace_bytes(int64_t M, int64_t I, int64_t K);
+int64_t stm_nf4_gated_keep_workspace_bytes(int64_t M, int64_t I, int64_t K);
 int stm_nf4_gated_fwd(const void* X, const uint8_t* packed, const float* absmax, void* H, int64_t M, int64_t I,
                       int64_t K, int blocksize, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 int stm_nf4_gated_bwd(const void* dH, const void* X, const uint8_t* packed, const float* absmax, void* dGU, int64_t M,

@@ -54,6 +54,7 @@ SIGNATURES = {
     "stm_swiglu_fwd": ([_P, _P, _I64, _I64, _I, _P], _I),
     "stm_swiglu_bwd": ([_P, _P, _P, _I64, _I64, _I, _P], _I),
     "stm_nf4_gated_workspace_bytes": ([_I64, _I64, _I64], _I64),
+    "stm_nf4_gated_keep_workspace_bytes": ([_I64, _I64, _I64], _I64),
     "stm_nf4_gated_fwd": ([_P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
     "stm_nf4_gated_bwd": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
     "stm_nf4_gated_sums_bytes": ([_I64, _I64, _I64], _I64),

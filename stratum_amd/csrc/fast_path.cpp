@@ -196,13 +196,15 @@ at::Tensor shaped(const at::Tensor& x, int64_t width) {
     return at::empty(shape, x.options().requires_grad(false));
 }
 
-// gated_fwd(function, workspace function, keeping function, sums function, x, packed, absmax, N, K, blocksize, stream)
+// gated_fwd(function, workspace function, keeping function, sums function, keeping workspace function, x, packed, absmax,
+//           N, K, blocksize, stream)
 //   -> h, or with a sums function (not 0) (h, the kept sums or None); None where the operands are not in the
 //   plain form (the Python layer copies or refuses them); a status if the call failed.
 PyObject* gated_fwd(PyObject*, PyObject* args) {
-    long long fn, ws_fn, keep_fn, sums_fn, N, K, bs, stream;
+    long long fn, ws_fn, keep_fn, sums_fn, keep_ws_fn, N, K, bs, stream;
     PyObject *px, *pq, *pa;
-    if (!PyArg_ParseTuple(args, "LLLLOOOLLLL", &fn, &ws_fn, &keep_fn, &sums_fn, &px, &pq, &pa, &N, &K, &bs, &stream))
+    if (!PyArg_ParseTuple(args, "LLLLLOOOLLLL", &fn, &ws_fn, &keep_fn, &sums_fn, &keep_ws_fn, &px, &pq, &pa, &N, &K, &bs,
+                          &stream))
         return nullptr;
     try {
         Weight w;
@@ -212,8 +214,8 @@ PyObject* gated_fwd(PyObject*, PyObject* args) {
         const int tag = dtype_tag(x.scalar_type());
         if ((tag != STM_BF16 && tag != STM_F16) || !rows_of(x, device, K)) Py_RETURN_NONE;
         const int64_t M = x.numel() / K, inter = N / 2;
-        const int64_t bytes = reinterpret_cast<GatedBytes>(ws_fn)(M, inter, K);
         const int64_t kept = sums_fn ? reinterpret_cast<GatedBytes>(sums_fn)(M, inter, K) : 0;
+        const int64_t bytes = reinterpret_cast<GatedBytes>(kept ? keep_ws_fn : ws_fn)(M, inter, K);
         if (bytes < 0 || kept < 0) return PyLong_FromLongLong(bytes < 0 ? bytes : kept);
         at::Tensor h = shaped(x, inter), ws, sums;
         if (bytes) ws = bytes_on(bytes, x);

@@ -409,7 +409,14 @@ int stm_nf4_gemm_bwd_dx(const void* dY, const uint8_t* packed, const float* absm
 int64_t stm_nf4_gated_workspace_bytes(int64_t M, int64_t I, int64_t K) {
     g_err[0] = 0;
     if (M < 0 || I < 0 || K < 0) return set_error(STM_ERR_INVALID, "gated_workspace_bytes: negative size");
-    return gated_workspace_bytes(M, I, K);
+    const int64_t plain = gated_workspace_bytes(M, I, K, 1), keep = gated_workspace_bytes(M, I, K, 3);
+    return plain > keep ? plain : keep;
+}
+
+int64_t stm_nf4_gated_keep_workspace_bytes(int64_t M, int64_t I, int64_t K) {
+    g_err[0] = 0;
+    if (M < 0 || I < 0 || K < 0) return set_error(STM_ERR_INVALID, "gated_keep_workspace_bytes: negative size");
+    return gated_workspace_bytes(M, I, K, 3);
 }
 
 // Every direction of the gated block: dH for the backward, sums for the forward that keeps them.
@@ -431,7 +438,7 @@ static int gated(const char* who, const void* dH, const void* X, const uint8_t* 
         return set_error(STM_ERR_INVALID, "%s: the sums must be 16-byte aligned and not NULL", who);
     if (mode == 3 && M <= kGatedKeepRows)
         return set_error(STM_ERR_UNSUPPORTED, "%s: takes more than %d rows", who, kGatedKeepRows);
-    const int64_t need = gated_workspace_bytes(M, I, K);
+    const int64_t need = gated_workspace_bytes(M, I, K, mode);
     if (need > 0 && !workspace) return set_error(STM_ERR_INVALID, "%s: a workspace of %lld bytes is needed", who, (long long)need);
     if ((rc = check_workspace(who, workspace, workspace_bytes, need)) != STM_OK) return rc;
     GemmArgs g{};

@@ -3610,10 +3610,9 @@ static int64_t gated_max_rows(int64_t N, int64_t K) {
     return (by_x < by_out ? by_x : by_out) / 256 * 256;
 }
 
-int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K) {
+int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K, int mode) {
     if (M <= 0 || I <= 0 || K <= 0) return 0;
-    const int64_t a = gated_plan(M, 2 * I, K, 1).partial, b = gated_plan(M, 2 * I, K, 3).partial;
-    return (a > b ? a : b) * (int64_t)sizeof(float);
+    return gated_plan(M, 2 * I, K, mode).partial * (int64_t)sizeof(float);
 }
 
 // A training step's two directions, us, the backward computing the sums again -> from kept ones.

@@ -85,7 +85,7 @@ int launch_gemm_fwd(const GemmArgs& g, int dtype, hipStream_t stream);
 int launch_gemm_bwd(const GemmArgs& g, int dtype, hipStream_t stream);
 // Gated block over W [2 I, K]: mode 1 = forward (out [M, I]), 2 = backward from dh (out
 // [M, 2 I]), 3 = forward that also keeps the sums (M > kGatedKeepRows); partial holds
-// gated_workspace_bytes(M, I, K).
+// gated_workspace_bytes(M, I, K, mode).
 constexpr int kGatedKeepRows = 64;
 int launch_gated(const GemmArgs& g, int mode, int dtype, hipStream_t stream);
 // Mode 2 from the kept sums, which g.partial holds.
@@ -95,7 +95,7 @@ int launch_gated_kept(const GemmArgs& g, int dtype, hipStream_t stream);
 int launch_gated_dense(const GemmArgs& g, const void* w, int mode, int dtype, unsigned grid, hipStream_t stream);
 int launch_dequantize_tiles(const uint8_t* packed, const float* absmax, int64_t inter, int64_t K, int bs, void* out,
                             int dtype, hipStream_t stream);
-int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K);
+int64_t gated_workspace_bytes(int64_t M, int64_t I, int64_t K, int mode);
 int64_t gated_sums_bytes(int64_t M, int64_t I, int64_t K);  // worth keeping; 0: not
 
 }  // namespace stm

@@ -550,7 +550,7 @@ def _gated_native() -> tuple:
     """The native callers of the forward and the backward, and the addresses that they take."""
     f, at = _lib.fast(), _lib.address
     return (f.gated_fwd, (at("stm_nf4_gated_fwd"), at("stm_nf4_gated_workspace_bytes"), at("stm_nf4_gated_fwd_keep")),
-            at("stm_nf4_gated_sums_bytes"),
+            (at("stm_nf4_gated_sums_bytes"), at("stm_nf4_gated_keep_workspace_bytes")),
             f.gated_bwd, (at("stm_nf4_gated_bwd"), at("stm_nf4_gated_workspace_bytes"), at("stm_gated_bwd_kept")),
             (at("stm_nf4_gemm_bwd_dx"), at("stm_nf4_gemm_workspace_bytes")))
 
@@ -560,7 +560,7 @@ def _gated_plain(x, packed, absmax, weight_shape, blocksize, keep=False):
     if not x.is_cuda:
         return None
     native, entries, sums = _gated_native()[:3]
-    y = native(*entries, sums if keep else 0, x, packed, absmax, int(weight_shape[0]), int(weight_shape[1]), blocksize,
+    y = native(*entries, *(sums if keep else (0, 0)), x, packed, absmax, int(weight_shape[0]), int(weight_shape[1]), blocksize,
                torch._C._cuda_getCurrentRawStream(x.get_device()))
     if type(y) is int:
         _lib.check(y, "stm_nf4_gated_fwd")
@@ -579,10 +579,11 @@ def _gated_plain_bwd(grad, saved, packed, absmax, weight_shape, blocksize, dx=Fa
     return y
 
 
-def _gated_workspace(M: int, inter: int, K: int, device) -> Optional[torch.Tensor]:
-    nbytes = int(_lib.lib().stm_nf4_gated_workspace_bytes(M, inter, K))
+def _gated_workspace(M: int, inter: int, K: int, device, keep: bool = False) -> Optional[torch.Tensor]:
+    name = "stm_nf4_gated_keep_workspace_bytes" if keep else "stm_nf4_gated_workspace_bytes"
+    nbytes = int(getattr(_lib.lib(), name)(M, inter, K))
     if nbytes < 0:
-        _lib.check(nbytes, "stm_nf4_gated_workspace_bytes")
+        _lib.check(nbytes, name)
     return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
 
 
@@ -623,7 +624,7 @@ def nf4_gated_fwd_keep(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tens
     h = torch.empty(*x.shape[:-1], inter, dtype=x.dtype, device=dev)
     sums = torch.empty(M, 2 * inter, dtype=torch.float32, device=dev)
     with _lib.device_guard(dev):
-        ws = _gated_workspace(M, inter, K, dev)
+        ws = _gated_workspace(M, inter, K, dev, keep=True)
         rc = _lib.lib().stm_nf4_gated_fwd_keep(
             x2.data_ptr(), _aligned(packed).data_ptr(), _aligned(absmax, 4).data_ptr(), h.data_ptr(), sums.data_ptr(), M,
             inter, K, blocksize, tag, ws.data_ptr() if ws is not None else None, 4 * ws.numel() if ws is not None else 0,
