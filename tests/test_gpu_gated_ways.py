@@ -7,7 +7,7 @@ import ctypes
 import pytest
 import torch
 
-from test_gpu_gated import assert_within, reference, seeded, weight
+from test_gpu_gated import U, assert_within, reference, seeded, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,36 @@ def test_the_keeping_forwards_space(cuda):
     before = torch.cuda.memory_allocated()
     h, sums = nf4_gated_fwd_keep(x, q, a, (2 * inter, K))
     assert torch.cuda.max_memory_allocated() - before <= h.numel() * 2 + sums.numel() * 4 + (4 << 20)
+
+
+@pytest.mark.parametrize("M,inter,K", [(6200, 5640, 2112), (8192, 2824, 1344)])
+def test_kept_sums_where_the_plain_forward_is_dense(cuda, M, inter, K):
+    from stratum_amd import _lib, nf4_gated_bwd_kept, nf4_gated_fwd, nf4_gated_fwd_keep
+    dtype = torch.bfloat16
+    assert _lib.lib().stm_nf4_gated_workspace_bytes(M, inter, K) == -(-inter // 128) * 256 * K * 2
+    q, a, w = weight(inter, K, dtype)
+    x, dh = (seeded((M, n), M + n, 1.0, dtype).cuda() for n in (K, inter))
+    h, sums = nf4_gated_fwd_keep(x, q, a, (2 * inter, K))
+    exact, size = x.double() @ w.t().contiguous(), x.double().abs() @ w.abs().t().contiguous()
+    assert ((sums.double() - exact).abs() <= K * U * size + 1e-30).all()
+    del exact, size
+    assert_within(h, *reference(x, w), dtype)
+    assert_within(nf4_gated_fwd(x, q, a, (2 * inter, K)), *reference(x, w), dtype)
+    assert_within(nf4_gated_bwd_kept(dh, sums), *reference(x, w, dh), dtype)
+
+
+def test_kept_sums_past_32_bit_offsets_and_in_stretches_of_rows(cuda):
+    """262 444 rows of 2 x 4096 sums (8.6 GB): the kernels run in stretches of 261 888 rows, and row
+    262 144 starts at element 2^31."""
+    from stratum_amd import nf4_gated_bwd_kept, nf4_gated_fwd_keep
+    M, inter, K, dtype = 262_444, 4096, 1280, torch.bfloat16
+    q, a, w = weight(inter, K, dtype)
+    x = torch.randn(M, K, device=cuda, dtype=torch.float32, generator=torch.Generator("cuda").manual_seed(1)).to(dtype)
+    dh = torch.ones(M, inter, device=cuda, dtype=dtype)
+    h, sums = nf4_gated_fwd_keep(x, q, a, (2 * inter, K))
+    dgu = nf4_gated_bwd_kept(dh, sums)
+    rows = torch.tensor([0, 1, 255, 131_071, 261_887, 261_888, 262_143, 262_144, M - 1], device=cuda)
+    exact, size = x[rows].double() @ w.t().contiguous(), x[rows].double().abs() @ w.abs().t().contiguous()
+    assert ((sums[rows].double() - exact).abs() <= K * U * size + 1e-30).all()
+    assert_within(h[rows], *reference(x[rows], w), dtype)
+    assert_within(dgu[rows], *reference(x[rows], w, dh[rows]), dtype)
