@@ -263,7 +263,8 @@ PyObject* gated_bwd(PyObject*, PyObject* args) {
         const int64_t M = g.numel() / inter;
         if (x.numel() != M * (kept ? N : K)) Py_RETURN_NONE;
         void* st = reinterpret_cast<void*>(stream);
-        at::Tensor dgu = shaped(g, N);
+        const at::Tensor& like = kept ? g : x;  // whose leading sizes the result has
+        at::Tensor dgu = shaped(like, N);
         int rc;
         if (kept) {
             rc = reinterpret_cast<GatedKept>(kept_fn)(g.data_ptr(), x.data_ptr<float>(), dgu.data_ptr(), M, inter, tag, st);
@@ -279,7 +280,7 @@ PyObject* gated_bwd(PyObject*, PyObject* args) {
         if (!dx_fn) return THPVariable_Wrap(dgu);
         const int64_t bytes = reinterpret_cast<GemmBytes>(dx_ws_fn)(M, N, K, 1);
         if (bytes < 0) return PyLong_FromLongLong(bytes);
-        at::Tensor dx = shaped(g, K), ws;
+        at::Tensor dx = shaped(like, K), ws;
         if (bytes) ws = bytes_on(bytes, g);
         rc = reinterpret_cast<GemmDx>(dx_fn)(dgu.data_ptr(), w.packed, w.absmax, nullptr, nullptr, 0, dx.data_ptr(), M, N,
                                              K, w.bs, tag, bytes ? ws.data_ptr() : nullptr, bytes, st);

@@ -73,3 +73,18 @@ def test_kept_sums_past_32_bit_offsets_and_in_stretches_of_rows(cuda):
     assert ((sums[rows].double() - exact).abs() <= K * U * size + 1e-30).all()
     assert_within(h[rows], *reference(x[rows], w), dtype)
     assert_within(dgu[rows], *reference(x[rows], w, dh[rows]), dtype)
+
+
+@pytest.mark.parametrize("M", [6, 300])
+def test_a_backward_has_the_leading_sizes_of_x(cuda, M):
+    """Whatever the gradient's are, and whether an operand has to be copied or not."""
+    from stratum_amd import nf4_gated_bwd
+    q, a, _ = weight(96, 128, torch.bfloat16)
+    x, dh = seeded((M, 128), 1, 1.0, torch.bfloat16).cuda(), seeded((M, 96), 2, 1.0, torch.bfloat16).cuda()
+    want = nf4_gated_bwd(dh, x, q, a, (192, 128))
+    folded, spread = x.view(2, M // 2, 128), torch.stack([x, x], 2)[..., 0].view(2, M // 2, 128)
+    assert not spread.is_contiguous()
+    for y in (folded, spread):
+        assert torch.equal(nf4_gated_bwd(dh, y, q, a, (192, 128)), want.view(2, M // 2, 192))
+    for y in (x, spread.reshape(M, 128)):
+        assert torch.equal(nf4_gated_bwd(dh.view(2, M // 2, 96), y, q, a, (192, 128)), want)
