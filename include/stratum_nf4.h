@@ -354,7 +354,7 @@ int stm_nf4_dequantize_aug(const uint8_t* packed, const float* absmax, const voi
  *
  * stm_grad_norm: out[0] = |g| / loss_scale over all elements of all tensors, out[1] =
  *   min(1, max_norm / (out[0] + 1e-6)) / loss_scale, the factor that clips and
- *   unscales the gradients; NaN where the norm is not finite. out: two floats on the
+ *   unscales the gradients; NaN where out[0] is not finite. out: two floats on the
  *   device. max_norm >= 0 (INFINITY: no clipping). Sums in fp64 in a fixed order.
  *   Workspace: stm_grad_norm_workspace_bytes(count, n) bytes, 8-byte aligned.
  *   count, grads, n: host arrays of device pointers and element counts; one dtype.

@@ -2,7 +2,7 @@
 // of all gradients, and one AdamW step over all tensors, each in few launches.
 //
 //   norm      out[0] = |g| / c, out[1] = min(1, max_norm / (out[0] + 1e-6)) / c, c the loss scale;
-//             out[1] = NaN where the norm is not finite
+//             out[1] = NaN where out[0] is not finite
 //   AdamW     g' = scale g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g' g'
 //             p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //             and nothing at all where scale is not finite
@@ -534,8 +534,8 @@ __global__ __launch_bounds__(kFinalThreads) void k_norm_final(const double* __re
     if (threadIdx.x == 0) {
         const double norm = sqrt(sum) / loss_scale;
         const double factor = max_norm / (norm + 1e-6);
-        out[0] = (float)norm;
-        out[1] = norm < (double)INFINITY ? (float)((factor < 1.0 ? factor : 1.0) / loss_scale) : NAN;
+        out[0] = (float)norm;  // as it is returned: infinite also where only fp32 ends
+        out[1] = out[0] < INFINITY ? (float)((factor < 1.0 ? factor : 1.0) / loss_scale) : NAN;
     }
 }
 

@@ -86,3 +86,23 @@ def test_the_optimizers_norm_over_many_tensors(cuda):
     for p, g in zip(ps, gs):
         m = 0.1 * g.double() * (0.5 / (want + 1e-6))
         assert ((opt.state[p]["exp_avg"].double() - m).abs() <= 8 * U * m.abs() + 1e-45).all()
+
+
+@pytest.mark.parametrize("kinds", [(torch.bfloat16,), (torch.bfloat16, torch.float32)])
+def test_a_norm_past_fp32_is_not_finite_for_the_factor_either(cuda, kinds):
+    """64 gradients of 3e38: 2.4e39, infinite in fp32, so the factor is NaN and a step changes nothing, with
+    one gradient type and with two."""
+    from stratum_amd.optim import AdamW, grad_norm
+    gs = [torch.full((64,), 3e38, dtype=kinds[0], device=cuda)] + [torch.ones(3, dtype=k, device=cuda) for k in kinds[1:]]
+    norm, factor = grad_norm(gs[:1], 1.0).tolist()
+    assert norm == math.inf and math.isnan(factor)
+    ps = [torch.nn.Parameter(torch.ones_like(g)) for g in gs]
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt = AdamW(ps, lr=0.1, max_grad_norm=1.0)
+    opt.step()
+    assert opt.grad_norm[0].item() == math.inf and all((p == 1).all() for p in ps)
+    # one that fp32 still holds is clipped
+    g = torch.full((64,), 2.0 ** 121, device=cuda)
+    norm, factor = grad_norm([g], 1.0).tolist()
+    assert norm == 2.0 ** 124 and factor == pytest.approx(2.0 ** -124, rel=1e-6)
