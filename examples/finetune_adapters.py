@@ -2,7 +2,7 @@
 
 A small decoder (random weights, synthetic tokens) with NF4 projections: adapters on the attention
 projections and the MLPs' down projections, the gate and up projections with their gating as one
-kernel, the frozen head under the chunked loss, and AdamW with 8-bit states, fp32 masters and
+operator, the frozen head under the chunked loss, and AdamW with 8-bit states, fp32 masters and
 clipping, whose step reads the gradient norm on the GPU.
 
     python examples/finetune_adapters.py [--steps 30] [--bits 8]

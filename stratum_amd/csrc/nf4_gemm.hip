@@ -36,7 +36,6 @@
 #include <type_traits>
 
 #include "gemm_tile.h"
-#include <cstdlib>
 #include "nf4_kernels.h"
 
 // Tile shapes (measured best on MI355X at M = 8192, N = 14336, K = 4096):
@@ -2704,7 +2703,8 @@ __global__ __launch_bounds__(256) void k_split_reduce(const float* __restrict__ 
 }
 
 // The gated block from partials [split][m][2 I], g and u in columns c and I + c: the forward (MODE 1), the
-// forward that also keeps the sums (3), and the backward (2), also from kept sums (one split).
+// forward that also keeps the sums (3), and the backward (2, rounded as store_gated says), also from kept sums
+// (one split).
 template <typename Tr, int MODE>
 __global__ __launch_bounds__(256) void k_gated_reduce(const float* __restrict__ partial, int splits, int64_t rows,
                                                       int64_t I, const uint16_t* __restrict__ dh,
@@ -3511,11 +3511,12 @@ double gated_rounds(int64_t tiles, int64_t steps, double c0, double c1, double f
 //  * the weight dequantized once and k_gated_dense over it: many rows.
 // The constants are fitted to 9 weights (K 640-5120, I 512-14336) x 20 row counts from 65 to
 // 8192, all ways timed on each: the pick is 0.2 % above the fastest on average and 4 % at
-// worst. E.g. us, [2 x 14336, 4096]:
+// worst, of the forward that keeps nothing. E.g. us, [2 x 14336, 4096]:
 // 100 rows 46 (128 rows, KW = 2; KW = 1 65, dense 129, split 66), 180 rows 53 (192, KW = 2; 128, KW = 1 67), 333 rows 85
 // (192; 256-row tiles 102), 1024 rows 207 (256; 192: 250), 8192 rows dense 1510 (256: 1600);
 // [2 x 512, 4096]: 509 rows 21 (eight ranges of 128 x 128; unsplit 50).
-// A forward that keeps its sums (mode 3) does not take the dense way, which loses more by the stores, us:
+// A forward that keeps its sums (mode 3) is priced alike, without its stores (509 rows on [2 x 5632, 2048]: 37 us
+// by the model, 45 measured); only it does not take the dense way, which loses more by them, us:
 // [2 x 14336, 4096] 4096 rows 884 against 841 (256-row tiles), 8192 rows 1724 against 1697, [2 x 8192, 4096]
 // 8192 rows 1029 against 958, [2 x 2816, 1024] 118 against 121.
 GatedPlan gated_plan(int64_t M, int64_t N, int64_t K, int mode) {

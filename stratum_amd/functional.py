@@ -591,9 +591,11 @@ def _gated_workspace(M: int, inter: int, K: int, device, keep: bool = False) -> 
 def nf4_gated_fwd(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, weight_shape: Sequence[int],
                   blocksize: int = 64, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``silu(x @ Wg.T) * (x @ Wu.T)`` as [..., I] in x's dtype, for the stacked NF4 weight
-    [Wg; Wu] of shape ``weight_shape`` = (2 I, K): both projections and the gating in one
-    kernel, fp32 throughout, one rounding. (``swiglu_fwd(nf4_gemm_fwd(...))`` rounds the
-    projections first and writes and reads them.) ``out`` as for :func:`nf4_gemm_fwd`."""
+    [Wg; Wu] of shape ``weight_shape`` = (2 I, K): the gating is applied to the projections'
+    fp32 sums, one rounding. One kernel for up to 16 rows and for a few hundred or
+    thousand; two, with fp32 parts of the sums or the dequantized weight in a workspace, for
+    the row counts between, narrow weights and many rows. (``swiglu_fwd(nf4_gemm_fwd(...))`` rounds
+    the projections first.) ``out`` as for :func:`nf4_gemm_fwd`."""
     if out is None:
         h = _gated_plain(x, packed, absmax, weight_shape, blocksize)
         if h is not None:
@@ -674,8 +676,8 @@ def nf4_gated_bwd(grad_out: torch.Tensor, x: torch.Tensor, packed: torch.Tensor,
                   weight_shape: Sequence[int], blocksize: int = 64,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of :func:`nf4_gated_fwd` with respect to the two projections' outputs:
-    [..., 2 I] = [d gate | d up] in x's dtype, both projections computed again in the same
-    kernel. The input's gradient is ``nf4_gemm_bwd_dx`` of it with the same weight."""
+    [..., 2 I] = [d gate | d up] in x's dtype, both projections computed again, as the forward
+    computes them. The input's gradient is ``nf4_gemm_bwd_dx`` of it with the same weight."""
     if out is None:
         dgu = None
         if x.dtype == grad_out.dtype:

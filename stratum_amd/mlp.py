@@ -26,8 +26,8 @@ work:
 * ``_ModuleRows`` otherwise: the module's own projections, with the input
   gradient of a chunk taken by a backward pass over that chunk's recompute.
 
-``NF4GatedMLP`` is the MLP for a whole batch at once: gate, up and the gating in one
-kernel (``nf4_gated``), then the module's own down projection, which may train a LoRA
+``NF4GatedMLP`` is the MLP for a whole batch at once: gate, up and the gating as one
+operator (``nf4_gated``), then the module's own down projection, which may train a LoRA
 adapter.
 """
 
@@ -336,7 +336,7 @@ class MemoryFlatFrozenMLP(nn.Module):
 
 class NF4GatedMLP(nn.Module):
     """``down(silu(gate(x)) * up(x))`` with the two frozen NF4 projections and the gating as
-    one kernel (``nf4_gated``). The backward keeps the projections' fp32 sums [tokens, 2 I], or
+    one operator (``nf4_gated``). The backward keeps the projections' fp32 sums [tokens, 2 I], or
     with ``recompute=True`` only x (and what the down projection keeps of h).
 
     ``module`` is an MLP whose gate and up projections are plain ``NF4Linear`` (``quantize_mlp_``

@@ -244,12 +244,14 @@ class _NF4GatedFn(torch.autograd.Function):
 def nf4_gated(x: torch.Tensor, packed: torch.Tensor, absmax: torch.Tensor, weight_shape: Sequence[int],
               blocksize: int = 64, recompute: bool = False) -> torch.Tensor:
     """``silu(x @ Wg.T) * (x @ Wu.T)`` with the stacked NF4 weight [Wg; Wu] of shape
-    ``weight_shape`` = (2 I, K) (``stack_nf4``, ``quantize_mlp_``), one kernel; differentiable in x. The
-    step ``act_fn(gate_proj(x)) * up_proj(x)`` of stratum/model/mlp_opt.py:178-180.
+    ``weight_shape`` = (2 I, K) (``stack_nf4``, ``quantize_mlp_``), one operator (:func:`nf4_gated_fwd`);
+    differentiable in x (reverse mode; a forward-mode dual is refused). The step
+    ``act_fn(gate_proj(x)) * up_proj(x)`` of stratum/model/mlp_opt.py:178-180.
 
     For the backward the projections' fp32 sums are kept, 8 bytes per output column and row
     (16 I bytes a row more than h), from the forward to the backward of this call;
-    ``recompute=True`` keeps x alone and computes them again."""
+    ``recompute=True`` keeps x alone and computes them again. The gradient of the projections is rounded to
+    x's dtype for its product with the weight: that doubles the variance of dx's rounding error."""
     shape = tuple(int(d) for d in weight_shape)
     # the raw kernel knows no autograd: a forward-mode dual goes to the function, which refuses it
     if not (torch.is_grad_enabled() and x.requires_grad) and forward_ad.unpack_dual(x).tangent is None:
