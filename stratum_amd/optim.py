@@ -406,7 +406,7 @@ class AdamW(torch.optim.Optimizer):
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
         for i, p in zip(saved, params):
-            if i in state_dict["state"]:
+            if state_dict["state"].get(i):  # empty: looked at, but never stepped
                 self.state[p] = self._taken(p, state_dict["state"][i])
 
     def _taken(self, p: torch.Tensor, saved: dict) -> dict:

@@ -211,3 +211,14 @@ def test_a_norm_refuses_a_tensor_of_more_work_groups_than_a_launch_takes():
     one, n = np.array([where], np.int64), np.array([most * 16384 + 1], np.int64)
     assert L.stm_grad_norm(1, one.ctypes.data, n.ctypes.data, 1, 1.0, 1.0, where, where, 1 << 40,
                            None) == _lib.STM_ERR_UNSUPPORTED
+
+
+def test_a_parameter_that_was_looked_at_and_never_stepped_loads(on_cpu):
+    ps, qs = ([parameter(), parameter()] for _ in range(2))
+    opt, other = optim.AdamW(ps), optim.AdamW(qs, lr=0.25)
+    ps[1].grad = None
+    opt.step()
+    assert len(opt.state[ps[1]]) == 0  # which leaves an empty entry
+    other.load_state_dict(opt.state_dict())
+    other.step()
+    assert (other.state[qs[0]]["step"], other.state[qs[1]]["step"]) == (2, 1)
