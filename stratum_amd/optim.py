@@ -394,9 +394,19 @@ class AdamW(torch.optim.Optimizer):
         """As torch's, but states keep fp32 or their codes (torch casts them to the parameter's type). A
         checkpoint of other settings, torch's own AdamW among them, is made one of these: its moments
         take ``state_bits``, and masters are made from the parameters, or dropped, as ``master_weights``
-        says."""
+        says. Groups that ask for another update (amsgrad, maximize, weight decay in the gradient) are
+        refused."""
         loaded: dict = {}  # what the hooks before loading leave of it
-        last = self.register_load_state_dict_pre_hook(lambda _, given: loaded.update(given))
+
+        def look(_, given: dict) -> None:
+            for group in given["param_groups"]:
+                for name in ("amsgrad", "maximize"):
+                    if group.get(name):
+                        raise ValueError(f"AdamW has no {name}, the state to load asks for it")
+                if group.get("weight_decay") and not group.get("decoupled_weight_decay", True):
+                    raise ValueError("AdamW's weight decay is decoupled, that of the state to load is not")
+            loaded.update(given)
+        last = self.register_load_state_dict_pre_hook(look)
         try:
             super().load_state_dict(state_dict)
         finally:

@@ -222,3 +222,25 @@ def test_a_parameter_that_was_looked_at_and_never_stepped_loads(on_cpu):
     other.load_state_dict(opt.state_dict())
     other.step()
     assert (other.state[qs[0]]["step"], other.state[qs[1]]["step"]) == (2, 1)
+
+
+@pytest.mark.parametrize("other,kw", [(torch.optim.AdamW, dict(amsgrad=True)), (torch.optim.AdamW, dict(maximize=True)),
+                                      (torch.optim.Adam, dict(weight_decay=0.1))])
+def test_a_state_of_another_update_is_refused_and_nothing_changes(on_cpu, other, kw):
+    p, q = parameter(), parameter()
+    theirs, mine = other([p], lr=0.5, **kw), optim.AdamW([q], lr=0.25)
+    theirs.step()
+    mine.step()
+    with pytest.raises(ValueError):
+        mine.load_state_dict(theirs.state_dict())
+    assert mine.param_groups[0]["lr"] == 0.25 and mine.state[q]["step"] == 1
+    assert not mine._optimizer_load_state_dict_pre_hooks
+
+
+def test_a_state_of_adam_without_weight_decay_loads(on_cpu):
+    p, q = parameter(), parameter()
+    theirs, mine = torch.optim.Adam([p], lr=0.5), optim.AdamW([q], lr=0.25)
+    theirs.step()
+    mine.load_state_dict(theirs.state_dict())
+    assert mine.param_groups[0]["weight_decay"] == 0 and mine.state[q]["step"] == 1
+    mine.step()
