@@ -417,6 +417,66 @@ int stm_state8_codes(const float* x, int64_t n, int is_signed, uint8_t* codes, f
 int stm_state8_values(const uint8_t* codes, const float* scales, int64_t n, int is_signed, float* out, void* stream);
 
 /*
+ * The sparse half of a decoder layer around the experts' products (stm_nf4_grouped_gemm_*): the norm before
+ * it, the router's choice, the rows in their experts' order and back. The reference leaves these to
+ * transformers' modules (stratum/model/qwen3_moe.py, stratum/moe.py). Pointers need their
+ * elements' alignment only; rows are contiguous; `dtype` is STM_F16, STM_BF16 or STM_F32.
+ *
+ * stm_rms_norm_fwd: s = x (+ residual), y = s / sqrt(mean(s^2) + eps) * weight, h = s rounded to residual_dtype
+ * (the rows' type or STM_F32; residual and h both NULL: neither). weight_dtype: the rows' type or STM_F32. rstd
+ * ([rows] fp32, or NULL) is what the backward takes.
+ * stm_rms_norm_bwd: from the gradients dy of y and dh of h (NULL: none), h (x where there was no
+ * residual) and rstd: the gradient of the sum as dx (rows' type) and dresidual (h_dtype), and dweight (weight_dtype),
+ * each NULL if not wanted; dweight needs stm_rms_norm_workspace_bytes(rows, cols) of workspace. Its sums over rows
+ * are taken in a fixed order.
+ */
+int stm_rms_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, int weight_dtype,
+                     void* y, void* h, float* rstd, int64_t rows, int64_t cols, double eps, int dtype, void* stream);
+int64_t stm_rms_norm_workspace_bytes(int64_t rows, int64_t cols);
+int stm_rms_norm_bwd(const void* dy, const void* dh, const void* h, int h_dtype, const float* rstd, const void* weight,
+                     int weight_dtype, void* dx, void* dresidual, void* dweight, int64_t rows, int64_t cols, int dtype,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* the router's scores */
+#define STM_MOE_SOFTMAX 0
+#define STM_MOE_SIGMOID 1
+/*
+ * stm_moe_route: for every token the top_k experts of its logits [tokens, num_experts] (at most 1024, top_k at most
+ * 64) in descending order of their keys, the lowest index among equal ones, and their weights, both [tokens, top_k].
+ * The key is the logit, or score + bias with a bias ([num_experts] fp32) or group_sums; experts stand in `groups`
+ * (at most 64) of equal size, of which the top_groups with the largest key (group_sums: the largest sum of two
+ * keys) are eligible. A weight is the score, divided by the chosen scores' sum if renormalize, times scale. An
+ * expert whose logit or key is -inf is never chosen; slots left over, and those of tokens whose mask byte is 0, hold
+ * expert -1 and weight 0.
+ * stm_moe_route_bwd: the gradient of the logits from that of the weights.
+ */
+int stm_moe_route(const void* logits, const float* bias, const uint8_t* mask, float* weights, int32_t* experts,
+                  int64_t tokens, int num_experts, int top_k, int score, int groups, int top_groups, int group_sums,
+                  int renormalize, double scale, int dtype, void* stream);
+int stm_moe_route_bwd(const float* dweights, const void* logits, const int32_t* experts, void* dlogits, int64_t tokens,
+                      int num_experts, int top_k, int score, int renormalize, double scale, int dtype, void* stream);
+/*
+ * stm_moe_sort: the n slots in the order of their experts (slots of one expert in their own order): offsets
+ * [num_experts + 1], slots [n] (row p holds slot slots[p]; -1 from offsets[num_experts] on) and positions [n] (slot's
+ * row, -1 for a slot whose expert is not in 0 .. num_experts - 1). Workspace: stm_moe_sort_workspace_bytes.
+ * stm_moe_gather: out[positions[t, j]] = x[t], out [tokens * top_k, hidden]; rows from offsets[num_experts] on are 0.
+ * stm_moe_combine: out[t] = residual[t] + sum over j of weights[t, j] * y[positions[t, j]], y [y_rows, hidden]; weights
+ * NULL: ones, residual NULL: none; both residual and out of out_dtype, y's type or STM_F32. A position outside 0 .. y_rows - 1 adds nothing.
+ * stm_moe_combine_bwd: dy[positions[t, j]] = weights[t, j] * dout[t] (rows from offsets[num_experts] on: 0) and
+ * dweights[t, j] = <dout[t], y[positions[t, j]]>, each NULL if not wanted.
+ */
+int64_t stm_moe_sort_workspace_bytes(int64_t n, int num_experts);
+int stm_moe_sort(const int32_t* experts, int64_t n, int num_experts, int32_t* offsets, int32_t* slots,
+                 int32_t* positions, void* workspace, int64_t workspace_bytes, void* stream);
+int stm_moe_gather(const void* x, const int32_t* positions, const int32_t* offsets, int num_experts, void* out,
+                   int64_t tokens, int top_k, int64_t hidden, int dtype, void* stream);
+int stm_moe_combine(const void* y, int64_t y_rows, const float* weights, const int32_t* positions, const void* residual,
+                    void* out, int out_dtype, int64_t tokens, int top_k, int64_t hidden, int dtype, void* stream);
+int stm_moe_combine_bwd(const void* dout, int dout_dtype, const void* y, int64_t y_rows, const float* weights, const int32_t* positions,
+                        const int32_t* offsets, int num_experts, void* dy, float* dweights, int64_t tokens, int top_k,
+                        int64_t hidden, int dtype, void* stream);
+
+/*
  * Host-only introspection used by the CPU test suite (no GPU work):
  * the 15 fp32 decision boundaries of a rounding rule (code > i iff s >= b[i]),
  * and the 65-cell table the quantize kernel indexes with

@@ -11,7 +11,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libstratum_nf4.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["nf4_abi.hip", "nf4_quant.hip", "nf4_gemm.hip", "swiglu.hip", "lora.hip", "gated_dense.hip",
-           "optim.hip"]
+           "optim.hip", "norm.hip", "moe.hip"]
 
 # The host code of launch-bound calls, a CPython module against torch's headers.
 FAST_SOURCE = "fast_path.cpp"

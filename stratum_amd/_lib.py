@@ -75,6 +75,16 @@ SIGNATURES = {
     "stm_adamw_step_table": ([_I, _P, _I, _I, _I, _I, _D, _D, _D, _D, _D, _I64, _P, _P], _I),
     "stm_state8_codes": ([_P, _I64, _I, _P, _P, _P], _I),
     "stm_state8_values": ([_P, _P, _I64, _I, _P, _P], _I),
+    "stm_rms_norm_fwd": ([_P, _P, _I, _P, _I, _P, _P, _P, _I64, _I64, _D, _I, _P], _I),
+    "stm_rms_norm_workspace_bytes": ([_I64, _I64], _I64),
+    "stm_rms_norm_bwd": ([_P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _I64, _I64, _I, _P, _I64, _P], _I),
+    "stm_moe_route": ([_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _D, _I, _P], _I),
+    "stm_moe_route_bwd": ([_P, _P, _P, _P, _I64, _I, _I, _I, _I, _D, _I, _P], _I),
+    "stm_moe_sort_workspace_bytes": ([_I64, _I], _I64),
+    "stm_moe_sort": ([_P, _I64, _I, _P, _P, _P, _P, _I64, _P], _I),
+    "stm_moe_gather": ([_P, _P, _P, _I, _P, _I64, _I, _I64, _I, _P], _I),
+    "stm_moe_combine": ([_P, _I64, _P, _P, _P, _P, _I, _I64, _I, _I64, _I, _P], _I),
+    "stm_moe_combine_bwd": ([_P, _I, _P, _I64, _P, _P, _P, _I, _P, _P, _I64, _I, _I64, _I, _P], _I),
     "stm_nf4_decision_boundaries": ([_I, _P], _I),
     "stm_nf4_cell_table": ([_I, _P, _P], _I),
 }

@@ -1,0 +1,489 @@
+// Root-mean-square norm over rows, with the residual's addition before it (gfx950).
+//
+//   s = x (+ residual),  r = 1 / sqrt(mean(s^2) + eps),  y = s r w,  h = s rounded to the residual's type
+//
+// backward, with n = h r (h as it was stored) and t = w dy:
+//
+//   ds = r (t - n mean(t n)) (+ dh),  dw = sum over rows of dy n
+//
+// ds is the gradient of x and of the residual. Everything between a load and a store is fp32; y comes from the sum
+// before its rounding to h, so each output is rounded once. The backward's n does use the rounded h: half a step of h in
+// a term that is itself rounded to that type.
+//
+// Bound by bytes. One pass: a row stays in registers between its sum and its result, 8 elements of a thread in one access.
+// A row belongs to 8 to 64 lanes of a wave (no barrier), or to a work-group of 256 or 1024 threads.
+#include <type_traits>
+
+#include "nf4_kernels.h"
+#include "rows.h"
+
+namespace stm {
+namespace {
+
+// 8 elements of a row whose type is known at run time only (the residual's, the weight's): f32 is uniform.
+template <typename Tr>
+__device__ __forceinline__ void load_as(const void* p, bool f32, int64_t at, int n, float (&f)[8]) {
+    if (f32) {
+        Eight<F32> e;
+        e.load(p, at, n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = e.get(i);
+    } else {
+        Eight<Tr> e;
+        e.load(p, at, n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = e.get(i);
+    }
+}
+
+template <typename Tr>
+__device__ __forceinline__ void store_as(void* p, bool f32, int64_t at, int n, const float (&f)[8]) {
+    if (f32) {
+        Eight<F32> e;
+        e.set(f);
+        e.store(p, at, n);
+    } else {
+        Eight<Tr> e;
+        e.set(f);
+        e.store(p, at, n);
+    }
+}
+
+// Sum over the T threads of a row; every one of them gets it. Above a wave through LDS, `turn` alternating between two
+// buffers so that one barrier a sum is enough.
+template <int T>
+__device__ __forceinline__ float row_sum(float v, int turn) {
+    if constexpr (T <= 64) {
+        return lanes_sum<T>(v);
+    } else {
+        __shared__ float part[2][T / 64];
+        v = lanes_sum<64>(v);
+        float* p = part[turn & 1];
+        if ((threadIdx.x & 63) == 0) p[threadIdx.x / 64] = v;
+        __syncthreads();
+        float s = p[0];
+#pragma unroll
+        for (int i = 1; i < T / 64; ++i) s += p[i];
+        return s;
+    }
+}
+
+template <int T>
+constexpr int kBlock = T <= 256 ? 256 : T;
+
+struct NormFwd {
+    const void *x, *res, *w;
+    void *y, *h;
+    float* rstd;
+    int64_t rows;
+    int cols;
+    float eps;
+    bool res32, w32;
+};
+
+// T threads a row, NV vectors of 8 a thread: cols <= 8 T NV.
+template <typename Tr, int T, int NV>
+__global__ __launch_bounds__(kBlock<T>) void k_rms_fwd(NormFwd a) {
+    constexpr int SLOTS = kBlock<T> / T;
+    const int t = threadIdx.x % T;
+    int turn = 0;
+    for (int64_t first = (int64_t)blockIdx.x * SLOTS; first < a.rows; first += (int64_t)gridDim.x * SLOTS, ++turn) {
+        const int64_t row = first + threadIdx.x / T;
+        const bool on = row < a.rows;
+        const int64_t at = row * a.cols;
+        float s[NV][8];
+        float q = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
+            load_as<Tr>(a.x, false, at + c, n, s[v]);
+            if (a.res) {
+                float r[8];
+                load_as<Tr>(a.res, a.res32, at + c, n, r);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[v][i] += r[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q = __builtin_fmaf(s[v][i], s[v][i], q);
+        }
+        q = row_sum<T>(q, turn);
+        const float r = 1.0f / sqrtf(q / (float)a.cols + a.eps);
+        if (on && t == 0 && a.rstd) a.rstd[row] = r;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
+            float w[8], y[8];
+            load_as<Tr>(a.w, a.w32, c, n, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = s[v][i] * r * w[i];
+            store_as<Tr>(a.y, false, at + c, n, y);
+            if (a.h) store_as<Tr>(a.h, a.res32, at + c, n, s[v]);
+        }
+    }
+}
+
+// Rows too long for registers: two passes over them, 1024 threads a row.
+template <typename Tr>
+__global__ __launch_bounds__(1024) void k_rms_fwd_long(NormFwd a) {
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
+        const int64_t at = row * a.cols;
+        float q = 0.0f;
+        for (int c = 8 * threadIdx.x; c < a.cols; c += 8 * 1024) {
+            float s[8], r[8];
+            load_as<Tr>(a.x, false, at + c, a.cols - c, s);
+            if (a.res) {
+                load_as<Tr>(a.res, a.res32, at + c, a.cols - c, r);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] += r[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q = __builtin_fmaf(s[i], s[i], q);
+        }
+        q = row_sum<1024>(q, turn);
+        const float rstd = 1.0f / sqrtf(q / (float)a.cols + a.eps);
+        if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd;
+        for (int c = 8 * threadIdx.x; c < a.cols; c += 8 * 1024) {
+            float s[8], r[8], w[8], y[8];
+            load_as<Tr>(a.x, false, at + c, a.cols - c, s);
+            if (a.res) {
+                load_as<Tr>(a.res, a.res32, at + c, a.cols - c, r);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] += r[i];
+            }
+            load_as<Tr>(a.w, a.w32, c, a.cols - c, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = s[i] * rstd * w[i];
+            store_as<Tr>(a.y, false, at + c, a.cols - c, y);
+            if (a.h) store_as<Tr>(a.h, a.res32, at + c, a.cols - c, s);
+        }
+    }
+}
+
+struct NormBwd {
+    const void *dy, *dh, *h, *w;
+    const float* rstd;
+    void *dx, *dres;
+    float* dw_part;  // [groups of the grid, cols], or null
+    int64_t rows;
+    int cols;
+    bool h32, w32;
+};
+
+// DW: a thread's columns are the same in every row of its work-group, so the weight's gradient gathers in registers over
+// the rows that the group takes (gridDim rows apart), then over the group's row slots in LDS, and leaves as one row of
+// partial sums; k_rms_dw adds those rows up in a fixed order.
+template <typename Tr, int T, int NV, bool DW>
+__global__ __launch_bounds__(kBlock<T>) void k_rms_bwd(NormBwd a) {
+    constexpr int SLOTS = kBlock<T> / T;
+    const int t = threadIdx.x % T, slot = threadIdx.x / T;
+    float dw[NV][8];
+    if (DW) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dw[v][i] = 0.0f;
+    }
+    int turn = 0;
+    for (int64_t first = (int64_t)blockIdx.x * SLOTS; first < a.rows; first += (int64_t)gridDim.x * SLOTS, ++turn) {
+        const int64_t row = first + slot;
+        const bool on = row < a.rows;
+        const int64_t at = row * a.cols;
+        const float r = on ? a.rstd[row] : 0.0f;
+        float g[NV][8], n_[NV][8];  // t = w dy, n = h r
+        float dot = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
+            float w[8];
+            load_as<Tr>(a.dy, false, at + c, n, g[v]);
+            load_as<Tr>(a.h, a.h32, at + c, n, n_[v]);
+            load_as<Tr>(a.w, a.w32, c, n, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                n_[v][i] *= r;
+                if (DW) dw[v][i] = __builtin_fmaf(g[v][i], n_[v][i], dw[v][i]);
+                g[v][i] *= w[i];
+                dot = __builtin_fmaf(g[v][i], n_[v][i], dot);
+            }
+        }
+        const float mean = row_sum<T>(dot, turn) / (float)a.cols;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
+            float d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = r * (g[v][i] - n_[v][i] * mean);
+            if (a.dh) {
+                float e[8];
+                load_as<Tr>(a.dh, a.h32, at + c, n, e);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] += e[i];
+            }
+            if (a.dx) store_as<Tr>(a.dx, false, at + c, n, d);
+            if (a.dres) store_as<Tr>(a.dres, a.h32, at + c, n, d);
+        }
+    }
+    if (!DW) return;
+    float* out = a.dw_part + (int64_t)blockIdx.x * a.cols;
+    if constexpr (SLOTS > 1) {
+        // slot by slot into one row of LDS, each column by the thread that owns it
+        __shared__ float sum[8 * T * NV];
+        for (int k = 0; k < SLOTS; ++k) {
+            if (slot == k) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float* p = &sum[8 * (t + T * v) + i];
+                        *p = k ? *p + dw[v][i] : dw[v][i];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < a.cols; c += kBlock<T>) out[c] = sum[c];
+    } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = 8 * (t + T * v);
+            store_as<F32>(out, true, c, a.cols - c, dw[v]);
+        }
+    }
+}
+
+template <typename Tr>
+__global__ __launch_bounds__(1024) void k_rms_bwd_long(NormBwd a) {
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
+        const int64_t at = row * a.cols;
+        const float r = a.rstd[row];
+        float dot = 0.0f;
+        for (int c = 8 * threadIdx.x; c < a.cols; c += 8 * 1024) {
+            float g[8], h[8], w[8];
+            load_as<Tr>(a.dy, false, at + c, a.cols - c, g);
+            load_as<Tr>(a.h, a.h32, at + c, a.cols - c, h);
+            load_as<Tr>(a.w, a.w32, c, a.cols - c, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(g[i] * w[i], h[i] * r, dot);
+        }
+        const float mean = row_sum<1024>(dot, turn) / (float)a.cols;
+        for (int c = 8 * threadIdx.x; c < a.cols; c += 8 * 1024) {
+            float g[8], h[8], w[8];
+            load_as<Tr>(a.dy, false, at + c, a.cols - c, g);
+            load_as<Tr>(a.h, a.h32, at + c, a.cols - c, h);
+            load_as<Tr>(a.w, a.w32, c, a.cols - c, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[i] = r * (g[i] * w[i] - h[i] * r * mean);
+            if (a.dh) {
+                load_as<Tr>(a.dh, a.h32, at + c, a.cols - c, h);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] += h[i];
+            }
+            if (a.dx) store_as<Tr>(a.dx, false, at + c, a.cols - c, g);
+            if (a.dres) store_as<Tr>(a.dres, a.h32, at + c, a.cols - c, g);
+        }
+    }
+}
+
+// The weight's gradient of rows too long for registers: a thread's 8 columns, rows blockIdx.y, + gridDim.y, ...
+template <typename Tr>
+__global__ __launch_bounds__(256) void k_rms_dw_long(NormBwd a) {
+    const int64_t c = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+    const int n = (int)min((int64_t)8, a.cols - c);
+    if (n <= 0) return;
+    float dw[8] = {};
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        float g[8], h[8];
+        const float r = a.rstd[row];
+        load_as<Tr>(a.dy, false, row * a.cols + c, n, g);
+        load_as<Tr>(a.h, a.h32, row * a.cols + c, n, h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[i] = __builtin_fmaf(g[i], h[i] * r, dw[i]);
+    }
+    store_as<F32>(a.dw_part + (int64_t)blockIdx.y * a.cols, true, c, n, dw);
+}
+
+// Sum of `parts` rows of partial sums: 32 columns a work-group, its 32 row slots added up in LDS.
+template <typename Tr>
+__global__ __launch_bounds__(1024) void k_rms_dw(const float* __restrict__ part, int parts, int cols, void* dw,
+                                                 bool w32) {
+    __shared__ float sum[32][33];
+    const int c = blockIdx.x * 32 + threadIdx.x % 32, slot = threadIdx.x / 32;
+    float s = 0.0f;
+    if (c < cols)
+        for (int p = slot; p < parts; p += 32) s += part[(int64_t)p * cols + c];
+    sum[slot][threadIdx.x % 32] = s;
+    __syncthreads();
+    if (slot || c >= cols) return;
+    for (int k = 1; k < 32; ++k) s += sum[k][threadIdx.x];
+    if (w32)
+        static_cast<float*>(dw)[c] = s;
+    else
+        static_cast<typename Eight<Tr>::elem*>(dw)[c] = Tr::from_f32(s);
+}
+
+// ------------------------------------------------------------ which form
+constexpr int64_t kMostGroups = 1 << 21;  // of 1024 threads; the kernels loop over what is left
+
+unsigned row_groups(int64_t rows, int per) {
+    const int64_t groups = (rows + per - 1) / per;
+    return (unsigned)(groups < kMostGroups ? groups : kMostGroups);
+}
+
+constexpr int64_t kRegisterCols = 1024 * 4 * 8;
+
+// Threads of a row. Up to 512 columns one vector a thread; above that a wave takes a row of up to 4096 columns where
+// there are rows enough to fill the GPU with waves (no barrier), else 256 threads of up to 4 vectors, then 1024.
+int row_threads(int64_t rows, int64_t cols) {
+    const int64_t vecs = (cols + 7) / 8;
+    if (vecs <= 8) return 8;
+    if (vecs <= 16) return 16;
+    if (vecs <= 32) return 32;
+    if (vecs <= 64) return 64;
+    if (vecs <= 512 && rows >= 2048) return 64;
+    return vecs <= 1024 ? 256 : 1024;
+}
+
+// Groups of the backward's grid that write partial sums.
+int dw_groups(int64_t rows, int64_t cols) {
+    if (cols > kRegisterCols) return (int)(rows < 64 ? rows : 64);
+    const int t = row_threads(rows, cols), slots = t <= 256 ? 256 / t : 1;
+    const int64_t groups = (rows + slots - 1) / slots;
+    return (int)(groups < 512 ? groups : 512);
+}
+
+template <typename F>
+int each_form(int t, int nv, F f) {
+#define STM_FORM(T, NV) \
+    if (t == T && nv <= NV) return f(std::integral_constant<int, T>{}, std::integral_constant<int, NV>{})
+    STM_FORM(8, 1);
+    STM_FORM(16, 1);
+    STM_FORM(32, 1);
+    STM_FORM(64, 1);
+    STM_FORM(64, 2);
+    STM_FORM(64, 4);
+    STM_FORM(64, 8);
+    STM_FORM(256, 1);
+    STM_FORM(256, 2);
+    STM_FORM(256, 4);
+    STM_FORM(1024, 2);
+    STM_FORM(1024, 4);
+#undef STM_FORM
+    return set_error(STM_ERR_UNSUPPORTED, "rms_norm: no form of %d threads and %d vectors", t, nv);
+}
+
+template <typename Tr>
+int fwd(const NormFwd& a, hipStream_t st) {
+    if (a.cols > kRegisterCols) {
+        hipLaunchKernelGGL(k_rms_fwd_long<Tr>, dim3(row_groups(a.rows, 1)), dim3(1024), 0, st, a);
+        return check_launch("rms_norm_fwd");
+    }
+    const int t = row_threads(a.rows, a.cols), nv = (a.cols + 8 * t - 1) / (8 * t);
+    return each_form(t, nv, [&](auto T, auto NV) {
+        constexpr int per = kBlock<T.value> / T.value;
+        hipLaunchKernelGGL((k_rms_fwd<Tr, T.value, NV.value>), dim3(row_groups(a.rows, per)),
+                           dim3(kBlock<T.value>), 0, st, a);
+        return check_launch("rms_norm_fwd");
+    });
+}
+
+template <typename Tr>
+int bwd(const NormBwd& a, void* dweight, hipStream_t st) {
+    const int parts = a.dw_part ? dw_groups(a.rows, a.cols) : 0;
+    if (a.rows == 0) {  // no row: the weight's gradient is zero
+    } else if (a.cols > kRegisterCols) {
+        if (a.dx || a.dres) hipLaunchKernelGGL(k_rms_bwd_long<Tr>, dim3(row_groups(a.rows, 1)), dim3(1024), 0, st, a);
+        if (a.dw_part)
+            hipLaunchKernelGGL(k_rms_dw_long<Tr>, dim3((unsigned)((a.cols + 2047) / 2048), (unsigned)parts), dim3(256), 0,
+                               st, a);
+    } else {
+        const int t = row_threads(a.rows, a.cols), nv = (a.cols + 8 * t - 1) / (8 * t);
+        const int rc = each_form(t, nv, [&](auto T, auto NV) {
+            constexpr int per = kBlock<T.value> / T.value;
+            if (a.dw_part)
+                hipLaunchKernelGGL((k_rms_bwd<Tr, T.value, NV.value, true>), dim3((unsigned)parts), dim3(kBlock<T.value>), 0,
+                                   st, a);
+            else
+                hipLaunchKernelGGL((k_rms_bwd<Tr, T.value, NV.value, false>), dim3(row_groups(a.rows, per)),
+                                   dim3(kBlock<T.value>), 0, st, a);
+            return STM_OK;
+        });
+        if (rc) return rc;
+    }
+    if (dweight)
+        hipLaunchKernelGGL(k_rms_dw<Tr>, dim3((unsigned)((a.cols + 31) / 32)), dim3(1024), 0, st, a.dw_part, parts, a.cols,
+                           dweight, a.w32);
+    return check_launch("rms_norm_bwd");
+}
+
+// Sizes and types that every call shares.
+int check_rows(const char* what, int64_t rows, int64_t cols, int dtype, int w_dtype) {
+    if (rows < 0 || cols < 0) return set_error(STM_ERR_INVALID, "%s: negative size", what);
+    if (dtype < 0 || dtype > STM_F32) return set_error(STM_ERR_INVALID, "%s: dtype must be fp16, bf16 or fp32", what);
+    if (w_dtype != dtype && w_dtype != STM_F32)
+        return set_error(STM_ERR_INVALID, "%s: the weight must be of the rows' type or fp32", what);
+    if (rows >= (1ll << 31) || cols >= (1ll << 30) || (rows && cols > (1ll << 60) / rows))
+        return set_error(STM_ERR_UNSUPPORTED, "%s: [%lld, %lld] is too large", what, (long long)rows, (long long)cols);
+    return STM_OK;
+}
+
+// Elements lie on multiples of their size.
+bool lies(const void* p, int dtype) { return aligned(p, dtype == STM_F32 ? 4 : 2); }
+
+}  // namespace
+}  // namespace stm
+
+using namespace stm;
+
+extern "C" int stm_rms_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight,
+                                int weight_dtype, void* y, void* h, float* rstd, int64_t rows, int64_t cols, double eps,
+                                int dtype, void* stream) {
+    const char* what = "rms_norm_fwd";
+    int rc = check_rows(what, rows, cols, dtype, weight_dtype);
+    if (rc) return rc;
+    if (residual && residual_dtype != dtype && residual_dtype != STM_F32)
+        return set_error(STM_ERR_INVALID, "%s: the residual must be of x's type or fp32", what);
+    if (!(eps >= 0.0)) return set_error(STM_ERR_INVALID, "%s: eps must not be negative", what);
+    if (rows == 0 || cols == 0) return STM_OK;
+    if (!x || !weight || !y) return set_error(STM_ERR_INVALID, "%s: null pointer", what);
+    if (!residual != !h) return set_error(STM_ERR_INVALID, "%s: a residual and its sum come together", what);
+    if (!lies(x, dtype) || !lies(y, dtype) || !lies(residual, residual_dtype) || !lies(h, residual_dtype) ||
+        !lies(weight, weight_dtype) || !lies(rstd, STM_F32))
+        return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
+    const NormFwd a{x,    residual, weight, y, h, rstd, rows, (int)cols, (float)eps, residual && residual_dtype == STM_F32,
+                    weight_dtype == STM_F32};
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == STM_BF16 ? fwd<BF16>(a, st) : dtype == STM_F16 ? fwd<F16>(a, st) : fwd<F32>(a, st);
+}
+
+extern "C" int64_t stm_rms_norm_workspace_bytes(int64_t rows, int64_t cols) {
+    const int rc = check_rows("rms_norm_workspace_bytes", rows, cols, STM_F32, STM_F32);
+    if (rc) return rc;
+    return rows && cols ? (int64_t)dw_groups(rows, cols) * cols * 4 : 0;
+}
+
+extern "C" int stm_rms_norm_bwd(const void* dy, const void* dh, const void* h, int h_dtype, const float* rstd,
+                                const void* weight, int weight_dtype, void* dx, void* dresidual, void* dweight, int64_t rows,
+                                int64_t cols, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* what = "rms_norm_bwd";
+    int rc = check_rows(what, rows, cols, dtype, weight_dtype);
+    if (rc) return rc;
+    if (h_dtype != dtype && h_dtype != STM_F32) return set_error(STM_ERR_INVALID, "%s: h must be of dy's type or fp32", what);
+    if (cols == 0) return STM_OK;
+    if (rows && (!dy || !h || !rstd || !weight)) return set_error(STM_ERR_INVALID, "%s: null pointer", what);
+    if (!lies(dy, dtype) || !lies(dx, dtype) || !lies(dh, h_dtype) || !lies(h, h_dtype) || !lies(dresidual, h_dtype) ||
+        !lies(weight, weight_dtype) || !lies(dweight, weight_dtype) || !lies(rstd, STM_F32) || !lies(workspace, STM_F32))
+        return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
+    if (dweight && rows) {
+        const int64_t need = stm_rms_norm_workspace_bytes(rows, cols);
+        if (!workspace || workspace_bytes < need)
+            return set_error(STM_ERR_INVALID, "%s: the weight's gradient needs a workspace of %lld bytes, got %lld", what,
+                             (long long)need, (long long)(workspace ? workspace_bytes : 0));
+    }
+    if (rows == 0 && !dweight) return STM_OK;
+    if (!dx && !dresidual && !dweight) return STM_OK;
+    const NormBwd a{dy,   dh,        h, weight, rstd, dx, dresidual, dweight && rows ? static_cast<float*>(workspace) : nullptr,
+                    rows, (int)cols, h_dtype == STM_F32, weight_dtype == STM_F32};
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == STM_BF16 ? bwd<BF16>(a, dweight, st) : dtype == STM_F16 ? bwd<F16>(a, dweight, st) : bwd<F32>(a, dweight, st);
+}

@@ -1,0 +1,257 @@
+"""GPU tests of the norm with the residual's addition, both directions, against the formulas in 64 bits.
+
+Bounds, per element, u = 2^-24: s = x + residual is one rounding. The sum of squares is taken in chains of at most
+max(64, 8 ceil(cols / 8192)) terms a thread, then over at most 6 + 16 partial sums, all positive: relative error at most
+(chain + 24) u, half of it in 1 / rms, 3 u more for the mean, the root and the quotient; y adds two products. One
+rounding to the type is half a step of the result. The backward's n uses h as it was stored: half a step of h's type
+more, in n and in the mean of t n."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF, FP, F4 = torch.bfloat16, torch.float16, torch.float32
+HALF = {BF: 2.0 ** -8, FP: 2.0 ** -11, F4: 2.0 ** -24}
+TINY = {BF: 0.0, FP: 2.0 ** -25, F4: 0.0}  # half a step of a subnormal result
+
+
+def seeded(shape, seed, std=1.0, dtype=F4):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * std).to(dtype).cuda()
+
+
+def chain(cols):
+    return max(64, 8 * -(-cols // 8192)) + 24
+
+
+def assert_within(got, ref, err, what):
+    assert got.shape == ref.shape, what
+    dtype = got.dtype
+    off = (got.double() - ref).abs() - (HALF[dtype] * ref.abs() + TINY[dtype] + err * (1 + HALF[dtype]))
+    if off.numel():
+        assert not off.isnan().any(), f"{what}: NaN"
+        worst = int(off.argmax())
+        assert off.max() <= 0, f"{what} [{worst}]: {got.reshape(-1)[worst]} for {ref.reshape(-1)[worst]}"
+
+
+def reference(x, w, eps, r=None, dy=None, dh=None, h_dtype=None):
+    """{name: (value, bound)} in 64 bits."""
+    cols = x.shape[-1]
+    s = x.double() if r is None else x.double() + r.double()
+    w = w.double()
+    rstd = (s.square().mean(-1, keepdim=True) + eps).rsqrt()
+    n = s * rstd
+    e_r = (chain(cols) / 2 + 3) * U
+    out = {"y": (n * w, (n * w).abs() * (e_r + 4 * U)), "h": (s, s.abs() * U)}
+    if dy is not None:
+        e_h = HALF[h_dtype] if r is not None else 0.0
+        t = dy.double() * w
+        m = (t * n).mean(-1, keepdim=True)
+        size = (t * n).abs().mean(-1, keepdim=True)
+        ds = rstd * (t - n * m)
+        e_n = e_h + e_r + 2 * U
+        err = rstd * (t.abs() * (e_r + 4 * U) + n.abs() * (size * (e_n + (chain(cols) + 3) * U) + m.abs() * (e_n + e_r + 4 * U)))
+        if dh is not None:
+            ds = ds + dh.double()
+        err = err + 2 * U * ds.abs()
+        if dh is not None:
+            err = err + U * dh.double().abs()
+        out["dx"] = out["dr"] = (ds, err)
+        p = dy.double() * n
+        rows = p.numel() // cols
+        # a thread's rows, the slots of a work-group, 32 chains over the partial sums, 32 of those
+        links = rows / 512 + 512 / 32 + 32 + 32 + rows / 64 * (cols > 32768)
+        out["dw"] = (p.reshape(-1, cols).sum(0), p.abs().reshape(-1, cols).sum(0) * (e_n + (links + 4) * U))
+    return out
+
+
+def check(shape, dtype, residual=None, weight=None, seed=1, eps=1e-6, with_dh=True, backward=True):
+    from stratum_amd import rms_norm
+    cols = shape[-1]
+    x, w = seeded(shape, seed, 1.0, dtype), (1 + seeded((cols,), seed + 1, 0.3)).to(weight or dtype)
+    r = seeded(shape, seed + 2, 2.0, residual) if residual else None
+    with torch.no_grad():
+        got = rms_norm(x, w, eps, r)
+    y, h = got if residual else (got, None)
+    dy = seeded(shape, seed + 3, 1.0, dtype)
+    dh = seeded(shape, seed + 4, 1.0, residual) if residual and with_dh else None
+    ref = reference(x, w, eps, r, dy if backward else None, dh, residual)
+    assert y.dtype == dtype
+    assert_within(y, *ref["y"], "y")
+    if residual:
+        assert h.dtype == residual
+        assert_within(h, *ref["h"], "h")
+    if not backward:
+        return
+    leaves = [t.requires_grad_(True) for t in (x, w, r) if t is not None]
+    got = rms_norm(x, w, eps, r)
+    outs = got if residual else (got,)
+    assert torch.equal(outs[0], y) and (not residual or torch.equal(outs[1], h))
+    used = [(o, g) for o, g in zip(outs, (dy, dh)) if g is not None]
+    grads = torch.autograd.grad([o for o, _ in used], leaves, [g for _, g in used])
+    for name, leaf, g in zip(("dx", "dw", "dr"), leaves, grads):
+        assert g.dtype == leaf.dtype
+        assert_within(g, *ref[name], name)
+
+
+TYPES = [(BF, None, BF), (BF, BF, BF), (FP, F4, F4), (FP, FP, FP), (F4, F4, F4), (BF, F4, BF), (F4, None, F4)]
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (2, 8), (3, 64), (5, 65), (2, 128), (17, 129), (9, 256), (33, 257),
+                                   (7, 512), (3, 513), (1, 2048), (2, 2050), (3, 4100), (2, 8192), (1, 8200), (2, 20001),
+                                   (2, 32768)])
+def test_widths_and_types(cuda, shape, types):
+    dtype, residual, weight = types
+    check(shape, dtype, residual, weight, seed=sum(shape))
+
+
+@pytest.mark.parametrize("types", [(BF, BF, BF), (FP, F4, FP), (F4, None, F4)])
+@pytest.mark.parametrize("shape", [(2048, 513), (2050, 1001), (2100, 2048), (2049, 4096), (2048, 4104), (5000, 128),
+                                   (9001, 80), (30000, 64), (4097, 40), (1500, 8192)])
+def test_many_rows(cuda, shape, types):
+    dtype, residual, weight = types
+    check(shape, dtype, residual, weight, seed=sum(shape))
+
+
+@pytest.mark.parametrize("types", [(BF, BF, F4), (F4, None, F4)])
+@pytest.mark.parametrize("shape", [(3, 32769), (70, 40000), (1, 100003)])
+def test_rows_longer_than_the_registers(cuda, shape, types):
+    dtype, residual, weight = types
+    check(shape, dtype, residual, weight, seed=sum(shape))
+
+
+def test_leading_sizes_and_only_some_gradients(cuda):
+    from stratum_amd import rms_norm
+    check((2, 3, 5, 96), BF, BF)
+    check((3, 96), FP, F4, with_dh=False)
+    x, w, r = seeded((4, 96), 1, 1.0, BF), seeded((96,), 2, 1.0, BF), seeded((4, 96), 3, 1.0, F4)
+    every = {}
+    for names in ("x", "w", "r", "xw", "xr", "wr", "xwr"):
+        leaves = {n: t.clone().requires_grad_(n in names) for n, t in zip("xwr", (x, w, r))}
+        y, h = rms_norm(leaves["x"], leaves["w"], 1e-6, leaves["r"])
+        wanted = [leaves[n] for n in names]
+        for n, g in zip(names, torch.autograd.grad((y, h), wanted, (x, r))):
+            assert torch.equal(every.setdefault(n, g), g)
+    # only the sum went on: its gradient is both summands'
+    a, b = x.clone().requires_grad_(True), r.clone().requires_grad_(True)
+    _, h = rms_norm(a, w, 1e-6, b)
+    ga, gb = torch.autograd.grad(h, (a, b), r)
+    assert torch.equal(gb, r) and torch.equal(ga, r.to(BF)) and ga.dtype == BF
+
+
+def test_layouts_of_inputs_and_gradients(cuda):
+    """Strided rows, columns that start off 16 bytes, expanded gradients: the contiguous copies' results."""
+    from stratum_amd import rms_norm
+    base = seeded((6, 3 * 130), 1, 1.0, BF)
+    x, r, w = base[:, 3:133], base[:, 130:260].t().contiguous().t(), seeded((131,), 2, 1.0, BF)[1:]
+    want = rms_norm(x.contiguous(), w.clone(), 1e-6, r.contiguous())
+    got = rms_norm(x, w, 1e-6, r)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    dy = seeded((6, 1), 3, 1.0, BF).expand(6, 130)
+    grads = []
+    for a, b, c, g in ((x, w, r, dy), (x.contiguous(), w.clone(), r.contiguous(), dy.contiguous())):
+        leaves = [t.detach().requires_grad_(True) for t in (a, b, c)]
+        y, h = rms_norm(leaves[0], leaves[1], 1e-6, leaves[2])
+        grads.append(torch.autograd.grad((y, h), leaves, (g, g)))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    # tensors of another step between the elements' and 16 bytes
+    flat = seeded((1 + 5 * 96,), 4, 1.0, FP)
+    odd = flat[1:].view(5, 96)
+    assert torch.equal(rms_norm(odd, w[:96].to(FP)), rms_norm(odd.clone(), w[:96].to(FP)))
+
+
+def test_no_rows_and_no_columns(cuda):
+    from stratum_amd import rms_norm
+    w = torch.ones(16, dtype=BF, device=cuda, requires_grad=True)
+    x = torch.empty(0, 16, dtype=BF, device=cuda, requires_grad=True)
+    y, h = rms_norm(x, w, 1e-6, x.detach())
+    assert y.shape == h.shape == (0, 16)
+    dx, dw = torch.autograd.grad(y, (x, w), y)
+    assert dx.shape == (0, 16) and torch.equal(dw, torch.zeros_like(w))
+    assert rms_norm(x.detach().reshape(0, 4, 16), w.detach()).shape == (0, 4, 16)
+    assert rms_norm(torch.empty(3, 0, dtype=BF, device=cuda), w.detach()[:0]).shape == (3, 0)
+
+
+def test_values_that_are_not_finite_stay_in_their_row(cuda):
+    from stratum_amd import rms_norm
+    x, w = seeded((6, 300), 1), seeded((300,), 2)
+    clean = rms_norm(x, w)
+    for bad in (float("nan"), float("inf")):
+        z = x.clone()
+        z[2, 17] = bad
+        got = rms_norm(z, w)
+        keep = torch.tensor([0, 1, 3, 4, 5], device=cuda)
+        assert torch.equal(got[keep], clean[keep]) and got[2, 17].isnan()
+    zero = rms_norm(torch.zeros(2, 300, device=cuda), w)
+    assert torch.equal(zero, torch.zeros_like(zero))
+    tiny = rms_norm(torch.full((2, 300), 1e-30, device=cuda), w, 0.25)  # eps alone
+    assert_within(tiny, (w.double() * 2e-30).expand(2, 300), w.double().abs() * 2e-30 * 20 * U, "eps")
+
+
+def test_the_gradient_against_differences(cuda):
+    """Directional differences of the fp32 forward at two steps: their distance bounds what the shorter one
+    leaves out; the forward's own error divided by the step is the noise."""
+    from stratum_amd import rms_norm
+    x, r, w = seeded((3, 200), 1), seeded((3, 200), 2), seeded((200,), 3)
+    dy, dh = seeded((3, 200), 4), seeded((3, 200), 5)
+    way = [seeded(t.shape, 6 + i) for i, t in enumerate((x, w, r))]
+
+    def value(e):
+        y, h = rms_norm(x + e * way[0], w + e * way[1], 1e-6, r + e * way[2])
+        return ((y.double() * dy).sum() + (h.double() * dh).sum()).item()
+
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, r)]
+    y, h = rms_norm(leaves[0], leaves[1], 1e-6, leaves[2])
+    grads = torch.autograd.grad((y, h), leaves, (dy, dh))
+    slope = sum((g.double() * d).sum().item() for g, d in zip(grads, way))
+    e = 2.0 ** -6
+    short, long = ((value(s) - value(-s)) / (2 * s) for s in (e, 2 * e))
+    noise = (chain(200) * U) * ((y.abs() * dy.abs()).sum() + (h.abs() * dh.abs()).sum()).item() / e
+    assert abs(slope - short) <= abs(long - short) + noise
+
+
+def test_the_weights_gradient_is_the_same_in_every_run(cuda):
+    from stratum_amd import rms_norm
+    x, w = seeded((5000, 512), 1, 1.0, BF).requires_grad_(True), seeded((512,), 2, 1.0, F4).requires_grad_(True)
+    dy = seeded((5000, 512), 3, 1.0, BF)
+    first = None
+    for _ in range(3):
+        got = torch.autograd.grad(rms_norm(x, w), (x, w), dy)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+def test_more_elements_than_2_to_the_31(cuda):
+    from stratum_amd import rms_norm
+    rows, cols = 1 << 20, 2112
+    x = torch.empty(rows, cols, dtype=BF, device=cuda).normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    w = seeded((cols,), 2, 1.0, BF)
+    y = rms_norm(x, w)
+    for row in (0, 1 << 19, rows - 3):
+        some = x[row:row + 3]
+        assert_within(y[row:row + 3], *reference(some, w, 1e-6)["y"], f"row {row}")
+    del y
+    x.requires_grad_(True)
+    dx, = torch.autograd.grad(rms_norm(x, w), x, x.detach())
+    for row in (0, 1 << 19, rows - 3):
+        some = x.detach()[row:row + 3]
+        assert_within(dx[row:row + 3], *reference(some, w, 1e-6, None, some)["dx"], f"row {row}")
+
+
+def test_module_and_streams(cuda):
+    from stratum_amd import RMSNorm, rms_norm
+    norm = RMSNorm(96, eps=1e-5, dtype=BF, device=cuda)
+    with torch.no_grad():
+        norm.weight.copy_(seeded((96,), 1))
+    x, r = seeded((4, 96), 2, 1.0, BF), seeded((4, 96), 3, 1.0, BF)
+    assert torch.equal(norm(x), rms_norm(x, norm.weight, 1e-5))
+    assert all(torch.equal(a, b) for a, b in zip(norm(x, r), rms_norm(x, norm.weight, 1e-5, r)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = norm(x, r)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, norm(x, r)))
