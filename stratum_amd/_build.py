@@ -14,7 +14,7 @@ SOURCES = ["nf4_abi.hip", "nf4_quant.hip", "nf4_gemm.hip", "swiglu.hip", "lora.h
            "optim.hip", "norm.hip", "moe.hip"]
 
 # The host code of launch-bound calls, a CPython module against torch's headers.
-FAST_SOURCE = "fast_path.cpp"
+FAST_SOURCES = ["fast_path.cpp", "sparse_path.cpp"]
 FAST_PATH = os.path.join(PKG_DIR, "_fast.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -63,17 +63,23 @@ def _finish(proc: subprocess.Popen, what: str, verbose: bool) -> None:
         print("\n".join(msgs), flush=True)
 
 
-def _start_fast(out: str, verbose: bool) -> subprocess.Popen:
+def _fast_compile(src: str, obj: str, verbose: bool) -> subprocess.Popen:
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
     include = [sysconfig.get_paths()["include"], os.path.join(root, "include"),
-               os.path.join(root, "include", "torch", "csrc", "api", "include")]
-    return _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+               os.path.join(root, "include", "torch", "csrc", "api", "include"), "/opt/rocm/include"]
+    return _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__",
                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-                 *(f"-I{d}" for d in include), os.path.join(CSRC, FAST_SOURCE), "-o", out,
-                 "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"], verbose)
+                 *(f"-I{d}" for d in include), "-c", os.path.join(CSRC, src), "-o", obj], verbose)
+
+
+def _fast_link(objs: list, out: str, verbose: bool) -> subprocess.Popen:
+    import torch
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return _run([os.environ.get("CXX", "g++"), "-shared", "-o", out, *objs, "-L" + lib, "-ltorch_python", "-ltorch_cpu",
+                 "-lc10_hip", "-lc10"], verbose)
 
 
 def build(verbose: bool = False) -> str:
@@ -84,7 +90,7 @@ def build(verbose: bool = False) -> str:
     compile_flags = [f for f in FLAGS if f != "-shared"]
     with tempfile.TemporaryDirectory(prefix="stm_build_") as tmpdir:
         objs, procs = [], []
-        fast = _start_fast(FAST_PATH + ".tmp", verbose)
+        fast = [(_fast_compile(src, os.path.join(tmpdir, src + ".o"), verbose), src) for src in FAST_SOURCES]
         for src in SOURCES:
             obj = os.path.join(tmpdir, os.path.splitext(src)[0] + ".o")
             objs.append(obj)
@@ -93,7 +99,10 @@ def build(verbose: bool = False) -> str:
                           src))
         for proc, src in procs:
             _finish(proc, src, verbose)
-        _finish(fast, FAST_SOURCE, verbose)
+        for proc, src in fast:
+            _finish(proc, src, verbose)
+        _finish(_fast_link([os.path.join(tmpdir, src + ".o") for src in FAST_SOURCES], FAST_PATH + ".tmp", verbose),
+                os.path.basename(FAST_PATH), verbose)
         tmp = LIB_PATH + ".tmp"
         _finish(_run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs], verbose), LIB_NAME,
                 verbose)

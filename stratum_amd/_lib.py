@@ -147,6 +147,29 @@ def fast():
     return _fast
 
 
+_SPARSE = ("stm_last_error", "stm_rms_norm_fwd", "stm_rms_norm_workspace_bytes", "stm_rms_norm_bwd", "stm_moe_route",
+           "stm_moe_route_bwd", "stm_moe_sort_workspace_bytes", "stm_moe_sort", "stm_moe_gather", "stm_moe_combine",
+           "stm_moe_combine_bwd")
+_sparse = None
+
+
+def sparse():
+    """:func:`fast` with the entry points that csrc/sparse_path.cpp calls."""
+    global _sparse
+    if _sparse is None:
+        module = fast()
+        module.sparse_setup([address(name) for name in _SPARSE])
+        _sparse = module
+    return _sparse
+
+
+def taken(what: str, out):
+    """*out* of a native call that was given checked operands."""
+    if out is None:
+        raise RuntimeError(f"{what}: the native host code does not take these operands")
+    return out
+
+
 @functools.lru_cache(maxsize=None)
 def address(name: str) -> int:
     """Address of an entry point, for native callers."""

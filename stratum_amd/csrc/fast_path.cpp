@@ -305,4 +305,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", "Host code of launch-bound
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fast(void) { return PyModule_Create(&module); }
+extern PyMethodDef stm_sparse_methods[];  // sparse_path.cpp
+
+PyMODINIT_FUNC PyInit__fast(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddFunctions(m, stm_sparse_methods) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -19,17 +19,17 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd import forward_ad
 
 from . import _lib
 from .functional import (_on_device, _rows, fused_supported, nf4_grouped_gemm, quantize_4bit, swiglu_bwd,
                          swiglu_fwd)
-from .norm import rms_norm
+from .norm import _plain
 
 __all__ = ["MoEOrder", "NF4MoE", "moe_combine", "moe_gather", "moe_route", "moe_sort"]
 
 SCORES = {"softmax": 0, "sigmoid": 1}
 GROUP_SCORES = {"max": 0, "top2": 1}
+MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 64, 64
 
 
 class MoEOrder(NamedTuple):
@@ -46,63 +46,34 @@ def _gpu(t: torch.Tensor, what: str) -> torch.device:
     return t.device
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return t.data_ptr() if t is not None else None
-
-
-def _dual(*tensors) -> bool:
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+def _slots(what: str, n: int) -> None:
+    if n >= 1 << 31:
+        raise ValueError(f"{what}: {n} slots are too many (2^31 - 1)")
 
 
 # ------------------------------------------------------------ route
-def _route_fwd(logits, bias, mask, top_k, score, groups, top_groups, sums, renormalize, scale):
-    dev, tag = _gpu(logits, "moe_route"), _lib.dtype_tag(logits.dtype)
+def _check_route(logits, bias, mask, top_k, groups, top_groups) -> None:
+    dev = _gpu(logits, "moe_route")
+    _lib.dtype_tag(logits.dtype)
     if logits.dim() < 1:
         raise ValueError("logits must be [..., experts]")
     E, lead = int(logits.shape[-1]), tuple(logits.shape[:-1])
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"1 to {MAX_EXPERTS} experts, got {E}")
+    if not 1 <= top_k <= min(E, MAX_TOP_K):
+        raise ValueError(f"top_k must be from 1 to min(experts, {MAX_TOP_K}), got {top_k} of {E} experts")
+    if not 1 <= groups <= MAX_GROUPS or E % groups:
+        raise ValueError(f"{E} experts do not make {groups} groups (1 to {MAX_GROUPS})")
+    if not 1 <= top_groups <= groups:
+        raise ValueError(f"top_groups must be from 1 to {groups}, got {top_groups}")
+    if top_k > E // groups * top_groups:
+        raise ValueError(f"{top_groups} groups of {E // groups} hold fewer than {top_k} experts")
     _on_device(dev, bias=bias, mask=mask)
     if bias is not None and (tuple(bias.shape) != (E,) or bias.dtype != torch.float32):
         raise ValueError(f"bias must be float32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
     if mask is not None and (tuple(mask.shape) != lead or mask.dtype != torch.bool):
         raise ValueError(f"mask must be bool {lead}, got {mask.dtype} {tuple(mask.shape)}")
-    if not 1 <= top_k <= min(E, 64):
-        raise ValueError(f"top_k must be from 1 to min(experts, 64), got {top_k} of {E} experts")
-    rows = _rows(logits, E).contiguous()
-    m = mask.contiguous() if mask is not None else None
-    b = bias.contiguous() if bias is not None else None
-    weights = torch.empty(*lead, top_k, dtype=torch.float32, device=dev)
-    experts = torch.empty(*lead, top_k, dtype=torch.int32, device=dev)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().stm_moe_route(rows.data_ptr(), _ptr(b), _ptr(m), weights.data_ptr(), experts.data_ptr(),
-                                      rows.shape[0], E, top_k, score, groups, top_groups, sums, int(renormalize),
-                                      float(scale), tag, _lib.stream_handle(dev))
-    _lib.check(rc, "stm_moe_route")
-    return weights, experts
-
-
-class _RouteFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, mask, top_k, score, groups, top_groups, sums, renormalize, scale):
-        weights, experts = _route_fwd(logits, bias, mask, top_k, score, groups, top_groups, sums, renormalize, scale)
-        ctx.args = top_k, score, int(renormalize), float(scale)
-        ctx.save_for_backward(logits, experts)
-        ctx.mark_non_differentiable(experts)
-        return weights, experts
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dweights, _):
-        logits, experts = ctx.saved_tensors
-        E, dev = int(logits.shape[-1]), logits.device
-        rows = _rows(logits, E).contiguous()
-        dw = dweights.contiguous()
-        dl = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        with _lib.device_guard(dev):
-            rc = _lib.lib().stm_moe_route_bwd(dw.data_ptr(), rows.data_ptr(), experts.data_ptr(), dl.data_ptr(),
-                                              rows.shape[0], E, *ctx.args, _lib.dtype_tag(logits.dtype),
-                                              _lib.stream_handle(dev))
-        _lib.check(rc, "stm_moe_route_bwd")
-        return dl, None, None, None, None, None, None, None, None, None
+    _slots("moe_route", logits.numel() // E * top_k)
 
 
 def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -121,17 +92,19 @@ def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias:
 
     ``mask`` (bool [...]) is False for tokens that take no part: their experts are -1, their weights 0 and
     nothing of their logits matters. An expert whose logit (or key) is -inf is never chosen; slots left over hold
-    -1 and 0 too. Differentiable in the logits through the weights (reverse mode), not in the bias."""
+    -1 and 0 too. Differentiable in the logits through the weights (reverse mode, once), not in the bias."""
     if score not in SCORES:
         raise ValueError(f"score must be one of {sorted(SCORES)}, got {score!r}")
     if group_score not in GROUP_SCORES:
         raise ValueError(f"group_score must be one of {sorted(GROUP_SCORES)}, got {group_score!r}")
-    args = (logits, bias, mask, int(top_k), SCORES[score], int(groups), int(top_groups), GROUP_SCORES[group_score],
-            renormalize, scale)
-    if not (torch.is_grad_enabled() and logits.requires_grad) and not _dual(logits):
-        with torch.no_grad():
-            return _route_fwd(*args)
-    return _RouteFn.apply(*args)
+    rest = (top_k, SCORES[score], groups, top_groups, GROUP_SCORES[group_score], bool(renormalize), scale)
+    out = _lib.sparse().route(logits, bias, mask, *rest)
+    if out is None:  # an operand to refuse or to convert, or another device than the current one
+        _check_route(logits, bias, mask, top_k, groups, top_groups)
+        logits, bias, mask = _plain("moe_route", logits, bias, mask)
+        with _lib.device_guard(logits.device):
+            out = _lib.taken("moe_route", _lib.sparse().route(logits, bias, mask, *rest))
+    return out
 
 
 # ------------------------------------------------------------ rows by expert
@@ -139,26 +112,18 @@ def moe_sort(experts: torch.Tensor, num_experts: int) -> MoEOrder:
     """The order by expert of the slots ``experts`` (int32 [..., top_k], as :func:`moe_route` gives them): rows of one
     expert keep the slots' order. A slot whose value is not in 0 .. num_experts - 1 (-1) gets no row; as many rows at the
     end stay without a slot. At most 1024 experts."""
-    dev = _gpu(experts, "moe_sort")
-    if experts.dtype != torch.int32 or experts.dim() < 1:
-        raise ValueError(f"experts must be int32 [..., top_k], got {experts.dtype} {tuple(experts.shape)}")
-    num_experts = int(num_experts)
-    if num_experts < 1:
-        raise ValueError(f"num_experts must be positive, got {num_experts}")
-    e = experts.contiguous()
-    n = e.numel()
-    nbytes = int(_lib.lib().stm_moe_sort_workspace_bytes(n, num_experts))
-    if nbytes < 0:
-        _lib.check(nbytes, "stm_moe_sort_workspace_bytes")
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    slots = torch.empty(n, dtype=torch.int32, device=dev)
-    positions = torch.empty(experts.shape, dtype=torch.int32, device=dev)
-    ws = torch.empty(nbytes // 4, dtype=torch.int32, device=dev) if nbytes else None
-    with _lib.device_guard(dev):
-        rc = _lib.lib().stm_moe_sort(e.data_ptr(), n, num_experts, offsets.data_ptr(), slots.data_ptr(),
-                                     positions.data_ptr(), _ptr(ws), nbytes, _lib.stream_handle(dev))
-    _lib.check(rc, "stm_moe_sort")
-    return MoEOrder(offsets, slots, positions)
+    out = _lib.sparse().sort(experts, num_experts)
+    if out is None:
+        dev = _gpu(experts, "moe_sort")
+        if experts.dtype != torch.int32 or experts.dim() < 1:
+            raise ValueError(f"experts must be int32 [..., top_k], got {experts.dtype} {tuple(experts.shape)}")
+        if not 1 <= num_experts <= MAX_EXPERTS:
+            raise ValueError(f"1 to {MAX_EXPERTS} experts, got {num_experts}")
+        _slots("moe_sort", experts.numel())
+        (experts,) = _plain("moe_sort", experts)
+        with _lib.device_guard(dev):
+            out = _lib.taken("moe_sort", _lib.sparse().sort(experts, num_experts))
+    return MoEOrder(*out)
 
 
 def _check_order(order: MoEOrder, dev: torch.device) -> tuple:
@@ -167,68 +132,30 @@ def _check_order(order: MoEOrder, dev: torch.device) -> tuple:
     for name, t in (("offsets", offsets), ("slots", slots), ("positions", positions)):
         if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
             raise ValueError(f"order.{name} must be contiguous int32 on {dev}, got {t.dtype} on {t.device}")
-    if positions.dim() < 1 or slots.numel() != positions.numel() or offsets.numel() < 2:
-        raise ValueError("order must be that of moe_sort")
+    if positions.dim() < 1 or positions.shape[-1] < 1 or slots.numel() != positions.numel() or offsets.numel() < 2:
+        raise ValueError("order must be that of moe_sort, of at least one slot a token")
     top_k = int(positions.shape[-1])
-    return (positions.numel() // top_k if top_k else 0), top_k
-
-
-def _gather_fwd(x, order):
-    dev, tag = _gpu(x, "moe_gather"), _lib.dtype_tag(x.dtype)
-    tokens, top_k = _check_order(order, dev)
-    hidden = int(x.shape[-1]) if x.dim() else 0
-    if x.dim() < 2 or x.numel() != tokens * hidden:
-        raise ValueError(f"x must hold [{tokens}, hidden], got {tuple(x.shape)}")
-    x2 = x.contiguous()
-    out = torch.empty(tokens * top_k, hidden, dtype=x.dtype, device=dev)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().stm_moe_gather(x2.data_ptr(), order.positions.data_ptr(), order.offsets.data_ptr(),
-                                       order.offsets.numel() - 1, out.data_ptr(), tokens, top_k, hidden, tag,
-                                       _lib.stream_handle(dev))
-    _lib.check(rc, "stm_moe_gather")
-    return out
-
-
-def _combine_fwd(y, weights, positions, residual, shape):
-    dev = y.device
-    tokens, top_k, hidden = positions.numel() // max(int(positions.shape[-1]), 1), int(positions.shape[-1]), int(y.shape[-1])
-    y2 = y.contiguous()
-    w = weights.contiguous() if weights is not None else None
-    r = residual.contiguous() if residual is not None else None
-    out = torch.empty(shape, dtype=y.dtype if r is None else r.dtype, device=dev)
-    with _lib.device_guard(dev):
-        rc = _lib.lib().stm_moe_combine(y2.data_ptr(), y2.shape[0], _ptr(w), positions.data_ptr(), _ptr(r), out.data_ptr(),
-                                        _lib.dtype_tag(out.dtype), tokens, top_k, hidden, _lib.dtype_tag(y.dtype),
-                                        _lib.stream_handle(dev))
-    _lib.check(rc, "stm_moe_combine")
-    return out
-
-
-class _GatherFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, offsets, slots, positions):
-        ctx.save_for_backward(positions)
-        ctx.shape = x.shape
-        return _gather_fwd(x, MoEOrder(offsets, slots, positions))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        (positions,) = ctx.saved_tensors
-        return _combine_fwd(grad, None, positions, None, ctx.shape), None, None, None
+    return positions.numel() // top_k, top_k
 
 
 def moe_gather(x: torch.Tensor, order: MoEOrder) -> torch.Tensor:
     """The rows of ``x`` [..., hidden] in the order ``order`` of its slots: [tokens * top_k, hidden], row p the row of
-    slot ``order.slots[p]``'s token, zeros where there is no slot. Differentiable in x: the gradient of a
-    token is the sum, in 32 bits, over its slots."""
-    if not (torch.is_grad_enabled() and x.requires_grad) and not _dual(x):
-        with torch.no_grad():
-            return _gather_fwd(x, order)
-    return _GatherFn.apply(x, *order)
+    slot ``order.slots[p]``'s token, zeros where there is no slot. Differentiable in x (reverse mode, once): the
+    gradient of a token is the sum, in 32 bits, over its slots."""
+    out = _lib.sparse().gather(x, order)
+    if out is None:
+        dev = _gpu(x, "moe_gather")
+        _lib.dtype_tag(x.dtype)
+        tokens, _ = _check_order(order, dev)
+        if x.dim() < 2 or x.numel() != tokens * x.shape[-1]:
+            raise ValueError(f"x must hold [{tokens}, hidden], got {tuple(x.shape)}")
+        x, *order = _plain("moe_gather", x, *order)
+        with _lib.device_guard(dev):
+            out = _lib.taken("moe_gather", _lib.sparse().gather(x, tuple(order)))
+    return out
 
 
-def _check_combine(y, weights, order, residual):
+def _check_combine(y, weights, order, residual) -> None:
     dev = _gpu(y, "moe_combine")
     _lib.dtype_tag(y.dtype)
     tokens, top_k = _check_order(order, dev)
@@ -239,58 +166,26 @@ def _check_combine(y, weights, order, residual):
         raise ValueError(f"weights must be float32 {tuple(order.positions.shape)}, got {weights.dtype} "
                          f"{tuple(weights.shape)}")
     hidden = int(y.shape[1])
-    if residual is None:
-        return (*order.positions.shape[:-1], hidden)
-    if residual.dtype not in (y.dtype, torch.float32) or residual.numel() != tokens * hidden or residual.shape[-1:] != y.shape[1:]:
-        raise ValueError(f"residual must be {y.dtype} or float32 [{tokens}, {hidden}], got {residual.dtype} {tuple(residual.shape)}")
-    return tuple(residual.shape)
-
-
-class _CombineFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, offsets, slots, positions, residual, shape):
-        need_y, need_w = ctx.needs_input_grad[:2]
-        (ctx.rows, ctx.hidden), ctx.dtype = y.shape, y.dtype
-        ctx.save_for_backward(y if need_w else None, weights if need_y else None, offsets, positions)
-        return _combine_fwd(y, weights, positions, residual, shape)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        y, weights, offsets, positions = ctx.saved_tensors
-        need_y, need_w = ctx.needs_input_grad[:2]
-        dev = grad.device
-        dy = dw = None
-        if need_y or need_w:
-            g = grad.contiguous()
-            y2 = y.contiguous() if need_w else None
-            w = weights.contiguous() if need_y else None
-            dy = torch.empty(ctx.rows, ctx.hidden, dtype=ctx.dtype, device=dev) if need_y else None
-            dw = torch.empty(positions.shape, dtype=torch.float32, device=dev) if need_w else None
-            top_k = int(positions.shape[-1])
-            with _lib.device_guard(dev):
-                rc = _lib.lib().stm_moe_combine_bwd(
-                    g.data_ptr(), _lib.dtype_tag(g.dtype), _ptr(y2), ctx.rows, _ptr(w), positions.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
-                    _ptr(dy), _ptr(dw), positions.numel() // max(top_k, 1), top_k, ctx.hidden, _lib.dtype_tag(ctx.dtype),
-                    _lib.stream_handle(dev))
-            _lib.check(rc, "stm_moe_combine_bwd")
-        return dy, dw, None, None, None, grad if ctx.needs_input_grad[5] else None, None
+    if residual is not None and (residual.dtype not in (y.dtype, torch.float32) or residual.numel() != tokens * hidden
+                                 or residual.shape[-1:] != y.shape[1:]):
+        raise ValueError(f"residual must be {y.dtype} or float32 [{tokens}, {hidden}], got {residual.dtype} "
+                         f"{tuple(residual.shape)}")
 
 
 def moe_combine(y: torch.Tensor, weights: torch.Tensor, order: MoEOrder,
                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``residual[t] + sum over j of weights[t, j] * y[order.positions[t, j]]`` for every token, in the residual's dtype
-    (y's without one): fp32 sums, one rounding. ``y`` [rows, hidden] holds the experts' rows in ``order``, all of them or the first
-    ``order.offsets[-1]``; ``weights`` is float32 [..., top_k]; ``residual`` (optional) [..., hidden], in y's dtype
-    or float32, gives the result its shape. A slot without a row adds nothing, whatever its weight. Differentiable in y, the weights and the
-    residual; rows of y that no slot has get a gradient of zeros."""
-    shape = _check_combine(y, weights, order, residual)
-    grad = torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad or
-                                        (residual is not None and residual.requires_grad))
-    if not grad and not _dual(y, weights, residual):
-        with torch.no_grad():
-            return _combine_fwd(y, weights, order.positions, residual, shape)
-    return _CombineFn.apply(y, weights, *order, residual, shape)
+    (y's without one): fp32 sums, one rounding. ``y`` [rows, hidden] holds the experts' rows in ``order``, all of them or
+    the first ``order.offsets[-1]``; ``weights`` is float32 [..., top_k]; ``residual`` (optional) [..., hidden], in y's dtype
+    or float32, gives the result its shape. A slot without a row adds nothing, whatever its weight. Differentiable in
+    y, the weights and the residual (reverse mode, once); rows of y that no slot has get a gradient of zeros."""
+    out = _lib.sparse().combine(y, weights, order, residual)
+    if out is None:
+        _check_combine(y, weights, order, residual)
+        y, weights, residual, *order = _plain("moe_combine", y, weights, residual, *order)
+        with _lib.device_guard(y.device):
+            out = _lib.taken("moe_combine", _lib.sparse().combine(y, weights, tuple(order), residual))
+    return out
 
 
 # ------------------------------------------------------------ the layer's feed-forward half

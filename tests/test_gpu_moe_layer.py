@@ -202,3 +202,45 @@ def test_a_changed_operand_is_noticed(cuda):
         leaf.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_gradients_are_differentiable_once(cuda):
+    """With create_graph the gradients are there and raise when they are differentiated."""
+    from stratum_amd import moe_combine, moe_gather, moe_route, moe_sort, rms_norm
+    x, w, r = (seeded(s, i).requires_grad_(True) for i, s in enumerate(((4, 16), (16,), (4, 16))))
+    order = moe_sort(torch.arange(8, dtype=torch.int32, device=cuda).view(4, 2) % 5, 5)
+    y, weights = seeded((8, 16), 3).requires_grad_(True), seeded((4, 2), 4).requires_grad_(True)
+    for call, leaves in ((lambda: rms_norm(x, w), (x, w)), (lambda: rms_norm(x, w, 1e-6, r)[0], (x, w, r)),
+                         (lambda: rms_norm(x, w, 1e-6, r)[0], (r,)), (lambda: moe_route(x, 2)[0], (x,)),
+                         (lambda: moe_gather(x, order), (x,)), (lambda: moe_combine(y, weights, order), (y, weights)),
+                         (lambda: moe_combine(y, weights, order, r), (weights, r))):
+        d = torch.ones_like(call())
+        plain = torch.autograd.grad(call(), leaves, d)
+        grads = torch.autograd.grad(call(), leaves, d, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            grads[0].sum().backward()
+
+
+def test_tensor_subclasses(cuda):
+    """Operands of a subclass give the results and gradients of their plain tensors."""
+    from stratum_amd import moe_combine, moe_gather, moe_route, moe_sort, rms_norm
+
+    class Named(torch.Tensor):
+        pass
+
+    x, w, r = seeded((4, 16), 1), seeded((16,), 2), seeded((4, 16), 3)
+    weights, e = moe_route(x, 2)
+    order = moe_sort(e, 16)
+    y = seeded((8, 16), 4)
+    for call, args in ((lambda x, w, r: rms_norm(x, w, 1e-6, r)[0], (x, w, r)), (lambda x: moe_route(x, 2)[0], (x,)),
+                       (lambda x: moe_gather(x, order), (x,)),
+                       (lambda y, w, r: moe_combine(y, w, order, r), (y, weights, r))):
+        results = []
+        for kind in (torch.Tensor, Named):
+            leaves = [t.detach().clone().as_subclass(kind).requires_grad_(True) for t in args]
+            out = call(*leaves)
+            grads = torch.autograd.grad(out, leaves, torch.ones(out.shape, device=cuda))
+            results.append([torch.Tensor(t.detach()) for t in (out, *grads)])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert all(torch.equal(a, b) for a, b in zip(moe_sort(e.as_subclass(Named), 16), order))
