@@ -11,7 +11,7 @@
 // a term that is itself rounded to that type.
 //
 // Bound by bytes. One pass: a row stays in registers between its sum and its result, 8 elements of a thread in one access.
-// A row belongs to 8 to 64 lanes of a wave (no barrier), or to a work-group of 256 or 1024 threads.
+// A row belongs to 8 to 64 lanes of a wave (no barrier), or to 128 to 1024 threads.
 #include <type_traits>
 
 #include "nf4_kernels.h"
@@ -49,6 +49,41 @@ __device__ __forceinline__ void store_as(void* p, bool f32, int64_t at, int n, c
     }
 }
 
+// 8 elements of such a row before their conversion, so that a load can be under way while an earlier row is worked on.
+template <typename Tr>
+struct Loaded {
+    u32x4_t v[2];
+
+    __device__ __forceinline__ void load(const void* p, bool f32, int64_t at, int n) {
+        if (f32) {
+            Eight<F32> e;
+            e.load(p, at, n);
+            v[0] = e.v[0], v[1] = e.v[1];
+        } else {
+            Eight<Tr> e;
+            e.load(p, at, n);
+            if constexpr (sizeof(e) == 32)
+                v[0] = e.v[0], v[1] = e.v[1];
+            else
+                v[0] = __builtin_bit_cast(u32x4_t, e);
+        }
+    }
+    __device__ __forceinline__ void get(bool f32, float (&f)[8]) const {
+        if (f32 || sizeof(Eight<Tr>) == 32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i / 4][i % 4]);
+        } else if constexpr (sizeof(Eight<Tr>) == 16) {
+            const Eight<Tr> e = __builtin_bit_cast(Eight<Tr>, v[0]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = e.get(i);
+        }
+    }
+};
+
+// A work-group holds one row of T threads, or 256 / T of them.
+template <int T>
+constexpr int kBlock = T <= 256 ? 256 : T;
+
 // Sum over the T threads of a row; every one of them gets it. Above a wave through LDS, `turn` alternating between two
 // buffers so that one barrier a sum is enough.
 template <int T>
@@ -56,20 +91,18 @@ __device__ __forceinline__ float row_sum(float v, int turn) {
     if constexpr (T <= 64) {
         return lanes_sum<T>(v);
     } else {
-        __shared__ float part[2][T / 64];
+        __shared__ float part[2][kBlock<T> / 64];
         v = lanes_sum<64>(v);
         float* p = part[turn & 1];
         if ((threadIdx.x & 63) == 0) p[threadIdx.x / 64] = v;
         __syncthreads();
+        p += threadIdx.x / T * (T / 64);
         float s = p[0];
 #pragma unroll
         for (int i = 1; i < T / 64; ++i) s += p[i];
         return s;
     }
 }
-
-template <int T>
-constexpr int kBlock = T <= 256 ? 256 : T;
 
 struct NormFwd {
     const void *x, *res, *w;
@@ -172,11 +205,15 @@ struct NormBwd {
 
 // DW: a thread's columns are the same in every row of its work-group, so the weight's gradient gathers in registers over
 // the rows that the group takes (gridDim rows apart), then over the group's row slots in LDS, and leaves as one row of
-// partial sums; k_rms_dw adds those rows up in a fixed order.
+// partial sums; k_rms_dw adds those rows up in a fixed order. With one vector a thread the next row is asked for before
+// this one's sum: few groups, so that there are few partial sums, would leave the memory idle in between ([8192, 4096] bf16,
+// us, with the sum of the parts: without the weight's gradient 48, with it 60 without and 54 with the look-ahead).
 template <typename Tr, int T, int NV, bool DW>
 __global__ __launch_bounds__(kBlock<T>) void k_rms_bwd(NormBwd a) {
     constexpr int SLOTS = kBlock<T> / T;
+    constexpr bool AHEAD = DW && NV == 1;
     const int t = threadIdx.x % T, slot = threadIdx.x / T;
+    const int64_t stride = (int64_t)gridDim.x * SLOTS;
     float dw[NV][8];
     if (DW) {
 #pragma unroll
@@ -184,21 +221,40 @@ __global__ __launch_bounds__(kBlock<T>) void k_rms_bwd(NormBwd a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) dw[v][i] = 0.0f;
     }
-    int turn = 0;
-    for (int64_t first = (int64_t)blockIdx.x * SLOTS; first < a.rows; first += (int64_t)gridDim.x * SLOTS, ++turn) {
-        const int64_t row = first + slot;
+    Loaded<Tr> dy[NV], h[NV], dh[NV], w_[NV];
+    float rstd = 0.0f;
+    auto ask = [&](int64_t row) {
         const bool on = row < a.rows;
-        const int64_t at = row * a.cols;
-        const float r = on ? a.rstd[row] : 0.0f;
-        float g[NV][8], n_[NV][8];  // t = w dy, n = h r
-        float dot = 0.0f;
+        rstd = on ? a.rstd[row] : 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
+            dy[v].load(a.dy, false, row * a.cols + c, n);
+            h[v].load(a.h, a.h32, row * a.cols + c, n);
+            if (a.dh) dh[v].load(a.dh, a.h32, row * a.cols + c, n);
+        }
+    };
+    int turn = 0;
+    int64_t first = (int64_t)blockIdx.x * SLOTS;
+    if (AHEAD) ask(first + slot);
+    if (NV == 1) w_[0].load(a.w, a.w32, 8 * t, a.cols - 8 * t);
+    for (; first < a.rows; first += stride, ++turn) {
+        const int64_t row = first + slot;
+        const bool on = row < a.rows;
+        const int64_t at = row * a.cols;
+        if (!AHEAD) ask(row);
+        const float r = rstd;
+        float g[NV][8], n_[NV][8], e[NV][8];  // t = w dy, n = h r
+        float dot = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = 8 * (t + T * v);
             float w[8];
-            load_as<Tr>(a.dy, false, at + c, n, g[v]);
-            load_as<Tr>(a.h, a.h32, at + c, n, n_[v]);
-            load_as<Tr>(a.w, a.w32, c, n, w);
+            dy[v].get(false, g[v]);
+            h[v].get(a.h32, n_[v]);
+            if (a.dh) dh[v].get(a.h32, e[v]);
+            if (NV > 1) w_[v].load(a.w, a.w32, c, a.cols - c);
+            w_[v].get(a.w32, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 n_[v][i] *= r;
@@ -207,18 +263,16 @@ __global__ __launch_bounds__(kBlock<T>) void k_rms_bwd(NormBwd a) {
                 dot = __builtin_fmaf(g[v][i], n_[v][i], dot);
             }
         }
+        if (AHEAD) ask(row + stride);
         const float mean = row_sum<T>(dot, turn) / (float)a.cols;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
             float d[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = r * (g[v][i] - n_[v][i] * mean);
-            if (a.dh) {
-                float e[8];
-                load_as<Tr>(a.dh, a.h32, at + c, n, e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] += e[i];
+            for (int i = 0; i < 8; ++i) {
+                d[i] = r * (g[v][i] - n_[v][i] * mean);
+                if (a.dh) d[i] += e[v][i];
             }
             if (a.dx) store_as<Tr>(a.dx, false, at + c, n, d);
             if (a.dres) store_as<Tr>(a.dres, a.h32, at + c, n, d);
@@ -303,7 +357,8 @@ __global__ __launch_bounds__(256) void k_rms_dw_long(NormBwd a) {
     store_as<F32>(a.dw_part + (int64_t)blockIdx.y * a.cols, true, c, n, dw);
 }
 
-// Sum of `parts` rows of partial sums: 32 columns a work-group, its 32 row slots added up in LDS.
+// Sum of `parts` rows of partial sums: 32 columns a work-group, its 32 row slots added up in LDS. A slot's rows are
+// asked for eight at a time.
 template <typename Tr>
 __global__ __launch_bounds__(1024) void k_rms_dw(const float* __restrict__ part, int parts, int cols, void* dw,
                                                  bool w32) {
@@ -311,7 +366,13 @@ __global__ __launch_bounds__(1024) void k_rms_dw(const float* __restrict__ part,
     const int c = blockIdx.x * 32 + threadIdx.x % 32, slot = threadIdx.x / 32;
     float s = 0.0f;
     if (c < cols)
-        for (int p = slot; p < parts; p += 32) s += part[(int64_t)p * cols + c];
+        for (int p0 = slot; p0 < parts; p0 += 32 * 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p0 + 32 * i < parts ? part[(int64_t)(p0 + 32 * i) * cols + c] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
     sum[slot][threadIdx.x % 32] = s;
     __syncthreads();
     if (slot || c >= cols) return;
@@ -332,24 +393,26 @@ unsigned row_groups(int64_t rows, int per) {
 
 constexpr int64_t kRegisterCols = 1024 * 4 * 8;
 
-// Threads of a row. Up to 512 columns one vector a thread; above that a wave takes a row of up to 4096 columns where
-// there are rows enough to fill the GPU with waves (no barrier), else 256 threads of up to 4 vectors, then 1024.
-int row_threads(int64_t rows, int64_t cols) {
+// Threads of a row: one vector each, up to 8192 columns; whole pairs of waves where that is more than a wave of them
+// ([8192, 5120] backward: 640 threads 67, 1024 80). More vectors a thread are slower, whether a wave then needs no
+// barrier or not ([8192, 4096] bf16 with a residual, us forward / backward: 64 threads of 8 vectors 55 / 115, 128 of 4
+// 55 / 61, 256 of 2 51 / 52, 512 of 1 49 / 48; [4096, 8192]: 256 57 / 59, 512 53 / 55, 1024 51 / 50).
+int row_threads(int64_t cols) {
     const int64_t vecs = (cols + 7) / 8;
-    if (vecs <= 8) return 8;
-    if (vecs <= 16) return 16;
-    if (vecs <= 32) return 32;
-    if (vecs <= 64) return 64;
-    if (vecs <= 512 && rows >= 2048) return 64;
-    return vecs <= 1024 ? 256 : 1024;
+    if (vecs > 256) return vecs < 1024 ? (int)(vecs + 127) / 128 * 128 : 1024;
+    int t = 8;
+    while (t < vecs) t *= 2;
+    return t;
 }
 
-// Groups of the backward's grid that write partial sums.
+// Groups of the backward's grid that write partial sums: as many as give each of the 256 compute units up to 1024 threads
+// and the same work ([8192, 4096] us: 256 groups of 512 threads 67, 384 60, 512 54, 768 61, 1024 58; [131072, 128], 256
+// threads: 512 34, 1024 28, 2048 33; [8192, 5120], 640 threads: 256 77, 384 96, 512 79).
 int dw_groups(int64_t rows, int64_t cols) {
     if (cols > kRegisterCols) return (int)(rows < 64 ? rows : 64);
-    const int t = row_threads(rows, cols), slots = t <= 256 ? 256 / t : 1;
-    const int64_t groups = (rows + slots - 1) / slots;
-    return (int)(groups < 512 ? groups : 512);
+    const int t = row_threads(cols), slots = t <= 256 ? 256 / t : 1, threads = t <= 256 ? 256 : t;
+    const int64_t groups = (rows + slots - 1) / slots, most = 256 * (1024 / threads);
+    return (int)(groups < most ? groups : most);
 }
 
 template <typename F>
@@ -360,12 +423,14 @@ int each_form(int t, int nv, F f) {
     STM_FORM(16, 1);
     STM_FORM(32, 1);
     STM_FORM(64, 1);
-    STM_FORM(64, 2);
-    STM_FORM(64, 4);
-    STM_FORM(64, 8);
+    STM_FORM(128, 1);
     STM_FORM(256, 1);
-    STM_FORM(256, 2);
-    STM_FORM(256, 4);
+    STM_FORM(384, 1);
+    STM_FORM(512, 1);
+    STM_FORM(640, 1);
+    STM_FORM(768, 1);
+    STM_FORM(896, 1);
+    STM_FORM(1024, 1);
     STM_FORM(1024, 2);
     STM_FORM(1024, 4);
 #undef STM_FORM
@@ -378,7 +443,7 @@ int fwd(const NormFwd& a, hipStream_t st) {
         hipLaunchKernelGGL(k_rms_fwd_long<Tr>, dim3(row_groups(a.rows, 1)), dim3(1024), 0, st, a);
         return check_launch("rms_norm_fwd");
     }
-    const int t = row_threads(a.rows, a.cols), nv = (a.cols + 8 * t - 1) / (8 * t);
+    const int t = row_threads(a.cols), nv = (a.cols + 8 * t - 1) / (8 * t);
     return each_form(t, nv, [&](auto T, auto NV) {
         constexpr int per = kBlock<T.value> / T.value;
         hipLaunchKernelGGL((k_rms_fwd<Tr, T.value, NV.value>), dim3(row_groups(a.rows, per)),
@@ -397,7 +462,7 @@ int bwd(const NormBwd& a, void* dweight, hipStream_t st) {
             hipLaunchKernelGGL(k_rms_dw_long<Tr>, dim3((unsigned)((a.cols + 2047) / 2048), (unsigned)parts), dim3(256), 0,
                                st, a);
     } else {
-        const int t = row_threads(a.rows, a.cols), nv = (a.cols + 8 * t - 1) / (8 * t);
+        const int t = row_threads(a.cols), nv = (a.cols + 8 * t - 1) / (8 * t);
         const int rc = each_form(t, nv, [&](auto T, auto NV) {
             constexpr int per = kBlock<T.value> / T.value;
             if (a.dw_part)
