@@ -23,15 +23,20 @@ unsigned groups_for(int64_t items, int per) {
 }
 
 // ------------------------------------------------------------ route
-// A token belongs to LANES lanes, lane l holds experts l * VPL .. l * VPL + VPL - 1, so that among equal keys the lowest
-// lane, and in it the first of its values, is the lowest expert.
+// A token belongs to LANES lanes of a wave, lane l holds experts l * VPL .. l * VPL + VPL - 1. No barrier: what a token has
+// in LDS is its wave's. One expert is taken per round: the maximum over a lane's keys, over the lanes (DPP), the lowest
+// index that holds it. Bound by instructions: with 8 values a lane the steps over the lanes, and the exponentials of
+// the weights, serve two to four tokens at a time (8192 tokens of 128 in bf16, top 8, us: 64 lanes of 2 values 7.4, 16 of 8
+// 4.3).
 //
-// Keys are unsigned integers in the order of the values they stand for, 0 for an expert that cannot be chosen (-inf), NaN
-// above all. Without a bias and without sums over groups the scores are in the order of the logits, which are compared as
-// they are (32 bits, exact). Otherwise score + bias is computed in 64 bits: two experts whose keys differ by less than an
-// fp32 rounding are still told apart, and the same ones are found as by any other program that computes them so.
-//
-// One key is taken per round: the maximum over a lane's values, over the lanes (DPP), the first lane that holds it.
+// Keys are compared as what they stand for, the lowest index first among equal ones; an expert that cannot be chosen
+// has none (-inf; as an unsigned integer 0). Without a bias and without sums over groups the scores are in the order of
+// the logits, which are compared as they are (integers in their order, NaN above all; of 16-bit types the low 10 bits,
+// which are free, hold the index, so that no two are equal and one maximum finds both). Otherwise the keys are those of
+// score + bias in 64 bits: two experts whose keys differ by less than an fp32 rounding are still told apart, and the same
+// ones are found as by any other program that computes them so. They are computed in 32 bits first, with a bound on what that
+// may be off. Where experts that follow each other are nearer than the bound, the keys of those taken are computed in
+// 64 bits, by a lane each; where groups are (or a value is not finite), all of them (16383 tokens of 256, sigmoid, bias, 8 groups, us: always 43, so 29).
 struct Route {
     const void* logits;
     const float* bias;
@@ -63,6 +68,10 @@ __device__ __forceinline__ double value_of(uint64_t k) {
     return __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
 }
 
+__device__ __forceinline__ float value_of(uint32_t k) {
+    return k == ~0u ? __builtin_nanf("") : __uint_as_float(k >> 31 ? k & ~(1u << 31) : ~k);
+}
+
 __device__ __forceinline__ float sigmoid_of(float x) {  // accurate on both sides
     const float e = expf(-fabsf(x));
     return (x < 0.0f ? e : 1.0f) / (1.0f + e);
@@ -74,113 +83,337 @@ __device__ __forceinline__ float logit(const void* logits, int64_t at) {
     return Tr::to_f32(static_cast<const typename Eight<Tr>::elem*>(logits)[at]);
 }
 
-// Best of LANES lanes: its key to all of them, and which lane of the token holds it first.
-template <int LANES, typename Key>
-__device__ __forceinline__ Key take(Key best, int* lane) {
-    const Key top = lanes_max<LANES>(best);
-    const uint64_t holders = __ballot(best == top);
-    const int first = threadIdx.x & 63 & ~(LANES - 1);
-    *lane = __ffsll((unsigned long long)(LANES == 64 ? holders : holders >> first & ((1ull << (LANES % 64)) - 1))) - 1;
-    return top;
+// A lane's N values of a row (of the n that are left), `fill` behind its end; whole ones in one access at any address.
+template <typename Tr, int N>
+struct Few {
+    typedef typename Eight<Tr>::elem elem;
+    typedef elem vec __attribute__((ext_vector_type(N)));
+    typedef vec loose __attribute__((aligned(sizeof(elem))));
+
+    static __device__ __forceinline__ void load(const void* base, int64_t at, int n, float fill, float (&f)[N]) {
+        const elem* p = static_cast<const elem*>(base) + at;
+        if (n >= N) {
+            const vec v = *reinterpret_cast<const loose*>(p);
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = Tr::to_f32(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = i < n ? Tr::to_f32(p[i]) : fill;
+        }
+    }
+    static __device__ __forceinline__ void store(void* base, int64_t at, int n, const float (&f)[N]) {
+        elem* p = static_cast<elem*>(base) + at;
+        if (n >= N) {
+            vec v;
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = Tr::from_f32(f[i]);
+            *reinterpret_cast<loose*>(p) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i < n) p[i] = Tr::from_f32(f[i]);
+        }
+    }
+};
+
+// What the wave wrote to LDS before is there for all its lanes (they execute in order; this holds the compiler to it).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int LANES>
-__device__ __forceinline__ int from_lane(int v, int lane) {
-    if constexpr (LANES == 64) return __builtin_amdgcn_readlane(v, __builtin_amdgcn_readfirstlane(lane));
-    return __shfl(v, lane, LANES);
+template <typename Key>
+__device__ __forceinline__ Key none() {
+    return std::is_same_v<Key, float> ? (Key)-INFINITY : (Key)0;
 }
 
-template <typename Tr, int LANES, int VPL, typename Key>
+template <typename Key>
+__device__ __forceinline__ Key larger(Key a, Key b) {
+    if constexpr (std::is_same_v<Key, float>)
+        return fmaxf(a, b);
+    else
+        return a > b ? a : b;
+}
+
+__device__ __forceinline__ float value_of(float k) { return k; }
+
+__device__ __forceinline__ uint32_t other_lane(uint32_t v, int step) {  // step is uniform
+    return step == 1 ? across<1>(v) : step == 2 ? across<2>(v) : step == 4 ? across<4>(v) : step == 8 ? across<8>(v) :
+           step == 16 ? across<16>(v) : across<32>(v);
+}
+
+__device__ __forceinline__ uint64_t other_lane(uint64_t v, int step) {
+    return (uint64_t)other_lane((uint32_t)(v >> 32), step) << 32 | other_lane((uint32_t)v, step);
+}
+
+__device__ __forceinline__ float other_lane(float v, int step) {
+    return __uint_as_float(other_lane(__float_as_uint(v), step));
+}
+
+// What decides between a token's groups.
+struct Border {
+    float least, next;  // the smallest value of an eligible group, the largest of the others (-inf: none)
+    float size;         // the largest sum of the magnitudes that make a value
+};
+
+// Takes away the keys of the groups that are not eligible. A group belongs to `share` lanes (a power of two), which read
+// its keys back from LDS, `mine` [LANES * VPL]. key: the experts' keys for this; out: those to take away from.
+template <int LANES, int VPL, typename Key, typename Out>
+__device__ __forceinline__ void keep_groups(const Route& a, const Key (&key)[VPL], Out (&out)[VPL], Key* mine, Border* border) {
+    typedef std::conditional_t<LANES <= 32, uint32_t, uint64_t> Bits;
+    const int l = threadIdx.x % LANES, size = a.E / a.groups;
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) mine[l * VPL + i] = key[i];
+    wave_sync();
+    const int bits = 31 - __clz(LANES / a.groups), share = 1 << bits, group = l >> bits;
+    Key best = none<Key>(), second = none<Key>();
+    if (group < a.groups)
+        for (int i = l & (share - 1); i < size; i += share) {
+            const Key k = mine[group * size + i];
+            second = larger(second, k > best ? best : k);
+            best = larger(best, k);
+        }
+    for (int step = 1; step < share; step <<= 1) {
+        const Key b = other_lane(best, step), s = other_lane(second, step);
+        second = larger(larger(second, s), b > best ? best : b);
+        best = larger(best, b);
+    }
+    border->size = 0.0f;
+    if (a.sums && second > none<Key>()) {
+        const auto v = value_of(best), w = value_of(second);
+        border->size = fabsf((float)v) + fabsf((float)w);
+        if constexpr (std::is_same_v<Key, float>)
+            best = v + w;
+        else
+            best = (Key)key_of(v + w);
+    }
+    border->size = lanes_max<LANES>(border->size);
+    Bits kept = 0;
+    Key least = none<Key>();
+    for (int j = 0; j < a.top_groups; ++j) {
+        least = lanes_max<LANES>(best);
+        const uint32_t g = lanes_min<LANES>(best == least ? (uint32_t)group : 63u);
+        if (least > none<Key>()) kept |= (Bits)1 << g;
+        if ((uint32_t)group == g) best = none<Key>();
+    }
+    const Key next = lanes_max<LANES>(best);
+    border->least = (float)value_of(least);
+    border->next = next > none<Key>() ? (float)value_of(next) : -INFINITY;
+    int g = l * VPL / size, left = (g + 1) * size - l * VPL;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        if (g < a.groups && !(kept >> g & 1)) out[i] = none<Out>();
+        if (--left == 0) ++g, left = size;
+    }
+}
+
+// The largest of a token's keys.
+template <int LANES, int VPL, typename Key>
+__device__ __forceinline__ Key largest(const Key (&key)[VPL]) {
+    Key top = key[0];
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) top = larger(top, key[i]);
+    return lanes_max<LANES>(top);
+}
+
+// Takes it away and says whose it is. PACKED: a key's low 10 bits are 1023 - its expert.
+template <int LANES, int VPL, bool PACKED, typename Key>
+__device__ __forceinline__ int take(Key (&key)[VPL], Key top) {
+    const int l = threadIdx.x % LANES;
+    if constexpr (PACKED) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (key[i] == top) key[i] = 0;
+        return 1023 - (int)(top & 1023);
+    } else {
+        uint32_t at = 1u << 20;
+#pragma unroll
+        for (int i = VPL - 1; i >= 0; --i)
+            if (key[i] == top) at = i;
+        const int e = (int)lanes_min<LANES>(at + l * VPL), mine = e - l * VPL;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (mine == i) key[i] = none<Key>();
+        return e;
+    }
+}
+
+// Lane j gets the token's j-th expert (or -1) and its key.
+template <int LANES, int VPL, bool PACKED, typename Key>
+__device__ __forceinline__ int best_experts(const Route& a, Key (&key)[VPL], Key* of) {
+    int chosen = -1;
+    *of = none<Key>();
+    for (int j = 0; j < a.top_k; ++j) {
+        const Key top = largest<LANES, VPL>(key);
+        const int e = take<LANES, VPL, PACKED>(key, top);
+        if ((int)(threadIdx.x % LANES) == j && top > none<Key>()) chosen = e, *of = top;
+    }
+    return chosen;
+}
+
+// SCORES: with a bias, or sums over groups.
+template <typename Tr, int LANES, int VPL, bool SCORES>
 __global__ __launch_bounds__(256) void k_route(Route a) {
+    typedef std::conditional_t<SCORES, uint64_t, uint32_t> Key;
     constexpr int TOKENS = 256 / LANES;
     __shared__ Key grouped[256 * VPL];
-    const int l = threadIdx.x % LANES;
+    const int l = threadIdx.x % LANES, left = a.E - l * VPL;
+    Key* mine = grouped + (threadIdx.x / LANES) * LANES * VPL;
+    float bias[VPL];
+    if constexpr (SCORES)
+        if (a.bias) Few<F32, VPL>::load(a.bias, l * VPL, left, 0.0f, bias);
     for (int64_t first = (int64_t)blockIdx.x * TOKENS; first < a.tokens; first += (int64_t)gridDim.x * TOKENS) {
         const int64_t token = first + threadIdx.x / LANES;
         const bool on = token < a.tokens && !(a.mask && !a.mask[token]);
         const int64_t row = token * a.E;
         float x[VPL];
-        float top = -INFINITY;
+        Few<Tr, VPL>::load(a.logits, row + l * VPL, on ? left : 0, -INFINITY, x);
+        float top = x[0];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const int e = l * VPL + i;
-            x[i] = on && e < a.E ? logit<Tr>(a.logits, row + e) : -INFINITY;
-            top = fmaxf(top, x[i]);
-        }
+        for (int i = 1; i < VPL; ++i) top = fmaxf(top, x[i]);
         top = lanes_max<LANES>(top);
-        Key key[VPL];
+        Border border;
+        int chosen;
+        float c;  // the chosen expert's logit
         bool spoiled = false;  // no score of the token is a number
-        if constexpr (sizeof(Key) == 4) {
+        if constexpr (!SCORES) {
+            constexpr bool PACKED = sizeof(typename Eight<Tr>::elem) == 2;
+            uint32_t key[VPL], of;
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) key[i] = key_of(x[i]);
+            for (int i = 0; i < VPL; ++i) {
+                key[i] = key_of(x[i]);
+                if (PACKED && key[i]) key[i] = (key[i] & ~1023u) | (1023 - (l * VPL + i));
+            }
+            if (a.groups > 1) keep_groups<LANES>(a, key, key, mine, &border);
+            chosen = best_experts<LANES, VPL, PACKED>(a, key, &of);
+            if constexpr (PACKED) {
+                if (of >> 10 == ~0u >> 10) c = __builtin_nanf("");
+                else c = __uint_as_float((of >> 31 ? of & ~(1u << 31) : ~of) & ~1023u);
+            } else {
+                c = value_of(of);
+            }
+            if (chosen < 0) c = -INFINITY;
         } else {
-            double s[VPL], total = 0.0;
+            // In units of u = 2^-24 a score is off by at most, where the exponential is 2^(x log2 e) with a relative error
+            // of 3 |x| + 2 and a reciprocal has 2: sigmoid, e = exp(-|x|), by the exponential ((3 |x| + 2) e, at most 4),
+            // 1 + e (1), the reciprocal (2) and the product with e (1): 8 u; softmax, by the exponential (with d = top - x
+            // (3 d + 2) exp(-d), at most 4), the sum of at most 16 values a lane over 64 lanes (22) of terms that are off by
+            // 3 d + 2 (on average d is at most ln 1024 = 7: 23), the reciprocal and the product (3): 52 u of the largest
+            // score. `off` takes 10 and 56. Adding the bias is off by u of the key; a group's sum by its keys' and u of itself.
+            constexpr float u = 0x1p-24f;
+            float key[VPL], order[VPL], total = 0.0f, off = 10.0f * u;
+            bool close = false;
+            constexpr float log2e = 1.44269504088896340736f;
+            if (a.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                s[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)top);
-                total += x[i] == -INFINITY ? 0.0 : s[i];
-            }
-            if (!a.sigmoid) {
-                total = lanes_sum<LANES>(total);
-                spoiled = total != total;
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) s[i] /= total;
-            }
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                const int e = l * VPL + i;
-                if (a.bias && e < a.E) s[i] += (double)a.bias[e];
-                key[i] = x[i] == -INFINITY ? 0 : key_of(s[i]);
-            }
-        }
-        if (a.groups > 1) {
-            // lane g reads its group's keys back from LDS (groups <= LANES)
-            Key* mine = grouped + (threadIdx.x / LANES) * LANES * VPL;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) mine[l * VPL + i] = key[i];
-            __syncthreads();
-            const int size = a.E / a.groups;
-            Key best = 0, second = 0;
-            if (l < a.groups)
-                for (int i = 0; i < size; ++i) {
-                    const Key k = mine[l * size + i];
-                    second = k > best ? best : k > second ? k : second;
-                    best = k > best ? k : best;
+                for (int i = 0; i < VPL; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(-log2e * fabsf(x[i])), r = __builtin_amdgcn_rcpf(1.0f + e);
+                    key[i] = x[i] < 0.0f ? e * r : r;
                 }
-            if constexpr (sizeof(Key) == 8)
-                if (a.sums && best && second) best = key_of(value_of(best) + value_of(second));
-            uint64_t kept = 0;
-            for (int j = 0; j < a.top_groups; ++j) {
-                int g;
-                if (take<LANES>(best, &g)) kept |= 1ull << g;
-                if (l == g) best = 0;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) {
+                    key[i] = x[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(log2e * (x[i] - top));
+                    total += key[i];
+                }
+                const float r = __builtin_amdgcn_rcpf(lanes_sum<LANES>(total));
+                off = 56.0f * u * r;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) key[i] *= r;
             }
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
-                const int e = l * VPL + i;
-                if (e < a.E && !(kept >> (e / size) & 1)) key[i] = 0;
+                key[i] = x[i] == -INFINITY ? -INFINITY : a.bias ? key[i] + bias[i] : key[i];
+                close |= !(key[i] < INFINITY && x[i] < INFINITY);
+                order[i] = a.bias ? key[i] : x[i];
             }
-            __syncthreads();
-        }
-        int chosen = -1;  // lane j: the token's j-th expert
-        for (int j = 0; j < a.top_k; ++j) {
-            Key best = key[0];
-            int at = 0;
-#pragma unroll
-            for (int i = 1; i < VPL; ++i)
-                if (key[i] > best) best = key[i], at = i;
-            int holder;
-            const Key most = take<LANES>(best, &holder);
-            const int e = from_lane<LANES>(l * VPL + at, holder);
-            if (l == j && most) chosen = e;
-            if (l == holder) {
-#pragma unroll
-                for (int i = 0; i < VPL; ++i)
-                    if (i == at) key[i] = 0;
+            if (a.groups > 1) {
+                keep_groups<LANES>(a, key, order, reinterpret_cast<float*>(mine), &border);
+                const float err = (a.sums ? 2.0f * off + u * border.size : off) +
+                                  u * (fabsf(border.least) + fabsf(border.next));
+                close |= border.next > -INFINITY && !(border.least - border.next > 2.0f * err);
             }
+            // Without a bias the scores are in the order of the logits, and equal where the logits are; that others are
+            // apart in 64 bits too is certain unless they are less than u apart or where the scores end (a sigmoid beyond
+            // 16 is 1 - exp(-x): u exp(-16) is 2^-47; exp(-700) is still normal).
+            // Lane j takes the j-th key, beyond top_k until the next one is smaller for certain.
+            bool mixed = false;
+            float before = 0.0f;
+            int taken = 0;
+            chosen = -1;
+            for (;; ++taken) {
+                const float k = largest<LANES, VPL>(order);
+                bool apart = true;
+                if (taken && k > -INFINITY) {
+                    const float gap = before - k;
+                    apart = a.bias ? gap > 2.0f * (off + u * (fabsf(before) + fabsf(k))) :
+                                     gap == 0.0f || (gap > u && (a.sigmoid ? before <= 16.0f && k > -700.0f : top - k < 700.0f));
+                }
+                mixed |= !apart;
+                if (taken >= a.top_k && !__any(!apart)) break;
+                if (taken == LANES) {
+                    close |= !apart;
+                    break;
+                }
+                const int e = take<LANES, VPL, false>(order, k);
+                if (l == taken && k > -INFINITY) chosen = e;
+                before = k;
+            }
+            // the softmax' sum in 64 bits
+            auto sum64 = [&]() {
+                double sum = 0.0;
+#pragma unroll 1
+                for (int i = 0; i < VPL; ++i) {
+                    const double v = on && i < left ? logit<Tr>(a.logits, row + l * VPL + i) : -INFINITY;
+                    sum += v == -INFINITY ? 0.0 : exp(v - (double)top);
+                }
+                return lanes_sum<LANES>(sum);
+            };
+            auto key64 = [&](double v, double sum, int e) -> Key {
+                if (v == -INFINITY) return 0;
+                const double t = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / sum;
+                return key_of(a.bias ? t + (double)a.bias[e] : t);
+            };
+            if (!__any(close)) {
+                if (__any(mixed)) {  // those that were taken, put in order by their keys in 64 bits
+                    const double sum = a.sigmoid ? 1.0 : sum64();
+                    const Key k = chosen >= 0 ? key64(logit<Tr>(a.logits, row + chosen), sum, chosen) : 0;
+                    int rank = 0;
+                    for (int i = 0; i < taken; ++i) {
+                        const Key other = __shfl((unsigned long long)k, i, LANES);
+                        const int e = __shfl(chosen, i, LANES);
+                        rank += other > k || (other == k && e < chosen);
+                    }
+                    int* place = reinterpret_cast<int*>(mine);
+                    wave_sync();
+                    place[l] = -1;
+                    wave_sync();
+                    if (chosen >= 0) place[rank] = chosen;
+                    wave_sync();
+                    chosen = place[l];
+                }
+                if (l >= a.top_k) chosen = -1;
+            } else {
+                Key wide[VPL], of64, *own = mine + l * VPL;
+                const double sum = a.sigmoid ? 1.0 : sum64();
+                spoiled = sum != sum;
+                wave_sync();
+#pragma unroll 1
+                for (int i = 0; i < VPL; ++i) {
+                    const double v = on && i < left ? logit<Tr>(a.logits, row + l * VPL + i) : -INFINITY;
+                    own[i] = key64(v, sum, l * VPL + i);
+                }
+                wave_sync();
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) wide[i] = own[i];
+                if (a.groups > 1) keep_groups<LANES>(a, wide, wide, mine, &border);
+                chosen = best_experts<LANES, VPL, false>(a, wide, &of64);
+            }
+            c = chosen >= 0 ? logit<Tr>(a.logits, row + chosen) : -INFINITY;
         }
         // the weights, each lane one
-        const float c = chosen >= 0 ? logit<Tr>(a.logits, row + chosen) : -INFINITY;
         float p = 0.0f, total = 1.0f;
         if (!a.sigmoid) {
             // renormalised, the scores' common factor drops out: the largest chosen logit takes its place
@@ -227,7 +460,7 @@ template <typename Tr, int LANES, int VPL>
 __global__ __launch_bounds__(256) void k_route_bwd(RouteBwd a) {
     constexpr int TOKENS = 256 / LANES;
     __shared__ float scattered[256 * VPL];
-    const int l = threadIdx.x % LANES;
+    const int l = threadIdx.x % LANES, left = a.E - l * VPL;
     float* mine = scattered + (threadIdx.x / LANES) * LANES * VPL;
     for (int64_t first = (int64_t)blockIdx.x * TOKENS; first < a.tokens; first += (int64_t)gridDim.x * TOKENS) {
         const int64_t token = first + threadIdx.x / LANES;
@@ -242,12 +475,9 @@ __global__ __launch_bounds__(256) void k_route_bwd(RouteBwd a) {
         float s[VPL], g, dot = 0.0f;
         if (whole) {
             float top = -INFINITY, total = 0.0f;
+            Few<Tr, VPL>::load(a.logits, row + l * VPL, any ? left : 0, -INFINITY, s);
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                const int e = l * VPL + i;
-                s[i] = any && e < a.E ? logit<Tr>(a.logits, row + e) : -INFINITY;
-                top = fmaxf(top, s[i]);
-            }
+            for (int i = 0; i < VPL; ++i) top = fmaxf(top, s[i]);
             top = lanes_max<LANES>(top);
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
@@ -269,20 +499,19 @@ __global__ __launch_bounds__(256) void k_route_bwd(RouteBwd a) {
         } else {
             g = d * sigmoid_of(c) * sigmoid_of(-c);
         }
+        wave_sync();
 #pragma unroll
         for (int i = 0; i < VPL; ++i) mine[l * VPL + i] = 0.0f;
-        __syncthreads();
+        wave_sync();
         if (chosen >= 0) mine[chosen] = g;
-        __syncthreads();
-        typename Eight<Tr>::elem* out = static_cast<typename Eight<Tr>::elem*>(a.dlogits);
+        wave_sync();
+        float v[VPL];
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int e = l * VPL + i;
-            float v = mine[e];
-            if (whole) v = s[i] * (v - dot);
-            if (on && e < a.E) out[row + e] = Tr::from_f32(v);
+            v[i] = mine[l * VPL + i];
+            if (whole) v[i] = s[i] * (v[i] - dot);
         }
-        __syncthreads();
+        Few<Tr, VPL>::store(a.dlogits, row + l * VPL, on ? left : 0, v);
     }
 }
 
@@ -331,20 +560,41 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(Sort a) {
 
 __global__ __launch_bounds__(kSortThreads) void k_sort(Sort a) {
     __shared__ int cnt[kSortWaves][kSortExperts];
-    __shared__ int total[kSortExperts + 1];
+    __shared__ int total[kSortExperts + 1], sums[2][kSortExperts];  // sums: parts * E <= max(kSortThreads, E)
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     count_slots(a, cnt);
-    // per expert: all rows, and those before this work-group's
+    // per expert: all rows, and those before this work-group's. The work-groups' counts of an expert are split between
+    // the threads that there are, which ask for 16 at a time (65536 slots, 128 experts: one thread an expert, one count at
+    // a time 19.5 us, so 6.6).
+    int parts = 1;
+    if (a.groups > 1) {
+        while (2 * parts * a.E <= kSortThreads) parts *= 2;
+        for (int i = threadIdx.x; i < parts * a.E; i += kSortThreads) {
+            const int part = i / a.E, e = i - part * a.E;
+            int before = 0, all = 0;
+            for (int g0 = part; g0 < a.groups; g0 += 16 * parts) {
+                int c[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int g = g0 + k * parts;
+                    c[k] = g < a.groups ? a.counts[(int64_t)g * a.E + e] : 0;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    before += g0 + k * parts < (int)blockIdx.x ? c[k] : 0;
+                    all += c[k];
+                }
+            }
+            sums[0][i] = before, sums[1][i] = all;
+        }
+        __syncthreads();
+    }
     for (int e = threadIdx.x; e < a.E; e += kSortThreads) {
         int before = 0, all = 0;
         if (a.groups == 1) {
             for (int w = 0; w < kSortWaves; ++w) all += cnt[w][e];
         } else {
-            for (int g = 0; g < a.groups; ++g) {
-                const int c = a.counts[(int64_t)g * a.E + e];
-                before += g < (int)blockIdx.x ? c : 0;
-                all += c;
-            }
+            for (int part = 0; part < parts; ++part) before += sums[0][part * a.E + e], all += sums[1][part * a.E + e];
         }
         total[e] = all;
         for (int w = 0; w < kSortWaves; ++w) {
@@ -417,7 +667,8 @@ int sort_groups(int64_t n, int64_t* stretch) {
 }
 
 // ------------------------------------------------------------ rows by expert, and back
-// A wave takes 512 columns of a token, 8 a lane; the token's positions are uniform.
+// A wave takes 512 columns of a token, 8 a lane: a work-group of four waves the same columns of four tokens, its x the
+// columns. The token's positions and weights are uniform.
 struct Rows {
     const void *in, *other;    // gather: x; combine: y and the residual; its gradients: dout and y
     const float* weights;      // null: ones
@@ -445,6 +696,24 @@ __device__ __forceinline__ void load_stream(const void* p, bool wide, int64_t at
     }
 }
 
+constexpr unsigned kMostColumnGroups = 1u << 15, kMostTokenGroups = 1u << 15;
+
+dim3 row_grid(int64_t tokens, int64_t hidden) {
+    const int64_t x = (hidden + 511) / 512, y = (tokens + 3) / 4;
+    return dim3((unsigned)(x < kMostColumnGroups ? x : kMostColumnGroups), (unsigned)(y < kMostTokenGroups ? y : kMostTokenGroups));
+}
+
+// f(token, column, how many of the 8 are there) for what the wave takes.
+template <typename F>
+__device__ __forceinline__ void each_part(const Rows& a, F f) {
+    const int w4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t token = (int64_t)blockIdx.y * 4 + w4; token < a.tokens; token += (int64_t)gridDim.y * 4)
+        for (int64_t c0 = (int64_t)blockIdx.x * 512; c0 < a.hidden; c0 += (int64_t)gridDim.x * 512) {
+            const int64_t c = c0 + 8 * (threadIdx.x & 63), left = a.hidden - c;
+            f(token, c, left < 8 ? (int)left : 8);
+        }
+}
+
 // Rows from offsets[E] on belong to no slot: zeros. Called by all waves, `wave` of `waves`.
 template <typename Tr>
 __device__ __forceinline__ void clear_tail(const Rows& a, void* out, int64_t wave, int64_t waves) {
@@ -463,40 +732,39 @@ __device__ __forceinline__ void clear_tail(const Rows& a, void* out, int64_t wav
 
 template <typename Tr>
 __global__ __launch_bounds__(256) void k_gather(Rows a) {
-    const int64_t chunks = (a.hidden + 511) / 512, waves = (int64_t)gridDim.x * 4;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int64_t i = wave; i < a.tokens * chunks; i += waves) {
-        const int64_t token = i / chunks, c = (i - token * chunks) * 512 + 8 * (threadIdx.x & 63);
-        const int64_t left = a.hidden - c;
-        const int n = left < 8 ? (int)left : 8;
+    each_part(a, [&](int64_t token, int64_t c, int n) {
         Eight<Tr> v;
         v.load(a.in, token * a.hidden + c, n);
         for (int j = 0; j < a.top_k; ++j) {
             const int64_t p = a.positions[token * a.top_k + j];
             if (p >= 0 && p < a.rows) v.store(a.out, p * a.hidden + c, n);
         }
-    }
-    clear_tail<Tr>(a, a.out, wave, waves);
+    });
+    const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, groups = (int64_t)gridDim.x * gridDim.y;
+    clear_tail<Tr>(a, a.out, group * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), groups * 4);
 }
 
-template <typename Tr>
+// J of the token's rows are asked for before the first is used.
+template <typename Tr, int J>
 __global__ __launch_bounds__(256) void k_combine(Rows a) {
-    const int64_t chunks = (a.hidden + 511) / 512, waves = (int64_t)gridDim.x * 4;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int64_t i = wave; i < a.tokens * chunks; i += waves) {
-        const int64_t token = i / chunks, c = (i - token * chunks) * 512 + 8 * (threadIdx.x & 63);
-        const int64_t left = a.hidden - c;
-        const int n = left < 8 ? (int)left : 8;
+    each_part(a, [&](int64_t token, int64_t c, int n) {
         float s[8] = {};
         if (a.other) load_stream<Tr>(a.other, a.wide, token * a.hidden + c, n, s);
-        for (int j = 0; j < a.top_k; ++j) {
-            const int64_t slot = token * a.top_k + j, p = a.positions[slot];
-            if (p < 0 || p >= a.rows) continue;
-            const float w = a.weights ? a.weights[slot] : 1.0f;
-            Eight<Tr> y;
-            y.load(a.in, p * a.hidden + c, n);
+        for (int j0 = 0; j0 < a.top_k; j0 += J) {
+            Eight<Tr> y[J];
+            float w[J];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s[k] = __builtin_fmaf(w, y.get(k), s[k]);
+            for (int j = 0; j < J; ++j) {
+                const int64_t slot = token * a.top_k + (j0 + j < a.top_k ? j0 + j : 0);
+                const int64_t p = j0 + j < a.top_k ? a.positions[slot] : -1;
+                const bool live = p >= 0 && p < a.rows;  // (what is not adds 1 * 0: its weight may be anything)
+                w[j] = live && a.weights ? a.weights[slot] : 1.0f;
+                y[j].load(a.in, p * a.hidden + c, live ? n : 0);
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[k] = __builtin_fmaf(w[j], y[j].get(k), s[k]);
         }
         if (a.wide) {
             Eight<F32> o;
@@ -507,7 +775,7 @@ __global__ __launch_bounds__(256) void k_combine(Rows a) {
             o.set(s);
             o.store(a.out, token * a.hidden + c, n);
         }
-    }
+    });
 }
 
 // A work-group takes a token: its waves walk the columns, and their sums meet in LDS. J slots at a time.
@@ -564,25 +832,24 @@ __global__ __launch_bounds__(256) void k_combine_bwd(Rows a) {
 bool known(int dtype) { return dtype == STM_F16 || dtype == STM_BF16 || dtype == STM_F32; }
 bool lies(const void* p, int dtype) { return aligned(p, dtype == STM_F32 ? 4 : 2); }
 
-// f(type, lanes, values a lane) of the form that holds a token's experts.
+// f(type, lanes, values a lane) of the form that holds a token's experts; its lanes hold one chosen expert and one group each.
 template <typename Tr, typename F>
-int each_width(int E, F f) {
+int each_form(int E, int least, F f) {
     using std::integral_constant;
-    if (E <= 8) return f(Tr{}, integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    if (E <= 16) return f(Tr{}, integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    if (E <= 32) return f(Tr{}, integral_constant<int, 32>{}, integral_constant<int, 1>{});
-    if (E <= 64) return f(Tr{}, integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    if (E <= 128) return f(Tr{}, integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    if (E <= 256) return f(Tr{}, integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    if (E <= 16 && least <= 16) return f(Tr{}, integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    if (E <= 32 && least <= 16) return f(Tr{}, integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    if (E <= 64 && least <= 16) return f(Tr{}, integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    if (E <= 128 && least <= 16) return f(Tr{}, integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    if (E <= 256 && least <= 32) return f(Tr{}, integral_constant<int, 32>{}, integral_constant<int, 8>{});
     if (E <= 512) return f(Tr{}, integral_constant<int, 64>{}, integral_constant<int, 8>{});
     return f(Tr{}, integral_constant<int, 64>{}, integral_constant<int, 16>{});
 }
 
 template <typename F>
-int each_route(int dtype, int E, F f) {
-    if (dtype == STM_BF16) return each_width<BF16>(E, f);
-    if (dtype == STM_F16) return each_width<F16>(E, f);
-    return each_width<F32>(E, f);
+int each_route(int dtype, int E, int least, F f) {
+    if (dtype == STM_BF16) return each_form<BF16>(E, least, f);
+    if (dtype == STM_F16) return each_form<F16>(E, least, f);
+    return each_form<F32>(E, least, f);
 }
 
 int check_route(const char* what, int64_t tokens, int E, int top_k, int score, int dtype) {
@@ -606,6 +873,16 @@ int check_rows(const char* what, int64_t tokens, int top_k, int64_t hidden, int 
         return set_error(STM_ERR_UNSUPPORTED, "%s: %lld tokens of %lld columns are too many", what, (long long)tokens,
                          (long long)hidden);
     return STM_OK;
+}
+
+// f(slots at a time) for a token's top_k.
+template <typename F>
+int each_chunk(int top_k, F f) {
+    using std::integral_constant;
+    if (top_k <= 1) return f(integral_constant<int, 1>{});
+    if (top_k <= 2) return f(integral_constant<int, 2>{});
+    if (top_k <= 4) return f(integral_constant<int, 4>{});
+    return f(integral_constant<int, 8>{});
 }
 
 template <typename F>
@@ -637,13 +914,13 @@ extern "C" int stm_moe_route(const void* logits, const float* bias, const uint8_
     const bool sums = group_sums && groups > 1;
     const Route a{logits, bias, mask, weights, experts, tokens, num_experts, top_k, groups, top_groups,
                   score == STM_MOE_SIGMOID, sums, renormalize != 0, (float)scale};
-    return each_route(dtype, num_experts, [&](auto tr, auto lanes, auto vpl) {
+    return each_route(dtype, num_experts, top_k > groups ? top_k : groups, [&](auto tr, auto lanes, auto vpl) {
         const dim3 grid(groups_for(tokens, 256 / lanes.value)), block(256);
         if (bias || sums)
-            hipLaunchKernelGGL((k_route<decltype(tr), lanes.value, vpl.value, uint64_t>), grid, block, 0,
+            hipLaunchKernelGGL((k_route<decltype(tr), lanes.value, vpl.value, true>), grid, block, 0,
                                (hipStream_t)stream, a);
         else
-            hipLaunchKernelGGL((k_route<decltype(tr), lanes.value, vpl.value, uint32_t>), grid, block, 0,
+            hipLaunchKernelGGL((k_route<decltype(tr), lanes.value, vpl.value, false>), grid, block, 0,
                                (hipStream_t)stream, a);
         return check_launch(what);
     });
@@ -661,7 +938,7 @@ extern "C" int stm_moe_route_bwd(const float* dweights, const void* logits, cons
         return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
     const RouteBwd a{dweights, logits, experts, dlogits, tokens, num_experts, top_k, score == STM_MOE_SIGMOID,
                      renormalize != 0, (float)scale};
-    return each_route(dtype, num_experts, [&](auto tr, auto lanes, auto vpl) {
+    return each_route(dtype, num_experts, top_k, [&](auto tr, auto lanes, auto vpl) {
         hipLaunchKernelGGL((k_route_bwd<decltype(tr), lanes.value, vpl.value>), dim3(groups_for(tokens, 256 / lanes.value)),
                            dim3(256), 0, (hipStream_t)stream, a);
         return check_launch(what);
@@ -717,8 +994,7 @@ extern "C" int stm_moe_gather(const void* x, const int32_t* positions, const int
         return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
     const Rows a{x, nullptr, nullptr, positions, offsets, out, nullptr, tokens, hidden, tokens * top_k, top_k, num_experts, false};
     return each_type(dtype, [&](auto tr) {
-        hipLaunchKernelGGL(k_gather<decltype(tr)>, dim3(groups_for(tokens * ((hidden + 511) / 512), 4)), dim3(256), 0,
-                           (hipStream_t)stream, a);
+        hipLaunchKernelGGL(k_gather<decltype(tr)>, row_grid(tokens, hidden), dim3(256), 0, (hipStream_t)stream, a);
         return check_launch(what);
     });
 }
@@ -740,9 +1016,11 @@ extern "C" int stm_moe_combine(const void* y, int64_t y_rows, const float* weigh
         return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
     const Rows a{y, residual, weights, positions, nullptr, out, nullptr, tokens, hidden, y_rows, top_k, 0, out_dtype == STM_F32};
     return each_type(dtype, [&](auto tr) {
-        hipLaunchKernelGGL(k_combine<decltype(tr)>, dim3(groups_for(tokens * ((hidden + 511) / 512), 4)), dim3(256), 0,
-                           (hipStream_t)stream, a);
-        return check_launch(what);
+        return each_chunk(top_k, [&](auto j) {
+            hipLaunchKernelGGL((k_combine<decltype(tr), j.value>), row_grid(tokens, hidden), dim3(256), 0, (hipStream_t)stream,
+                               a);
+            return check_launch(what);
+        });
     });
 }
 
@@ -769,14 +1047,9 @@ extern "C" int stm_moe_combine_bwd(const void* dout, int dout_dtype, const void*
     return each_type(dtype, [&](auto tr) {
         const dim3 grid((unsigned)(tokens < (1 << 22) ? tokens : 1 << 22)), block(256);
         hipStream_t st = (hipStream_t)stream;
-        if (top_k <= 1)
-            hipLaunchKernelGGL((k_combine_bwd<decltype(tr), 1>), grid, block, 0, st, a);
-        else if (top_k <= 2)
-            hipLaunchKernelGGL((k_combine_bwd<decltype(tr), 2>), grid, block, 0, st, a);
-        else if (top_k <= 4)
-            hipLaunchKernelGGL((k_combine_bwd<decltype(tr), 4>), grid, block, 0, st, a);
-        else
-            hipLaunchKernelGGL((k_combine_bwd<decltype(tr), 8>), grid, block, 0, st, a);
-        return check_launch(what);
+        return each_chunk(top_k, [&](auto j) {
+            hipLaunchKernelGGL((k_combine_bwd<decltype(tr), j.value>), grid, block, 0, st, a);
+            return check_launch(what);
+        });
     });
 }

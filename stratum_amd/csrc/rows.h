@@ -91,13 +91,28 @@ struct Eight<F32> {
 };
 
 // ------------------------------------------------------------ lanes
-// The value of the lane that is 1, 2, 4, 8, 16 or 32 away, where all lanes of each smaller group hold one value already:
-// within 16 lanes a DPP move (swap neighbours, swap pairs, mirror 8, mirror 16), across them the two row swaps.
+// op(v, the other lane's v), the other one 1, 2, 4, 8, 16 or 32 away, where all lanes of each smaller group hold one value
+// already: within 16 lanes a DPP move (swap neighbours, swap pairs, mirror 8, mirror 16), across them the two row swaps,
+// which give every lane both values. op commutes.
+template <int STEP, typename Op>
+__device__ __forceinline__ uint32_t with_other(uint32_t v, Op op) {
+    if constexpr (STEP <= 8) {
+        constexpr int ctrl = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;
+        return op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, true));
+    } else if constexpr (STEP == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return op(r[0], r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return op(r[0], r[1]);
+    }
+}
+
+// The other lane's value itself.
 template <int STEP>
 __device__ __forceinline__ uint32_t across(uint32_t v) {
     if constexpr (STEP <= 8) {
-        constexpr int ctrl = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;
-        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, true);
+        return with_other<STEP>(v, [](uint32_t, uint32_t o) { return o; });
     } else if constexpr (STEP == 16) {
         const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
         return (threadIdx.x & 16) ? r[0] : r[1];
@@ -111,7 +126,7 @@ __device__ __forceinline__ uint32_t across(uint32_t v) {
 template <int LANES, int STEP = 1, typename Op>
 __device__ __forceinline__ uint32_t over_lanes(uint32_t v, Op op) {
     if constexpr (STEP < LANES) {
-        return over_lanes<LANES, STEP * 2>(op(v, across<STEP>(v)), op);
+        return over_lanes<LANES, STEP * 2>(with_other<STEP>(v, op), op);
     } else {
         return v;
     }
@@ -134,6 +149,11 @@ __device__ __forceinline__ float lanes_max(float v) {
 template <int LANES>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     return over_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
+    return over_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 }
 
 // 64-bit keys: the largest upper half, then the largest lower half among its holders.
