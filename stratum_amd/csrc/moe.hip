@@ -696,6 +696,8 @@ __device__ __forceinline__ void load_stream(const void* p, bool wide, int64_t at
     }
 }
 
+enum class Far { none, loads, both };  // accesses to the experts' rows that pass the caches by
+
 constexpr unsigned kMostColumnGroups = 1u << 15, kMostTokenGroups = 1u << 15;
 
 dim3 row_grid(int64_t tokens, int64_t hidden) {
@@ -730,14 +732,14 @@ __device__ __forceinline__ void clear_tail(const Rows& a, void* out, int64_t wav
     }
 }
 
-template <typename Tr>
+template <typename Tr, Far FAR>
 __global__ __launch_bounds__(256) void k_gather(Rows a) {
     each_part(a, [&](int64_t token, int64_t c, int n) {
         Eight<Tr> v;
         v.load(a.in, token * a.hidden + c, n);
         for (int j = 0; j < a.top_k; ++j) {
             const int64_t p = a.positions[token * a.top_k + j];
-            if (p >= 0 && p < a.rows) v.store(a.out, p * a.hidden + c, n);
+            if (p >= 0 && p < a.rows) v.template store<(FAR == Far::both)>(a.out, p * a.hidden + c, n);
         }
     });
     const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, groups = (int64_t)gridDim.x * gridDim.y;
@@ -745,7 +747,7 @@ __global__ __launch_bounds__(256) void k_gather(Rows a) {
 }
 
 // J of the token's rows are asked for before the first is used.
-template <typename Tr, int J>
+template <typename Tr, int J, Far FAR>
 __global__ __launch_bounds__(256) void k_combine(Rows a) {
     each_part(a, [&](int64_t token, int64_t c, int n) {
         float s[8] = {};
@@ -759,7 +761,7 @@ __global__ __launch_bounds__(256) void k_combine(Rows a) {
                 const int64_t p = j0 + j < a.top_k ? a.positions[slot] : -1;
                 const bool live = p >= 0 && p < a.rows;  // (what is not adds 1 * 0: its weight may be anything)
                 w[j] = live && a.weights ? a.weights[slot] : 1.0f;
-                y[j].load(a.in, p * a.hidden + c, live ? n : 0);
+                y[j].template load<(FAR != Far::none)>(a.in, p * a.hidden + c, live ? n : 0);
             }
 #pragma unroll
             for (int j = 0; j < J; ++j)
@@ -779,7 +781,7 @@ __global__ __launch_bounds__(256) void k_combine(Rows a) {
 }
 
 // A work-group takes a token: its waves walk the columns, and their sums meet in LDS. J slots at a time.
-template <typename Tr, int J>
+template <typename Tr, int J, Far FAR>
 __global__ __launch_bounds__(256) void k_combine_bwd(Rows a) {
     __shared__ float part[4][J];
     const int lane = threadIdx.x & 63, w4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -798,7 +800,7 @@ __global__ __launch_bounds__(256) void k_combine_bwd(Rows a) {
                     if (p < 0 || p >= a.rows) continue;
                     if (a.dweights) {
                         Eight<Tr> y;
-                        y.load(a.other, p * a.hidden + c, n);
+                        y.template load<(FAR != Far::none)>(a.other, p * a.hidden + c, n);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) dot[j] = __builtin_fmaf(d[k], y.get(k), dot[j]);
                     }
@@ -809,7 +811,7 @@ __global__ __launch_bounds__(256) void k_combine_bwd(Rows a) {
                         for (int k = 0; k < 8; ++k) g[k] = w * d[k];
                         Eight<Tr> o;
                         o.set(g);
-                        o.store(a.out, p * a.hidden + c, n);
+                        o.template store<(FAR == Far::both)>(a.out, p * a.hidden + c, n);
                     }
                 }
             }
@@ -883,6 +885,19 @@ int each_chunk(int top_k, F f) {
     if (top_k <= 2) return f(integral_constant<int, 2>{});
     if (top_k <= 4) return f(integral_constant<int, 4>{});
     return f(integral_constant<int, 8>{});
+}
+
+// f(which accesses to the experts' rows pass the caches by). Read once, rows of a good part of the 256 MB memory-side cache
+// leave it to what is read again; written, rows that do not fit it gain from passing it by, smaller ones are there for the
+// product that takes them (bf16, 8 slots a token of 2048 columns, us; nothing / loads / both): combination of 3000 tokens
+// 25.1 / 25.0, of 4096 32.1 / 29.3, of 8192 65 / 56; gather of 4096 and their combination 58 / 50 / 57, of 8192
+// 136 / 109 / 107; the gradient of 1024 14 / 20, of 8192 123 / 119 / 114.
+template <typename F>
+int each_distance(int64_t rows, int64_t hidden, int dtype, F f) {
+    const int64_t bytes = rows * hidden * (dtype == STM_F32 ? 4 : 2);
+    if (bytes < 96ll << 20) return f(std::integral_constant<Far, Far::none>{});
+    if (bytes < 256ll << 20) return f(std::integral_constant<Far, Far::loads>{});
+    return f(std::integral_constant<Far, Far::both>{});
 }
 
 template <typename F>
@@ -994,8 +1009,11 @@ extern "C" int stm_moe_gather(const void* x, const int32_t* positions, const int
         return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
     const Rows a{x, nullptr, nullptr, positions, offsets, out, nullptr, tokens, hidden, tokens * top_k, top_k, num_experts, false};
     return each_type(dtype, [&](auto tr) {
-        hipLaunchKernelGGL(k_gather<decltype(tr)>, row_grid(tokens, hidden), dim3(256), 0, (hipStream_t)stream, a);
-        return check_launch(what);
+        return each_distance(tokens * top_k, hidden, dtype, [&](auto far) {
+            hipLaunchKernelGGL((k_gather<decltype(tr), far.value>), row_grid(tokens, hidden), dim3(256), 0, (hipStream_t)stream,
+                               a);
+            return check_launch(what);
+        });
     });
 }
 
@@ -1017,9 +1035,11 @@ extern "C" int stm_moe_combine(const void* y, int64_t y_rows, const float* weigh
     const Rows a{y, residual, weights, positions, nullptr, out, nullptr, tokens, hidden, y_rows, top_k, 0, out_dtype == STM_F32};
     return each_type(dtype, [&](auto tr) {
         return each_chunk(top_k, [&](auto j) {
-            hipLaunchKernelGGL((k_combine<decltype(tr), j.value>), row_grid(tokens, hidden), dim3(256), 0, (hipStream_t)stream,
-                               a);
-            return check_launch(what);
+            return each_distance(y_rows, hidden, dtype, [&](auto far) {
+                hipLaunchKernelGGL((k_combine<decltype(tr), j.value, far.value>), row_grid(tokens, hidden), dim3(256), 0,
+                                   (hipStream_t)stream, a);
+                return check_launch(what);
+            });
         });
     });
 }
@@ -1048,8 +1068,10 @@ extern "C" int stm_moe_combine_bwd(const void* dout, int dout_dtype, const void*
         const dim3 grid((unsigned)(tokens < (1 << 22) ? tokens : 1 << 22)), block(256);
         hipStream_t st = (hipStream_t)stream;
         return each_chunk(top_k, [&](auto j) {
-            hipLaunchKernelGGL((k_combine_bwd<decltype(tr), j.value>), grid, block, 0, st, a);
-            return check_launch(what);
+            return each_distance(y_rows, hidden, dtype, [&](auto far) {
+                hipLaunchKernelGGL((k_combine_bwd<decltype(tr), j.value, far.value>), grid, block, 0, st, a);
+                return check_launch(what);
+            });
         });
     });
 }

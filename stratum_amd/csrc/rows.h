@@ -13,19 +13,41 @@ struct F32 {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-// 8 consecutive elements of a row as they lie in memory. A row starts wherever its width puts it, so the 16-byte
-// accesses are declared with the alignment of one element: the hardware takes them at any address.
+// 16 bytes at an element's alignment (the typedef's alignment does not pass through a template's argument).
+#define STM_LOOSE(NAME, A)                                                                        \
+    struct NAME {                                                                                 \
+        typedef u32x4_t __attribute__((aligned(A))) type;                                         \
+        template <bool STREAM>                                                                    \
+        static __device__ __forceinline__ u32x4_t load(const void* p) {                           \
+            if constexpr (STREAM) return __builtin_nontemporal_load(static_cast<const type*>(p)); \
+            return *static_cast<const type*>(p);                                                  \
+        }                                                                                         \
+        template <bool STREAM>                                                                    \
+        static __device__ __forceinline__ void store(u32x4_t v, void* p) {                        \
+            if constexpr (STREAM)                                                                 \
+                __builtin_nontemporal_store(v, static_cast<type*>(p));                            \
+            else                                                                                  \
+                *static_cast<type*>(p) = v;                                                       \
+        }                                                                                         \
+    }
+STM_LOOSE(Loose2, 2);
+STM_LOOSE(Loose4, 4);
+#undef STM_LOOSE
+
+// 8 consecutive elements of a row as they lie in memory. STREAM: what is read or written will not be met again soon, so the
+// caches need not keep it. A row starts wherever its width puts it, so the 16-byte accesses are declared with the
+// alignment of one element: the hardware takes them at any address.
 template <typename Tr>
 struct Eight {
     typedef uint16_t elem;
-    typedef u32x4_t __attribute__((aligned(2))) loose;
     u32x4_t v;
 
     // the first n elements at p (n < 8 at a row's end; n <= 0: none), zeros behind them
+    template <bool STREAM = false>
     __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
         const elem* p = static_cast<const elem*>(base) + at;
         if (n >= 8) {
-            v = *reinterpret_cast<const loose*>(p);
+            v = Loose2::load<STREAM>(p);
             return;
         }
         v = u32x4_t{0, 0, 0, 0};
@@ -33,10 +55,11 @@ struct Eight {
         for (int i = 0; i < 8; ++i)
             if (i < n) v[i / 2] |= (uint32_t)p[i] << (16 * (i % 2));
     }
+    template <bool STREAM = false>
     __device__ __forceinline__ void store(void* base, int64_t at, int n) const {
         elem* p = static_cast<elem*>(base) + at;
         if (n >= 8) {
-            *reinterpret_cast<loose*>(p) = v;
+            Loose2::store<STREAM>(v, p);
             return;
         }
 #pragma unroll
@@ -56,14 +79,14 @@ struct Eight {
 template <>
 struct Eight<F32> {
     typedef float elem;
-    typedef u32x4_t __attribute__((aligned(4))) loose;
     u32x4_t v[2];
 
+    template <bool STREAM = false>
     __device__ __forceinline__ void load(const void* base, int64_t at, int n) {
         const elem* p = static_cast<const elem*>(base) + at;
         if (n >= 8) {
-            v[0] = *reinterpret_cast<const loose*>(p);
-            v[1] = *reinterpret_cast<const loose*>(p + 4);
+            v[0] = Loose4::load<STREAM>(p);
+            v[1] = Loose4::load<STREAM>(p + 4);
             return;
         }
         clear();
@@ -71,11 +94,12 @@ struct Eight<F32> {
         for (int i = 0; i < 8; ++i)
             if (i < n) v[i / 4][i % 4] = __float_as_uint(p[i]);
     }
+    template <bool STREAM = false>
     __device__ __forceinline__ void store(void* base, int64_t at, int n) const {
         elem* p = static_cast<elem*>(base) + at;
         if (n >= 8) {
-            *reinterpret_cast<loose*>(p) = v[0];
-            *reinterpret_cast<loose*>(p + 4) = v[1];
+            Loose4::store<STREAM>(v[0], p);
+            Loose4::store<STREAM>(v[1], p + 4);
             return;
         }
 #pragma unroll
