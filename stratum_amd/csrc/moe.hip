@@ -716,10 +716,9 @@ __device__ __forceinline__ void each_part(const Rows& a, F f) {
         }
 }
 
-// Rows from offsets[E] on belong to no slot: zeros. Called by all waves, `wave` of `waves`.
+// Rows from `live` = offsets[E] on belong to no slot: zeros. Called by all waves, `wave` of `waves`.
 template <typename Tr>
-__device__ __forceinline__ void clear_tail(const Rows& a, void* out, int64_t wave, int64_t waves) {
-    int64_t live = a.offsets[a.E];
+__device__ __forceinline__ void clear_tail(const Rows& a, void* out, int64_t live, int64_t wave, int64_t waves) {
     if (live < 0) live = 0;
     if (live >= a.rows) return;
     const int64_t chunks = (a.hidden + 511) / 512;
@@ -734,6 +733,7 @@ __device__ __forceinline__ void clear_tail(const Rows& a, void* out, int64_t wav
 
 template <typename Tr, Far FAR>
 __global__ __launch_bounds__(256) void k_gather(Rows a) {
+    const int64_t live = a.offsets[a.E];
     each_part(a, [&](int64_t token, int64_t c, int n) {
         Eight<Tr> v;
         v.load(a.in, token * a.hidden + c, n);
@@ -743,7 +743,7 @@ __global__ __launch_bounds__(256) void k_gather(Rows a) {
         }
     });
     const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, groups = (int64_t)gridDim.x * gridDim.y;
-    clear_tail<Tr>(a, a.out, group * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), groups * 4);
+    clear_tail<Tr>(a, a.out, live, group * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), groups * 4);
 }
 
 // J of the token's rows are asked for before the first is used.
@@ -780,38 +780,55 @@ __global__ __launch_bounds__(256) void k_combine(Rows a) {
     });
 }
 
-// A work-group takes a token: its waves walk the columns, and their sums meet in LDS. J slots at a time.
-template <typename Tr, int J, Far FAR>
+// A work-group takes 4 / W tokens, W waves each, which walk its columns; their sums meet in LDS. J slots at a time, whose
+// rows are asked for before the first is used.
+template <typename Tr, int J, int W, Far FAR>
 __global__ __launch_bounds__(256) void k_combine_bwd(Rows a) {
+    constexpr int TOKENS = 4 / W;
     __shared__ float part[4][J];
     const int lane = threadIdx.x & 63, w4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+    const int64_t live = a.out ? a.offsets[a.E] : 0;
+    for (int64_t first = (int64_t)blockIdx.x * TOKENS; first < a.tokens; first += (int64_t)gridDim.x * TOKENS) {
+        const int64_t token = first + w4 / W;
+        const bool on = token < a.tokens;
         for (int j0 = 0; j0 < a.top_k; j0 += J) {
-            float dot[J] = {};
-            for (int64_t c = 8 * threadIdx.x; c < a.hidden; c += 2048) {
+            int64_t p[J];
+            float w[J], dot[J] = {};
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                p[j] = -1, w[j] = 0.0f;
+                if (!on || j0 + j >= a.top_k) continue;
+                const int64_t slot = token * a.top_k + j0 + j;
+                p[j] = a.positions[slot];
+                if (p[j] >= a.rows) p[j] = -1;
+                if (a.out && p[j] >= 0) w[j] = a.weights[slot];
+            }
+#pragma unroll 1
+            for (int64_t c = 8 * (lane + 64 * (w4 % W)); c < a.hidden && on; c += 512 * W) {
                 const int64_t left = a.hidden - c;
                 const int n = left < 8 ? (int)left : 8;
+                Eight<Tr> y[J];
                 float d[8];
                 load_stream<Tr>(a.in, a.wide, token * a.hidden + c, n, d);
+                if (a.dweights) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+                        y[j].template load<(FAR != Far::none)>(a.other, p[j] * a.hidden + c, p[j] >= 0 ? n : 0);
+                }
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
-                    if (j0 + j >= a.top_k) continue;
-                    const int64_t slot = token * a.top_k + j0 + j, p = a.positions[slot];
-                    if (p < 0 || p >= a.rows) continue;
+                    if (p[j] < 0) continue;
                     if (a.dweights) {
-                        Eight<Tr> y;
-                        y.template load<(FAR != Far::none)>(a.other, p * a.hidden + c, n);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) dot[j] = __builtin_fmaf(d[k], y.get(k), dot[j]);
+                        for (int k = 0; k < 8; ++k) dot[j] = __builtin_fmaf(d[k], y[j].get(k), dot[j]);
                     }
                     if (a.out) {
-                        const float w = a.weights[slot];
                         float g[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) g[k] = w * d[k];
+                        for (int k = 0; k < 8; ++k) g[k] = w[j] * d[k];
                         Eight<Tr> o;
                         o.set(g);
-                        o.template store<(FAR == Far::both)>(a.out, p * a.hidden + c, n);
+                        o.template store<(FAR == Far::both)>(a.out, p[j] * a.hidden + c, n);
                     }
                 }
             }
@@ -819,16 +836,25 @@ __global__ __launch_bounds__(256) void k_combine_bwd(Rows a) {
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 dot[j] = lanes_sum<64>(dot[j]);
-                if (lane == 0) part[w4][j] = dot[j];
+                if (W > 1 && lane == 0) part[w4][j] = dot[j];
             }
-            __syncthreads();
-            if (threadIdx.x < J && j0 + (int)threadIdx.x < a.top_k)
-                a.dweights[token * a.top_k + j0 + threadIdx.x] =
-                    part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
-            __syncthreads();
+            if constexpr (W > 1) __syncthreads();
+            if (w4 % W == 0) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    float s = dot[j];
+                    if constexpr (W > 1) {
+                        s = part[w4][j];
+#pragma unroll
+                        for (int k = 1; k < W; ++k) s += part[w4 + k][j];
+                    }
+                    if (lane == j && on && j0 + j < a.top_k) a.dweights[token * a.top_k + j0 + j] = s;
+                }
+            }
+            if constexpr (W > 1) __syncthreads();
         }
     }
-    if (a.out) clear_tail<Tr>(a, a.out, (int64_t)blockIdx.x * 4 + w4, (int64_t)gridDim.x * 4);
+    if (a.out) clear_tail<Tr>(a, a.out, live, (int64_t)blockIdx.x * 4 + w4, (int64_t)gridDim.x * 4);
 }
 
 bool known(int dtype) { return dtype == STM_F16 || dtype == STM_BF16 || dtype == STM_F32; }
@@ -891,12 +917,13 @@ int each_chunk(int top_k, F f) {
 // leave it to what is read again; written, rows that do not fit it gain from passing it by, smaller ones are there for the
 // product that takes them (bf16, 8 slots a token of 2048 columns, us; nothing / loads / both): combination of 3000 tokens
 // 25.1 / 25.0, of 4096 32.1 / 29.3, of 8192 65 / 56; gather of 4096 and their combination 58 / 50 / 57, of 8192
-// 136 / 109 / 107; the gradient of 1024 14 / 20, of 8192 123 / 119 / 114.
+// 136 / 109 / 107; the gradient of 1024 14 / 20, of 8192 125 / 113 / 108. Stores that do so have to fill their 128-byte
+// lines, as those of whole 16-bit chunks do (fp32, two halves of a line apart: gather of 4096 tokens 62 / 130).
 template <typename F>
 int each_distance(int64_t rows, int64_t hidden, int dtype, F f) {
     const int64_t bytes = rows * hidden * (dtype == STM_F32 ? 4 : 2);
     if (bytes < 96ll << 20) return f(std::integral_constant<Far, Far::none>{});
-    if (bytes < 256ll << 20) return f(std::integral_constant<Far, Far::loads>{});
+    if (bytes < 256ll << 20 || dtype == STM_F32 || hidden % 64) return f(std::integral_constant<Far, Far::loads>{});
     return f(std::integral_constant<Far, Far::both>{});
 }
 
@@ -1065,13 +1092,19 @@ extern "C" int stm_moe_combine_bwd(const void* dout, int dout_dtype, const void*
     const Rows a{dout, y, weights, positions, offsets, y_rows ? dy : nullptr, dweights, tokens, hidden, y_rows, top_k, num_experts,
                  dout_dtype == STM_F32};
     return each_type(dtype, [&](auto tr) {
-        const dim3 grid((unsigned)(tokens < (1 << 22) ? tokens : 1 << 22)), block(256);
-        hipStream_t st = (hipStream_t)stream;
-        return each_chunk(top_k, [&](auto j) {
-            return each_distance(y_rows, hidden, dtype, [&](auto far) {
-                hipLaunchKernelGGL((k_combine_bwd<decltype(tr), j.value, far.value>), grid, block, 0, st, a);
-                return check_launch(what);
+        const auto run = [&](auto w) {
+            const int64_t groups = (tokens + 4 / w.value - 1) / (4 / w.value);
+            const dim3 grid((unsigned)(groups < (1 << 22) ? groups : 1 << 22));
+            return each_chunk(top_k, [&](auto j) {
+                return each_distance(y_rows, hidden, dtype, [&](auto far) {
+                    hipLaunchKernelGGL((k_combine_bwd<decltype(tr), j.value, w.value, far.value>), grid, dim3(256), 0,
+                                       (hipStream_t)stream, a);
+                    return check_launch(what);
+                });
             });
-        });
+        };
+        if (hidden <= 512) return run(std::integral_constant<int, 1>{});
+        if (hidden <= 1024) return run(std::integral_constant<int, 2>{});
+        return run(std::integral_constant<int, 4>{});
     });
 }
