@@ -77,7 +77,7 @@ SIGNATURES = {
     "stm_state8_values": ([_P, _P, _I64, _I, _P, _P], _I),
     "stm_rms_norm_fwd": ([_P, _P, _I, _P, _I, _P, _P, _P, _I64, _I64, _D, _I, _P], _I),
     "stm_rms_norm_workspace_bytes": ([_I64, _I64], _I64),
-    "stm_rms_norm_bwd": ([_P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _I64, _I64, _I, _P, _I64, _P], _I),
+    "stm_rms_norm_bwd": ([_P, _P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _I64, _I64, _I, _P, _I64, _P], _I),
     "stm_moe_route": ([_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _D, _I, _P], _I),
     "stm_moe_route_bwd": ([_P, _P, _P, _P, _I64, _I, _I, _I, _I, _D, _I, _P], _I),
     "stm_moe_sort_workspace_bytes": ([_I64, _I], _I64),

@@ -7,8 +7,8 @@
 //   ds = r (t - n mean(t n)) (+ dh),  dw = sum over rows of dy n
 //
 // ds is the gradient of x and of the residual. Everything between a load and a store is fp32; y comes from the sum
-// before its rounding to h, so each output is rounded once. The backward's n does use the rounded h: half a step of h in
-// a term that is itself rounded to that type.
+// before its rounding to h, so each output is rounded once. The backward's n uses the rounded h where what it gives is
+// rounded to that type itself; a weight's gradient that is wider than h takes x and the residual again.
 //
 // Bound by bytes. One pass: a row stays in registers between its sum and its result, 8 elements of a thread in one access.
 // A row belongs to 8 to 64 lanes of a wave (no barrier), or to 128 to 1024 threads.
@@ -195,6 +195,7 @@ __global__ __launch_bounds__(1024) void k_rms_fwd_long(NormFwd a) {
 
 struct NormBwd {
     const void *dy, *dh, *h, *w;
+    const void* res;  // in h's 16-bit type: h is x, and this its residual (null: h is the sum)
     const float* rstd;
     void *dx, *dres;
     float* dw_part;  // [groups of the grid, cols], or null
@@ -203,105 +204,95 @@ struct NormBwd {
     bool h32, w32;
 };
 
-// DW: a thread's columns are the same in every row of its work-group, so the weight's gradient gathers in registers over
-// the rows that the group takes (gridDim rows apart), then over the group's row slots in LDS, and leaves as one row of
-// partial sums; k_rms_dw adds those rows up in a fixed order. With one vector a thread the next row is asked for before
-// this one's sum: few groups, so that there are few partial sums, would leave the memory idle in between ([8192, 4096] bf16,
-// us, with the sum of the parts: without the weight's gradient 48, with it 60 without and 54 with the look-ahead).
-template <typename Tr, int T, int NV, bool DW>
+// T threads a row, 8 columns each: cols <= 8 T. DW: a thread's columns are the same in every row of its work-group, so the
+// weight's gradient gathers in registers over the rows that the group takes (gridDim rows apart), then over the group's
+// row slots in LDS, and leaves as one row of partial sums; k_rms_dw adds those rows up in a fixed order. The next row is
+// then asked for before this one's sum: few groups, so that there are few partial sums, would leave the memory idle in
+// between ([8192, 4096] bf16, us, with the sum of the parts: without the weight's gradient 48, with it 60 without and 54 with
+// the look-ahead).
+template <typename Tr, int T, bool DW>
 __global__ __launch_bounds__(kBlock<T>) void k_rms_bwd(NormBwd a) {
     constexpr int SLOTS = kBlock<T> / T;
-    constexpr bool AHEAD = DW && NV == 1;
-    const int t = threadIdx.x % T, slot = threadIdx.x / T;
+    const int t = threadIdx.x % T, slot = threadIdx.x / T, c = 8 * t;
     const int64_t stride = (int64_t)gridDim.x * SLOTS;
-    float dw[NV][8];
-    if (DW) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dw[v][i] = 0.0f;
-    }
-    Loaded<Tr> dy[NV], h[NV], dh[NV], w_[NV];
+    float dw[8] = {};
+    Loaded<Tr> dy, h, res, dh, weight;
     float rstd = 0.0f;
     auto ask = [&](int64_t row) {
         const bool on = row < a.rows;
+        const int n = on ? a.cols - c : 0;
         rstd = on ? a.rstd[row] : 0.0f;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
-            dy[v].load(a.dy, false, row * a.cols + c, n);
-            h[v].load(a.h, a.h32, row * a.cols + c, n);
-            if (a.dh) dh[v].load(a.dh, a.h32, row * a.cols + c, n);
-        }
+        dy.load(a.dy, false, row * a.cols + c, n);
+        h.load(a.h, a.h32, row * a.cols + c, n);
+        if (a.res) res.load(a.res, false, row * a.cols + c, n);
+        if (a.dh) dh.load(a.dh, a.h32, row * a.cols + c, n);
     };
     int turn = 0;
     int64_t first = (int64_t)blockIdx.x * SLOTS;
-    if (AHEAD) ask(first + slot);
-    if (NV == 1) w_[0].load(a.w, a.w32, 8 * t, a.cols - 8 * t);
+    if (DW) ask(first + slot);
+    weight.load(a.w, a.w32, c, a.cols - c);
     for (; first < a.rows; first += stride, ++turn) {
         const int64_t row = first + slot;
-        const bool on = row < a.rows;
-        const int64_t at = row * a.cols;
-        if (!AHEAD) ask(row);
+        if (!DW) ask(row);
         const float r = rstd;
-        float g[NV][8], n_[NV][8], e[NV][8];  // t = w dy, n = h r
+        float g[8], n_[8], e[8], w[8];  // t = w dy, n = h r
         float dot = 0.0f;
+        dy.get(false, g);
+        h.get(a.h32, n_);
+        if (a.res) {
+            float s[8];
+            res.get(false, s);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = 8 * (t + T * v);
-            float w[8];
-            dy[v].get(false, g[v]);
-            h[v].get(a.h32, n_[v]);
-            if (a.dh) dh[v].get(a.h32, e[v]);
-            if (NV > 1) w_[v].load(a.w, a.w32, c, a.cols - c);
-            w_[v].get(a.w32, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                n_[v][i] *= r;
-                if (DW) dw[v][i] = __builtin_fmaf(g[v][i], n_[v][i], dw[v][i]);
-                g[v][i] *= w[i];
-                dot = __builtin_fmaf(g[v][i], n_[v][i], dot);
-            }
+            for (int i = 0; i < 8; ++i) n_[i] += s[i];
         }
-        if (AHEAD) ask(row + stride);
+        if (a.dh) dh.get(a.h32, e);
+        weight.get(a.w32, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            n_[i] *= r;
+            if (DW) dw[i] = __builtin_fmaf(g[i], n_[i], dw[i]);
+            g[i] *= w[i];
+            dot = __builtin_fmaf(g[i], n_[i], dot);
+        }
+        if (DW) ask(row + stride);
         const float mean = row_sum<T>(dot, turn) / (float)a.cols;
+        const int n = row < a.rows ? a.cols - c : 0;
+        float d[8];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = 8 * (t + T * v), n = on ? a.cols - c : 0;
-            float d[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                d[i] = r * (g[v][i] - n_[v][i] * mean);
-                if (a.dh) d[i] += e[v][i];
-            }
-            if (a.dx) store_as<Tr>(a.dx, false, at + c, n, d);
-            if (a.dres) store_as<Tr>(a.dres, a.h32, at + c, n, d);
+        for (int i = 0; i < 8; ++i) {
+            d[i] = r * (g[i] - n_[i] * mean);
+            if (a.dh) d[i] += e[i];
         }
+        if (a.dx) store_as<Tr>(a.dx, false, row * a.cols + c, n, d);
+        if (a.dres) store_as<Tr>(a.dres, a.h32, row * a.cols + c, n, d);
     }
     if (!DW) return;
     float* out = a.dw_part + (int64_t)blockIdx.x * a.cols;
     if constexpr (SLOTS > 1) {
         // slot by slot into one row of LDS, each column by the thread that owns it
-        __shared__ float sum[8 * T * NV];
+        __shared__ float sum[8 * T];
         for (int k = 0; k < SLOTS; ++k) {
             if (slot == k) {
 #pragma unroll
-                for (int v = 0; v < NV; ++v)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float* p = &sum[8 * (t + T * v) + i];
-                        *p = k ? *p + dw[v][i] : dw[v][i];
-                    }
+                for (int i = 0; i < 8; ++i) sum[c + i] = k ? sum[c + i] + dw[i] : dw[i];
             }
             __syncthreads();
         }
-        for (int c = threadIdx.x; c < a.cols; c += kBlock<T>) out[c] = sum[c];
+        for (int i = threadIdx.x; i < a.cols; i += kBlock<T>) out[i] = sum[i];
     } else {
+        store_as<F32>(out, true, c, a.cols - c, dw);
+    }
+}
+
+// Rows too long for that (with a second vector a thread the registers do not do): two passes, 1024 threads a row.
+template <typename Tr>
+__device__ __forceinline__ void load_sum(const NormBwd& a, int64_t at, int n, float (&h)[8]) {
+    load_as<Tr>(a.h, a.h32, at, n, h);
+    if (a.res) {
+        float r[8];
+        load_as<Tr>(a.res, false, at, n, r);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = 8 * (t + T * v);
-            store_as<F32>(out, true, c, a.cols - c, dw[v]);
-        }
+        for (int i = 0; i < 8; ++i) h[i] += r[i];
     }
 }
 
@@ -315,7 +306,7 @@ __global__ __launch_bounds__(1024) void k_rms_bwd_long(NormBwd a) {
         for (int c = 8 * threadIdx.x; c < a.cols; c += 8 * 1024) {
             float g[8], h[8], w[8];
             load_as<Tr>(a.dy, false, at + c, a.cols - c, g);
-            load_as<Tr>(a.h, a.h32, at + c, a.cols - c, h);
+            load_sum<Tr>(a, at + c, a.cols - c, h);
             load_as<Tr>(a.w, a.w32, c, a.cols - c, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(g[i] * w[i], h[i] * r, dot);
@@ -324,7 +315,7 @@ __global__ __launch_bounds__(1024) void k_rms_bwd_long(NormBwd a) {
         for (int c = 8 * threadIdx.x; c < a.cols; c += 8 * 1024) {
             float g[8], h[8], w[8];
             load_as<Tr>(a.dy, false, at + c, a.cols - c, g);
-            load_as<Tr>(a.h, a.h32, at + c, a.cols - c, h);
+            load_sum<Tr>(a, at + c, a.cols - c, h);
             load_as<Tr>(a.w, a.w32, c, a.cols - c, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) g[i] = r * (g[i] * w[i] - h[i] * r * mean);
@@ -350,7 +341,7 @@ __global__ __launch_bounds__(256) void k_rms_dw_long(NormBwd a) {
         float g[8], h[8];
         const float r = a.rstd[row];
         load_as<Tr>(a.dy, false, row * a.cols + c, n, g);
-        load_as<Tr>(a.h, a.h32, row * a.cols + c, n, h);
+        load_sum<Tr>(a, row * a.cols + c, n, h);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw[i] = __builtin_fmaf(g[i], h[i] * r, dw[i]);
     }
@@ -391,7 +382,7 @@ unsigned row_groups(int64_t rows, int per) {
     return (unsigned)(groups < kMostGroups ? groups : kMostGroups);
 }
 
-constexpr int64_t kRegisterCols = 1024 * 4 * 8;
+constexpr int64_t kForwardCols = 1024 * 4 * 8, kBackwardCols = 1024 * 8;  // what registers hold of a row
 
 // Threads of a row: one vector each, up to 8192 columns; whole pairs of waves where that is more than a wave of them
 // ([8192, 5120] backward: 640 threads 67, 1024 80). More vectors a thread are slower, whether a wave then needs no
@@ -409,7 +400,7 @@ int row_threads(int64_t cols) {
 // and the same work ([8192, 4096] us: 256 groups of 512 threads 67, 384 60, 512 54, 768 61, 1024 58; [131072, 128], 256
 // threads: 512 34, 1024 28, 2048 33; [8192, 5120], 640 threads: 256 77, 384 96, 512 79).
 int dw_groups(int64_t rows, int64_t cols) {
-    if (cols > kRegisterCols) return (int)(rows < 64 ? rows : 64);
+    if (cols > kBackwardCols) return (int)(rows < 256 ? rows : 256);
     const int t = row_threads(cols), slots = t <= 256 ? 256 / t : 1, threads = t <= 256 ? 256 : t;
     const int64_t groups = (rows + slots - 1) / slots, most = 256 * (1024 / threads);
     return (int)(groups < most ? groups : most);
@@ -439,7 +430,7 @@ int each_form(int t, int nv, F f) {
 
 template <typename Tr>
 int fwd(const NormFwd& a, hipStream_t st) {
-    if (a.cols > kRegisterCols) {
+    if (a.cols > kForwardCols) {
         hipLaunchKernelGGL(k_rms_fwd_long<Tr>, dim3(row_groups(a.rows, 1)), dim3(1024), 0, st, a);
         return check_launch("rms_norm_fwd");
     }
@@ -456,21 +447,19 @@ template <typename Tr>
 int bwd(const NormBwd& a, void* dweight, hipStream_t st) {
     const int parts = a.dw_part ? dw_groups(a.rows, a.cols) : 0;
     if (a.rows == 0) {  // no row: the weight's gradient is zero
-    } else if (a.cols > kRegisterCols) {
+    } else if (a.cols > kBackwardCols) {
         if (a.dx || a.dres) hipLaunchKernelGGL(k_rms_bwd_long<Tr>, dim3(row_groups(a.rows, 1)), dim3(1024), 0, st, a);
         if (a.dw_part)
             hipLaunchKernelGGL(k_rms_dw_long<Tr>, dim3((unsigned)((a.cols + 2047) / 2048), (unsigned)parts), dim3(256), 0,
                                st, a);
     } else {
-        const int t = row_threads(a.cols), nv = (a.cols + 8 * t - 1) / (8 * t);
-        const int rc = each_form(t, nv, [&](auto T, auto NV) {
+        const int rc = each_form(row_threads(a.cols), 1, [&](auto T, auto) {
             constexpr int per = kBlock<T.value> / T.value;
             if (a.dw_part)
-                hipLaunchKernelGGL((k_rms_bwd<Tr, T.value, NV.value, true>), dim3((unsigned)parts), dim3(kBlock<T.value>), 0,
-                                   st, a);
+                hipLaunchKernelGGL((k_rms_bwd<Tr, T.value, true>), dim3((unsigned)parts), dim3(kBlock<T.value>), 0, st, a);
             else
-                hipLaunchKernelGGL((k_rms_bwd<Tr, T.value, NV.value, false>), dim3(row_groups(a.rows, per)),
-                                   dim3(kBlock<T.value>), 0, st, a);
+                hipLaunchKernelGGL((k_rms_bwd<Tr, T.value, false>), dim3(row_groups(a.rows, per)), dim3(kBlock<T.value>), 0, st,
+                                   a);
             return STM_OK;
         });
         if (rc) return rc;
@@ -527,16 +516,19 @@ extern "C" int64_t stm_rms_norm_workspace_bytes(int64_t rows, int64_t cols) {
     return rows && cols ? (int64_t)dw_groups(rows, cols) * cols * 4 : 0;
 }
 
-extern "C" int stm_rms_norm_bwd(const void* dy, const void* dh, const void* h, int h_dtype, const float* rstd,
-                                const void* weight, int weight_dtype, void* dx, void* dresidual, void* dweight, int64_t rows,
+extern "C" int stm_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* residual, int h_dtype,
+                                const float* rstd, const void* weight, int weight_dtype, void* dx, void* dresidual, void* dweight, int64_t rows,
                                 int64_t cols, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
     const char* what = "rms_norm_bwd";
     int rc = check_rows(what, rows, cols, dtype, weight_dtype);
     if (rc) return rc;
     if (h_dtype != dtype && h_dtype != STM_F32) return set_error(STM_ERR_INVALID, "%s: h must be of dy's type or fp32", what);
+    if (residual && h_dtype == STM_F32)
+        return set_error(STM_ERR_INVALID, "%s: a residual apart from its sum is taken in 16 bits", what);
     if (cols == 0) return STM_OK;
     if (rows && (!dy || !h || !rstd || !weight)) return set_error(STM_ERR_INVALID, "%s: null pointer", what);
-    if (!lies(dy, dtype) || !lies(dx, dtype) || !lies(dh, h_dtype) || !lies(h, h_dtype) || !lies(dresidual, h_dtype) ||
+    if (!lies(dy, dtype) || !lies(dx, dtype) || !lies(dh, h_dtype) || !lies(h, h_dtype) || !lies(residual, h_dtype) ||
+        !lies(dresidual, h_dtype) ||
         !lies(weight, weight_dtype) || !lies(dweight, weight_dtype) || !lies(rstd, STM_F32) || !lies(workspace, STM_F32))
         return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
     if (dweight && rows) {
@@ -547,8 +539,9 @@ extern "C" int stm_rms_norm_bwd(const void* dy, const void* dh, const void* h, i
     }
     if (rows == 0 && !dweight) return STM_OK;
     if (!dx && !dresidual && !dweight) return STM_OK;
-    const NormBwd a{dy,   dh,        h, weight, rstd, dx, dresidual, dweight && rows ? static_cast<float*>(workspace) : nullptr,
-                    rows, (int)cols, h_dtype == STM_F32, weight_dtype == STM_F32};
+    const NormBwd a{dy, dh, h, weight, residual, rstd, dx, dresidual,
+                    dweight && rows ? static_cast<float*>(workspace) : nullptr, rows, (int)cols, h_dtype == STM_F32,
+                    weight_dtype == STM_F32};
     hipStream_t st = (hipStream_t)stream;
     return dtype == STM_BF16 ? bwd<BF16>(a, dweight, st) : dtype == STM_F16 ? bwd<F16>(a, dweight, st) : bwd<F32>(a, dweight, st);
 }

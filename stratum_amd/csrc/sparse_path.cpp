@@ -125,7 +125,11 @@ struct NormFn : torch::autograd::Function<NormFn> {
         const Normed n = norm_fwd(x, w, eps, residual ? *residual : Tensor(), true);
         ctx->set_materialize_grads(false);
         ctx->saved_data["type"] = (int64_t)x.scalar_type();
-        ctx->save_for_backward({residual ? n.h : x, w, n.rstd});
+        // a gradient of the weight that is wider than h as it was rounded takes the sum's terms
+        if (residual && w.requires_grad() && w.scalar_type() == at::kFloat && n.h.scalar_type() != at::kFloat)
+            ctx->save_for_backward({x, w, n.rstd, *residual});
+        else
+            ctx->save_for_backward({residual ? n.h : x, w, n.rstd});
         return residual ? variable_list{n.y, n.h} : variable_list{n.y};
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -143,7 +147,8 @@ struct NormFn : torch::autograd::Function<NormFn> {
             }
         } else {
             const c10::DeviceGuard guard(h.device());
-            const Tensor dy = grads[0].contiguous(), hc = h.contiguous(), wc = w.contiguous();
+            const Tensor dy = grads[0].contiguous(), hc = h.contiguous(), wc = w.contiguous(),
+                         rc = saved.size() == 4 ? saved[3].contiguous() : Tensor();
             const Tensor dh = residual && grads[1].defined() ? grads[1].contiguous() : Tensor();
             const int64_t cols = dy.size(-1), rows = cols ? dy.numel() / cols : 0;
             const bool apart = need_r && h.scalar_type() != type;
@@ -156,7 +161,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
                 dw = like(w, w.sizes(), w.scalar_type());
                 ws = like(dy, {bytes / 4}, at::kFloat);
             }
-            check(lib.norm_bwd(data(dy), data(dh), data(hc), tag_of(h.scalar_type()), static_cast<float*>(data(rstd)),
+            check(lib.norm_bwd(data(dy), data(dh), data(hc), data(rc), tag_of(h.scalar_type()), static_cast<float*>(data(rstd)),
                                data(wc), tag_of(w.scalar_type()), data(dx), data(dr), data(dw), rows, cols, tag_of(type),
                                data(ws), bytes, stream_on(h.device())),
                   "stm_rms_norm_bwd");

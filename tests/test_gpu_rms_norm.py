@@ -255,3 +255,20 @@ def test_module_and_streams(cuda):
         got = norm(x, r)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, norm(x, r)))
+
+
+@pytest.mark.parametrize("shape", [(1, 96), (101, 384), (2000, 64), (300, 1000), (257, 4100), (70, 9000), (3, 40000)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_the_gradient_of_a_wider_weight(cuda, shape, dtype):
+    """An fp32 weight's gradient is as exact as the sum, not as h rounded to 16 bits."""
+    from stratum_amd import rms_norm
+    x, r, w = seeded(shape, 1, 1.0, dtype), seeded(shape, 2, 2.0, dtype), 1 + seeded(shape[-1:], 3, 0.3)
+    dy, dh = seeded(shape, 4, 1.0, dtype), seeded(shape, 5, 1.0, dtype)
+    ref = reference(x, w, 1e-6, r, dy, dh, F4)
+    leaves = [t.requires_grad_(True) for t in (x, w, r)]
+    dx, dw, dr = torch.autograd.grad(rms_norm(x, w, 1e-6, r), leaves, (dy, dh))
+    for name, got in (("dx", dx), ("dw", dw), ("dr", dr)):
+        assert_within(got, *ref[name], name)
+    # the others are the same whichever are asked for
+    again, = torch.autograd.grad(rms_norm(x, w, 1e-6, r), (x,), (dy, dh))
+    assert torch.equal(again, dx)

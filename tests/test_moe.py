@@ -24,8 +24,8 @@ def norm_fwd(L, x=BASE, r=None, rt=1, w=BASE, wt=1, y=BASE, h=None, rstd=None, r
 
 
 def norm_bwd(L, dy=BASE, dh=None, h=BASE, ht=1, rstd=BASE, w=BASE, wt=1, dx=BASE, dr=None, dw=None, rows=1, cols=64, dtype=1,
-             ws=None, bytes=0):
-    return L.stm_rms_norm_bwd(dy, dh, h, ht, rstd, w, wt, dx, dr, dw, rows, cols, dtype, ws, bytes, None)
+             ws=None, bytes=0, r=None):
+    return L.stm_rms_norm_bwd(dy, dh, h, r, ht, rstd, w, wt, dx, dr, dw, rows, cols, dtype, ws, bytes, None)
 
 
 def test_the_norms_c_abi_refuses(L):
@@ -36,7 +36,7 @@ def test_the_norms_c_abi_refuses(L):
                 dict(rows=1 << 31), dict(cols=1 << 30), dict(r=BASE, h=BASE + 2, rt=2)):
         assert norm_fwd(L, **bad) < 0 and "rms_norm" in err(), bad
     for bad in (dict(dy=None), dict(h=None), dict(rstd=None), dict(w=None), dict(ht=0), dict(wt=0), dict(rows=-1),
-                dict(dtype=9), dict(dw=BASE), dict(dw=BASE, ws=BASE, bytes=255), dict(dh=BASE + 1), dict(dw=BASE + 1)):
+                dict(dtype=9), dict(dw=BASE), dict(dw=BASE, ws=BASE, bytes=255), dict(r=BASE, ht=2), dict(r=BASE + 1), dict(dh=BASE + 1), dict(dw=BASE + 1)):
         assert norm_bwd(L, **bad) < 0 and "rms_norm" in err(), bad
     # nothing to do
     assert norm_fwd(L, x=None, w=None, y=None, rows=0) == 0 and norm_fwd(L, x=None, w=None, y=None, cols=0) == 0
