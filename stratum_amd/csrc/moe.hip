@@ -36,7 +36,8 @@ unsigned groups_for(int64_t items, int per) {
 // score + bias in 64 bits: two experts whose keys differ by less than an fp32 rounding are still told apart, and the same
 // ones are found as by any other program that computes them so. They are computed in 32 bits first, with a bound on what that
 // may be off. Where experts that follow each other are nearer than the bound, the keys of those taken are computed in
-// 64 bits, by a lane each; where groups are (or a value is not finite), all of them (16383 tokens of 256, sigmoid, bias, 8 groups, us: always 43, so 29).
+// 64 bits, by a lane each; where groups are (or a value is not finite), all of them (16383 tokens of 256, sigmoid, bias, 8
+// groups, us: always 43, so 29; 22 if no token needed them).
 struct Route {
     const void* logits;
     const float* bias;
@@ -860,7 +861,9 @@ __global__ __launch_bounds__(256) void k_combine_bwd(Rows a) {
 bool known(int dtype) { return dtype == STM_F16 || dtype == STM_BF16 || dtype == STM_F32; }
 bool lies(const void* p, int dtype) { return aligned(p, dtype == STM_F32 ? 4 : 2); }
 
-// f(type, lanes, values a lane) of the form that holds a token's experts; its lanes hold one chosen expert and one group each.
+// f(type, lanes, values a lane) of the form that holds a token's experts; its lanes hold one chosen expert and one group
+// each. Twice the values on half the lanes, us: 16383 tokens of 256 in bf16 9.8 -> 8.6, with bias and groups 29 -> 37, one
+// token 3.8 -> 5.1.
 template <typename Tr, typename F>
 int each_form(int E, int least, F f) {
     using std::integral_constant;
