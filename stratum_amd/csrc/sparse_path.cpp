@@ -10,9 +10,11 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -99,6 +101,24 @@ variable_list once(variable_list grads, const char* name) {
     return grads;
 }
 
+// A gradient that is captured into a graph must end where the capture can follow: a leaf that an eager graph still holds
+// is tied to that graph's stream, and torch's engine, passing a gradient on from the capture to it, ends the process.
+void check_capture(const char* name) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const c10::Stream now = c10::hip::getCurrentHIPStream().unwrap();
+    for (const auto& edge : node->next_edges()) {
+        if (!edge.is_valid()) continue;
+        const auto stream = edge.function->stream();
+        if (stream && stream->id() != now.id())
+            throw std::runtime_error(std::string(name) +
+                                     ": its gradient is captured into a graph, but an operand of it belongs to an eager graph on "
+                                     "another stream; capture on operands of its own (t.detach().requires_grad_()) or let "
+                                     "go of the eager graph first");
+    }
+}
+
 std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
 // ------------------------------------------------------------ norm
@@ -134,6 +154,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
         return residual ? variable_list{n.y, n.h} : variable_list{n.y};
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_capture("rms_norm");
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
         const bool residual = grads.size() == 2;
@@ -242,6 +263,7 @@ struct RouteFn : torch::autograd::Function<RouteFn> {
         return {weights, experts};
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_capture("moe_route");
         const variable_list saved = ctx->get_saved_variables();
         const auto args = ctx->saved_data["args"].toDoubleVector();
         if (!grads[0].defined()) return {Tensor(), Tensor()};
@@ -376,6 +398,7 @@ struct GatherFn : torch::autograd::Function<GatherFn> {
         return gather_fwd(x, *o);
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_capture("moe_gather");
         const c10::DeviceGuard guard(grads[0].device());
         const Tensor dx = combine_fwd(grads[0], Tensor(), ctx->get_saved_variables()[0], Tensor(),
                                       ctx->saved_data["sizes"].toIntVector());
@@ -410,6 +433,7 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
         return combine_fwd(y, weights, o->positions, residual ? *residual : Tensor(), *sizes);
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_capture("moe_combine");
         const variable_list saved = ctx->get_saved_variables();
         const auto y_is = ctx->saved_data["y"].toIntVector();
         const Tensor &y = saved[0], &weights = saved[1], &offsets = saved[2], &positions = saved[3];

@@ -11,7 +11,7 @@ order. Here is what comes before and after it:
 :class:`NF4MoE` runs them around an NF4 expert bank, with the norm and the residual's addition before.
 The reference runs transformers' ``Qwen3MoeExperts`` and router there (``stratum/model/qwen3_moe.py``,
 ``stratum/moe.py``). None of the four reads anything back to the host; all can be captured into a graph, with their
-gradients too (as for any operator of torch, on leaves that no eager graph holds: ``t.detach().requires_grad_()``).
+gradients too: of operands that belong to no eager graph (``t.detach().requires_grad_()``), others are refused.
 """
 
 from __future__ import annotations

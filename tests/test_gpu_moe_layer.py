@@ -244,3 +244,42 @@ def test_tensor_subclasses(cuda):
             results.append([torch.Tensor(t.detach()) for t in (out, *grads)])
         assert all(torch.equal(a, b) for a, b in zip(*results))
     assert all(torch.equal(a, b) for a, b in zip(moe_sort(e.as_subclass(Named), 16), order))
+
+
+def test_a_captured_gradient_of_an_eager_graphs_leaf_is_refused(cuda):
+    """The engine cannot pass a gradient on from a capture to a leaf that an eager graph ties to another stream."""
+    from stratum_amd import moe_combine, moe_gather, moe_route, moe_sort, rms_norm
+    x, w = seeded((12, 64), 1), seeded((64,), 2)
+    order = moe_sort(moe_route(x[:, :8], 2)[1], 8)
+    rows, weights = seeded((24, 64), 3), seeded((12, 2), 4)
+    for name, op, operand in (("rms_norm", lambda t: rms_norm(t, w), x), ("moe_route", lambda t: moe_route(t, 2)[0], x),
+                              ("moe_gather", lambda t: moe_gather(t, order), x),
+                              ("moe_combine", lambda t: moe_combine(t, weights, order), rows)):
+        leaf = operand.clone().requires_grad_(True)
+        eager = op(leaf)
+        d = torch.ones_like(eager)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match=f"{name}.*captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(op(leaf), leaf, d)
+        torch.cuda.synchronize()
+        want, = torch.autograd.grad(eager, leaf, d)
+        del eager
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(op(leaf), leaf, d)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
+
+
+def test_no_columns(cuda):
+    from stratum_amd import moe_combine, moe_gather, moe_sort
+    order = moe_sort(torch.tensor([[0, 1], [2, 0]], dtype=torch.int32, device=cuda), 4)
+    y, w = torch.zeros(4, 0, dtype=BF, device=cuda, requires_grad=True), seeded((2, 2), 1).requires_grad_(True)
+    out = moe_combine(y, w, order)
+    assert out.shape == (2, 0)
+    dy, dw = torch.autograd.grad(out, (y, w), torch.zeros_like(out))
+    assert dy.shape == (4, 0) and torch.equal(dw, torch.zeros_like(w))
+    assert moe_gather(torch.zeros(2, 0, dtype=BF, device=cuda), order).shape == (4, 0)
