@@ -1086,13 +1086,14 @@ extern "C" int stm_moe_combine_bwd(const void* dout, int dout_dtype, const void*
     if (y_rows < 0 || y_rows > tokens * top_k)
         return set_error(STM_ERR_INVALID, "%s: %lld rows for %lld slots", what, (long long)y_rows,
                          (long long)(tokens * top_k));
+    if (y_rows == 0 || hidden == 0) dy = nullptr;  // nothing of it
     if (tokens == 0 || top_k == 0 || (!dy && !dweights)) return STM_OK;
     if (!positions || (hidden && (!dout || (y_rows && ((dweights && !y) || (dy && (!weights || !offsets)))))))
         return set_error(STM_ERR_INVALID, "%s: null pointer", what);
     if (!lies(dout, dout_dtype) || !lies(y, dtype) || !lies(dy, dtype) || !aligned(positions, 4) || !aligned(weights, 4) ||
         !aligned(offsets, 4) || !aligned(dweights, 4))
         return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
-    const Rows a{dout, y, weights, positions, offsets, y_rows ? dy : nullptr, dweights, tokens, hidden, y_rows, top_k, num_experts,
+    const Rows a{dout, y, weights, positions, offsets, dy, dweights, tokens, hidden, y_rows, top_k, num_experts,
                  dout_dtype == STM_F32};
     return each_type(dtype, [&](auto tr) {
         const auto run = [&](auto w) {

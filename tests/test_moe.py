@@ -109,6 +109,7 @@ def test_the_rows_c_abi_refuses(L):
                 dict(dtype=8), dict(dw=BASE + 2), dict(d=BASE + 1)):
         assert bwd(**bad) < 0 and "moe_combine" in err(), bad
     assert bwd(dy=None, dw=None, d=None) == 0 and bwd(T=0, d=None, rows=0) == 0
+    assert bwd(H=0, dw=None, d=None, y=None, w=None, o=None) == 0 and bwd(rows=0, dw=None, d=BASE, y=None, w=None, o=None) == 0
 
 
 def order(tokens=4, k=2, E=8):
