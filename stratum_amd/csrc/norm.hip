@@ -354,24 +354,28 @@ template <typename Tr>
 __global__ __launch_bounds__(1024) void k_rms_dw(const float* __restrict__ part, int parts, int cols, void* dw,
                                                  bool w32) {
     __shared__ float sum[32][33];
-    const int c = blockIdx.x * 32 + threadIdx.x % 32, slot = threadIdx.x / 32;
-    float s = 0.0f;
-    if (c < cols)
-        for (int p0 = slot; p0 < parts; p0 += 32 * 8) {
-            float v[8];
+    const int slot = threadIdx.x / 32;
+    for (int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x % 32; c - threadIdx.x % 32 < cols; c += (int64_t)gridDim.x * 32) {
+        float s = 0.0f;
+        if (c < cols)
+            for (int p0 = slot; p0 < parts; p0 += 32 * 8) {
+                float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = p0 + 32 * i < parts ? part[(int64_t)(p0 + 32 * i) * cols + c] : 0.0f;
+                for (int i = 0; i < 8; ++i) v[i] = p0 + 32 * i < parts ? part[(int64_t)(p0 + 32 * i) * cols + c] : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i];
+                for (int i = 0; i < 8; ++i) s += v[i];
+            }
+        sum[slot][threadIdx.x % 32] = s;
+        __syncthreads();
+        if (slot == 0 && c < cols) {
+            for (int k = 1; k < 32; ++k) s += sum[k][threadIdx.x];
+            if (w32)
+                static_cast<float*>(dw)[c] = s;
+            else
+                static_cast<typename Eight<Tr>::elem*>(dw)[c] = Tr::from_f32(s);
         }
-    sum[slot][threadIdx.x % 32] = s;
-    __syncthreads();
-    if (slot || c >= cols) return;
-    for (int k = 1; k < 32; ++k) s += sum[k][threadIdx.x];
-    if (w32)
-        static_cast<float*>(dw)[c] = s;
-    else
-        static_cast<typename Eight<Tr>::elem*>(dw)[c] = Tr::from_f32(s);
+        __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------ which form
@@ -465,8 +469,7 @@ int bwd(const NormBwd& a, void* dweight, hipStream_t st) {
         if (rc) return rc;
     }
     if (dweight)
-        hipLaunchKernelGGL(k_rms_dw<Tr>, dim3((unsigned)((a.cols + 31) / 32)), dim3(1024), 0, st, a.dw_part, parts, a.cols,
-                           dweight, a.w32);
+        hipLaunchKernelGGL(k_rms_dw<Tr>, dim3(row_groups(a.cols, 32)), dim3(1024), 0, st, a.dw_part, parts, a.cols, dweight, a.w32);
     return check_launch("rms_norm_bwd");
 }
 

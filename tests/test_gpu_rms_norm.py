@@ -272,3 +272,17 @@ def test_the_gradient_of_a_wider_weight(cuda, shape, dtype):
     # the others are the same whichever are asked for
     again, = torch.autograd.grad(rms_norm(x, w, 1e-6, r), (x,), (dy, dh))
     assert torch.equal(again, dx)
+
+
+def test_a_very_long_row(cuda):
+    """More columns than one launch of the weight's sum has work-groups for (2^21, of 32 columns each)."""
+    from stratum_amd import rms_norm
+    cols = (1 << 26) + 40
+    x = torch.empty(1, cols, dtype=BF, device=cuda).normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    w = torch.ones(cols, dtype=BF, device=cuda)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    y = rms_norm(*leaves)
+    dx, dw = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    # one row: dw = n = y where the weights are one, each rounded once
+    assert torch.equal(dw, y[0])
+    assert dx.shape == x.shape and dx[0, -40:].isfinite().all()
