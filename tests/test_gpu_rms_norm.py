@@ -258,11 +258,11 @@ def test_module_and_streams(cuda):
 
 
 @pytest.mark.parametrize("shape", [(1, 96), (101, 384), (2000, 64), (300, 1000), (257, 4100), (70, 9000), (3, 40000)])
-@pytest.mark.parametrize("dtype", [BF, FP])
-def test_the_gradient_of_a_wider_weight(cuda, shape, dtype):
-    """An fp32 weight's gradient is as exact as the sum, not as h rounded to 16 bits."""
+@pytest.mark.parametrize("dtype,weight", [(BF, F4), (FP, F4), (BF, BF), (FP, FP)])
+def test_the_weights_gradient_takes_the_sum(cuda, shape, dtype, weight):
+    """It is as exact as the sum, not as h rounded to 16 bits."""
     from stratum_amd import rms_norm
-    x, r, w = seeded(shape, 1, 1.0, dtype), seeded(shape, 2, 2.0, dtype), 1 + seeded(shape[-1:], 3, 0.3)
+    x, r, w = seeded(shape, 1, 1.0, dtype), seeded(shape, 2, 2.0, dtype), (1 + seeded(shape[-1:], 3, 0.3)).to(weight)
     dy, dh = seeded(shape, 4, 1.0, dtype), seeded(shape, 5, 1.0, dtype)
     ref = reference(x, w, 1e-6, r, dy, dh, F4)
     leaves = [t.requires_grad_(True) for t in (x, w, r)]
