@@ -210,10 +210,11 @@ def _own_norm(state, step):
     from stratum_amd import rms_norm
     x, weight, residual = state["x"], state["weight"], state["residual"]
     y = rms_norm(x, weight, EPS, residual)
-    out = {"y": y} if residual is None else {"y": y[0], "h": y[1]}
+    out, grads = ({"y": y}, (state["dy"],)) if step or residual is None else ({"y": y[0], "h": y[1]}, None)
+    if residual is not None and step:
+        out, grads = {"y": y[0], "h": y[1]}, (state["dy"], state["dh"])
     if not step:
         return out
-    grads = (state["dy"],) if residual is None else (state["dy"], state["dh"])
     wanted = {"dx": x, "dresidual": residual, "dweight": weight if weight.requires_grad else None}
     wanted = {name: t for name, t in wanted.items() if t is not None}
     got = torch.autograd.grad(tuple(out.values()), tuple(wanted.values()), grads)
