@@ -428,8 +428,8 @@ int stm_state8_values(const uint8_t* codes, const float* scales, int64_t n, int 
  * stm_rms_norm_bwd: from the gradients dy of y and dh of h (NULL: none), h (x where there was no
  * residual) and rstd: the gradient of the sum as dx (rows' type) and dresidual (h_dtype), and dweight (weight_dtype),
  * each NULL if not wanted; dweight needs stm_rms_norm_workspace_bytes(rows, cols) of workspace. Its sums over rows
- * are taken in a fixed order. `residual` (or NULL): h is x and this its residual, both of a 16-bit h_dtype: for a
- * dweight that is to be more exact than the sum as it was rounded.
+ * are taken in a fixed order. `residual` (or NULL): h is x and this its residual, both of a 16-bit h_dtype: for
+ * gradients that are to be more exact than those of the sum as it was rounded.
  */
 int stm_rms_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, int weight_dtype,
                      void* y, void* h, float* rstd, int64_t rows, int64_t cols, double eps, int dtype, void* stream);

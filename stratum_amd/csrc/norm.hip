@@ -2,14 +2,15 @@
 //
 //   s = x (+ residual),  r = 1 / sqrt(mean(s^2) + eps),  y = s r w,  h = s rounded to the residual's type
 //
-// backward, with n = h r (h as it was stored) and t = w dy:
+// backward, with n = s r and t = w dy:
 //
 //   ds = r (t - n mean(t n)) (+ dh),  dw = sum over rows of dy n
 //
 // ds is the gradient of x and of the residual. Everything between a load and a store is fp32; y comes from the sum
-// before its rounding to h, so each output is rounded once. The backward's n may use the rounded h: half a step of h in a
-// term of ds, which is rounded to that type itself. A weight's gradient takes x and the residual again (bf16, 763 rows of
-// 5058: 2.4e-3 off with the rounded h, 1.8e-3, its own rounding, without).
+// before its rounding to h, so each output is rounded once. The backward's s is h where h is exact (x without a residual,
+// an fp32 stream) and x + residual again where h has 16 bits: with h as it was rounded a weight's gradient is 2.4e-3 off
+// (bf16, 763 rows of 5058) and not the 1.8e-3 of its own rounding, and ds differs by 2.1e-4 ([8192, 4096] bf16) from
+// the plain form's.
 //
 // Bound by bytes. One pass: a row stays in registers between its sum and its result, 8 elements of a thread in one access.
 // A row belongs to 8 to 64 lanes of a wave (no barrier), or to 128 to 1024 threads.

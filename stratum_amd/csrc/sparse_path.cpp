@@ -146,8 +146,8 @@ struct NormFn : torch::autograd::Function<NormFn> {
         const Normed n = norm_fwd(x, w, eps, residual ? *residual : Tensor(), true);
         ctx->set_materialize_grads(false);
         ctx->saved_data["type"] = (int64_t)x.scalar_type();
-        // the weight's gradient takes the sum's terms where h was rounded to 16 bits
-        if (residual && w.requires_grad() && n.h.scalar_type() != at::kFloat)
+        // the gradients take the sum's terms where h was rounded to 16 bits
+        if (residual && n.h.scalar_type() != at::kFloat)
             ctx->save_for_backward({x, w, n.rstd, *residual});
         else
             ctx->save_for_backward({residual ? n.h : x, w, n.rstd});

@@ -57,9 +57,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     With ``residual`` (x's shape; x's dtype or fp32) the rows are ``h = x + residual``, and the result is
     ``(y, h)``, h in the residual's dtype: y comes from the sum in 32 bits, each output is rounded once.
     ``weight``: [columns] in x's dtype or fp32. Differentiable in x, the residual and the weight (reverse
-    mode, once); the weight's gradient is a sum in a fixed order. Kept for the backward: h (x without a residual;
-    x and the residual where h has 16 bits and the weight a gradient: h as it was rounded would add as much error to
-    it as its own rounding does) and 4 bytes a row."""
+    mode, once); the weight's gradient is a sum in a fixed order. Kept for the backward: h (x without a residual; x and
+    the residual where h has 16 bits: the gradients are those of the sum, and do not depend on which of them are asked
+    for) and 4 bytes a row."""
     out = _lib.sparse().norm(x, weight, eps, residual)
     if out is None:  # an operand to refuse or to convert, or another device than the current one
         _check(x, weight, eps, residual)
