@@ -336,21 +336,39 @@ __global__ __launch_bounds__(256) void k_route(Route a) {
                                   u * (fabsf(border.least) + fabsf(border.next));
                 close |= border.next > -INFINITY && !(border.least - border.next > 2.0f * err);
             }
-            // Without a bias the scores are in the order of the logits, and equal where the logits are; that others are
-            // apart in 64 bits too is certain unless they are less than u apart or where the scores end (a sigmoid beyond
-            // 16 is 1 - exp(-x): u exp(-16) is 2^-47; exp(-700) is still normal).
+            // Without a bias the scores are in the order of the logits, and equal where the logits are. Different logits have
+            // scores that are certainly apart in 64 bits too (`parted`, of the larger and the smaller) unless they are less
+            // than u apart or where the scores end (a sigmoid beyond 16 is 1 - exp(-x): u exp(-16) is 2^-47; exp(-700) is
+            // still normal). Equal logits are in the right order by themselves, but not if one of them may have the score of a
+            // logit outside: of a larger one (`linked`), or of a smaller one with a lower index.
             // Lane j takes the j-th key, beyond top_k until the next one is smaller for certain.
-            bool mixed = false;
+            const auto parted = [&](float more, float less) {
+                return more - less > u && (a.sigmoid ? more <= 16.0f && less > -700.0f : top - less < 700.0f);
+            };
+            bool mixed = false, linked = false;
             float before = 0.0f;
             int taken = 0;
             chosen = -1;
             for (;; ++taken) {
                 const float k = largest<LANES, VPL>(order);
-                bool apart = true;
+                bool apart = true, ends = false;  // ends: the choice among equal logits, if no smaller one has their score
                 if (taken && k > -INFINITY) {
-                    const float gap = before - k;
-                    apart = a.bias ? gap > 2.0f * (off + u * (fabsf(before) + fabsf(k))) :
-                                     gap == 0.0f || (gap > u && (a.sigmoid ? before <= 16.0f && k > -700.0f : top - k < 700.0f));
+                    if (a.bias) {
+                        apart = before - k > 2.0f * (off + u * (fabsf(before) + fabsf(k)));
+                    } else if (before == k) {
+                        apart = !linked;
+                        ends = apart && taken >= a.top_k;
+                    } else {
+                        apart = parted(before, k);
+                        linked = !apart;
+                    }
+                }
+                if (!a.bias && __any(ends)) {
+                    float below = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) below = fmaxf(below, order[i] < k ? order[i] : -INFINITY);
+                    below = lanes_max<LANES>(below);
+                    if (ends && below > -INFINITY) apart = parted(k, below);
                 }
                 mixed |= !apart;
                 if (taken >= a.top_k && !__any(!apart)) break;
