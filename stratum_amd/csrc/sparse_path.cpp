@@ -10,7 +10,6 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -23,6 +22,8 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/stratum_nf4.h"
 
@@ -101,21 +102,44 @@ variable_list once(variable_list grads, const char* name) {
     return grads;
 }
 
+// The graph that a stream is being captured into (0: none; the null stream cannot be).
+unsigned long long capture_of(hipStream_t stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (!stream) return 0;
+    if (hipStreamGetCaptureInfo(stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 // A gradient that is captured into a graph must end where the capture can follow: a leaf that an eager graph still holds
-// is tied to that graph's stream, and torch's engine, passing a gradient on from the capture to it, ends the process.
+// is tied to that graph's stream, and torch's engine, passing a gradient on from the capture to it, ends the process. So
+// what follows a node in this backward pass is looked through first, on other streams of the same capture too; what
+// nobody asked for is not followed.
 void check_capture(const char* name) {
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const unsigned long long now = capture_of(c10::hip::getCurrentHIPStream().stream());
+    if (!now) return;
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
-    const c10::Stream now = c10::hip::getCurrentHIPStream().unwrap();
-    for (const auto& edge : node->next_edges()) {
-        if (!edge.is_valid()) continue;
-        const auto stream = edge.function->stream();
-        if (stream && stream->id() != now.id())
-            throw std::runtime_error(std::string(name) +
-                                     ": its gradient is captured into a graph, but an operand of it belongs to an eager graph on "
-                                     "another stream; capture on operands of its own (t.detach().requires_grad_()) or let "
-                                     "go of the eager graph first");
+    std::vector<torch::autograd::Node*> left{node.get()};
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!left.empty()) {
+        torch::autograd::Node* n = left.back();
+        left.pop_back();
+        for (uint32_t i = 0; i < n->num_outputs(); ++i) {
+            if (!n->task_should_compute_output(i)) continue;
+            torch::autograd::Node* next = n->next_edge(i).function.get();
+            if (!seen.insert(next).second) continue;
+            const auto stream = next->stream();
+            if (stream && capture_of(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *stream).stream()) != now)
+                throw std::runtime_error(std::string(name) +
+                                         ": its gradient is captured into a graph, but goes on to a leaf of an eager graph, "
+                                         "whose stream takes no part in the capture; capture on leaves of its own "
+                                         "(t.detach().requires_grad_()) or let go of the eager graph first");
+            left.push_back(next);
+        }
     }
 }
 
