@@ -224,7 +224,7 @@ class NF4MoE(nn.Module):
     ``(packed, QuantState)`` of the stacked banks [E, 2 I, H] ([gate; up] of each expert) and [E, H, I], as
     ``quantize_4bit`` makes them from 3-D weights. ``norm`` is an :class:`~stratum_amd.norm.RMSNorm` or None (y = x; out
     then has the residual added if one is given, and nothing else). The remaining arguments are those of
-    :func:`moe_route`; ``bias`` becomes a float32 buffer.
+    :func:`moe_route`; ``bias`` becomes a float32 buffer, which ``.to(dtype)`` and ``.half()`` leave in 32 bits.
 
     Differentiable in x, the residual, the norm's weight and the router's parameters. The experts' row counts are read
     back once per call (the products' launch needs them)."""
@@ -286,6 +286,13 @@ class NF4MoE(nn.Module):
         out = self.experts(moe_gather(rows, order), order)
         stream = _rows(h, self.hidden) if h is not None else None
         return moe_combine(out, weights, order, stream).reshape(x.shape)
+
+    def _apply(self, fn, recurse=True):
+        bias = self.bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.bias.dtype != torch.float32:  # .to(dtype), .half(): it moves and stays as exact
+            self.bias = bias.float().to(self.bias.device)
+        return self
 
     def extra_repr(self) -> str:
         return (f"{self.num_experts} experts of [{self.hidden}, {self.inter}], top {self.top_k}, "
