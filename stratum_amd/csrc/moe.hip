@@ -715,7 +715,7 @@ __device__ __forceinline__ void load_stream(const void* p, bool wide, int64_t at
     }
 }
 
-enum class Far { none, loads, both };  // accesses to the experts' rows that pass the caches by
+enum class Far { none, loads, both };  // accesses of the gradient to the experts' rows that pass the caches by
 
 constexpr unsigned kMostColumnGroups = 1u << 15, kMostTokenGroups = 1u << 15;
 
@@ -750,7 +750,8 @@ __device__ __forceinline__ void clear_tail(const Rows& a, void* out, int64_t liv
     }
 }
 
-template <typename Tr, Far FAR>
+// FAR: the stores of the experts' rows pass the caches by; in k_combine the loads.
+template <typename Tr, bool FAR>
 __global__ __launch_bounds__(256) void k_gather(Rows a) {
     const int64_t live = a.offsets[a.E];
     each_part(a, [&](int64_t token, int64_t c, int n) {
@@ -758,7 +759,7 @@ __global__ __launch_bounds__(256) void k_gather(Rows a) {
         v.load(a.in, token * a.hidden + c, n);
         for (int j = 0; j < a.top_k; ++j) {
             const int64_t p = a.positions[token * a.top_k + j];
-            if (p >= 0 && p < a.rows) v.template store<(FAR == Far::both)>(a.out, p * a.hidden + c, n);
+            if (p >= 0 && p < a.rows) v.template store<FAR>(a.out, p * a.hidden + c, n);
         }
     });
     const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, groups = (int64_t)gridDim.x * gridDim.y;
@@ -766,7 +767,7 @@ __global__ __launch_bounds__(256) void k_gather(Rows a) {
 }
 
 // J of the token's rows are asked for before the first is used.
-template <typename Tr, int J, Far FAR>
+template <typename Tr, int J, bool FAR>
 __global__ __launch_bounds__(256) void k_combine(Rows a) {
     each_part(a, [&](int64_t token, int64_t c, int n) {
         float s[8] = {};
@@ -780,7 +781,7 @@ __global__ __launch_bounds__(256) void k_combine(Rows a) {
                 const int64_t p = j0 + j < a.top_k ? a.positions[slot] : -1;
                 const bool live = p >= 0 && p < a.rows;  // (what is not adds 1 * 0: its weight may be anything)
                 w[j] = live && a.weights ? a.weights[slot] : 1.0f;
-                y[j].template load<(FAR != Far::none)>(a.in, p * a.hidden + c, live ? n : 0);
+                y[j].template load<FAR>(a.in, p * a.hidden + c, live ? n : 0);
             }
 #pragma unroll
             for (int j = 0; j < J; ++j)
@@ -934,18 +935,24 @@ int each_chunk(int top_k, F f) {
     return f(integral_constant<int, 8>{});
 }
 
-// f(which accesses to the experts' rows pass the caches by). Read once, rows of a good part of the 256 MB memory-side cache
+// Which accesses to the experts' rows pass the caches by. Read once, rows of a good part of the 256 MB memory-side cache
 // leave it to what is read again; written, rows that do not fit it gain from passing it by, smaller ones are there for the
-// product that takes them (bf16, 8 slots a token of 2048 columns, us; nothing / loads / both): combination of 3000 tokens
-// 25.1 / 25.0, of 4096 32.1 / 29.3, of 8192 65 / 56; gather of 4096 and their combination 58 / 50 / 57, of 8192
-// 136 / 109 / 107; the gradient of 1024 14 / 20, of 8192 125 / 113 / 108. Stores that do so have to fill their 128-byte
-// lines, as those of whole 16-bit chunks do (fp32, two halves of a line apart: gather of 4096 tokens 62 / 130).
-template <typename F>
-int each_distance(int64_t rows, int64_t hidden, int dtype, F f) {
-    const int64_t bytes = rows * hidden * (dtype == STM_F32 ? 4 : 2);
-    if (bytes < 96ll << 20) return f(std::integral_constant<Far, Far::none>{});
-    if (bytes < 256ll << 20 || dtype == STM_F32 || hidden % 64) return f(std::integral_constant<Far, Far::loads>{});
-    return f(std::integral_constant<Far, Far::both>{});
+// product that takes them. Stores that do so have to fill their 128-byte lines, as those of whole 16-bit chunks do (fp32,
+// two halves of a line apart: gather of 256 MiB 64 / 130). bf16, 8 slots a token of 2048 columns, us, nothing / loads / both:
+//   MiB                                            62            128            188            256            512
+//   combination                                    14 / 15       32 / 29        45 / 42        65 / 56        129 / 106
+//   gather, its rows read by a combination         27 / 27 / 30  59 / 50 / 57   80 / 81 / 82   135 / 109 / 108  263 / 226 / 229
+//   gather alone                                   13 / 13 / 15  30 / 30 / 28   44 / 44 / 40   59 / 59 / 51   117 / 117 / 104
+//   combination and its gradient                   52 / 46 / 48  101 / 95 / 87  145 / 136 / 126  193 / 182 / 162  376 / 360 / 338
+// Other rows gain less and lose as often, nothing / loads: fp32 of 125 MiB, combination 31 / 33, after a gather 60 / 55, with
+// its gradient 95 / 100; of 512 MiB 134 / 121, 292 / 261 and 371 / 374. bf16 of 1001 columns, 122 MiB 39 / 38, 73 / 74 and
+// 131 / 147; 244 MiB 77 / 74, 153 / 144 and 262 / 282.
+int64_t row_bytes(int64_t rows, int64_t hidden, int dtype) { return rows * hidden * (dtype == STM_F32 ? 4 : 2); }
+
+bool far_loads(int64_t rows, int64_t hidden, int dtype) { return row_bytes(rows, hidden, dtype) >= 96ll << 20; }
+
+bool far_stores(int64_t rows, int64_t hidden, int dtype) {
+    return row_bytes(rows, hidden, dtype) >= 256ll << 20 && dtype != STM_F32 && hidden % 64 == 0;
 }
 
 template <typename F>
@@ -1057,11 +1064,14 @@ extern "C" int stm_moe_gather(const void* x, const int32_t* positions, const int
         return set_error(STM_ERR_INVALID, "%s: pointers must be aligned to their elements", what);
     const Rows a{x, nullptr, nullptr, positions, offsets, out, nullptr, tokens, hidden, tokens * top_k, top_k, num_experts, false};
     return each_type(dtype, [&](auto tr) {
-        return each_distance(tokens * top_k, hidden, dtype, [&](auto far) {
+        const auto run = [&](auto far) {
             hipLaunchKernelGGL((k_gather<decltype(tr), far.value>), row_grid(tokens, hidden), dim3(256), 0, (hipStream_t)stream,
                                a);
             return check_launch(what);
-        });
+        };
+        if constexpr (!std::is_same_v<decltype(tr), F32>)
+            if (far_stores(tokens * top_k, hidden, dtype)) return run(std::true_type{});
+        return run(std::false_type{});
     });
 }
 
@@ -1083,11 +1093,12 @@ extern "C" int stm_moe_combine(const void* y, int64_t y_rows, const float* weigh
     const Rows a{y, residual, weights, positions, nullptr, out, nullptr, tokens, hidden, y_rows, top_k, 0, out_dtype == STM_F32};
     return each_type(dtype, [&](auto tr) {
         return each_chunk(top_k, [&](auto j) {
-            return each_distance(y_rows, hidden, dtype, [&](auto far) {
+            const auto run = [&](auto far) {
                 hipLaunchKernelGGL((k_combine<decltype(tr), j.value, far.value>), row_grid(tokens, hidden), dim3(256), 0,
                                    (hipStream_t)stream, a);
                 return check_launch(what);
-            });
+            };
+            return far_loads(y_rows, hidden, dtype) ? run(std::true_type{}) : run(std::false_type{});
         });
     });
 }
@@ -1118,11 +1129,15 @@ extern "C" int stm_moe_combine_bwd(const void* dout, int dout_dtype, const void*
             const int64_t groups = (tokens + 4 / w.value - 1) / (4 / w.value);
             const dim3 grid((unsigned)(groups < (1 << 22) ? groups : 1 << 22));
             return each_chunk(top_k, [&](auto j) {
-                return each_distance(y_rows, hidden, dtype, [&](auto far) {
+                const auto launch = [&](auto far) {
                     hipLaunchKernelGGL((k_combine_bwd<decltype(tr), j.value, w.value, far.value>), grid, dim3(256), 0,
                                        (hipStream_t)stream, a);
                     return check_launch(what);
-                });
+                };
+                if constexpr (!std::is_same_v<decltype(tr), F32>)
+                    if (far_stores(y_rows, hidden, dtype)) return launch(std::integral_constant<Far, Far::both>{});
+                if (far_loads(y_rows, hidden, dtype)) return launch(std::integral_constant<Far, Far::loads>{});
+                return launch(std::integral_constant<Far, Far::none>{});
             });
         };
         if (hidden <= 512) return run(std::integral_constant<int, 1>{});
