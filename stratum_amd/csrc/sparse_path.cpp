@@ -114,10 +114,15 @@ unsigned long long capture_of(hipStream_t stream) {
     return status == hipStreamCaptureStatusActive ? id : 0;
 }
 
-// A gradient that is captured into a graph must end where the capture can follow: a leaf that an eager graph still holds
-// is tied to that graph's stream, and torch's engine, passing a gradient on from the capture to it, ends the process. So
-// what follows a node in this backward pass is looked through first, on other streams of the same capture too; what
-// nobody asked for is not followed.
+bool can_join(hipStream_t stream, unsigned long long capture) {
+    const unsigned long long own = capture_of(stream);
+    return stream && (own == 0 || own == capture);
+}
+
+// A gradient that is captured into a graph must end where the capture can follow: torch's engine makes the stream of each
+// node wait for the one before, by which a stream becomes part of the capture; but not the null stream, to which a leaf
+// is tied by an eager graph from there that still holds it, nor one of another capture. The engine then ends the process.
+// So what follows a node in this backward pass is looked through first; what nobody asked for is not followed.
 void check_capture(const char* name) {
     const unsigned long long now = capture_of(c10::hip::getCurrentHIPStream().stream());
     if (!now) return;
@@ -133,10 +138,10 @@ void check_capture(const char* name) {
             torch::autograd::Node* next = n->next_edge(i).function.get();
             if (!seen.insert(next).second) continue;
             const auto stream = next->stream();
-            if (stream && capture_of(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *stream).stream()) != now)
+            if (stream && !can_join(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *stream).stream(), now))
                 throw std::runtime_error(std::string(name) +
                                          ": its gradient is captured into a graph, but goes on to a leaf of an eager graph, "
-                                         "whose stream takes no part in the capture; capture on leaves of its own "
+                                         "whose stream cannot take part in the capture; capture on leaves of its own "
                                          "(t.detach().requires_grad_()) or let go of the eager graph first");
             left.push_back(next);
         }

@@ -12,7 +12,8 @@ order. Here is what comes before and after it:
 The reference runs transformers' ``Qwen3MoeExperts`` and router there (``stratum/model/qwen3_moe.py``,
 ``stratum/moe.py``). None of the four reads anything back to the host; all can be captured into a graph, with their
 gradients too, on as many streams as take part in the capture. A captured gradient that would go on from one of them to a
-leaf that an eager graph holds is refused (capture on leaves of its own: ``t.detach().requires_grad_()``).
+leaf that an eager graph on the default stream holds is refused (capture on leaves of its own:
+``t.detach().requires_grad_()``).
 """
 
 from __future__ import annotations

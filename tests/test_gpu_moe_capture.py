@@ -117,3 +117,22 @@ def test_captured_gradients_that_accumulate(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a.grad, b.grad) for a, b in zip(leaves, want))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_leaf_of_an_eager_graph_on_a_stream_that_can_join(cuda, name):
+    """Work on any but the null stream becomes part of a capture when it waits for it, as the engine makes it do."""
+    op, value = operators()[name]
+    leaf = value.clone().requires_grad_(True)
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        eager = op(leaf)
+        d = torch.ones_like(eager) + torch.arange(eager.shape[-1], device=cuda)
+        want, = torch.autograd.grad(eager, leaf, d, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(op(leaf * 1.0), leaf, d)
+    replays_equal(graph, got, want)
+    assert torch.equal(torch.autograd.grad(eager, leaf, d)[0], want)
