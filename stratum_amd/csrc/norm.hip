@@ -210,8 +210,10 @@ struct NormBwd {
 // weight's gradient gathers in registers over the rows that the group takes (gridDim rows apart), then over the group's
 // row slots in LDS, and leaves as one row of partial sums; k_rms_dw adds those rows up in a fixed order. The next row is
 // then asked for before this one's sum: few groups, so that there are few partial sums, would leave the memory idle in
-// between ([8192, 4096] bf16, us, with the sum of the parts: without the weight's gradient 48, with it 60 without and 54 with
-// the look-ahead).
+// between. bf16 with a residual's gradient, us in a graph with the sum of the parts, look-ahead / none (x and residual read
+// again): [8192, 5120] 66 / 74 (80 / 85), [4096, 8192] 54 / 56 (66 / 67), [8192, 4096] 55 / 54 (70 / 67), [131072, 128]
+// 32 / 32 (39 / 38); the prologue costs a short launch 1 ([1021, 2050] 14.4 / 13.2). Without the weight's gradient
+// [8192, 4096] takes 52 (62).
 template <typename Tr, int T, bool DW>
 __global__ __launch_bounds__(kBlock<T>) void k_rms_bwd(NormBwd a) {
     constexpr int SLOTS = kBlock<T> / T;
@@ -392,8 +394,8 @@ constexpr int64_t kForwardCols = 1024 * 4 * 8, kBackwardCols = 1024 * 8;  // wha
 
 // Threads of a row: one vector each, up to 8192 columns; whole pairs of waves where that is more than a wave of them
 // ([8192, 5120] backward: 640 threads 67, 1024 80). More vectors a thread are slower, whether a wave then needs no
-// barrier or not ([8192, 4096] bf16 with a residual, us forward / backward: 64 threads of 8 vectors 55 / 115, 128 of 4
-// 55 / 61, 256 of 2 51 / 52, 512 of 1 49 / 48; [4096, 8192]: 256 57 / 59, 512 53 / 55, 1024 51 / 50).
+// barrier or not ([8192, 4096] bf16 with a residual, us forward / backward of h alone: 64 threads of 8 vectors 55 / 115, 128
+// of 4 55 / 61, 256 of 2 51 / 52, 512 of 1 49 / 48; [4096, 8192]: 256 57 / 59, 512 53 / 55, 1024 51 / 50).
 int row_threads(int64_t cols) {
     const int64_t vecs = (cols + 7) / 8;
     if (vecs > 256) return vecs < 1024 ? (int)(vecs + 127) / 128 * 128 : 1024;
@@ -403,8 +405,10 @@ int row_threads(int64_t cols) {
 }
 
 // Groups of the backward's grid that write partial sums: as many as give each of the 256 compute units up to 1024 threads
-// and the same work ([8192, 4096] us: 256 groups of 512 threads 67, 384 60, 512 54, 768 61, 1024 58; [131072, 128], 256
-// threads: 512 34, 1024 28, 2048 33; [8192, 5120], 640 threads: 256 77, 384 96, 512 79).
+// and the same work; half or twice as many are within a tenth of them or slower (bf16 with a residual's gradient, us in a
+// graph: [8192, 4096], 512 threads, 256 groups 51, 384 57, 512 55, 768 59, 1024 58; [40000, 2048], 256 threads, 256 159, 512
+// 115, 1024 127; [131072, 128], 256 threads, 512 31, 1024 32, 2048 36; [8192, 5120], 640 threads, 256 66, 384 78, 512 70;
+// [1021, 2050], 384 threads, 256 16, 512 14, 1021 21).
 int dw_groups(int64_t rows, int64_t cols) {
     if (cols > kBackwardCols) return (int)(rows < 256 ? rows : 256);
     const int t = row_threads(cols), slots = t <= 256 ? 256 / t : 1, threads = t <= 256 ? 256 : t;

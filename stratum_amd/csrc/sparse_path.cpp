@@ -1,7 +1,8 @@
 // Host code of the sparse layer's operators (functions of the CPython module stratum_amd._fast): their
 // calls and autograd nodes, whose time is the host's where a batch is small. One token through the norm, us a call:
-// from Python 15, here 6; 8192 tokens routed with their gradient 102, here 48, of which torch's engine takes 44 for any
-// node (it wakes the device's thread).
+// from Python 15, here 6; 8192 tokens routed with their gradient 102, here 48. A step of torch's own product with a number
+// takes 42 to 48 beside it, one of a view 31 to 35: the engine wakes the device's thread. Of the norm's steps one of x takes
+// 46, of x and the residual 62, of the weight too 73.
 //
 // Operands that are not as they have to be are handed back (None): the Python layer says what is wrong with them, or
 // converts them (subclasses) or changes the device and calls again.
